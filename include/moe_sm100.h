@@ -46,7 +46,7 @@ extern "C" {
 
 #define MOE_DTYPE_BF16 0
 #define MOE_DTYPE_F16 1
-#define MOE_DTYPE_F32 2 /* accepted by moe_router_topk and moe_router_tail only */
+#define MOE_DTYPE_F32 2 /* accepted by the router's entry points and for the norm's weight only */
 
 #define MOE_ACT_NONE 0
 #define MOE_ACT_SILU 1
@@ -103,6 +103,43 @@ int moe_router_topk(const void* logits, void* scores, int64_t* indices, int32_t*
  * fp32 logits.  E <= 1024, k <= min(32, E). */
 int moe_router_tail(const void* logits, const float* bias, void* scores, int64_t* indices, int64_t num_tokens, int num_experts,
                     int topk, int softmax_before_topk, int normalize, int dtype, int scores_dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Routing to experts in groups, in one launch: p = sigmoid or softmax of the logits [T, E]; c = p + bias (fp32 [E], may be NULL;
+ * for the selection only); the experts are num_groups equal runs, a group's score is the sum of its best `group_best`
+ * (1 or 2) c; the topk best c inside the topk_groups best groups are selected; scores [T, topk] = scale * p, divided by the
+ * sum of the selected p + 1e-20 when normalize; indices int64 [T, topk] in descending order of c.  The selection is that of exact
+ * arithmetic on the logits as they are given: values too close for fp32 are compared in 64 bits.  Equal values: lowest
+ * index first; NaN after everything else.  E <= 1024, num_groups <= 32, topk <= 32.  dtype (logits), scores_dtype:
+ * MOE_DTYPE_BF16 / F16 / F32.  No counterpart in the reference (its routers are moe_router_topk's and moe_router_tail's).
+ * moe_grouped_topk_backward: d_logits [T, E] (dtype) from d_scores [T, topk] (scores_dtype) and the selection;
+ * the selection itself and the bias have no gradient.
+ * --------------------------------------------------------------------------------- */
+int moe_grouped_topk(const void* logits, const float* bias, void* scores, int64_t* indices, int64_t num_tokens,
+                     int num_experts, int num_groups, int topk_groups, int group_best, int topk, int sigmoid,
+                     int normalize, float scale, int dtype, int scores_dtype, void* stream);
+int moe_grouped_topk_backward(const void* logits, const int64_t* indices, const void* d_scores, void* d_logits,
+                              int64_t num_tokens, int num_experts, int topk, int sigmoid, int normalize, float scale,
+                              int dtype, int scores_dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Root-mean-square norm of rows x [num_rows, cols] (row stride x_stride elements), with the residual's addition:
+ *   h = x + residual (rounded to `dtype`; x itself without a residual);  r = 1 / sqrt(mean h^2 + eps);  y = h * r * weight
+ * y [num_rows, cols] in `dtype` and / or in 8 bits: q (e4m3) and scales fp32 [num_rows, ceil(cols / 128)], where a
+ * block's scale is max(max |y|, 2^-80) / 448 and q = y / scale.  h (may be NULL), y, q and rstd (fp32 [num_rows], may
+ * be NULL) are dense.  weight [cols]: `dtype`, or fp32.  cols a multiple of 8, at most 16384; pointers and row strides 16-byte
+ * aligned.
+ * Backward: dx = dh + r (g - h r mean(g h r)) with g = dy * weight (dh may be NULL; dx is also the residual's gradient), dw =
+ * sum over the rows of dy h r in weight_dtype, added up in a fixed order.  partials: fp32 [moe_rms_norm_partials(num_rows),
+ * cols], overwritten.  No counterpart in the reference (its layer begins behind the norm).
+ * --------------------------------------------------------------------------------- */
+int moe_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                 int weight_dtype, void* h, void* y, void* q, float* scales, float* rstd, int64_t num_rows, int cols,
+                 float eps, int dtype, void* stream);
+int64_t moe_rms_norm_partials(int64_t num_rows);
+int moe_rms_norm_backward(const void* dy, const void* dh, const void* h, int64_t h_stride, const void* weight,
+                          int weight_dtype, const float* rstd, void* dx, void* dw, float* partials,
+                          int64_t num_rows, int cols, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * (a) Routing metadata.  Replaces get_token_indices (src/moe_explore/expert_permute.py:19-41):

@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
-from ctypes import c_int, c_int32, c_int64, c_size_t, c_void_p, c_char_p, POINTER
+from ctypes import c_float, c_int, c_int32, c_int64, c_size_t, c_void_p, c_char_p, POINTER
 
 import torch
 
@@ -78,6 +78,12 @@ SIGNATURES = {
     "moe_layout_from_groups": (c_int, [c_void_p, c_int64, c_int] + [c_void_p] * 7 + [c_void_p]),
     "moe_router_topk": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "moe_router_tail": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "moe_grouped_topk": (c_int, [c_void_p] * 4 + [c_int64] + [c_int] * 7 + [c_float, c_int, c_int, c_void_p]),
+    "moe_grouped_topk_backward": (c_int, [c_void_p] * 4 + [c_int64] + [c_int] * 4 + [c_float, c_int, c_int, c_void_p]),
+    "moe_rms_norm": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int] + [c_void_p] * 5 +
+                     [c_int64, c_int, c_float, c_int, c_void_p]),
+    "moe_rms_norm_partials": (c_int64, [c_int64]),
+    "moe_rms_norm_backward": (c_int, [c_void_p] * 3 + [c_int64, c_void_p, c_int] + [c_void_p] * 4 + [c_int64, c_int, c_int, c_void_p]),
     "moe_store_to_host": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "moe_copy_blocks": (c_int, [POINTER(c_void_p), POINTER(c_void_p), POINTER(c_size_t), c_int, c_void_p]),
     "moe_zero_padding_rows": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
@@ -190,6 +196,11 @@ def _ptr(t):
 def _stream():
     # what torch.cuda.current_stream().cuda_stream reads, without building a Stream object (2 us a call)
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which the launches go to the current stream of the tensor's device."""
+    return _NO_SECTION if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def dtype_code(dtype: torch.dtype) -> int:
@@ -369,6 +380,59 @@ def router_tail(logits, topk: int, softmax_before_topk: bool, normalize: int, bi
     _check("moe_router_tail", rc)
     _count(1)
     return scores, indices
+
+
+def grouped_topk(logits, bias, num_groups: int, topk_groups: int, group_best: int, topk: int, sigmoid: bool, normalize: bool,
+                 scale: float, dtype):
+    """Scores [T, k] in ``dtype`` and indices int64 [T, k] (see moe_grouped_topk)."""
+    T, E = logits.shape
+    scores = torch.empty(T, topk, dtype=dtype, device=logits.device)
+    indices = torch.empty(T, topk, dtype=torch.int64, device=logits.device)
+    with timed("router:topk"):
+        rc = load().moe_grouped_topk(logits.data_ptr(), _ptr(bias), scores.data_ptr(), indices.data_ptr(), T, E, num_groups,
+                                     topk_groups, group_best, topk, sigmoid, normalize, scale, float_code(logits.dtype),
+                                     float_code(dtype), _stream())
+    _check("moe_grouped_topk", rc)
+    _count(1)
+    return scores, indices
+
+
+def grouped_topk_backward(logits, indices, d_scores, sigmoid: bool, normalize: bool, scale: float):
+    """The gradient of ``grouped_topk``'s logits."""
+    T, E = logits.shape
+    d_logits = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
+    with timed("router:bwd"):
+        rc = load().moe_grouped_topk_backward(logits.data_ptr(), indices.data_ptr(), d_scores.data_ptr(), d_logits.data_ptr(), T, E,
+                                              indices.size(1), sigmoid, normalize, scale, float_code(logits.dtype),
+                                              float_code(d_scores.dtype), _stream())
+    _check("moe_grouped_topk_backward", rc)
+    _count(1)
+    return d_logits
+
+
+def rms_norm(x, residual, weight, eps: float, h=None, y=None, q=None, scales=None, rstd=None):
+    """Rows ``x`` [R, d] (row stride allowed) into the outputs that are given (see moe_rms_norm)."""
+    with timed("rows:norm"):
+        rc = load().moe_rms_norm(x.data_ptr(), x.stride(0), _ptr(residual), 0 if residual is None else residual.stride(0),
+                                 weight.data_ptr(), float_code(weight.dtype), _ptr(h), _ptr(y), _ptr(q), _ptr(scales), _ptr(rstd),
+                                 x.size(0), x.size(1), eps, dtype_code(x.dtype), _stream())
+    _check("moe_rms_norm", rc)
+    _count(1)
+
+
+def rms_norm_backward(dy, dh, h, weight, rstd):
+    """(dx, dw) (see moe_rms_norm_backward)."""
+    rows, cols = h.shape
+    dx = torch.empty(rows, cols, dtype=h.dtype, device=h.device)
+    dw = torch.empty_like(weight)
+    partials = torch.empty(int(load().moe_rms_norm_partials(rows)), cols, dtype=torch.float32, device=h.device)
+    with timed("rows:norm_bwd"):
+        rc = load().moe_rms_norm_backward(dy.data_ptr(), _ptr(dh), h.data_ptr(), h.stride(0), weight.data_ptr(), float_code(weight.dtype),
+                                          rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), partials.data_ptr(), rows, cols,
+                                          dtype_code(h.dtype), _stream())
+    _check("moe_rms_norm_backward", rc)
+    _count(2)
+    return dx, dw
 
 
 _PINNED = {}

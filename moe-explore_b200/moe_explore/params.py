@@ -77,6 +77,22 @@ class ErnieRouterParams(RouterParams):
 
 
 @dataclass
+class GroupedTopkRouterParams(RouterParams):
+    """Sigmoid or softmax scores, a bias that balances the load (added for the selection only), experts in ``num_groups``
+    equal groups of which the ``topk_groups`` best stay open (a group's score: the sum of its best ``group_best``
+    biased scores, 1 or 2), top-k inside them, weights renormalised and scaled.  No reference counterpart."""
+    router_weight: torch.Tensor           # [d, E]; fp32: the logits are computed in fp32
+    topk: int
+    bias: Optional[torch.Tensor] = None   # [E], fp32
+    num_groups: int = 1
+    topk_groups: int = 1
+    group_best: int = 2
+    score_function: str = "sigmoid"       # or "softmax"
+    normalize_routing: bool = True
+    scale: float = 1.0
+
+
+@dataclass
 class MOEParams:
     router_params: RouterParams
     expert_params: FFNParams

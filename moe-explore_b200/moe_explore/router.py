@@ -12,7 +12,7 @@ import torch.nn.functional as F
 from torch.autograd import forward_ad
 
 from moe_explore import _native
-from moe_explore.params import ErnieRouterParams, RouterParams, TopkRouterParams
+from moe_explore.params import ErnieRouterParams, GroupedTopkRouterParams, RouterParams, TopkRouterParams
 
 
 def softmax(x: torch.Tensor) -> torch.Tensor:
@@ -26,6 +26,8 @@ def router(input: torch.Tensor, params: RouterParams):
         return topk_router(input, params)
     if isinstance(params, ErnieRouterParams):
         return ernie_router(input, params)
+    if isinstance(params, GroupedTopkRouterParams):
+        return grouped_topk_router(input, params)
     raise ValueError(f"Unsupported router type: {type(params)}")
 
 
@@ -142,3 +144,59 @@ def ernie_router(input: torch.Tensor, router_params: ErnieRouterParams):
         picked = torch.gather(probs, dim=-1, index=indices)
         picked = picked / torch.clamp(picked.sum(dim=-1, keepdim=True), min=1e-12)
         return picked.to(input.dtype), indices
+
+
+class _GroupedTopk(torch.autograd.Function):
+    """scores, indices of ``logits``; differentiable with respect to the logits, given the selection."""
+
+    @staticmethod
+    def forward(ctx, logits, bias, p, dtype):
+        sigmoid = p.score_function == "sigmoid"
+        scores, indices = _native.grouped_topk(logits, bias, p.num_groups, p.topk_groups, _group_best(p), p.topk, sigmoid,
+                                               bool(p.normalize_routing), float(p.scale), dtype)
+        ctx.save_for_backward(logits, indices)
+        ctx.cfg = (sigmoid, bool(p.normalize_routing), float(p.scale))
+        ctx.mark_non_differentiable(indices)
+        return scores, indices
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_scores, _d_indices):
+        logits, indices = ctx.saved_tensors
+        return _native.grouped_topk_backward(logits, indices, d_scores.contiguous(), *ctx.cfg), None, None, None
+
+
+def _group_best(p: GroupedTopkRouterParams) -> int:
+    return p.group_best if p.num_groups > 1 else 1   # one group has no rank
+
+
+def grouped_topk_of_logits(logits: torch.Tensor, params: GroupedTopkRouterParams, dtype: torch.dtype = None):
+    """Everything of ``grouped_topk_router`` after the linear layer: ``logits`` [T, E] (bf16, fp16 or fp32) -> (scores [T, k] in
+    ``dtype`` (the logits'), indices int64 [T, k], in descending order of the biased score).  One kernel; the selection is that of
+    exact arithmetic, equal values by ascending index, NaN last.  Differentiable with respect to the logits."""
+    dtype = logits.dtype if dtype is None else dtype
+    _native.require_cuda(logits, params.bias)
+    if logits.dim() != 2:
+        raise ValueError(f"logits are [tokens, experts], got {tuple(logits.shape)}")
+    if params.score_function not in ("sigmoid", "softmax"):
+        raise ValueError(f"score_function is 'sigmoid' or 'softmax', got {params.score_function!r}")
+    bias = params.bias
+    if bias is not None:
+        if bias.dtype is not torch.float32 or bias.shape != logits.shape[1:] or bias.device != logits.device:
+            raise ValueError("bias is fp32 [experts] on the device of the logits")
+        bias = bias.detach().contiguous()
+    with _native.on_device_of(logits):
+        return _GroupedTopk.apply(logits.contiguous(), bias, params, dtype)
+
+
+def grouped_topk_router(input: torch.Tensor, params: GroupedTopkRouterParams):
+    """Linear logits -> scores -> biased, group-limited top-k -> renormalised, scaled weights in the input's dtype (see
+    ``GroupedTopkRouterParams``).  With an fp32 router weight the logits are computed in fp32, as the selection of such models is
+    sensitive to the rounding of the logits."""
+    weight = params.router_weight
+    if weight.dtype is torch.float32:
+        with torch.autocast(device_type=input.device.type, enabled=False):
+            logits = input.float() @ weight
+    else:
+        logits = input @ weight
+    return grouped_topk_of_logits(logits, params, input.dtype)
