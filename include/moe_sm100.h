@@ -550,6 +550,78 @@ size_t moe_rows_pass_size(void);
 #define MOE_ROWS_ALL 7
 int moe_rows_gemm(const moe_rows_pass* pass, int steps, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Products in 8 bits (for serving: forward only).  No counterpart in the reference.
+ * Rows: e4m3 [rows, K] with fp32 scales [rows, ceil(K / 128)], a scale per row and block of 128 columns.  Weights: e4m3 [E, N, K]
+ * (K contiguous) with fp32 scales [E, ceil(N / 128), ceil(K / 128)], a scale per 128 x 128 block; gated ones [E, 2, N, K]
+ * (gate, up) with scales [E, 2, ceil(N / 128), ceil(K / 128)].  Products of a block are summed in fp32 by the tensor cores, then
+ * multiplied by the two scales and added in fp32.  K a multiple of 16, N of 8 (of 16 where the result is in 8 bits); e4m3
+ * pointers 16-byte aligned.
+ * --------------------------------------------------------------------------------- */
+
+/* 16-bit rows [num_rows, cols] -> q (e4m3) and scales: per block scale = max(max |x|, 2^-80) / 448, q = x / scale rounded once
+ * to nearest even.  cols a multiple of 16. */
+int moe_f8_quantize_rows(const void* x, void* q, float* scales, int64_t num_rows, int cols, int dtype, void* stream);
+
+/* The experts of a layer: rows to 8 bits -> w1 with the activation, result in 8 bits again (a scale per row and 128 columns of
+ * the activated product, from its fp32 values) -> w2 -> weighted fold.  `steps` selects the launches as in moe_expert_forward.
+ * x [num_tokens, d] in `dtype`, or, with x_scales != NULL, rows that are in 8 bits already; w1 [E, 2, inter, d] (gated) or
+ * [E, inter, d], w2 [E, d, inter]; xs [padded_rows, d], hidden [padded_rows, inter] in 8 bits with their scales; ys
+ * [padded_rows, d], out, addend (may be NULL) [num_tokens, d] and scores [num_tokens, topk] in `dtype`.  Index arrays, status
+ * and workspace as in moe_expert_pass; padded_rows = moe_padded_rows_bound(num_tokens * topk, num_experts). */
+typedef struct moe_f8_pass {
+  int64_t num_tokens, padded_rows;
+  int32_t d, inter, num_experts, topk, act, dtype;
+  const int64_t* expert_idx;
+  const void* x;
+  const float* x_scales;
+  const void *scores, *w1;
+  const float* w1_scales;
+  const void* w2;
+  const float* w2_scales;
+  int32_t *group_indices, *pad_offsets, *row_src, *dst_row, *mtile_expert, *tile_pairs, *num_mtiles, *status;
+  void* workspace;
+  size_t workspace_bytes;
+  void* xs;
+  float* xs_scales;
+  void* hidden;
+  float* hidden_scales;
+  void *ys, *out;
+  const void* addend;
+} moe_f8_pass;
+
+size_t moe_f8_pass_size(void);
+
+#define MOE_F8_ROUTE 1
+#define MOE_F8_DISPATCH 2
+#define MOE_F8_UP 4
+#define MOE_F8_DOWN 8
+#define MOE_F8_FOLD 16
+#define MOE_F8_ALL 31
+int moe_f8_expert_forward(const moe_f8_pass* pass, int steps, void* stream);
+
+/* The functional product: out[o(r)] = act(x[i(r)] @ w[expert of r]^T) for rows r < num_rows grouped by group_indices [E + 1]
+ * (NULL: one expert, no maps needed); i(r) = perm[r] / topk with gather, else r; o(r) = perm[r] with scatter, else r.  x [x_rows,
+ * k_dim]; gathered rows go through `gathered` [num_rows, k_dim] and its scales.  Negative entries of perm: a zero row / not
+ * stored.  act: none or element-wise.  Steps: MOE_ROWS_*. */
+typedef struct moe_f8_rows_pass {
+  int64_t num_rows, x_rows;
+  int32_t num_experts, k_dim, n_dim, topk, act, dtype, gather, scatter;
+  const void* x;
+  const float* x_scales;
+  const void* w;
+  const float* w_scales;
+  void* out;
+  const int32_t* group_indices;
+  const int64_t* perm;
+  int32_t *pad_offsets, *mtile_expert, *tile_pairs, *num_mtiles, *status;
+  void* gathered;
+  float* gathered_scales;
+} moe_f8_rows_pass;
+
+size_t moe_f8_rows_pass_size(void);
+int moe_f8_rows_gemm(const moe_f8_rows_pass* pass, int steps, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,10 @@ constexpr int kF8Block = 128;
 constexpr float kF8Top = 448.0f;
 constexpr float kF8Least = 8.271806125530277e-25f;  // 2^-80
 
+// The wait of the kernels in this family for the one they are chained to: nothing before it touches global memory, and what was
+// said about such kernels at grid_wait() holds for them (no __restrict__, no __ldg).
+__device__ __forceinline__ void await_predecessor() { grid_wait(); }
+
 __device__ __forceinline__ uint32_t f8x4(float a, float b, float c, float d) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);

@@ -1,0 +1,862 @@
+// Grouped products of 8-bit rows and 8-bit weights on the tensor cores, a scale per row and 128 columns on one side and per 128 x 128
+// block on the other:
+//
+//   out[r, n] = sum over the blocks b of K:  sx[r, b] * sw[n / 128, b] * sum over k in b: x[r, k] * w[e][n, k]
+//
+// The inner sums are tcgen05.mma (kind::f8f6f4, e4m3 x e4m3) over one 128-byte-deep stage into an accumulator of their own in TMEM; the
+// epilogue warps fetch it, multiply by the two scales and add in fp32 registers while the tensor cores work on the next block.
+// (The scales are fp32, not powers of two, so the tensor cores' own block scaling cannot apply them.)
+//
+// Two kernels, chosen by how many rows an expert has (f8_gemm.cu):
+//   f8_pair_kernel   rows on the accumulator's lanes: a CTA pair covers 256 rows x 256 weight rows of one expert
+//   f8_lanes_kernel  weights on the lanes: a CTA covers 128 weight rows (of gate AND up where gated) and up to R rows of one
+//                    expert, so that few rows cost few columns and the weights stream at the rate of the memory
+//
+// Operands are described to the copy engine as pairs of bytes (16-bit elements, 64 to a 128-byte swizzle row); loads past an edge
+// read zeros, which are zeros in e4m3 too.
+#pragma once
+
+#include "f8.cuh"
+#include "gemm_kernel.cuh"
+
+namespace moe {
+
+// What a product's results become.
+enum F8Out : int {
+  F8_ROWS = 0,       // 16-bit rows, element-wise activation
+  F8_QUANT = 1,      // 8-bit rows with scales, element-wise activation
+  F8_GLU_QUANT = 2,  // 8-bit rows with scales of act(gate) * up; w holds [E][gate, up][I][K]
+};
+
+// A product as the host asks for it (f8_gemm.cu).
+struct F8Product {
+  int kind;  // F8Out
+  const void* x;            // [x_rows, K]
+  const float* x_scales;    // [x_rows, ceil(K / 128)]
+  int64_t x_rows;
+  const void* w;            // [E, N, K], gated [E, 2, N, K]
+  const float* w_scales;    // [E(, 2), ceil(N / 128), ceil(K / 128)]
+  void* out;
+  float* out_scales;
+  int K, N, num_experts, act, dtype;
+  int64_t routed_rows;      // about how many rows there are
+  bool dense;
+  int compact;
+  const int64_t* out_perm;
+  int64_t out_rows;
+  const int32_t *mtile_expert, *tile_pairs, *num_mtiles, *pad_offsets, *group_indices;
+  int32_t* status;
+};
+int f8_product(const char* name, const F8Product& p, void* stream);
+
+struct F8Args {
+  // The rows of the experts: maps of the padded layout, or dense_rows >= 0: one expert, rows 0 .. dense_rows - 1, no maps.
+  const int32_t *mtile_expert, *tile_pairs, *num_mtiles, *pad_offsets, *group_indices;
+  int64_t dense_rows;
+  int32_t compact;       // x and out hold the rows without padding, expert by expert
+  int64_t total_rows;    // rows of x
+  const float* x_scales;
+  const float* w_scales;
+  void* out;
+  float* out_scales;
+  const int64_t* out_perm;  // F8_ROWS: row r of x goes to row out_perm[r] of out (negative: nowhere)
+  int64_t out_rows;
+  int32_t n_dim;            // columns of out
+  int32_t k_dim;
+  int32_t act;
+  int32_t group_m;
+  long long wait_limit;
+  int32_t* status;
+};
+
+// One work item of a CTA: `rows` rows of x from a_row on (0: nothing to do for this CTA of a pair), result columns from n0 on.
+struct F8Item {
+  int a_row, n0, expert, rows;
+  bool valid;
+};
+
+// The items of one worker, decoded 32 at a time, one per lane (a chain of dependent loads each), and taken from the lanes in turn.
+// Row units (two row tiles of one expert for a CTA pair, one otherwise) are walked in groups of group_m, inside a group column
+// tile by column tile, so that the workers running at one time share weight and row tiles in L2.
+template <int CTAS> struct F8Walk {
+  F8Item mine;
+  int first, stride, count, units, nt, rank;
+  __device__ __forceinline__ F8Walk(const F8Args& a, int worker, int workers, int cols_per_tile, int rank_)
+      : mine{}, first(worker), stride(workers), rank(rank_) {
+    nt = (a.n_dim + cols_per_tile - 1) / cols_per_tile;
+    units = a.dense_rows >= 0 ? static_cast<int>((a.dense_rows + CTAS * BM - 1) / (CTAS * BM)) : map_word(a.num_mtiles + (CTAS == 2 ? 1 : 0));
+    count = units * nt;
+  }
+  __device__ __forceinline__ F8Item decode(int t, const F8Args& a, int cols_per_tile) const {
+    const int groups = (units + a.group_m - 1) / a.group_m;
+    const int group_m = (units + groups - 1) / groups;
+    const int g = t / (group_m * nt);
+    const int rem = t - g * group_m * nt;
+    const int gm = min(group_m, units - g * group_m);
+    const int n_idx = rem / gm;
+    const int unit = g * group_m + rem - n_idx * gm;
+    F8Item c;
+    c.n0 = n_idx * cols_per_tile;
+    c.valid = true;
+    if (a.dense_rows >= 0) {
+      c.expert = 0;
+      c.a_row = (unit * CTAS + rank) * BM;
+      const int64_t left = a.dense_rows - c.a_row;
+      c.rows = left < 0 ? 0 : left < BM ? static_cast<int>(left) : BM;
+      return c;
+    }
+    int tile = unit;
+    bool active = true;
+    if (CTAS == 2) {
+      const uint32_t info = static_cast<uint32_t>(map_word(a.tile_pairs + unit));
+      tile = static_cast<int>(info & 0xFFFFFu);
+      c.expert = static_cast<int>((info >> 20) & 0x7FFu);
+      if (rank == 1) {
+        if (info >> 31) ++tile;
+        else active = false;  // re-reads the first tile and stores nothing
+      }
+    } else {
+      c.expert = map_word(a.mtile_expert + unit);
+    }
+    const int base = map_word(a.pad_offsets + c.expert);
+    const int begin = map_word(a.group_indices + c.expert), end = map_word(a.group_indices + c.expert + 1);
+    const int inside = tile * BM - base;
+    c.a_row = a.compact ? begin + inside : tile * BM;
+    int rows = end - begin - inside;
+    if (rows > BM) rows = BM;
+    if (rows > a.total_rows - c.a_row) rows = static_cast<int>(a.total_rows - c.a_row);  // (whatever the prefix says)
+    c.rows = active && rows > 0 && c.a_row >= 0 ? rows : 0;
+    return c;
+  }
+  __device__ __forceinline__ F8Item get(int i, const F8Args& a, int cols_per_tile) {
+    if ((i & 31) == 0) {
+      const int t = first + (i + static_cast<int>(threadIdx.x & 31)) * stride;
+      if (t < count) mine = decode(t, a, cols_per_tile);
+      __syncwarp();
+    }
+    const int src = i & 31;
+    F8Item c;
+    c.valid = first + i * stride < count;
+    c.a_row = __shfl_sync(0xFFFFFFFFu, mine.a_row, src);
+    c.n0 = __shfl_sync(0xFFFFFFFFu, mine.n0, src);
+    c.expert = __shfl_sync(0xFFFFFFFFu, mine.expert, src);
+    c.rows = __shfl_sync(0xFFFFFFFFu, mine.rows, src);
+    return c;
+  }
+};
+
+// e4m3 x e4m3 -> fp32, both operands K-major: the instruction descriptor without the extents.
+constexpr uint32_t kF8Idesc = 1u << 4;
+__host__ __device__ constexpr uint32_t f8_idesc(int m, int n) {
+  return kF8Idesc | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 lanes x 16 consecutive fp32 columns.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Waits for the warp's TMEM loads; the registers pass through, so that nothing that reads them is moved before the wait.
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
+}
+// a += v * f on two fp32 values at once.
+__device__ __forceinline__ void fma2(uint64_t& a, uint32_t v0, uint32_t v1, uint64_t f) {
+  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(a) : "r"(v0), "r"(v1), "l"(f));
+}
+__device__ __forceinline__ uint64_t twice(float f) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(f));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+// The element-wise activation of a register row; the choice is made once per row, so that the elements interleave.
+template <int N> __device__ __forceinline__ void act_row(float (&v)[N], int act) {
+  if (act == MOE_ACT_SILU || act == MOE_ACT_SWIGLU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = silu_f(v[i]);
+  } else if (act == MOE_ACT_GELU || act == MOE_ACT_GEGLU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = gelu_f(v[i]);
+  } else if (act == MOE_ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = gelu_tanh_f(v[i]);
+  }
+}
+// Warps: 0 producer, 1 MMA issuer, 2 and 3 none, 4 to 11 epilogue: whole warpgroups, so that the epilogue's take the registers that
+// the first one gives back (40 + 2 * 232 = 3 * 168, what the launch has).
+constexpr int kF8Threads = 384;
+constexpr int kF8LaunchRegs = 168, kF8FewRegs = 40, kF8EpilogueRegs = 232;
+static_assert(kF8FewRegs + 2 * kF8EpilogueRegs <= 3 * kF8LaunchRegs, "register split");
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8FewRegs)); }
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8EpilogueRegs)); }
+
+constexpr int kF8K = 128;                    // bytes (= elements) of K in one stage: one swizzle row
+constexpr int kF8Tile = BM * kF8K;           // 16 KB: 128 rows of an operand
+constexpr int kF8MmaK = 32;                  // K of one instruction
+
+// ------------------------------------------------------------------------------------------------------------------
+// Rows on the lanes, CTA pairs.
+//
+// A pair's tile is 256 rows x 256 weight rows (128 gate + 128 up rows where gated); per 128 of K each CTA loads 16 KB of rows and
+// 16 KB of weights, and the leader's four instructions (M 256, N 256, K 32) fill one of the two accumulator stages.  Each of
+// the eight epilogue warps of a CTA owns 32 rows x 128 of the columns: 128 fp32 sums per thread, fetched from TMEM 16 columns
+// at a time, the next 16 on their way while the last are added (two additions per instruction).  A thread's row is its lane, so
+// the row's scale is one register, and so is the weight block's.
+// ------------------------------------------------------------------------------------------------------------------
+struct F8PairPlan {
+  static constexpr int kStageBytes = 2 * kF8Tile;
+  static constexpr int kStages = 6;
+  static constexpr int kStagingTile = 32 * 128;
+  static constexpr int kStagingBytes = kEpilogueWarps * kStagingTile;
+  static constexpr int kBarrierBytes = 1024;
+  static constexpr int kTotal = kStages * kStageBytes + kStagingBytes + kBarrierBytes + 1024;
+  static_assert(kTotal <= 232448, "shared memory");
+};
+
+template <typename T, int OUT>
+__global__ void __launch_bounds__(kF8Threads, 1)
+f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const F8Args args) {
+  using Plan = F8PairPlan;
+  constexpr int kStages = Plan::kStages;
+  constexpr bool kGlu = OUT == F8_GLU_QUANT;
+  constexpr int kCols = kGlu ? 128 : 256;  // result columns of a tile
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t tiles_addr = (raw_addr + 1023u) & ~1023u;
+  uint8_t* tiles = smem_raw + (tiles_addr - raw_addr);
+  const uint32_t staging_addr = tiles_addr + kStages * Plan::kStageBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kStages * Plan::kStageBytes + Plan::kStagingBytes);
+  const uint32_t full_bar = smem_u32(bars);                      // [kStages]  (used in the leader CTA)
+  const uint32_t empty_bar = smem_u32(bars + kStages);           // [kStages]  (one set per CTA)
+  const uint32_t tfull_bar = smem_u32(bars + 2 * kStages);       // [2]        (one set per CTA)
+  const uint32_t tempty_bar = smem_u32(bars + 2 * kStages + 2);  // [2]        (used in the leader CTA)
+  const uint32_t meet_bar = smem_u32(bars + 2 * kStages + 4);    // [4]        the two warps of a quadrant
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  WaitCtx wctx;
+  wctx.abort_flag = abort_flag;
+  wctx.peer_abort = mapa_shared(smem_u32(const_cast<int*>(abort_flag)), static_cast<uint32_t>(rank ^ 1));
+  wctx.status = args.status;
+  wctx.limit = args.wait_limit;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar + 8 * s, 2);
+      mbar_init(empty_bar + 8 * s, 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar + 8 * a, 1);
+      mbar_init(tempty_bar + 8 * a, kEpilogueWarps * 2);
+    }
+    for (int q = 0; q < 4; ++q) mbar_init(meet_bar + 8 * q, 2);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_x);
+    tma_prefetch_desc(&tmap_w);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  await_predecessor();
+  const uint32_t tmem_base = *tmem_slot;
+  F8Walk<2> walk(args, blockIdx.x >> 1, gridDim.x >> 1, kCols, rank);
+  const int kiters = (args.k_dim + kF8K - 1) / kF8K;
+
+  if (warp >= 4) {
+    more_registers();
+    // ------------------------------ epilogue ----------------------------------
+    const int quad = warp & 3;
+    const int half = (warp - 4) >> 2;
+    const uint32_t tempty_leader = mapa_shared(tempty_bar, 0);
+    const uint32_t stage_base = staging_addr + (warp - 4) * Plan::kStagingTile;
+    const int kblocks = kiters;
+    // first accumulator column of the thread's two groups of 64
+    const int col_a = kGlu ? 64 * half : 128 * half;
+    const int col_b = kGlu ? 128 + 64 * half : 128 * half + 64;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      const F8Item c = walk.get(i, args, kCols);
+      if (!c.valid) break;
+      const int r = quad * 32 + lane;
+      const bool live = quad * 32 < c.rows;  // some of this warp's rows exist
+      const int64_t row = static_cast<int64_t>(c.a_row) + (r < c.rows ? r : c.rows > 0 ? c.rows - 1 : 0);
+      const float* xs = args.x_scales + row * kblocks;
+      const int nblocks = (args.n_dim + kF8Block - 1) / kF8Block;
+      // (a tile's second block of columns may lie past the last one: its products are zeros, any scale serves)
+      const int nb = kGlu ? c.n0 / kF8Block : min(c.n0 / kF8Block + half, nblocks - 1);
+      const float* wa = args.w_scales + (static_cast<int64_t>(c.expert) * (kGlu ? 2 : 1) * nblocks + nb) * kblocks;
+      const float* wb = wa + static_cast<int64_t>(nblocks) * kblocks;
+      uint64_t sum[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) sum[j] = 0;
+      float x0 = 0.0f, a0 = 0.0f, b0 = 0.0f, x1 = 0.0f, a1 = 0.0f, b1 = 0.0f;
+      if (live) {
+        x0 = xs[0];
+        a0 = wa[0];
+        if (kGlu) b0 = wb[0];
+        if (kiters > 1) {
+          x1 = xs[1];
+          a1 = wa[1];
+          if (kGlu) b1 = wb[1];
+        }
+      }
+      for (int kb = 0; kb < kiters; ++kb) {
+        const uint64_t fa = twice(x0 * a0), fb = kGlu ? twice(x0 * b0) : fa;
+        x0 = x1;
+        a0 = a1;
+        b0 = b1;
+        if (live && kb + 2 < kiters) {
+          x1 = xs[kb + 2];
+          a1 = wa[kb + 2];
+          if (kGlu) b1 = wb[kb + 2];
+        }
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar + 8 * acc, acc_phase, wctx, DS_TIMEOUT_EPILOGUE))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (live) {
+          const uint32_t t0 = tmem_base + lanes + acc * 256;
+          uint32_t v[2][16];
+          tmem_ld_32x16(t0 + col_a, v[0]);
+          tmem_ld_wait16(v[0]);
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch) {
+            if (ch < 7) tmem_ld_32x16(t0 + (ch + 1 < 4 ? col_a + 16 * (ch + 1) : col_b + 16 * (ch - 3)), v[(ch + 1) & 1]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) fma2(sum[ch * 8 + j], v[ch & 1][2 * j], v[ch & 1][2 * j + 1], ch < 4 ? fa : fb);
+            if (ch < 7) tmem_ld_wait16(v[(ch + 1) & 1]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * acc);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+      if (!ok) break;
+      if constexpr (OUT == F8_ROWS) {
+        if (!live) continue;
+        // 64 columns at a time through the warp's staging tile, so that a store covers four whole 128-byte row segments
+        long long out_row = -1;
+        if (r < c.rows) {
+          out_row = args.out_perm != nullptr ? args.out_perm[c.a_row + r] : c.a_row + r;
+          if (out_row >= args.out_rows) out_row = -1;
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int col0 = c.n0 + 128 * half + 64 * g;
+          if (col0 >= args.n_dim) break;
+          float f[64];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float2 p = halves(sum[g * 32 + j]);
+            f[2 * j] = p.x;
+            f[2 * j + 1] = p.y;
+          }
+          act_row(f, args.act);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint4 u = pack8<T>(f + 8 * q);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage_base + lane * 128 + ((q ^ (lane & 7)) << 4)), "r"(u.x),
+                         "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+          }
+          __syncwarp();
+          const int ck = lane & 7;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int rr = j * 4 + (lane >> 3);
+            const long long to = __shfl_sync(0xFFFFFFFFu, out_row, rr);
+            uint4 u;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                         : "r"(stage_base + rr * 128 + ((ck ^ (rr & 7)) << 4)));
+            const int col = col0 + ck * 8;
+            if (to >= 0 && col < args.n_dim) *reinterpret_cast<uint4*>(static_cast<T*>(args.out) + to * args.n_dim + col) = u;
+          }
+          __syncwarp();
+        }
+      } else {
+        // 8-bit rows: the block's largest value is this thread's (128 columns of its own), or its and its partner's (64 each)
+        uint8_t* out = static_cast<uint8_t*>(args.out);
+        const int blocks = nblocks;
+        float most = kF8Least;
+        constexpr int kMine = kGlu ? 64 : 128;
+        float f[kMine];
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < kMine / 2; ++j) {
+            const float2 p = halves(sum[j]);
+            f[2 * j] = p.x;
+            f[2 * j + 1] = p.y;
+          }
+          act_row(f, args.act);
+          if (kGlu) {
+#pragma unroll
+            for (int j = 0; j < kMine / 2; ++j) {
+              const float2 u = halves(sum[32 + j]);
+              f[2 * j] *= u.x;
+              f[2 * j + 1] *= u.y;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kMine; ++j) most = fmaxf(most, fabsf(f[j]));
+        }
+        if (kGlu) {
+          // two places used in turn, so that one meeting of the quadrant's warps is enough
+          float* mine = reinterpret_cast<float*>(tiles + kStages * Plan::kStageBytes) + (i & 1) * 256;
+          mine[half * 128 + r] = most;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(meet_bar + 8 * quad);
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(meet_bar + 8 * quad, i & 1, wctx, DS_TIMEOUT_EPILOGUE))) break;
+          most = fmaxf(most, mine[(half ^ 1) * 128 + r]);
+        }
+        if (r < c.rows) {
+          const float inv = kF8Top / most;
+          const int col0 = kGlu ? c.n0 + 64 * half : c.n0 + 128 * half;
+          const int64_t to = static_cast<int64_t>(c.a_row) + r;
+#pragma unroll
+          for (int q = 0; q < kMine / 16; ++q) {
+            const int col = col0 + 16 * q;
+            if (col < args.n_dim)
+              *reinterpret_cast<uint4*>(out + to * args.n_dim + col) =
+                  make_uint4(f8x4(f[16 * q] * inv, f[16 * q + 1] * inv, f[16 * q + 2] * inv, f[16 * q + 3] * inv),
+                             f8x4(f[16 * q + 4] * inv, f[16 * q + 5] * inv, f[16 * q + 6] * inv, f[16 * q + 7] * inv),
+                             f8x4(f[16 * q + 8] * inv, f[16 * q + 9] * inv, f[16 * q + 10] * inv, f[16 * q + 11] * inv),
+                             f8x4(f[16 * q + 12] * inv, f[16 * q + 13] * inv, f[16 * q + 14] * inv, f[16 * q + 15] * inv));
+          }
+          if ((!kGlu || half == 0) && col0 < args.n_dim) args.out_scales[to * blocks + col0 / kF8Block] = most / kF8Top;
+        }
+      }
+    }
+  } else {
+    fewer_registers();
+    if (warp == 0) {
+      // ------------------------------ TMA producer ------------------------------
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint64_t pol = l2_policy_evict_normal();
+      const uint32_t full_leader = mapa_shared(full_bar, 0);
+      for (int i = 0; ok; ++i) {
+        const F8Item c = walk.get(i, args, kCols);
+        if (!c.valid) break;
+        const int wz = kGlu ? 2 * c.expert + rank : c.expert;
+        const int wrow = kGlu ? c.n0 : c.n0 + rank * BM;
+        for (int kb = 0; kb < kiters; ++kb) {
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, wctx, DS_TIMEOUT_PRODUCER))) {
+            ok = false;
+            break;
+          }
+          if (elect_one()) {
+            const uint32_t sx = tiles_addr + stage * Plan::kStageBytes;
+            const uint32_t fb = full_leader + 8 * stage;
+            mbar_arrive_expect_tx_cluster(fb, Plan::kStageBytes);
+            tma_load_2d_pair(sx, &tmap_x, kb * (kF8K / 2), c.a_row, fb, pol);
+            tma_load_3d_pair(sx + kF8Tile, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
+          }
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+        }
+      }
+      grid_release();
+      if (!ok || *abort_flag) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies already issued land before the CTA ends
+      }
+    } else if (warp == 1) {
+      // ------------------------------ MMA issuer (leader CTA only) --------------
+      if (rank == 0) {
+        constexpr uint32_t idesc = f8_idesc(2 * BM, 256);
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int i = 0; ok; ++i) {
+          const F8Item c = walk.get(i, args, kCols);
+          if (!c.valid) break;
+          for (int kb = 0; kb < kiters; ++kb) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1, wctx, DS_TIMEOUT_MMA)) ||
+                !__all_sync(0xFFFFFFFFu, mbar_wait(full_bar + 8 * stage, phase, wctx, DS_TIMEOUT_MMA))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t sx = tiles_addr + stage * Plan::kStageBytes;
+#pragma unroll
+              for (int k = 0; k < kF8K / kF8MmaK; ++k)
+                umma_f8_pair(tmem_base + acc * 256, make_desc(sx + k * kF8MmaK, 16, 1024), make_desc(sx + kF8Tile + k * kF8MmaK, 16, 1024),
+                             idesc, k != 0 ? 1u : 0u);
+              umma_commit_pair_both(empty_bar + 8 * stage);
+              umma_commit_pair_both(tfull_bar + 8 * acc);
+            }
+            __syncwarp();
+            if (++stage == kStages) { stage = 0; phase ^= 1; }
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1;
+          }
+        }
+        if (!ok || *abort_flag) {
+          for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA may end while its peer can still touch its memory or barriers
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// Weights on the lanes.
+//
+// A tile is 128 result columns (weight rows on the lanes; gate and up rows where gated: two accumulators) x the rows of one row
+// tile, R at a time.  The instruction's N is the rows there are, in steps of 16, and so are the rows loaded per stage: with one
+// token a stage is 16 (32) KB of weights and 2 KB of rows.  The ring holds about 190 KB, what an SM needs in flight to stream
+// weights at the memory's rate.  Epilogue warp w owns the 32 lanes of quadrant w % 4 and every other group of 16 rows; a row's scale
+// is handed around by shuffles.  (CTA pairs bring nothing here: there is nothing to share but the few rows.)
+// ------------------------------------------------------------------------------------------------------------------
+template <int R, bool GLU> struct F8LanesPlan {
+  static constexpr int kWBytes = (GLU ? 2 : 1) * kF8Tile;
+  static constexpr int kStageBytes = kWBytes + R * kF8K;
+  static constexpr int kExtra = 2 * 4 * R * 4;  // block maxima of the quadrants, two places used in turn
+  static constexpr int kBarrierBytes = 1024;
+  static constexpr int kBudget = 232448 - 1024 - kBarrierBytes - kExtra;
+  static constexpr int kStages = kBudget / kStageBytes > 10 ? 10 : kBudget / kStageBytes;
+  static constexpr int kTotal = kStages * kStageBytes + kExtra + kBarrierBytes + 1024;
+  static constexpr int kAccCols = (GLU ? 2 : 1) * R;
+  static constexpr int kAccs = 512 / kAccCols > 4 ? 4 : 512 / kAccCols;
+};
+
+template <typename T, int OUT, int R>
+__global__ void __launch_bounds__(kF8Threads, 1)
+f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const F8Args args) {
+  constexpr bool kGlu = OUT == F8_GLU_QUANT;
+  using Plan = F8LanesPlan<R, kGlu>;
+  constexpr int kStages = Plan::kStages, kAccs = Plan::kAccs;
+  constexpr int kMats = kGlu ? 2 : 1;
+  constexpr int kChunks = R / 32;  // groups of 16 rows per warp
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t tiles_addr = (raw_addr + 1023u) & ~1023u;
+  uint8_t* tiles = smem_raw + (tiles_addr - raw_addr);
+  float* maxima = reinterpret_cast<float*>(tiles + kStages * Plan::kStageBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kStages * Plan::kStageBytes + Plan::kExtra);
+  const uint32_t full_bar = smem_u32(bars);
+  const uint32_t empty_bar = smem_u32(bars + kStages);
+  const uint32_t tfull_bar = smem_u32(bars + 2 * kStages);
+  const uint32_t tempty_bar = smem_u32(bars + 2 * kStages + kAccs);
+  const uint32_t meet_bar = smem_u32(bars + 2 * kStages + 2 * kAccs);  // the epilogue warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kAccs + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  WaitCtx wctx;
+  wctx.abort_flag = abort_flag;
+  wctx.peer_abort = 0;
+  wctx.status = args.status;
+  wctx.limit = args.wait_limit;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full_bar + 8 * s, 1);
+      mbar_init(empty_bar + 8 * s, 1);
+    }
+    for (int a = 0; a < kAccs; ++a) {
+      mbar_init(tfull_bar + 8 * a, 1);
+      mbar_init(tempty_bar + 8 * a, kEpilogueWarps);
+    }
+    mbar_init(meet_bar, kEpilogueWarps);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_x);
+    tma_prefetch_desc(&tmap_w);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  await_predecessor();
+  const uint32_t tmem_base = *tmem_slot;
+  F8Walk<1> walk(args, blockIdx.x, gridDim.x, 128, 0);
+  const int kiters = (args.k_dim + kF8K - 1) / kF8K;
+
+  if (warp >= 4) {
+    more_registers();
+    // ------------------------------ epilogue ----------------------------------
+    const int quad = warp & 3;
+    const int half = (warp - 4) >> 2;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const int kblocks = kiters;
+    const int nblocks = (args.n_dim + kF8Block - 1) / kF8Block;
+    int acc = 0, turn = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      const F8Item c = walk.get(i, args, 128);
+      if (!c.valid) break;
+      const int n = c.n0 + quad * 32 + lane;  // this lane's result column
+      const float* wa = args.w_scales + (static_cast<int64_t>(c.expert) * kMats * nblocks + c.n0 / kF8Block) * kblocks;
+      const float* wb = wa + static_cast<int64_t>(nblocks) * kblocks;
+      for (int r0 = 0; r0 < c.rows && ok; r0 += R, ++turn) {
+        const int rows = min(c.rows - r0, R);
+        // group ch of this warp: rows r0 + 16 * (2 * ch + half) ...; its lanes' scales (lanes 16 to 31 repeat them)
+        const float* xs[kChunks];
+        float x0[kChunks], x1[kChunks];
+        float sum[kMats][kChunks][16];
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+          const int rr = min(16 * (2 * ch + half) + (lane & 15), rows - 1);
+          xs[ch] = args.x_scales + (static_cast<int64_t>(c.a_row) + r0 + rr) * kblocks;
+          x0[ch] = xs[ch][0];
+          x1[ch] = kiters > 1 ? xs[ch][1] : 0.0f;
+#pragma unroll
+          for (int m = 0; m < kMats; ++m)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum[m][ch][j] = 0.0f;
+        }
+        float a0 = wa[0], b0 = kGlu ? wb[0] : 0.0f;
+        float a1 = kiters > 1 ? wa[1] : 0.0f, b1 = kGlu && kiters > 1 ? wb[1] : 0.0f;
+        for (int kb = 0; kb < kiters; ++kb) {
+          float x2[kChunks], a2 = 0.0f, b2 = 0.0f;
+          const bool more = kb + 2 < kiters;
+          if (more) {
+            a2 = wa[kb + 2];
+            if (kGlu) b2 = wb[kb + 2];
+          }
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch) x2[ch] = more ? xs[ch][kb + 2] : 0.0f;
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar + 8 * acc, acc_phase, wctx, DS_TIMEOUT_EPILOGUE))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t t0 = tmem_base + lanes + acc * Plan::kAccCols;
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch) {
+            const int col = 16 * (2 * ch + half);
+            if (col < rows) {
+              uint32_t v[kMats][16];
+#pragma unroll
+              for (int m = 0; m < kMats; ++m) tmem_ld_32x16(t0 + m * R + col, v[m]);
+#pragma unroll
+              for (int m = 0; m < kMats; ++m) tmem_ld_wait16(v[m]);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float x = __shfl_sync(0xFFFFFFFFu, x0[ch], j);
+                sum[0][ch][j] = fmaf(__uint_as_float(v[0][j]), x * a0, sum[0][ch][j]);
+                if (kGlu) sum[kMats - 1][ch][j] = fmaf(__uint_as_float(v[kMats - 1][j]), x * b0, sum[kMats - 1][ch][j]);
+              }
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tempty_bar + 8 * acc);
+          if (++acc == kAccs) { acc = 0; acc_phase ^= 1; }
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch) {
+            x0[ch] = x1[ch];
+            x1[ch] = x2[ch];
+          }
+          a0 = a1;
+          a1 = a2;
+          b0 = b1;
+          b1 = b2;
+        }
+        if (!ok) break;
+        // the results: activation in place
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+          act_row(sum[0][ch], args.act);
+          if (kGlu) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum[0][ch][j] *= sum[kMats - 1][ch][j];
+          }
+        }
+        const int64_t first = static_cast<int64_t>(c.a_row) + r0;
+        if constexpr (OUT == F8_ROWS) {
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int rr = 16 * (2 * ch + half) + j;
+              if (rr >= rows) continue;
+              const int64_t to = args.out_perm != nullptr ? args.out_perm[first + rr] : first + rr;
+              if (n < args.n_dim && to >= 0 && to < args.out_rows)
+                static_cast<T*>(args.out)[to * args.n_dim + n] = Elem<T>::from_float(sum[0][ch][j]);
+            }
+        } else {
+          float* place = maxima + (turn & 1) * 4 * R;
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch) {
+            float keep = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              // (non-negative floats order as integers; NaN stays out of the maximum, as in fmaxf)
+              const float v = fabsf(sum[0][ch][j]);
+              const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, v == v ? __float_as_uint(v) : 0u);
+              if ((lane & 15) == j) keep = __uint_as_float(m);
+            }
+            if (lane < 16) place[quad * R + 16 * (2 * ch + half) + lane] = keep;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(meet_bar);
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(meet_bar, turn & 1, wctx, DS_TIMEOUT_EPILOGUE))) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch) {
+            const int rr0 = 16 * (2 * ch + half);
+            if (rr0 >= rows) continue;
+            float most = kF8Least;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) most = fmaxf(most, place[q * R + rr0 + (lane & 15)]);
+            if (quad == 0 && lane < 16 && rr0 + lane < rows)
+              args.out_scales[(first + rr0 + lane) * nblocks + c.n0 / kF8Block] = most / kF8Top;
+            const float inv = kF8Top / most;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float v = sum[0][ch][j] * __shfl_sync(0xFFFFFFFFu, inv, j);
+              if (rr0 + j < rows && n < args.n_dim)
+                static_cast<uint8_t*>(args.out)[(first + rr0 + j) * args.n_dim + n] =
+                    static_cast<uint8_t>(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3));
+            }
+          }
+        }
+      }
+    }
+  } else {
+    fewer_registers();
+    if (warp == 0) {
+      // ------------------------------ TMA producer ------------------------------
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint64_t pol = l2_policy_evict_normal();
+      for (int i = 0; ok; ++i) {
+        const F8Item c = walk.get(i, args, 128);
+        if (!c.valid) break;
+        for (int r0 = 0; r0 < c.rows && ok; r0 += R) {
+          const int groups = (min(c.rows - r0, R) + 15) >> 4;
+          for (int kb = 0; kb < kiters; ++kb) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, wctx, DS_TIMEOUT_PRODUCER))) {
+              ok = false;
+              break;
+            }
+            if (elect_one()) {
+              const uint32_t sw = tiles_addr + stage * Plan::kStageBytes;
+              const uint32_t fb = full_bar + 8 * stage;
+              mbar_arrive_expect_tx(fb, Plan::kWBytes + groups * 16 * kF8K);
+#pragma unroll
+              for (int m = 0; m < kMats; ++m)
+                tma_load_3d(sw + m * kF8Tile, &tmap_w, kb * (kF8K / 2), c.n0, kMats * c.expert + m, fb, pol);
+              for (int g = 0; g < groups; ++g)
+                tma_load_2d(sw + Plan::kWBytes + g * 16 * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + r0 + 16 * g, fb, pol);
+            }
+            __syncwarp();
+            if (++stage == kStages) { stage = 0; phase ^= 1; }
+          }
+        }
+      }
+      grid_release();
+      if (!ok || *abort_flag) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+      }
+    } else if (warp == 1) {
+      // ------------------------------ MMA issuer --------------------------------
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const F8Item c = walk.get(i, args, 128);
+        if (!c.valid) break;
+        for (int r0 = 0; r0 < c.rows && ok; r0 += R) {
+          const uint32_t idesc = f8_idesc(BM, (min(c.rows - r0, R) + 15) & ~15);
+          for (int kb = 0; kb < kiters; ++kb) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1, wctx, DS_TIMEOUT_MMA)) ||
+                !__all_sync(0xFFFFFFFFu, mbar_wait(full_bar + 8 * stage, phase, wctx, DS_TIMEOUT_MMA))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t sw = tiles_addr + stage * Plan::kStageBytes;
+#pragma unroll
+              for (int m = 0; m < kMats; ++m)
+#pragma unroll
+                for (int k = 0; k < kF8K / kF8MmaK; ++k)
+                  umma_f8(tmem_base + acc * Plan::kAccCols + m * R, make_desc(sw + m * kF8Tile + k * kF8MmaK, 16, 1024),
+                          make_desc(sw + Plan::kWBytes + k * kF8MmaK, 16, 1024), idesc, k != 0 ? 1u : 0u);
+              umma_commit(empty_bar + 8 * stage);
+              umma_commit(tfull_bar + 8 * acc);
+            }
+            __syncwarp();
+            if (++stage == kStages) { stage = 0; phase ^= 1; }
+            if (++acc == kAccs) { acc = 0; acc_phase ^= 1; }
+          }
+        }
+      }
+      if (!ok || *abort_flag) {
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+}  // namespace moe

@@ -92,8 +92,8 @@ static int g_tmap_used = 0, g_tmap_next = 0;
 
 // Tensor map (by default with the 128-byte swizzle); dims[0] is the contiguous dimension.  `strides` (bytes, for dims 1..rank-1)
 // may be null for a dense row-major tensor.
-static int make_tmap(CUtensorMap* map, int dtype, const void* ptr, int rank, const uint64_t* dims,
-                     const uint32_t* box, const uint64_t* strides = nullptr, bool swizzle = true) {
+int make_tmap(CUtensorMap* map, int dtype, const void* ptr, int rank, const uint64_t* dims, const uint32_t* box,
+              const uint64_t* strides, bool swizzle) {
   TmapKey key{};
   key.ptr = ptr;
   key.dtype = dtype;

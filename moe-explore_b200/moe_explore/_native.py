@@ -59,6 +59,25 @@ class RowsPass(ctypes.Structure):
                                         "mtile_expert", "tile_pairs", "num_mtiles", "status", "padded", "counters")]
 
 
+class F8Pass(ctypes.Structure):
+    """``moe_f8_pass``: sizes and buffers of one forward pass over experts in 8 bits."""
+    _fields_ = [(f, c_int64) for f in ("num_tokens", "padded_rows")] + \
+               [(f, c_int32) for f in ("d", "inter", "num_experts", "topk", "act", "dtype")] + \
+               [(f, c_void_p) for f in ("expert_idx", "x", "x_scales", "scores", "w1", "w1_scales", "w2", "w2_scales", "group_indices",
+                                        "pad_offsets", "row_src", "dst_row", "mtile_expert", "tile_pairs", "num_mtiles", "status",
+                                        "workspace")] + \
+               [("workspace_bytes", c_size_t)] + \
+               [(f, c_void_p) for f in ("xs", "xs_scales", "hidden", "hidden_scales", "ys", "out", "addend")]
+
+
+class F8RowsPass(ctypes.Structure):
+    """``moe_f8_rows_pass``: sizes and buffers of one functional product in 8 bits."""
+    _fields_ = [(f, c_int64) for f in ("num_rows", "x_rows")] + \
+               [(f, c_int32) for f in ("num_experts", "k_dim", "n_dim", "topk", "act", "dtype", "gather", "scatter")] + \
+               [(f, c_void_p) for f in ("x", "x_scales", "w", "w_scales", "out", "group_indices", "perm", "pad_offsets", "mtile_expert",
+                                        "tile_pairs", "num_mtiles", "status", "gathered", "gathered_scales")]
+
+
 # name -> (restype, argtypes); the single source for both binding and the symbol-export test
 _OPT = POINTER(GemmOptions)
 SIGNATURES = {
@@ -100,6 +119,11 @@ SIGNATURES = {
     "moe_expert_pass_size": (c_size_t, []),
     "moe_expert_forward": (c_int, [POINTER(ExpertPass), c_int, c_void_p]),
     "moe_expert_backward": (c_int, [POINTER(ExpertPass), c_int, c_void_p]),
+    "moe_f8_quantize_rows": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p]),
+    "moe_f8_pass_size": (c_size_t, []),
+    "moe_f8_expert_forward": (c_int, [POINTER(F8Pass), c_int, c_void_p]),
+    "moe_f8_rows_pass_size": (c_size_t, []),
+    "moe_f8_rows_gemm": (c_int, [POINTER(F8RowsPass), c_int, c_void_p]),
     "moe_rows_pass_size": (c_size_t, []),
     "moe_rows_gemm": (c_int, [POINTER(RowsPass), c_int, c_void_p]),
     "moe_dispatch_rows_only": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int, c_int, c_void_p]),
@@ -180,6 +204,8 @@ def load() -> ctypes.CDLL:
             raise ImportError(f"{LIB_PATH} was built with another layout of moe_expert_pass: rebuild it")
         if lib.moe_rows_pass_size() != ctypes.sizeof(RowsPass):
             raise ImportError(f"{LIB_PATH} was built with another layout of moe_rows_pass: rebuild it")
+        if lib.moe_f8_pass_size() != ctypes.sizeof(F8Pass) or lib.moe_f8_rows_pass_size() != ctypes.sizeof(F8RowsPass):
+            raise ImportError(f"{LIB_PATH} was built with another layout of moe_f8_pass or moe_f8_rows_pass: rebuild it")
         _lib = lib
     return _lib
 
@@ -264,6 +290,7 @@ def _opt(options):
 
 
 ROWS_LAYOUT, ROWS_GATHER, ROWS_GEMM = 1, 2, 4
+F8_ROUTE, F8_DISPATCH, F8_UP, F8_DOWN, F8_FOLD = 1, 2, 4, 8, 16
 FWD_ROUTE, FWD_DISPATCH, FWD_UP, FWD_DOWN, FWD_FOLD, FWD_TAIL = 1, 2, 4, 8, 16, 32
 BWD_FOLD, BWD_DOWN, BWD_UP, BWD_FOLD_DX, BWD_DW1, BWD_DW2, BWD_ROUTER = 1, 2, 4, 8, 16, 32, 64
 
@@ -433,6 +460,15 @@ def rms_norm_backward(dy, dh, h, weight, rstd):
     _check("moe_rms_norm_backward", rc)
     _count(2)
     return dx, dw
+
+
+def f8_quantize_rows(x, q, scales):
+    """16-bit rows [R, K] in 8 bits with a scale per 128 columns (see moe_f8_quantize_rows)."""
+    with timed("rows:f8"):
+        rc = load().moe_f8_quantize_rows(x.data_ptr(), q.data_ptr(), scales.data_ptr(), x.size(0), x.size(1), dtype_code(x.dtype),
+                                         _stream())
+    _check("moe_f8_quantize_rows", rc)
+    _count(1)
 
 
 _PINNED = {}

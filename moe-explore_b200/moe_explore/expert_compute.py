@@ -19,7 +19,8 @@ import torch
 
 from moe_explore import _native
 from moe_explore.functional.activation import is_glu
-from moe_explore.params import ErnieRouterParams, TopkRouterParams
+from moe_explore.functional.fp8 import Fp8Rows, _dense, blocks
+from moe_explore.params import ErnieRouterParams, Fp8ExpertParams, TopkRouterParams
 from moe_explore.router import ernie_router, fused_topk_of_logits, nothing_watches, tail_in_one_kernel, topk_of_logits
 from moe_explore.routing_plan import RoutingPlan, device_status, packed_layout
 
@@ -432,3 +433,61 @@ def inference_pass(x, router_params, weight1, weight2, num_experts: int, topk: i
     # (topk is the layer's: the router's may be anything that torch.topk takes and that equals it)
     return _forward(x, scores, weight1, weight2, (indices, num_experts, topk), None if act is None else str(act),
                     bool(gather_in_gemm), bool(fused_combine), False, addend, tail)[0]
+
+
+def fp8_expert_compute(x, scores, indices, params: Fp8ExpertParams, addend=None) -> torch.Tensor:
+    """out[t] = sum_s scores[t, s] * (act(x[t] @ up[e]^T) @ down[e]^T) with e = indices[t, s], the products in 8 bits: rows (unless
+    they are ``Fp8Rows`` already) and the activated products get a scale per 128 columns; everything is added in fp32 and
+    each expert's row is rounded to the 16-bit result type before the fold.  ``x`` [T, d] in bf16 / fp16 or ``Fp8Rows`` (result in
+    their ``dtype``), ``scores`` and ``indices`` (int64) [T, k]; slots with an expert id out of range add nothing (and are
+    reported by the status word).  ``addend`` [T, d] is added by the fold.  For serving: no gradients.  d and I multiples of 16."""
+    rows = isinstance(x, Fp8Rows)
+    data = x.checked().data if rows else x
+    dtype = x.dtype
+    params.up.checked(4, "up")
+    params.down.checked(3, "down")
+    _native.require_cuda(data, scores, indices, addend)
+    act = str(params.activation)
+    E, gates, inter, d = params.up.data.shape
+    if act not in _native.ACT_CODES or gates != (2 if is_glu(act) else 1):
+        raise ValueError(f"up has {gates} matrices per expert, which does not fit the activation {act!r}")
+    if params.down.data.shape != (E, d, inter) or data.dim() != 2 or data.size(1) != d:
+        raise ValueError(f"shapes do not match: input {tuple(data.shape)}, up {tuple(params.up.data.shape)}, down {tuple(params.down.data.shape)}")
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"fp8_expert_compute takes bf16 or fp16 rows, or Fp8Rows, got {dtype}")
+    T, topk = indices.shape if indices.dim() == 2 else (-1, 0)
+    if T != data.size(0) or indices.dtype is not torch.int64 or scores.shape != indices.shape:
+        raise ValueError("indices (int64) and scores are [tokens, k]")
+    if any(t.device != data.device for t in (scores, indices, params.up.data, params.down.data) + (() if addend is None else (addend,))):
+        raise ValueError("all tensors lie on the device of the input")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (data, scores, addend)):
+        raise RuntimeError("experts in 8 bits have no backward pass: call this under torch.no_grad(), or train 16-bit experts")
+    if addend is not None and (addend.shape != (T, d) or addend.dtype is not dtype):
+        raise ValueError("addend is like the result")
+    with _native.on_device_of(data):
+        out = torch.empty(T, d, dtype=dtype, device=data.device)
+        if T == 0:
+            return out
+        data, ids, scores = _dense(data.detach()), indices.contiguous(), scores.detach().to(dtype).contiguous()
+        x_scales = x.scales.contiguous() if rows else None
+        up, up_scales, down, down_scales = (_dense(params.up.data), params.up.scales.contiguous(), _dense(params.down.data),
+                                            params.down.scales.contiguous())
+        addend = None if addend is None else _dense(addend.detach())
+        num_rows = T * topk
+        rp, offsets, num_words = packed_layout(num_rows, E)
+        launches = _native.routing_launches(num_rows, E)
+        workspace = None
+        if launches > 1:
+            workspace = torch.empty(max(_native.routing_workspace_bytes(num_rows, E), 16), dtype=torch.uint8, device=data.device)
+        held, (words, xs, xs_scales, hidden, hidden_scales, ys) = _buffers(
+            (4 * num_words, rp * d, 4 * rp * blocks(d), rp * inter, 4 * rp * blocks(inter), 2 * rp * d), data.device)
+        ptr = _native._ptr
+        p = _native.F8Pass(T, rp, d, inter, E, topk, _native.ACT_CODES[act], _native.dtype_code(dtype), ids.data_ptr(), data.data_ptr(),
+                           ptr(x_scales), scores.data_ptr(), up.data_ptr(), up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(),
+                           *_packed_pointers(words, offsets, device_status(data.get_device())), ptr(workspace),
+                           0 if workspace is None else workspace.numel(), xs, xs_scales, hidden, hidden_scales, ys, out.data_ptr(),
+                           ptr(addend))
+        _native.run_pass("moe_f8_expert_forward", p, [
+            (_native.F8_ROUTE, "routing", launches), (_native.F8_DISPATCH, "rows:gather", 1), (_native.F8_UP, "f8_gemm:up", 1),
+            (_native.F8_DOWN, "f8_gemm:down", 1), (_native.F8_FOLD, "rows:combine", 1)], num_rows)
+    return out

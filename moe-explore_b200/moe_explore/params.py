@@ -13,6 +13,7 @@ from typing import Optional
 import torch
 
 from moe_explore.functional.activation import Activation
+from moe_explore.functional.fp8 import Fp8Weight
 
 
 @dataclass
@@ -53,6 +54,15 @@ class SharedExpertParams(FFNParams):
     (functional/topk_moe.py:56-62) without declaring a type for them."""
     up_weight: torch.Tensor
     down_weight: torch.Tensor
+    activation: Activation
+
+
+@dataclass
+class Fp8ExpertParams(FFNParams):
+    """Experts in 8 bits, for serving (``moe_explore.functional.fp8.quantize_experts`` makes them of 16-bit ones): ``up`` [E, 2, I, d]
+    (gate, up) for swiglu / geglu, else [E, 1, I, d]; ``down`` [E, d, I].  No reference counterpart."""
+    up: Fp8Weight
+    down: Fp8Weight
     activation: Activation
 
 

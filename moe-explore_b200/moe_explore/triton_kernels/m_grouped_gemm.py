@@ -16,12 +16,13 @@ import torch
 
 from moe_explore import _native
 from moe_explore.functional.activation import is_glu
+from moe_explore.functional.fp8 import Fp8Rows, Fp8Weight, fp8_rows_gemm
 from moe_explore.routing_plan import device_status
 
 
 @dataclass
 class MGroupedGEMMParams:
-    weight: torch.Tensor                      # [E, K, N]
+    weight: torch.Tensor                      # [E, K, N]; or an Fp8Weight [E, N, K], for tokens that are Fp8Rows
     group_indices: torch.Tensor               # int32 [E+1], exclusive prefix of rows per expert
     permute_indices: Optional[torch.Tensor]   # int64 [T*topk], required with gather or scatter
     gather: bool                              # input row of sorted position r is token[permute_indices[r] // topk]
@@ -40,7 +41,12 @@ def m_grouped_gemm(token: torch.Tensor, params: MGroupedGEMMParams, autotune_mod
     optional scatter of the output rows.  As in the reference kernel the scatter happens inside the GEMM's epilogue
     (m_grouped_gemm.py:168-172): no un-scattered copy of the output exists.  Gathered input rows are copied into
     128-row-aligned expert segments first (one HBM-bound pass) so that the GEMM loads whole tiles; rows that are in expert
-    order already are read where they are."""
+    order already are read where they are.
+
+    In 8 bits (``token`` an ``Fp8Rows``, ``params.weight`` an ``Fp8Weight`` [E, N, K]): the same without gated activations, the
+    result in ``token.dtype``; forward only."""
+    if isinstance(token, Fp8Rows) or isinstance(params.weight, Fp8Weight):
+        return _m_grouped_gemm_fp8(token, params)
     assert token.dim() == 2
     assert params.weight.dim() == 3
     assert token.size(1) == params.weight.size(1)
@@ -83,6 +89,25 @@ def m_grouped_gemm(token: torch.Tensor, params: MGroupedGEMMParams, autotune_mod
         out.data_ptr(), groups.data_ptr(), ptr(perm), *[base + o for o in offsets[:-1]],
         device_status(token.get_device()).data_ptr(), ptr(padded), base + offsets[-1]), steps, rows)
     return out
+
+
+def _m_grouped_gemm_fp8(token: Fp8Rows, params: MGroupedGEMMParams) -> torch.Tensor:
+    if not (isinstance(token, Fp8Rows) and isinstance(params.weight, Fp8Weight)):
+        raise TypeError("8-bit rows are multiplied with 8-bit weights: both of Fp8Rows and Fp8Weight, or neither")
+    moved = params.gather or params.scatter
+    assert not moved or params.permute_indices is not None
+    _native.require_cuda(params.group_indices)
+    rows = params.num_tokens * params.topk if moved else params.num_tokens
+    num_experts = params.weight.data.size(0)
+    assert params.group_indices.dim() == 1 and params.group_indices.numel() == num_experts + 1
+    assert params.gather or token.data.size(0) >= rows, "fewer rows than the groups hold"
+    perm = None
+    if moved:
+        _native.require_cuda(params.permute_indices)
+        perm = params.permute_indices.to(torch.int64).contiguous()
+        assert perm.numel() >= rows, "permute_indices is shorter than the routed rows"
+    return fp8_rows_gemm(token, params.weight, params.group_indices.to(torch.int32).contiguous(), perm, params.gather, params.scatter,
+                         rows, params.topk, None if params.activation is None else str(params.activation))
 
 
 @functools.lru_cache(maxsize=256)
