@@ -7,9 +7,8 @@ namespace moe {
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <int CTAS, typename Kernel>
-static int launch_f8(Kernel kernel, int smem, std::atomic<int> (&grids)[64], const CUtensorMap& tx, const CUtensorMap& tw,
-                     const F8Args& args, cudaStream_t s) {
+template <int CTAS, typename Kernel, typename... Args>
+static int launch_f8(Kernel kernel, int threads, int smem, std::atomic<int> (&grids)[64], cudaStream_t s, const Args&... args) {
   LaunchParams lp;
   lp.stream = s;
   lp.max_ctas = 0;
@@ -17,20 +16,20 @@ static int launch_f8(Kernel kernel, int smem, std::atomic<int> (&grids)[64], con
   PersistentLaunch l;
   const int rc = configure<CTAS>(l, kernel, smem, grids, lp);
   if (rc != MOE_OK) return rc;
-  l.cfg.blockDim = dim3(kF8Threads, 1, 1);
-  MOE_CUDA(cudaLaunchKernelEx(&l.cfg, kernel, tx, tw, args));
+  l.cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  MOE_CUDA(cudaLaunchKernelEx(&l.cfg, kernel, args...));
   return MOE_OK;
 }
 
 template <typename T, int OUT>
-static int launch_f8_pair(const CUtensorMap& tx, const CUtensorMap& tw, const F8Args& args, cudaStream_t s) {
+static int launch_f8_pair(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& to, const F8Args& args, cudaStream_t s) {
   static std::atomic<int> grids[64];
-  return launch_f8<2>(f8_pair_kernel<T, OUT>, F8PairPlan::kTotal, grids, tx, tw, args, s);
+  return launch_f8<2>(f8_pair_kernel<T, OUT>, kF8Threads, F8PairPlan::kTotal, grids, s, tx, tw, to, args);
 }
 template <typename T, int OUT, int R>
 static int launch_f8_lanes(const CUtensorMap& tx, const CUtensorMap& tw, const F8Args& args, cudaStream_t s) {
   static std::atomic<int> grids[64];
-  return launch_f8<1>(f8_lanes_kernel<T, OUT, R>, F8LanesPlan<R, OUT == F8_GLU_QUANT>::kTotal, grids, tx, tw, args, s);
+  return launch_f8<1>(f8_lanes_kernel<T, OUT, R>, kF8Threads, F8LanesPlan<R, OUT == F8_GLU_QUANT>::kTotal, grids, s, tx, tw, args);
 }
 
 // Rows [rows, K] and weights [mats, N, K] in bytes, described as pairs of bytes.
@@ -69,6 +68,7 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
   a.group_indices = p.group_indices;
   a.dense_rows = p.dense ? p.x_rows : -1;
   a.compact = p.compact;
+  a.padded = !p.compact && !p.dense;
   a.total_rows = p.x_rows;
   a.x_scales = p.x_scales;
   a.w_scales = p.w_scales;
@@ -90,9 +90,16 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
   if (rc != MOE_OK) return rc;
   const bool bf16 = p.dtype == MOE_DTYPE_BF16;
   if (!lanes) {
-    if (p.kind == F8_GLU_QUANT) return launch_f8_pair<__nv_bfloat16, F8_GLU_QUANT>(tx, tw, a, s);
-    if (p.kind == F8_QUANT) return launch_f8_pair<__nv_bfloat16, F8_QUANT>(tx, tw, a, s);
-    return bf16 ? launch_f8_pair<__nv_bfloat16, F8_ROWS>(tx, tw, a, s) : launch_f8_pair<__half, F8_ROWS>(tx, tw, a, s);
+    CUtensorMap to = tx;
+    if (p.kind == F8_ROWS && p.out_perm == nullptr) {
+      const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.x_rows)};
+      const uint32_t box[2] = {64, 32};
+      const int rc2 = make_tmap(&to, p.dtype, p.out, 2, dims, box);
+      if (rc2 != MOE_OK) return rc2;
+    }
+    if (p.kind == F8_GLU_QUANT) return launch_f8_pair<__nv_bfloat16, F8_GLU_QUANT>(tx, tw, to, a, s);
+    if (p.kind == F8_QUANT) return launch_f8_pair<__nv_bfloat16, F8_QUANT>(tx, tw, to, a, s);
+    return bf16 ? launch_f8_pair<__nv_bfloat16, F8_ROWS>(tx, tw, to, a, s) : launch_f8_pair<__half, F8_ROWS>(tx, tw, to, a, s);
   }
 #define MOE_F8_LANES(R)                                                                                              \
   do {                                                                                                               \

@@ -53,6 +53,7 @@ struct F8Args {
   // The rows of the experts: maps of the padded layout, or dense_rows >= 0: one expert, rows 0 .. dense_rows - 1, no maps.
   const int32_t *mtile_expert, *tile_pairs, *num_mtiles, *pad_offsets, *group_indices;
   int64_t dense_rows;
+  int32_t padded;        // out has rows for whole tiles: what is stored past an expert's last row is read by nobody
   int32_t compact;       // x and out hold the rows without padding, expert by expert
   int64_t total_rows;    // rows of x
   const float* x_scales;
@@ -184,19 +185,20 @@ __device__ __forceinline__ void tmem_ld_wait16(uint32_t (&v)[16]) {
                :
                : "memory");
 }
-// a += v * f on two fp32 values at once.
-__device__ __forceinline__ void fma2(uint64_t& a, uint32_t v0, uint32_t v1, uint64_t f) {
-  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(a) : "r"(v0), "r"(v1), "l"(f));
+// The same for 32 columns (tmem_ld_32x32 loads them).
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
+                 "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                 "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+               :
+               : "memory");
 }
-__device__ __forceinline__ uint64_t twice(float f) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(f));
-  return r;
-}
-__device__ __forceinline__ float2 halves(uint64_t a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-  return r;
+// An arrival in either CTA of the pair that publishes no memory (TMEM reads are ordered by the tcgen05 fence before it): a releasing
+// one would wait for the loads of the scales that are under way.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // The element-wise activation of a register row; the choice is made once per row, so that the elements interleave.
 template <int N> __device__ __forceinline__ void act_row(float (&v)[N], int act) {
@@ -228,9 +230,9 @@ constexpr int kF8MmaK = 32;                  // K of one instruction
 //
 // A pair's tile is 256 rows x 256 weight rows (128 gate + 128 up rows where gated); per 128 of K each CTA loads 16 KB of rows and
 // 16 KB of weights, and the leader's four instructions (M 256, N 256, K 32) fill one of the two accumulator stages.  Each of
-// the eight epilogue warps of a CTA owns 32 rows x 128 of the columns: 128 fp32 sums per thread, fetched from TMEM 16 columns
-// at a time, the next 16 on their way while the last are added (two additions per instruction).  A thread's row is its lane, so
-// the row's scale is one register, and so is the weight block's.
+// the eight epilogue warps of a CTA owns 32 rows x 128 of the columns: 128 fp32 sums per thread, fetched from TMEM
+// 32 at a time, the next 32 on their way while the last are added.  A thread's row is its lane, so a step's factor is one register
+// (two where gated).
 // ------------------------------------------------------------------------------------------------------------------
 struct F8PairPlan {
   static constexpr int kStageBytes = 2 * kF8Tile;
@@ -244,7 +246,8 @@ struct F8PairPlan {
 
 template <typename T, int OUT>
 __global__ void __launch_bounds__(kF8Threads, 1)
-f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const F8Args args) {
+f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
+               const __grid_constant__ CUtensorMap tmap_out, const F8Args args) {
   using Plan = F8PairPlan;
   constexpr int kStages = Plan::kStages;
   constexpr bool kGlu = OUT == F8_GLU_QUANT;
@@ -285,6 +288,7 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     mbar_fence_init();
     tma_prefetch_desc(&tmap_x);
     tma_prefetch_desc(&tmap_w);
+    if (OUT == F8_ROWS) tma_prefetch_desc(&tmap_out);
   }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
@@ -311,6 +315,7 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     const int col_a = kGlu ? 64 * half : 128 * half;
     const int col_b = kGlu ? 128 + 64 * half : 128 * half + 64;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const int nblocks = (args.n_dim + kF8Block - 1) / kF8Block;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -321,14 +326,10 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       const bool live = quad * 32 < c.rows;  // some of this warp's rows exist
       const int64_t row = static_cast<int64_t>(c.a_row) + (r < c.rows ? r : c.rows > 0 ? c.rows - 1 : 0);
       const float* xs = args.x_scales + row * kblocks;
-      const int nblocks = (args.n_dim + kF8Block - 1) / kF8Block;
       // (a tile's second block of columns may lie past the last one: its products are zeros, any scale serves)
       const int nb = kGlu ? c.n0 / kF8Block : min(c.n0 / kF8Block + half, nblocks - 1);
       const float* wa = args.w_scales + (static_cast<int64_t>(c.expert) * (kGlu ? 2 : 1) * nblocks + nb) * kblocks;
       const float* wb = wa + static_cast<int64_t>(nblocks) * kblocks;
-      uint64_t sum[64];
-#pragma unroll
-      for (int j = 0; j < 64; ++j) sum[j] = 0;
       float x0 = 0.0f, a0 = 0.0f, b0 = 0.0f, x1 = 0.0f, a1 = 0.0f, b1 = 0.0f;
       if (live) {
         x0 = xs[0];
@@ -340,8 +341,11 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
           if (kGlu) b1 = wb[1];
         }
       }
+      float sum[128];
+#pragma unroll
+      for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
       for (int kb = 0; kb < kiters; ++kb) {
-        const uint64_t fa = twice(x0 * a0), fb = kGlu ? twice(x0 * b0) : fa;
+        const float fa = x0 * a0, fb = kGlu ? x0 * b0 : fa;
         x0 = x1;
         a0 = a1;
         b0 = b1;
@@ -357,29 +361,37 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         tc_fence_after();
         if (live) {
           const uint32_t t0 = tmem_base + lanes + acc * 256;
-          uint32_t v[2][16];
-          tmem_ld_32x16(t0 + col_a, v[0]);
-          tmem_ld_wait16(v[0]);
+          uint32_t v[2][32];
+          tmem_ld_32x32(t0 + col_a, v[0]);
+          tmem_ld_wait32(v[0]);
 #pragma unroll
-          for (int ch = 0; ch < 8; ++ch) {
-            if (ch < 7) tmem_ld_32x16(t0 + (ch + 1 < 4 ? col_a + 16 * (ch + 1) : col_b + 16 * (ch - 3)), v[(ch + 1) & 1]);
+          for (int ch = 0; ch < 4; ++ch) {
+            if (ch < 3) {
+              tmem_ld_32x32(t0 + (ch == 0 ? col_a + 32 : ch == 1 ? col_b : col_b + 32), v[(ch + 1) & 1]);
+            } else {
+              // before the last additions: the stage is in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) fma2(sum[ch * 8 + j], v[ch & 1][2 * j], v[ch & 1][2 * j + 1], ch < 4 ? fa : fb);
-            if (ch < 7) tmem_ld_wait16(v[(ch + 1) & 1]);
+            for (int j = 0; j < 32; ++j) sum[ch * 32 + j] = fmaf(__uint_as_float(v[ch & 1][j]), ch < 2 ? fa : fb, sum[ch * 32 + j]);
+            if (ch < 3) tmem_ld_wait32(v[(ch + 1) & 1]);
           }
+        } else {
+          if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(tempty_leader + 8 * acc);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
       if (!ok) break;
       if constexpr (OUT == F8_ROWS) {
         if (!live) continue;
-        // 64 columns at a time through the warp's staging tile, so that a store covers four whole 128-byte row segments
+        // 64 columns at a time through the warp's staging tile: a tensor copy where all 32 rows are this expert's own (in the padded
+        // layout they always are), else, or by a row map, stores of whole 128-byte row segments
+        const bool whole = args.out_perm == nullptr && (args.padded || quad * 32 + 32 <= c.rows);
         long long out_row = -1;
-        if (r < c.rows) {
+        if (!whole && r < c.rows) {
           out_row = args.out_perm != nullptr ? args.out_perm[c.a_row + r] : c.a_row + r;
           if (out_row >= args.out_rows) out_row = -1;
         }
@@ -390,16 +402,27 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
           float f[64];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const float2 p = halves(sum[g * 32 + j]);
+            const float2 p = make_float2(sum[g * 64 + 2 * j], sum[g * 64 + 2 * j + 1]);
             f[2 * j] = p.x;
             f[2 * j + 1] = p.y;
           }
           act_row(f, args.act);
+          if (lane == 0) bulk_wait_read_all();  // the copy that last read the tile
+          __syncwarp();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const uint4 u = pack8<T>(f + 8 * q);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage_base + lane * 128 + ((q ^ (lane & 7)) << 4)), "r"(u.x),
                          "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+          }
+          if (whole) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmap_out, col0, c.a_row + quad * 32, stage_base);
+              bulk_commit();
+            }
+            continue;
           }
           __syncwarp();
           const int ck = lane & 7;
@@ -425,7 +448,7 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         if (live) {
 #pragma unroll
           for (int j = 0; j < kMine / 2; ++j) {
-            const float2 p = halves(sum[j]);
+            const float2 p = make_float2(sum[2 * j], sum[2 * j + 1]);
             f[2 * j] = p.x;
             f[2 * j + 1] = p.y;
           }
@@ -433,7 +456,7 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
           if (kGlu) {
 #pragma unroll
             for (int j = 0; j < kMine / 2; ++j) {
-              const float2 u = halves(sum[32 + j]);
+              const float2 u = make_float2(sum[64 + 2 * j], sum[64 + 2 * j + 1]);
               f[2 * j] *= u.x;
               f[2 * j + 1] *= u.y;
             }
@@ -468,6 +491,7 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         }
       }
     }
+    if (OUT == F8_ROWS && lane == 0) bulk_wait_all();
   } else {
     fewer_registers();
     if (warp == 0) {
@@ -513,8 +537,9 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
           const F8Item c = walk.get(i, args, kCols);
           if (!c.valid) break;
           for (int kb = 0; kb < kiters; ++kb) {
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1, wctx, DS_TIMEOUT_MMA)) ||
-                !__all_sync(0xFFFFFFFFu, mbar_wait(full_bar + 8 * stage, phase, wctx, DS_TIMEOUT_MMA))) {
+            // (the operands first: they are there before the accumulator stage is, and a wait that passes takes its 100 cycles too)
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait(full_bar + 8 * stage, phase, wctx, DS_TIMEOUT_MMA)) ||
+                !__all_sync(0xFFFFFFFFu, mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1, wctx, DS_TIMEOUT_MMA))) {
               ok = false;
               break;
             }
@@ -525,8 +550,8 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
               for (int k = 0; k < kF8K / kF8MmaK; ++k)
                 umma_f8_pair(tmem_base + acc * 256, make_desc(sx + k * kF8MmaK, 16, 1024), make_desc(sx + kF8Tile + k * kF8MmaK, 16, 1024),
                              idesc, k != 0 ? 1u : 0u);
-              umma_commit_pair_both(empty_bar + 8 * stage);
               umma_commit_pair_both(tfull_bar + 8 * acc);
+              umma_commit_pair_both(empty_bar + 8 * stage);
             }
             __syncwarp();
             if (++stage == kStages) { stage = 0; phase ^= 1; }
