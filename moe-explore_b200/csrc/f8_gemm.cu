@@ -11,7 +11,7 @@ template <int CTAS, typename Kernel, typename... Args>
 static int launch_f8(Kernel kernel, int threads, int smem, std::atomic<int> (&grids)[64], cudaStream_t s, const Args&... args) {
   LaunchParams lp;
   lp.stream = s;
-  lp.max_ctas = 0;
+  lp.max_ctas = CTAS == 1 ? kF8MaxWorkers : 0;
   lp.chained = chained_launches();
   PersistentLaunch l;
   const int rc = configure<CTAS>(l, kernel, smem, grids, lp);
@@ -41,6 +41,21 @@ static int f8_maps(CUtensorMap* tx, CUtensorMap* tw, const void* x, int64_t rows
   const uint64_t dw[3] = {static_cast<uint64_t>(K / 2), static_cast<uint64_t>(N), static_cast<uint64_t>(mats)};
   const uint32_t bw[3] = {kF8K / 2, BM, 1};
   return make_tmap(tw, MOE_DTYPE_BF16, w, 3, dw, bw);
+}
+
+__global__ void __launch_bounds__(256) f8_zero_kernel(uint32_t* counters, int num_counters) {
+  await_predecessor();
+  grid_release();
+  for (int i = threadIdx.x; i < num_counters; i += 256) counters[i] = 0;
+}
+
+int f8_lane_rows(int64_t routed_rows, int num_experts) {
+  const int64_t mean = routed_rows / num_experts;
+  return mean > 128 ? 0 : mean > 48 ? 128 : 64;
+}
+static int f8_workers() {
+  const int n = sm_count();
+  return n < kF8MaxWorkers ? n : kF8MaxWorkers;
 }
 
 int f8_product(const char* name, const F8Product& p, void* stream) {
@@ -83,12 +98,19 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
   a.wait_limit = wait_limit_cycles();
   a.status = p.status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t mean = p.routed_rows / p.num_experts;
-  const bool lanes = mean <= 128;
+  const int lane_rows = f8_lane_rows(p.routed_rows, p.num_experts);
+  const bool lanes = lane_rows != 0;
+  MOE_CHECK_ARG(!lanes || (p.counters != nullptr && aligned16(p.counters)), "%s: 16-byte aligned partials are needed", name);
+  a.counters = p.counters;
+  a.partials = p.partials;
   CUtensorMap tx, tw;
   const int rc = f8_maps(&tx, &tw, p.x, p.x_rows, p.w, static_cast<int64_t>(p.num_experts) * (glu ? 2 : 1), p.N, p.K, lanes ? 16 : BM);
   if (rc != MOE_OK) return rc;
   const bool bf16 = p.dtype == MOE_DTYPE_BF16;
+  if (lanes && p.zero_counters) {
+    MOE_CUDA(launch_kernel(f8_zero_kernel, 1, 256, s, p.counters, kF8MaxWorkers));
+    chained_launches() = true;
+  }
   if (!lanes) {
     CUtensorMap to = tx;
     if (p.kind == F8_ROWS && p.out_perm == nullptr) {
@@ -107,7 +129,7 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
     if (p.kind == F8_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_QUANT, R>(tx, tw, a, s);                        \
     return bf16 ? launch_f8_lanes<__nv_bfloat16, F8_ROWS, R>(tx, tw, a, s) : launch_f8_lanes<__half, F8_ROWS, R>(tx, tw, a, s); \
   } while (0)
-  if (mean <= 48) MOE_F8_LANES(64);
+  if (lane_rows == 64) MOE_F8_LANES(64);
   MOE_F8_LANES(128);
 #undef MOE_F8_LANES
 }
@@ -128,9 +150,12 @@ template <typename T> __device__ __forceinline__ void to_floats(const uint4& u, 
 // T: a 16-bit type (rows are converted) or uint8_t (8-bit rows with `scales_in` are copied).
 template <typename T>
 __global__ void __launch_bounds__(256)
-f8_rows_kernel(const T* x, const float* scales_in, const int32_t* dst_row, int copies, uint2* out, float* scales, int64_t rows, int cols) {
+f8_rows_kernel(const T* x, const float* scales_in, const int32_t* dst_row, int copies, uint2* out, float* scales, int64_t rows, int cols,
+               uint32_t* counters, int num_counters) {
   await_predecessor();  // before the release: what comes up next reads the routing metadata
   grid_release();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < num_counters; i += 256) counters[i] = 0;
   const int blocks = (cols + kF8Block - 1) / kF8Block;
   const int vecs = cols / 8;
   const int lane16 = threadIdx.x & 15;
@@ -196,7 +221,7 @@ static int f8_row_grid(int64_t rows, int cols) {
 }
 
 int f8_rows(const char* name, const void* x, const float* x_scales, const int32_t* dst_row, int copies, void* out, float* scales,
-            int64_t rows, int cols, int dtype, void* stream) {
+            int64_t rows, int cols, int dtype, uint32_t* counters, int num_counters, void* stream) {
   MOE_CHECK_ARG(rows >= 0 && cols > 0 && copies > 0, "%s: negative or zero size", name);
   if (cols % 16 != 0) {
     set_error("%s: 8-bit rows have a multiple of 16 columns, got %d", name, cols);
@@ -210,12 +235,20 @@ int f8_rows(const char* name, const void* x, const float* x_scales, const int32_
   const int grid = f8_row_grid(rows, cols);
   uint2* o = static_cast<uint2*>(out);
   if (x_scales != nullptr)
-    MOE_CUDA(launch_kernel(f8_rows_kernel<uint8_t>, grid, 256, s, static_cast<const uint8_t*>(x), x_scales, dst_row, copies, o, scales, rows, cols));
+    MOE_CUDA(launch_kernel(f8_rows_kernel<uint8_t>, grid, 256, s, static_cast<const uint8_t*>(x), x_scales, dst_row, copies, o, scales, rows, cols,
+                           counters, num_counters));
   else if (dtype == MOE_DTYPE_BF16)
-    MOE_CUDA(launch_kernel(f8_rows_kernel<__nv_bfloat16>, grid, 256, s, static_cast<const __nv_bfloat16*>(x), x_scales, dst_row, copies, o, scales, rows, cols));
+    MOE_CUDA(launch_kernel(f8_rows_kernel<__nv_bfloat16>, grid, 256, s, static_cast<const __nv_bfloat16*>(x), x_scales, dst_row, copies, o, scales, rows, cols,
+                           counters, num_counters));
   else
-    MOE_CUDA(launch_kernel(f8_rows_kernel<__half>, grid, 256, s, static_cast<const __half*>(x), x_scales, dst_row, copies, o, scales, rows, cols));
+    MOE_CUDA(launch_kernel(f8_rows_kernel<__half>, grid, 256, s, static_cast<const __half*>(x), x_scales, dst_row, copies, o, scales, rows, cols,
+                           counters, num_counters));
   return MOE_OK;
+}
+
+// Floats of the workers' slots.
+static size_t f8_slot_floats(int64_t routed_rows, int num_experts, bool glu) {
+  return static_cast<size_t>(2 * f8_workers()) * (glu ? 2 : 1) * f8_lane_rows(routed_rows, num_experts) * 128;
 }
 
 static bool glu(int act) { return act == MOE_ACT_SWIGLU || act == MOE_ACT_GEGLU; }
@@ -225,7 +258,7 @@ static bool glu(int act) { return act == MOE_ACT_SWIGLU || act == MOE_ACT_GEGLU;
 using namespace moe;
 
 extern "C" int moe_f8_quantize_rows(const void* x, void* q, float* scales, int64_t num_rows, int cols, int dtype, void* stream) {
-  return f8_rows("moe_f8_quantize_rows", x, nullptr, nullptr, 1, q, scales, num_rows, cols, dtype, stream);
+  return f8_rows("moe_f8_quantize_rows", x, nullptr, nullptr, 1, q, scales, num_rows, cols, dtype, nullptr, 0, stream);
 }
 
 extern "C" size_t moe_f8_pass_size(void) { return sizeof(moe_f8_pass); }
@@ -244,8 +277,12 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
   if (steps & MOE_F8_ROUTE)
     MOE_STEP(routing_metadata(p->expert_idx, rows, p->num_experts, p->group_indices, nullptr, p->pad_offsets, p->row_src, p->dst_row,
                               p->mtile_expert, p->tile_pairs, p->num_mtiles, p->status, p->workspace, p->workspace_bytes, false, stream));
+  // counters of the two products, then the slots that both use in turn
+  uint32_t* const counters = static_cast<uint32_t*>(p->partials);
+  const bool lanes = f8_lane_rows(rows, p->num_experts) != 0;
   if (steps & MOE_F8_DISPATCH)
-    MOE_STEP(f8_rows("moe_f8_expert_forward", p->x, p->x_scales, p->dst_row, p->topk, p->xs, p->xs_scales, p->num_tokens, p->d, p->dtype, stream));
+    MOE_STEP(f8_rows("moe_f8_expert_forward", p->x, p->x_scales, p->dst_row, p->topk, p->xs, p->xs_scales, p->num_tokens, p->d, p->dtype,
+                     counters, lanes && counters != nullptr ? 2 * kF8MaxWorkers : 0, stream));
   F8Product g{};
   g.x_rows = p->padded_rows;
   g.routed_rows = rows;
@@ -257,8 +294,10 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
   g.pad_offsets = p->pad_offsets;
   g.group_indices = p->group_indices;
   g.status = p->status;
+  g.partials = reinterpret_cast<float*>(counters + 2 * kF8MaxWorkers);
   if (steps & MOE_F8_UP) {
     g.kind = glu(p->act) ? F8_GLU_QUANT : F8_QUANT;
+    g.counters = counters;
     g.x = p->xs;
     g.x_scales = p->xs_scales;
     g.w = p->w1;
@@ -272,6 +311,7 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
   }
   if (steps & MOE_F8_DOWN) {
     g.kind = F8_ROWS;
+    g.counters = counters + kF8MaxWorkers;
     g.x = p->hidden;
     g.x_scales = p->hidden_scales;
     g.w = p->w2;
@@ -287,6 +327,11 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
     MOE_STEP(combine_topk(p->ys, p->scores, p->dst_row, p->out, p->num_tokens, p->topk, p->d, p->dtype, p->addend, nullptr, nullptr,
                           nullptr, stream));
   return MOE_OK;
+}
+
+extern "C" size_t moe_f8_partial_bytes(int64_t num_rows, int num_experts, int act) {
+  if (num_rows <= 0 || num_experts <= 0 || f8_lane_rows(num_rows, num_experts) == 0) return 0;
+  return 2 * kF8MaxWorkers * sizeof(uint32_t) + f8_slot_floats(num_rows, num_experts, glu(act)) * sizeof(float);
 }
 
 extern "C" size_t moe_f8_rows_pass_size(void) { return sizeof(moe_f8_rows_pass); }
@@ -320,6 +365,9 @@ extern "C" int moe_f8_rows_gemm(const moe_f8_rows_pass* p, int steps, void* stre
   }
   if (steps & MOE_ROWS_GEMM) {
     F8Product g{};
+    g.counters = static_cast<uint32_t*>(p->partials);
+    g.partials = reinterpret_cast<float*>(g.counters + 2 * kF8MaxWorkers);
+    g.zero_counters = true;
     g.kind = F8_ROWS;
     g.x = p->gather ? p->gathered : p->x;
     g.x_scales = p->gather ? p->gathered_scales : p->x_scales;

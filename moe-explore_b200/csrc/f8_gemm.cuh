@@ -19,6 +19,8 @@
 #include "f8.cuh"
 #include "gemm_kernel.cuh"
 
+#include <type_traits>
+
 namespace moe {
 
 // What a product's results become.
@@ -40,6 +42,9 @@ struct F8Product {
   float* out_scales;
   int K, N, num_experts, act, dtype;
   int64_t routed_rows;      // about how many rows there are
+  float* partials;          // F8Args
+  uint32_t* counters;
+  bool zero_counters;       // by a launch of their own (else a kernel before has done it)
   bool dense;
   int compact;
   const int64_t* out_perm;
@@ -48,6 +53,8 @@ struct F8Product {
   int32_t* status;
 };
 int f8_product(const char* name, const F8Product& p, void* stream);
+// Rows per pass of the kernel with the weights on the lanes; 0: the other kernel.
+int f8_lane_rows(int64_t routed_rows, int num_experts);
 
 struct F8Args {
   // The rows of the experts: maps of the padded layout, or dense_rows >= 0: one expert, rows 0 .. dense_rows - 1, no maps.
@@ -66,6 +73,8 @@ struct F8Args {
   int32_t k_dim;
   int32_t act;
   int32_t group_m;
+  float* partials;        // f8_lanes_kernel: two slots per worker
+  uint32_t* counters;     // f8_lanes_kernel: kF8MaxWorkers words, zero
   long long wait_limit;
   int32_t* status;
 };
@@ -129,19 +138,24 @@ template <int CTAS> struct F8Walk {
     c.rows = active && rows > 0 && c.a_row >= 0 ? rows : 0;
     return c;
   }
+  // What lane `src` decoded.
+  __device__ __forceinline__ F8Item held(int src) const {
+    F8Item c;
+    c.valid = true;
+    c.a_row = __shfl_sync(0xFFFFFFFFu, mine.a_row, src);
+    c.n0 = __shfl_sync(0xFFFFFFFFu, mine.n0, src);
+    c.expert = __shfl_sync(0xFFFFFFFFu, mine.expert, src);
+    c.rows = __shfl_sync(0xFFFFFFFFu, mine.rows, src);
+    return c;
+  }
   __device__ __forceinline__ F8Item get(int i, const F8Args& a, int cols_per_tile) {
     if ((i & 31) == 0) {
       const int t = first + (i + static_cast<int>(threadIdx.x & 31)) * stride;
       if (t < count) mine = decode(t, a, cols_per_tile);
       __syncwarp();
     }
-    const int src = i & 31;
-    F8Item c;
+    F8Item c = held(i & 31);
     c.valid = first + i * stride < count;
-    c.a_row = __shfl_sync(0xFFFFFFFFu, mine.a_row, src);
-    c.n0 = __shfl_sync(0xFFFFFFFFu, mine.n0, src);
-    c.expert = __shfl_sync(0xFFFFFFFFu, mine.expert, src);
-    c.rows = __shfl_sync(0xFFFFFFFFu, mine.rows, src);
     return c;
   }
 };
@@ -214,12 +228,13 @@ template <int N> __device__ __forceinline__ void act_row(float (&v)[N], int act)
   }
 }
 // Warps: 0 producer, 1 MMA issuer, 2 and 3 none, 4 to 11 epilogue: whole warpgroups, so that the epilogue's take the registers that
-// the first one gives back (40 + 2 * 232 = 3 * 168, what the launch has).
+// the first one gives back (its own and twice theirs make 3 * 168, what the launch has).
 constexpr int kF8Threads = 384;
-constexpr int kF8LaunchRegs = 168, kF8FewRegs = 40, kF8EpilogueRegs = 232;
-static_assert(kF8FewRegs + 2 * kF8EpilogueRegs <= 3 * kF8LaunchRegs, "register split");
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kF8FewRegs)); }
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kF8EpilogueRegs)); }
+constexpr int kF8LaunchRegs = 168;
+template <int FEW> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW)); }
+template <int FEW> __device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"((3 * kF8LaunchRegs - FEW) / 2));
+}
 
 constexpr int kF8K = 128;                    // bytes (= elements) of K in one stage: one swizzle row
 constexpr int kF8Tile = BM * kF8K;           // 16 KB: 128 rows of an operand
@@ -304,7 +319,7 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   const int kiters = (args.k_dim + kF8K - 1) / kF8K;
 
   if (warp >= 4) {
-    more_registers();
+    more_registers<40>();
     // ------------------------------ epilogue ----------------------------------
     const int quad = warp & 3;
     const int half = (warp - 4) >> 2;
@@ -493,7 +508,7 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     }
     if (OUT == F8_ROWS && lane == 0) bulk_wait_all();
   } else {
-    fewer_registers();
+    fewer_registers<40>();
     if (warp == 0) {
       // ------------------------------ TMA producer ------------------------------
       int stage = 0;
@@ -584,17 +599,97 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
 // token a stage is 16 (32) KB of weights and 2 KB of rows.  The ring holds about 190 KB, what an SM needs in flight to stream
 // weights at the memory's rate.  Epilogue warp w owns the 32 lanes of quadrant w % 4 and every other group of 16 rows; a row's scale
 // is handed around by shuffles.  (CTA pairs bring nothing here: there is nothing to share but the few rows.)
+//
+// SPLIT ALONG K.  As many items as there are workers, as often as that goes, are dealt out whole; what is left (everything, where
+// there are fewer items than workers) is one run of steps of 128 of K, of which every worker takes an equal part, wherever that
+// begins and ends.  An item that several workers share is summed by each over its own steps into a slot of its own in `partials`, and
+// whoever arrives last (a counter per first worker of a shared item) adds the slots in the order of the workers and goes on to
+// the results.  Nobody waits for anybody, and the sums do not depend on who was last.  The shared steps come first and are joined
+// last.  Bound by HBM: one token through 2 of 8 experts of 4096 x 14336 has 224 and 64 items
+// for 148 SMs, which dealt out whole left half of them idle.  (All items as one run of steps, 14 in a row per worker: 1.9 GB of
+// weights at 5.0 TB/s instead of 6.0; neighbours then no longer stream neighbouring weights.)
+// (An item with more than R rows takes more than one pass over its weights and is not shared: its first worker does all of it.)
+//
+// The weights of the first stages are asked for before the wait for the kernel before: that one writes the rows, while the maps
+// and counts were complete before it let this kernel up (it waited for them itself).
 // ------------------------------------------------------------------------------------------------------------------
+constexpr int kF8MaxWorkers = 256;
+constexpr int kF8LeastSteps = 4;  // of a worker; with fewer, what the joining costs is more than the streaming
+
+// The work of one worker, item by item.
+struct F8Part {
+  F8Item c;
+  int kb0, kb1;  // steps of this item (kb0 >= kb1: none)
+  int item;
+  bool shared;
+  bool valid;
+};
+struct F8Split {
+  F8Walk<1> walk;             // decodes; its lanes 0 to 15 hold items of the shared run, 16 to 31 whole ones
+  int64_t begin, end, steps;  // the shared run: this worker's part of it, and all of it
+  int worker, all_workers, workers, kiters, item0, items, wholes, loose;
+  __device__ __forceinline__ F8Split(const F8Args& a, int worker_, int all_workers_, int kiters_)
+      : walk(a, 0, 1, 128, 0), worker(worker_), all_workers(all_workers_), kiters(kiters_) {
+    wholes = walk.count / all_workers;
+    loose = walk.count - wholes * all_workers;  // items of the shared run
+    steps = static_cast<int64_t>(loose) * kiters;
+    const int64_t most = steps / kF8LeastSteps;
+    workers = most < 1 ? 1 : most < all_workers ? static_cast<int>(most) : all_workers;
+    begin = worker < workers ? steps * worker / workers : steps;
+    end = worker < workers ? steps * (worker + 1) / workers : steps;
+    item0 = static_cast<int>(begin / kiters);
+    items = begin < end ? static_cast<int>((end - 1) / kiters) - item0 + 1 : 0;
+    decode(0, 0, a);
+  }
+  // Decodes shared items from `shared0` and whole ones from `whole0` on, 16 of each: one chain of dependent loads for both.
+  __device__ __forceinline__ void decode(int shared0, int whole0, const F8Args& a) {
+    const int lane = threadIdx.x & 31;
+    const int i = lane < 16 ? shared0 + lane : whole0 + lane - 16;
+    if (i < (lane < 16 ? items : wholes)) walk.mine = walk.decode(lane < 16 ? item0 + i : loose + worker + i * all_workers, a, 128);
+    __syncwarp();
+  }
+  // The i-th of this worker; i = 0, 1, 2, ... in this order, by all lanes of the warp (shared ones also again afterwards, from 0 on).
+  __device__ __forceinline__ F8Part get(int i, const F8Args& a, int most_rows) {
+    F8Part p;
+    p.valid = i < items + wholes;
+    if (!p.valid) return p;
+    const bool is_shared = i < items;
+    const int j = is_shared ? i : i - items;
+    if ((j & 15) == 0 && (j > 0 || items > 16)) decode(is_shared ? j : 0, is_shared ? 0 : j, a);
+    p.item = is_shared ? item0 + i : loose + worker + j * all_workers;
+    p.c = walk.held((is_shared ? 0 : 16) + (j & 15));
+    p.kb0 = 0;
+    p.kb1 = kiters;
+    p.shared = false;
+    if (!is_shared) return p;
+    if (i == 0) p.kb0 = static_cast<int>(begin - static_cast<int64_t>(item0) * kiters);
+    if (i == items - 1) p.kb1 = static_cast<int>(end - static_cast<int64_t>(p.item) * kiters);
+    p.shared = p.kb0 > 0 || p.kb1 < kiters;
+    if (p.shared && p.c.rows > most_rows) {
+      p.shared = false;
+      p.kb1 = p.kb0 == 0 ? kiters : p.kb0;
+    }
+    return p;
+  }
+  __device__ __forceinline__ int worker_of(int64_t step) const { return static_cast<int>(((step + 1) * workers - 1) / steps); }
+};
+
 template <int R, bool GLU> struct F8LanesPlan {
   static constexpr int kWBytes = (GLU ? 2 : 1) * kF8Tile;
   static constexpr int kStageBytes = kWBytes + R * kF8K;
-  static constexpr int kExtra = 2 * 4 * R * 4;  // block maxima of the quadrants, two places used in turn
+  static constexpr int kAccCols = (GLU ? 2 : 1) * R;
+  static constexpr int kAccs = 512 / kAccCols > 4 ? 4 : 512 / kAccCols;
+  // the results' way from lanes to rows: 16 rows x 128 columns in fp32
+  static constexpr int kStaging = (GLU ? 2 : 1) * 16 * 128 * 4;
+  // the scales of as many steps as fit: [step][row], and [matrix][step] of the weights
+  static constexpr int kTable = 2048;
+  static constexpr int kTableSteps = 128;
+  static constexpr int kExtra = kStaging + (kTable + 2 * kTableSteps) * 4;
   static constexpr int kBarrierBytes = 1024;
   static constexpr int kBudget = 232448 - 1024 - kBarrierBytes - kExtra;
   static constexpr int kStages = kBudget / kStageBytes > 10 ? 10 : kBudget / kStageBytes;
   static constexpr int kTotal = kStages * kStageBytes + kExtra + kBarrierBytes + 1024;
-  static constexpr int kAccCols = (GLU ? 2 : 1) * R;
-  static constexpr int kAccs = 512 / kAccCols > 4 ? 4 : 512 / kAccCols;
+  static_assert(kTable >= 16 * R, "scales of 16 steps at least");
 };
 
 template <typename T, int OUT, int R>
@@ -604,12 +699,14 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   using Plan = F8LanesPlan<R, kGlu>;
   constexpr int kStages = Plan::kStages, kAccs = Plan::kAccs;
   constexpr int kMats = kGlu ? 2 : 1;
-  constexpr int kChunks = R / 32;  // groups of 16 rows per warp
+  constexpr int kChunks = R / 32;  // groups of 16 rows whose results a warp sees to
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t tiles_addr = (raw_addr + 1023u) & ~1023u;
   uint8_t* tiles = smem_raw + (tiles_addr - raw_addr);
-  float* maxima = reinterpret_cast<float*>(tiles + kStages * Plan::kStageBytes);
+  float* const staging = reinterpret_cast<float*>(tiles + kStages * Plan::kStageBytes);
+  float* const table = staging + Plan::kStaging / 4;
+  float* const weight_table = table + Plan::kTable;
   uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kStages * Plan::kStageBytes + Plan::kExtra);
   const uint32_t full_bar = smem_u32(bars);
   const uint32_t empty_bar = smem_u32(bars + kStages);
@@ -618,6 +715,7 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   const uint32_t meet_bar = smem_u32(bars + 2 * kStages + 2 * kAccs);  // the epilogue warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kAccs + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* joined = reinterpret_cast<volatile int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -648,189 +746,327 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  await_predecessor();
   const uint32_t tmem_base = *tmem_slot;
-  F8Walk<1> walk(args, blockIdx.x, gridDim.x, 128, 0);
   const int kiters = (args.k_dim + kF8K - 1) / kF8K;
+  F8Split split(args, blockIdx.x, gridDim.x, kiters);
 
   if (warp >= 4) {
-    more_registers();
+    more_registers<72>();
     // ------------------------------ epilogue ----------------------------------
     const int quad = warp & 3;
     const int half = (warp - 4) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const int kblocks = kiters;
     const int nblocks = (args.n_dim + kF8Block - 1) / kF8Block;
-    int acc = 0, turn = 0;
+    int acc = 0, meets = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int i = 0; ok; ++i) {
-      const F8Item c = walk.get(i, args, 128);
-      if (!c.valid) break;
-      const int n = c.n0 + quad * 32 + lane;  // this lane's result column
-      const float* wa = args.w_scales + (static_cast<int64_t>(c.expert) * kMats * nblocks + c.n0 / kF8Block) * kblocks;
-      const float* wb = wa + static_cast<int64_t>(nblocks) * kblocks;
-      for (int r0 = 0; r0 < c.rows && ok; r0 += R, ++turn) {
+    const auto meet = [&]() {  // of the epilogue warps
+      __syncwarp();
+      if (lane == 0) mbar_arrive(meet_bar);
+      return __all_sync(0xFFFFFFFFu, mbar_wait(meet_bar, meets++ & 1, wctx, DS_TIMEOUT_EPILOGUE));
+    };
+    // Shared items a second time, at the end: their parts are written on the way, and by then the writes are long complete (waiting for
+    // them, and for the counter, at once took 5 us under a saturated memory, twice per worker, and the weights' stream stood).
+    const int parts = split.items + split.wholes;
+    // One warp tells the counters that this worker's parts are written, and which shared items are left to this worker: in the middle of
+    // a whole item, where its waiting costs nothing, else at the end.  A meeting of the warps since the writes lies before.
+    bool arrived = false;
+    const auto arrive = [&]() {
+      arrived = true;
+      if (warp != 4) return;
+      for (int j = 0; j < split.items; ++j) {
+        const F8Part p = split.get(j, args, R);
+        if (!p.shared || p.kb0 >= p.kb1 || lane != 0) continue;
+        __threadfence();  // (what the others wrote before the meeting is covered)
+        const int first_worker = split.worker_of(static_cast<int64_t>(p.item) * kiters);
+        const int last_worker = split.worker_of(static_cast<int64_t>(p.item + 1) * kiters - 1);
+        joined[j] = atomicAdd(args.counters + first_worker, 1u) == static_cast<uint32_t>(last_worker - first_worker) ? 1 : 0;
+        __threadfence();
+      }
+      __syncwarp();
+    };
+    await_predecessor();
+    for (int i = 0; ok && i < parts + split.items; ++i) {
+      const bool joining = i >= parts;
+      const F8Part part = split.get(joining ? i - parts : i, args, R);
+      if (part.kb0 >= part.kb1) continue;  // (done by the item's first worker)
+      if (joining) {
+        if (!part.shared) continue;
+        if (!arrived) {
+          if (!meet()) break;
+          arrive();
+        }
+        if (!meet()) break;
+        if (joined[i - parts] == 0) continue;  // someone else goes on with this item
+      }
+      const F8Item& c = part.c;
+      const float* ws = args.w_scales + (static_cast<int64_t>(c.expert) * kMats * nblocks + c.n0 / kF8Block) * kblocks;
+      for (int r0 = 0; r0 < c.rows && ok; r0 += R) {
         const int rows = min(c.rows - r0, R);
-        // group ch of this warp: rows r0 + 16 * (2 * ch + half) ...; its lanes' scales (lanes 16 to 31 repeat them)
-        const float* xs[kChunks];
-        float x0[kChunks], x1[kChunks];
+        const int rows16 = (rows + 15) & ~15;
+        const int64_t first = static_cast<int64_t>(c.a_row) + r0;
         float sum[kMats][kChunks][16];
 #pragma unroll
-        for (int ch = 0; ch < kChunks; ++ch) {
-          const int rr = min(16 * (2 * ch + half) + (lane & 15), rows - 1);
-          xs[ch] = args.x_scales + (static_cast<int64_t>(c.a_row) + r0 + rr) * kblocks;
-          x0[ch] = xs[ch][0];
-          x1[ch] = kiters > 1 ? xs[ch][1] : 0.0f;
+        for (int ch = 0; ch < kChunks; ++ch)
 #pragma unroll
           for (int m = 0; m < kMats; ++m)
 #pragma unroll
             for (int j = 0; j < 16; ++j) sum[m][ch][j] = 0.0f;
-        }
-        float a0 = wa[0], b0 = kGlu ? wb[0] : 0.0f;
-        float a1 = kiters > 1 ? wa[1] : 0.0f, b1 = kGlu && kiters > 1 ? wb[1] : 0.0f;
-        for (int kb = 0; kb < kiters; ++kb) {
-          float x2[kChunks], a2 = 0.0f, b2 = 0.0f;
-          const bool more = kb + 2 < kiters;
-          if (more) {
-            a2 = wa[kb + 2];
-            if (kGlu) b2 = wb[kb + 2];
+        const int most = min(Plan::kTable / rows16, Plan::kTableSteps);
+        int filled = part.kb0, base = part.kb0;  // the table holds the scales of steps [base, filled)
+        for (int kb = joining ? part.kb1 : part.kb0; kb < part.kb1;) {
+          if (kb == filled) {
+            if (!meet()) {  // (everyone is done with what it held)
+              ok = false;
+              break;
+            }
+            base = kb;
+            const int steps = min(part.kb1 - kb, most);
+            filled = kb + steps;
+#pragma unroll 1
+            for (int rr = warp - 4; rr < rows; rr += kEpilogueWarps)
+              for (int s = lane; s < steps; s += 32) table[s * rows16 + rr] = args.x_scales[(first + rr) * kblocks + kb + s];
+            if (warp < 4 + kMats)
+              for (int s = lane; s < steps; s += 32)
+                weight_table[(warp - 4) * Plan::kTableSteps + s] = ws[static_cast<int64_t>(warp - 4) * nblocks * kblocks + kb + s];
+            if (!meet()) {
+              ok = false;
+              break;
+            }
           }
+          if (!arrived && i >= split.items && kb - base >= 8) arrive();
+          // Two steps at a time where there are two: a step is a chain of waits (sums there, sums fetched) of about 350 ns, which is what
+          // 16 KB of weights take to arrive.
+          constexpr int kTogether = kAccs >= 4 ? 2 : 1;
+          const int together = kTogether == 2 && kb + 1 < filled && (acc & 1) == 0 ? 2 : 1;
 #pragma unroll
-          for (int ch = 0; ch < kChunks; ++ch) x2[ch] = more ? xs[ch][kb + 2] : 0.0f;
-          if (!__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar + 8 * acc, acc_phase, wctx, DS_TIMEOUT_EPILOGUE))) {
-            ok = false;
-            break;
-          }
+          for (int t = 0; t < kTogether; ++t)
+            if (t < together && ok &&
+                !__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar + 8 * (acc + t), acc_phase, wctx, DS_TIMEOUT_EPILOGUE))) ok = false;
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t t0 = tmem_base + lanes + acc * Plan::kAccCols;
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch) {
             const int col = 16 * (2 * ch + half);
             if (col < rows) {
-              uint32_t v[kMats][16];
+              uint32_t v[kTogether][kMats][16];
 #pragma unroll
-              for (int m = 0; m < kMats; ++m) tmem_ld_32x16(t0 + m * R + col, v[m]);
+              for (int t = 0; t < kTogether; ++t)
+                if (t < together) {
 #pragma unroll
-              for (int m = 0; m < kMats; ++m) tmem_ld_wait16(v[m]);
+                  for (int m = 0; m < kMats; ++m) tmem_ld_32x16(tmem_base + lanes + (acc + t) * Plan::kAccCols + m * R + col, v[t][m]);
+                }
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float x = __shfl_sync(0xFFFFFFFFu, x0[ch], j);
-                sum[0][ch][j] = fmaf(__uint_as_float(v[0][j]), x * a0, sum[0][ch][j]);
-                if (kGlu) sum[kMats - 1][ch][j] = fmaf(__uint_as_float(v[kMats - 1][j]), x * b0, sum[kMats - 1][ch][j]);
-              }
+              for (int t = 0; t < kTogether; ++t)
+                if (t < together) {
+                  const float* xs = table + (kb + t - base) * rows16 + col;
+                  const float a0 = weight_table[kb + t - base], b0 = kGlu ? weight_table[Plan::kTableSteps + kb + t - base] : 0.0f;
+                  float x[16];
+#pragma unroll
+                  for (int j = 0; j < 16; j += 4) {
+                    const float4 q = *reinterpret_cast<const float4*>(xs + j);
+                    x[j] = q.x;
+                    x[j + 1] = q.y;
+                    x[j + 2] = q.z;
+                    x[j + 3] = q.w;
+                  }
+#pragma unroll
+                  for (int m = 0; m < kMats; ++m) tmem_ld_wait16(v[t][m]);
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) {
+                    sum[0][ch][j] = fmaf(__uint_as_float(v[t][0][j]), x[j] * a0, sum[0][ch][j]);
+                    if (kGlu) sum[kMats - 1][ch][j] = fmaf(__uint_as_float(v[t][kMats - 1][j]), x[j] * b0, sum[kMats - 1][ch][j]);
+                  }
+                }
             }
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(tempty_bar + 8 * acc);
-          if (++acc == kAccs) { acc = 0; acc_phase ^= 1; }
-#pragma unroll
-          for (int ch = 0; ch < kChunks; ++ch) {
-            x0[ch] = x1[ch];
-            x1[ch] = x2[ch];
-          }
-          a0 = a1;
-          a1 = a2;
-          b0 = b1;
-          b1 = b2;
+          if (lane < together) mbar_arrive(tempty_bar + 8 * (acc + lane));
+          kb += together;
+          acc += together;
+          if (acc == kAccs) { acc = 0; acc_phase ^= 1; }
         }
         if (!ok) break;
-        // the results: activation in place
+        if (part.shared) {
+          // (R rows at most: one pass)
+          constexpr int kSlot = kMats * R * 128;  // floats: [matrix][four rows][lane][row of the four]
+          const int first_worker = split.worker_of(static_cast<int64_t>(part.item) * kiters);
+          const int last_worker = split.worker_of(static_cast<int64_t>(part.item + 1) * kiters - 1);
+          // a worker's slots: of the item it shares with those before it, and of the one it begins
+          const auto slot_of = [&](int worker) {
+            return reinterpret_cast<float4*>(args.partials + static_cast<int64_t>(2 * worker + (worker == first_worker ? 1 : 0)) * kSlot) +
+                   quad * 32 + lane;
+          };
+          if (!joining) {
+            float4* mine = slot_of(blockIdx.x);
 #pragma unroll
-        for (int ch = 0; ch < kChunks; ++ch) {
-          act_row(sum[0][ch], args.act);
-          if (kGlu) {
+            for (int ch = 0; ch < kChunks; ++ch) {
+              const int col = 16 * (2 * ch + half);
+              if (col >= rows) continue;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sum[0][ch][j] *= sum[kMats - 1][ch][j];
-          }
-        }
-        const int64_t first = static_cast<int64_t>(c.a_row) + r0;
-        if constexpr (OUT == F8_ROWS) {
+              for (int m = 0; m < kMats; ++m)
 #pragma unroll
-          for (int ch = 0; ch < kChunks; ++ch)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int rr = 16 * (2 * ch + half) + j;
-              if (rr >= rows) continue;
-              const int64_t to = args.out_perm != nullptr ? args.out_perm[first + rr] : first + rr;
-              if (n < args.n_dim && to >= 0 && to < args.out_rows)
-                static_cast<T*>(args.out)[to * args.n_dim + n] = Elem<T>::from_float(sum[0][ch][j]);
+                for (int j = 0; j < 16; j += 4)
+                  __stcg(mine + (m * R + col + j) / 4 * 128,
+                         make_float4(sum[m][ch][j], sum[m][ch][j + 1], sum[m][ch][j + 2], sum[m][ch][j + 3]));
             }
-        } else {
-          float* place = maxima + (turn & 1) * 4 * R;
+            continue;
+          }
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch) {
-            float keep = 0.0f;
+            const int col = 16 * (2 * ch + half);
+            if (col >= rows) continue;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              // (non-negative floats order as integers; NaN stays out of the maximum, as in fmaxf)
-              const float v = fabsf(sum[0][ch][j]);
-              const uint32_t m = __reduce_max_sync(0xFFFFFFFFu, v == v ? __float_as_uint(v) : 0u);
-              if ((lane & 15) == j) keep = __uint_as_float(m);
+            for (int m = 0; m < kMats; ++m)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) sum[m][ch][j] = 0.0f;
+#pragma unroll 2
+            for (int w = first_worker; w <= last_worker; ++w) {
+              const float4* from = slot_of(w);
+              float4 v[kMats][4];
+#pragma unroll
+              for (int m = 0; m < kMats; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[m][j] = __ldcg(from + ((m * R + col) / 4 + j) * 128);
+#pragma unroll
+              for (int m = 0; m < kMats; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  sum[m][ch][4 * j] += v[m][j].x;
+                  sum[m][ch][4 * j + 1] += v[m][j].y;
+                  sum[m][ch][4 * j + 2] += v[m][j].z;
+                  sum[m][ch][4 * j + 3] += v[m][j].w;
+                }
             }
-            if (lane < 16) place[quad * R + 16 * (2 * ch + half) + lane] = keep;
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(meet_bar);
-          if (!__all_sync(0xFFFFFFFFu, mbar_wait(meet_bar, turn & 1, wctx, DS_TIMEOUT_EPILOGUE))) {
+        }
+        // The results, 16 rows at a time: the warps that have them leave them in shared memory, then every warp takes rows, 128 columns
+        // (a block) over its lanes.  A loop of little code: the weights that stream through L2 throw instructions out of it, and
+        // each line that has to be fetched again behind them takes a microsecond (unrolled over rows and groups this took 5 us
+        // after the last step, at one token).
+#pragma unroll 1
+        for (int q = 0; 16 * q < rows; ++q) {
+          if ((q & 1) == half) {
+            // (constant indexes, group by group: an index that varies would put the sums into local memory)
+            float* to = staging + quad * 32 + lane;
+            const auto put = [&](auto group) {
+              constexpr int ch = decltype(group)::value;
+              if constexpr (ch < kChunks) {
+#pragma unroll
+                for (int m = 0; m < kMats; ++m)
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) to[(m * 16 + j) * 128] = sum[m][ch][j];
+              }
+            };
+            switch (q >> 1) {
+              case 0: put(std::integral_constant<int, 0>()); break;
+              case 1: put(std::integral_constant<int, 1>()); break;
+              case 2: put(std::integral_constant<int, 2>()); break;
+              default: put(std::integral_constant<int, 3>()); break;
+            }
+          }
+          if (!meet()) {
             ok = false;
             break;
           }
-#pragma unroll
-          for (int ch = 0; ch < kChunks; ++ch) {
-            const int rr0 = 16 * (2 * ch + half);
-            if (rr0 >= rows) continue;
-            float most = kF8Least;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) most = fmaxf(most, place[q * R + rr0 + (lane & 15)]);
-            if (quad == 0 && lane < 16 && rr0 + lane < rows)
-              args.out_scales[(first + rr0 + lane) * nblocks + c.n0 / kF8Block] = most / kF8Top;
-            const float inv = kF8Top / most;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float v = sum[0][ch][j] * __shfl_sync(0xFFFFFFFFu, inv, j);
-              if (rr0 + j < rows && n < args.n_dim)
-                static_cast<uint8_t*>(args.out)[(first + rr0 + j) * args.n_dim + n] =
-                    static_cast<uint8_t>(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3));
+          const int live = min(rows - 16 * q, 16);
+          const int col = c.n0 + 4 * lane;
+#pragma unroll 1
+          for (int rr = warp - 4; rr < live; rr += kEpilogueWarps) {
+            const float4 v = *reinterpret_cast<const float4*>(staging + rr * 128 + 4 * lane);
+            float f[4] = {v.x, v.y, v.z, v.w};
+            act_row(f, args.act);
+            if (kGlu) {
+              const float4 u = *reinterpret_cast<const float4*>(staging + (16 + rr) * 128 + 4 * lane);
+              f[0] *= u.x;
+              f[1] *= u.y;
+              f[2] *= u.z;
+              f[3] *= u.w;
             }
+            int64_t row = first + 16 * q + rr;
+            if constexpr (OUT == F8_ROWS) {
+              if (args.out_perm != nullptr) row = args.out_perm[row];
+              if (row >= 0 && row < args.out_rows && col < args.n_dim)
+                *reinterpret_cast<uint2*>(static_cast<T*>(args.out) + row * args.n_dim + col) =
+                    make_uint2(Elem<T>::pack2(f[0], f[1]), Elem<T>::pack2(f[2], f[3]));
+            } else {
+              float most = kF8Least;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(f[j]));
+              most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));  // (non-negative: ordered as integers)
+              const float inv = kF8Top / most;
+              if (col < args.n_dim)
+                *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(args.out) + row * args.n_dim + col) =
+                    f8x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+              if (lane == 0) args.out_scales[row * nblocks + c.n0 / kF8Block] = most / kF8Top;
+            }
+          }
+          if (!meet()) {  // (everyone is done with the staged rows)
+            ok = false;
+            break;
           }
         }
       }
     }
   } else {
-    fewer_registers();
+    fewer_registers<72>();
     if (warp == 0) {
       // ------------------------------ TMA producer ------------------------------
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       const uint64_t pol = l2_policy_evict_normal();
+      const auto load_weights = [&](int st, int kb, const F8Item& c, int groups) {
+        const uint32_t sw = tiles_addr + st * Plan::kStageBytes;
+        mbar_arrive_expect_tx(full_bar + 8 * st, Plan::kWBytes + groups * 16 * kF8K);
+#pragma unroll
+        for (int m = 0; m < kMats; ++m)
+          tma_load_3d(sw + m * kF8Tile, &tmap_w, kb * (kF8K / 2), c.n0, kMats * c.expert + m, full_bar + 8 * st, pol);
+      };
+      const auto load_rows = [&](int st, int kb, const F8Item& c, int r0, int groups) {
+        const uint32_t sx = tiles_addr + st * Plan::kStageBytes + Plan::kWBytes;
+        for (int g = 0; g < groups; ++g)
+          tma_load_2d(sx + g * 16 * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + r0 + 16 * g, full_bar + 8 * st, pol);
+      };
+      bool waited = false;
       for (int i = 0; ok; ++i) {
-        const F8Item c = walk.get(i, args, 128);
-        if (!c.valid) break;
+        const F8Part part = split.get(i, args, R);
+        if (!part.valid) break;
+        const F8Item& c = part.c;
+        if (part.kb0 >= part.kb1) continue;
         for (int r0 = 0; r0 < c.rows && ok; r0 += R) {
           const int groups = (min(c.rows - r0, R) + 15) >> 4;
-          for (int kb = 0; kb < kiters; ++kb) {
+          int kb = part.kb0;
+          if (!waited) {
+            const int ahead = min(part.kb1 - kb, kStages);
+            if (elect_one())
+              for (int st = 0; st < ahead; ++st) load_weights(st, kb + st, c, groups);
+            __syncwarp();
+            await_predecessor();
+            waited = true;
+            if (elect_one())
+              for (int st = 0; st < ahead; ++st) load_rows(st, kb + st, c, r0, groups);
+            __syncwarp();
+            kb += ahead;
+            if ((stage = ahead) == kStages) { stage = 0; phase = 1; }
+          }
+          for (; kb < part.kb1; ++kb) {
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, wctx, DS_TIMEOUT_PRODUCER))) {
               ok = false;
               break;
             }
             if (elect_one()) {
-              const uint32_t sw = tiles_addr + stage * Plan::kStageBytes;
-              const uint32_t fb = full_bar + 8 * stage;
-              mbar_arrive_expect_tx(fb, Plan::kWBytes + groups * 16 * kF8K);
-#pragma unroll
-              for (int m = 0; m < kMats; ++m)
-                tma_load_3d(sw + m * kF8Tile, &tmap_w, kb * (kF8K / 2), c.n0, kMats * c.expert + m, fb, pol);
-              for (int g = 0; g < groups; ++g)
-                tma_load_2d(sw + Plan::kWBytes + g * 16 * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + r0 + 16 * g, fb, pol);
+              load_weights(stage, kb, c, groups);
+              load_rows(stage, kb, c, r0, groups);
             }
             __syncwarp();
             if (++stage == kStages) { stage = 0; phase ^= 1; }
           }
         }
       }
+      if (!waited) await_predecessor();
       grid_release();
       if (!ok || *abort_flag) {
         for (int i = 0; i < 2000; ++i) __nanosleep(1000);
@@ -840,12 +1076,14 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
+      await_predecessor();  // (the limits of the waits below are not to run out on the kernel before)
       for (int i = 0; ok; ++i) {
-        const F8Item c = walk.get(i, args, 128);
-        if (!c.valid) break;
+        const F8Part part = split.get(i, args, R);
+        if (!part.valid) break;
+        const F8Item& c = part.c;
         for (int r0 = 0; r0 < c.rows && ok; r0 += R) {
           const uint32_t idesc = f8_idesc(BM, (min(c.rows - r0, R) + 15) & ~15);
-          for (int kb = 0; kb < kiters; ++kb) {
+          for (int kb = part.kb0; kb < part.kb1; ++kb) {
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1, wctx, DS_TIMEOUT_MMA)) ||
                 !__all_sync(0xFFFFFFFFu, mbar_wait(full_bar + 8 * stage, phase, wctx, DS_TIMEOUT_MMA))) {
               ok = false;
