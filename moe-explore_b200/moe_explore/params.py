@@ -67,6 +67,13 @@ class Fp8ExpertParams(FFNParams):
 
 
 @dataclass
+class RMSNormParams:
+    """Root-mean-square norm in front of the layer (``moe_explore.functional.rms_norm``)."""
+    weight: torch.Tensor   # [d], in the rows' dtype or fp32
+    eps: float = 1e-6
+
+
+@dataclass
 class RouterParams:
     """Base of the router parameter bundles."""
 
@@ -109,6 +116,7 @@ class MOEParams:
     num_experts: int
     topk: int
     shared_expert_params: Optional[FFNParams] = None
+    norm_params: Optional["RMSNormParams"] = None   # the layer's own norm in front of router and experts
 
 
 @dataclass
