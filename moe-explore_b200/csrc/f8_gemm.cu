@@ -26,10 +26,38 @@ static int launch_f8_pair(const CUtensorMap& tx, const CUtensorMap& tw, const CU
   static std::atomic<int> grids[64];
   return launch_f8<2>(f8_pair_kernel<T, OUT>, kF8Threads, F8PairPlan::kTotal, grids, s, tx, tw, to, args);
 }
-template <typename T, int OUT, int R>
+template <typename T, int OUT>
 static int launch_f8_lanes(const CUtensorMap& tx, const CUtensorMap& tw, const F8Args& args, cudaStream_t s) {
   static std::atomic<int> grids[64];
-  return launch_f8<1>(f8_lanes_kernel<T, OUT, R>, kF8Threads, F8LanesPlan<R, OUT == F8_GLU_QUANT>::kTotal, grids, s, tx, tw, args);
+  return launch_f8<1>(f8_lanes_kernel<T, OUT, false>, kF8Threads, F8LanesPlan<OUT == F8_GLU_QUANT>::kTotal, grids, s, tx, tw, args);
+}
+// One cluster of `ranks` CTAs per item.
+template <typename T>
+static int launch_f8_clusters(const CUtensorMap& tx, const CUtensorMap& tw, const F8Args& args, int items, int ranks, cudaStream_t s) {
+  const auto kernel = f8_lanes_kernel<T, F8_ROWS, true>;
+  constexpr int smem = F8LanesPlan<false>::kTotal;
+  static std::atomic<bool> prepared[64];
+  int dev = 0;
+  MOE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !prepared[dev].load(std::memory_order_acquire)) {
+    MOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev < 64) prepared[dev].store(true, std::memory_order_release);
+  }
+  PersistentLaunch l;
+  l.cfg.gridDim = dim3(static_cast<unsigned>(items * ranks), 1, 1);
+  l.cfg.blockDim = dim3(kF8Threads, 1, 1);
+  l.cfg.dynamicSmemBytes = smem;
+  l.cfg.stream = s;
+  l.attr[0].id = cudaLaunchAttributeClusterDimension;
+  l.attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
+  l.attr[0].val.clusterDim.y = 1;
+  l.attr[0].val.clusterDim.z = 1;
+  l.attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  l.attr[1].val.programmaticStreamSerializationAllowed = 1;
+  l.cfg.attrs = l.attr;
+  l.cfg.numAttrs = chained_launches() ? 2 : 1;
+  MOE_CUDA(cudaLaunchKernelEx(&l.cfg, kernel, tx, tw, args));
+  return MOE_OK;
 }
 
 // Rows [rows, K] and weights [mats, N, K] in bytes, described as pairs of bytes.
@@ -49,9 +77,20 @@ __global__ void __launch_bounds__(256) f8_zero_kernel(uint32_t* counters, int nu
   for (int i = threadIdx.x; i < num_counters; i += 256) counters[i] = 0;
 }
 
-int f8_lane_rows(int64_t routed_rows, int num_experts) {
-  const int64_t mean = routed_rows / num_experts;
-  return mean > 128 ? 0 : mean > 48 ? 128 : 64;
+// Rows per expert up to which the weights lie on the lanes.  us with the weights on the lanes / the rows, by rows per expert:
+//   64 experts of 7168 x 2048   16: 184 / 246   24: 203 / 259   32: 220 / 264   48: 336 / 274
+//   64 experts of 2048 x 1024   16:  50 /  49   24:  57 /  49   32:  64 /  50   48:  75 /  49
+//   60 experts of 2000 x 1416   16:  61 /  71   24:  69 /  69   32:  74 /  67   48:  92 /  67
+//   one matrix of 7168 x 4096   16:  XX /  34   32:  XX /  30   64:  XX /  31   96:  59 /  31
+bool f8_on_lanes(int64_t routed_rows, int num_experts) {
+  return routed_rows / num_experts <= (num_experts == 1 ? kF8LaneRows : 24);
+}
+// CTAs that share an item of one matrix: as many as leave every CTA an SM (a cluster lies within a processing cluster of 16 to 20 SMs,
+// so that some stay without) and steps enough.
+static int f8_ranks(int items, int kiters) {
+  for (int ranks = kF8MostRanks; ranks > 1; ranks /= 2)
+    if (items * ranks * 8 <= sm_count() * 7 && kiters >= ranks * kF8LeastSteps) return ranks;
+  return 1;
 }
 static int f8_workers() {
   const int n = sm_count();
@@ -98,8 +137,7 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
   a.wait_limit = wait_limit_cycles();
   a.status = p.status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int lane_rows = f8_lane_rows(p.routed_rows, p.num_experts);
-  const bool lanes = lane_rows != 0;
+  const bool lanes = f8_on_lanes(p.routed_rows, p.num_experts);
   MOE_CHECK_ARG(!lanes || (p.counters != nullptr && aligned16(p.counters)), "%s: 16-byte aligned partials are needed", name);
   a.counters = p.counters;
   a.partials = p.partials;
@@ -107,6 +145,11 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
   const int rc = f8_maps(&tx, &tw, p.x, p.x_rows, p.w, static_cast<int64_t>(p.num_experts) * (glu ? 2 : 1), p.N, p.K, lanes ? 16 : BM);
   if (rc != MOE_OK) return rc;
   const bool bf16 = p.dtype == MOE_DTYPE_BF16;
+  if (lanes && p.dense && p.kind == F8_ROWS && p.out_perm == nullptr && p.x_rows <= kF8LaneRows) {
+    const int items = (p.N + 127) / 128, ranks = f8_ranks(items, (p.K + kF8K - 1) / kF8K);
+    if (items <= sm_count())
+      return bf16 ? launch_f8_clusters<__nv_bfloat16>(tx, tw, a, items, ranks, s) : launch_f8_clusters<__half>(tx, tw, a, items, ranks, s);
+  }
   if (lanes && p.zero_counters) {
     MOE_CUDA(launch_kernel(f8_zero_kernel, 1, 256, s, p.counters, kF8MaxWorkers));
     chained_launches() = true;
@@ -123,15 +166,9 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
     if (p.kind == F8_QUANT) return launch_f8_pair<__nv_bfloat16, F8_QUANT>(tx, tw, to, a, s);
     return bf16 ? launch_f8_pair<__nv_bfloat16, F8_ROWS>(tx, tw, to, a, s) : launch_f8_pair<__half, F8_ROWS>(tx, tw, to, a, s);
   }
-#define MOE_F8_LANES(R)                                                                                              \
-  do {                                                                                                               \
-    if (p.kind == F8_GLU_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_GLU_QUANT, R>(tx, tw, a, s);                \
-    if (p.kind == F8_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_QUANT, R>(tx, tw, a, s);                        \
-    return bf16 ? launch_f8_lanes<__nv_bfloat16, F8_ROWS, R>(tx, tw, a, s) : launch_f8_lanes<__half, F8_ROWS, R>(tx, tw, a, s); \
-  } while (0)
-  if (lane_rows == 64) MOE_F8_LANES(64);
-  MOE_F8_LANES(128);
-#undef MOE_F8_LANES
+  if (p.kind == F8_GLU_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_GLU_QUANT>(tx, tw, a, s);
+  if (p.kind == F8_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_QUANT>(tx, tw, a, s);
+  return bf16 ? launch_f8_lanes<__nv_bfloat16, F8_ROWS>(tx, tw, a, s) : launch_f8_lanes<__half, F8_ROWS>(tx, tw, a, s);
 }
 
 // ---- rows to 8 bits, and their way to the experts ----
@@ -247,8 +284,8 @@ int f8_rows(const char* name, const void* x, const float* x_scales, const int32_
 }
 
 // Floats of the workers' slots.
-static size_t f8_slot_floats(int64_t routed_rows, int num_experts, bool glu) {
-  return static_cast<size_t>(2 * f8_workers()) * (glu ? 2 : 1) * f8_lane_rows(routed_rows, num_experts) * 128;
+static size_t f8_slot_floats(bool glu) {
+  return static_cast<size_t>(2 * f8_workers()) * (glu ? 2 : 1) * kF8LaneRows * 128;
 }
 
 static bool glu(int act) { return act == MOE_ACT_SWIGLU || act == MOE_ACT_GEGLU; }
@@ -279,7 +316,7 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
                               p->mtile_expert, p->tile_pairs, p->num_mtiles, p->status, p->workspace, p->workspace_bytes, false, stream));
   // counters of the two products, then the slots that both use in turn
   uint32_t* const counters = static_cast<uint32_t*>(p->partials);
-  const bool lanes = f8_lane_rows(rows, p->num_experts) != 0;
+  const bool lanes = f8_on_lanes(rows, p->num_experts);
   if (steps & MOE_F8_DISPATCH)
     MOE_STEP(f8_rows("moe_f8_expert_forward", p->x, p->x_scales, p->dst_row, p->topk, p->xs, p->xs_scales, p->num_tokens, p->d, p->dtype,
                      counters, lanes && counters != nullptr ? 2 * kF8MaxWorkers : 0, stream));
@@ -330,8 +367,8 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
 }
 
 extern "C" size_t moe_f8_partial_bytes(int64_t num_rows, int num_experts, int act) {
-  if (num_rows <= 0 || num_experts <= 0 || f8_lane_rows(num_rows, num_experts) == 0) return 0;
-  return 2 * kF8MaxWorkers * sizeof(uint32_t) + f8_slot_floats(num_rows, num_experts, glu(act)) * sizeof(float);
+  if (num_rows <= 0 || num_experts <= 0 || !f8_on_lanes(num_rows, num_experts)) return 0;
+  return 2 * kF8MaxWorkers * sizeof(uint32_t) + f8_slot_floats(glu(act)) * sizeof(float);
 }
 
 extern "C" size_t moe_f8_rows_pass_size(void) { return sizeof(moe_f8_rows_pass); }

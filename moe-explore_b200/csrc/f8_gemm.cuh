@@ -53,8 +53,8 @@ struct F8Product {
   int32_t* status;
 };
 int f8_product(const char* name, const F8Product& p, void* stream);
-// Rows per pass of the kernel with the weights on the lanes; 0: the other kernel.
-int f8_lane_rows(int64_t routed_rows, int num_experts);
+// Whether the kernel with the weights on the lanes does it.
+bool f8_on_lanes(int64_t routed_rows, int num_experts);
 
 struct F8Args {
   // The rows of the experts: maps of the padded layout, or dense_rows >= 0: one expert, rows 0 .. dense_rows - 1, no maps.
@@ -209,22 +209,32 @@ __device__ __forceinline__ void tmem_ld_wait32(uint32_t (&v)[32]) {
                :
                : "memory");
 }
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t cluster_addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
+  return v;
+}
 // An arrival in either CTA of the pair that publishes no memory (TMEM reads are ordered by the tcgen05 fence before it): a releasing
 // one would wait for the loads of the scales that are under way.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// The element-wise activation of a register row; the choice is made once per row, so that the elements interleave.
-template <int N> __device__ __forceinline__ void act_row(float (&v)[N], int act) {
+// The element-wise activation of N registers of a row; the choice is made once, so that the elements interleave.
+template <int N, int M> __device__ __forceinline__ void act_row(float (&v)[M], int act, int from = 0) {
   if (act == MOE_ACT_SILU || act == MOE_ACT_SWIGLU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = silu_f(v[i]);
+    for (int i = 0; i < N; ++i) v[from + i] = silu_f(v[from + i]);
   } else if (act == MOE_ACT_GELU || act == MOE_ACT_GEGLU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = gelu_f(v[i]);
+    for (int i = 0; i < N; ++i) v[from + i] = gelu_f(v[from + i]);
   } else if (act == MOE_ACT_GELU_TANH) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = gelu_tanh_f(v[i]);
+    for (int i = 0; i < N; ++i) v[from + i] = gelu_tanh_f(v[from + i]);
   }
 }
 // Warps: 0 producer, 1 MMA issuer, 2 and 3 none, 4 to 11 epilogue: whole warpgroups, so that the epilogue's take the registers that
@@ -334,28 +344,31 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int i = 0; ok; ++i) {
-      const F8Item c = walk.get(i, args, kCols);
-      if (!c.valid) break;
-      const int r = quad * 32 + lane;
-      const bool live = quad * 32 < c.rows;  // some of this warp's rows exist
-      const int64_t row = static_cast<int64_t>(c.a_row) + (r < c.rows ? r : c.rows > 0 ? c.rows - 1 : 0);
-      const float* xs = args.x_scales + row * kblocks;
+    F8Item c = walk.get(0, args, kCols);
+    const int r = quad * 32 + lane;
+    const float *xs = args.x_scales, *wa = args.w_scales, *wb = args.w_scales;
+    float x0 = 0.0f, a0 = 0.0f, b0 = 0.0f, x1 = 0.0f, a1 = 0.0f, b1 = 0.0f;
+    const auto begin = [&]() {  // the scales of the first two steps of item c
+      if (!c.valid || quad * 32 >= c.rows) return;
+      const int64_t row = static_cast<int64_t>(c.a_row) + (r < c.rows ? r : c.rows - 1);
+      xs = args.x_scales + row * kblocks;
       // (a tile's second block of columns may lie past the last one: its products are zeros, any scale serves)
       const int nb = kGlu ? c.n0 / kF8Block : min(c.n0 / kF8Block + half, nblocks - 1);
-      const float* wa = args.w_scales + (static_cast<int64_t>(c.expert) * (kGlu ? 2 : 1) * nblocks + nb) * kblocks;
-      const float* wb = wa + static_cast<int64_t>(nblocks) * kblocks;
-      float x0 = 0.0f, a0 = 0.0f, b0 = 0.0f, x1 = 0.0f, a1 = 0.0f, b1 = 0.0f;
-      if (live) {
-        x0 = xs[0];
-        a0 = wa[0];
-        if (kGlu) b0 = wb[0];
-        if (kiters > 1) {
-          x1 = xs[1];
-          a1 = wa[1];
-          if (kGlu) b1 = wb[1];
-        }
+      wa = args.w_scales + (static_cast<int64_t>(c.expert) * (kGlu ? 2 : 1) * nblocks + nb) * kblocks;
+      wb = wa + static_cast<int64_t>(nblocks) * kblocks;
+      x0 = xs[0];
+      a0 = wa[0];
+      if (kGlu) b0 = wb[0];
+      if (kiters > 1) {
+        x1 = xs[1];
+        a1 = wa[1];
+        if (kGlu) b1 = wb[1];
       }
+    };
+    begin();
+    F8Item next;
+    for (int i = 0; ok && c.valid; ++i, c = next) {
+      const bool live = quad * 32 < c.rows;  // some of this warp's rows exist
       float sum[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
@@ -400,6 +413,12 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         if (acc == 0) acc_phase ^= 1;
       }
       if (!ok) break;
+      // the next item's scales come while this one's results go (waiting for them then took as long as two steps)
+      const F8Item done = c;
+      next = walk.get(i + 1, args, kCols);
+      c = next;
+      begin();
+      c = done;
       if constexpr (OUT == F8_ROWS) {
         if (!live) continue;
         // 64 columns at a time through the warp's staging tile: a tensor copy where all 32 rows are this expert's own (in the padded
@@ -414,19 +433,12 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         for (int g = 0; g < 2; ++g) {
           const int col0 = c.n0 + 128 * half + 64 * g;
           if (col0 >= args.n_dim) break;
-          float f[64];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float2 p = make_float2(sum[g * 64 + 2 * j], sum[g * 64 + 2 * j + 1]);
-            f[2 * j] = p.x;
-            f[2 * j + 1] = p.y;
-          }
-          act_row(f, args.act);
+          act_row<64>(sum, args.act, g * 64);
           if (lane == 0) bulk_wait_read_all();  // the copy that last read the tile
           __syncwarp();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
-            const uint4 u = pack8<T>(f + 8 * q);
+            const uint4 u = pack8<T>(sum + g * 64 + 8 * q);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage_base + lane * 128 + ((q ^ (lane & 7)) << 4)), "r"(u.x),
                          "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
           }
@@ -459,25 +471,14 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         const int blocks = nblocks;
         float most = kF8Least;
         constexpr int kMine = kGlu ? 64 : 128;
-        float f[kMine];
         if (live) {
-#pragma unroll
-          for (int j = 0; j < kMine / 2; ++j) {
-            const float2 p = make_float2(sum[2 * j], sum[2 * j + 1]);
-            f[2 * j] = p.x;
-            f[2 * j + 1] = p.y;
-          }
-          act_row(f, args.act);
+          act_row<kMine>(sum, args.act);
           if (kGlu) {
 #pragma unroll
-            for (int j = 0; j < kMine / 2; ++j) {
-              const float2 u = make_float2(sum[64 + 2 * j], sum[64 + 2 * j + 1]);
-              f[2 * j] *= u.x;
-              f[2 * j + 1] *= u.y;
-            }
+            for (int j = 0; j < kMine; ++j) sum[j] *= sum[(64 + j) & 127];
           }
 #pragma unroll
-          for (int j = 0; j < kMine; ++j) most = fmaxf(most, fabsf(f[j]));
+          for (int j = 0; j < kMine; ++j) most = fmaxf(most, fabsf(sum[j]));
         }
         if (kGlu) {
           // two places used in turn, so that one meeting of the quadrant's warps is enough
@@ -497,10 +498,10 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
             const int col = col0 + 16 * q;
             if (col < args.n_dim)
               *reinterpret_cast<uint4*>(out + to * args.n_dim + col) =
-                  make_uint4(f8x4(f[16 * q] * inv, f[16 * q + 1] * inv, f[16 * q + 2] * inv, f[16 * q + 3] * inv),
-                             f8x4(f[16 * q + 4] * inv, f[16 * q + 5] * inv, f[16 * q + 6] * inv, f[16 * q + 7] * inv),
-                             f8x4(f[16 * q + 8] * inv, f[16 * q + 9] * inv, f[16 * q + 10] * inv, f[16 * q + 11] * inv),
-                             f8x4(f[16 * q + 12] * inv, f[16 * q + 13] * inv, f[16 * q + 14] * inv, f[16 * q + 15] * inv));
+                  make_uint4(f8x4(sum[16 * q] * inv, sum[16 * q + 1] * inv, sum[16 * q + 2] * inv, sum[16 * q + 3] * inv),
+                             f8x4(sum[16 * q + 4] * inv, sum[16 * q + 5] * inv, sum[16 * q + 6] * inv, sum[16 * q + 7] * inv),
+                             f8x4(sum[16 * q + 8] * inv, sum[16 * q + 9] * inv, sum[16 * q + 10] * inv, sum[16 * q + 11] * inv),
+                             f8x4(sum[16 * q + 12] * inv, sum[16 * q + 13] * inv, sum[16 * q + 14] * inv, sum[16 * q + 15] * inv));
           }
           if ((!kGlu || half == 0) && col0 < args.n_dim) args.out_scales[to * blocks + col0 / kF8Block] = most / kF8Top;
         }
@@ -608,12 +609,17 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
 // last.  Bound by HBM: one token through 2 of 8 experts of 4096 x 14336 has 224 and 64 items
 // for 148 SMs, which dealt out whole left half of them idle.  (All items as one run of steps, 14 in a row per worker: 1.9 GB of
 // weights at 5.0 TB/s instead of 6.0; neighbours then no longer stream neighbouring weights.)
+// A product of one matrix whose items are fewer than half the SMs is split over clusters instead (CLUSTERED): each CTA of a
+// cluster has an equal part of K of one item and leaves its sums in its shared memory, and the CTAs share out the rows of the results.
+// 64 rows of 7168 by 4096 columns: XXX us instead of 30 with slots and counters (and a launch that zeroes them).
+//
 // (An item with more than R rows takes more than one pass over its weights and is not shared: its first worker does all of it.)
 //
 // The weights of the first stages are asked for before the wait for the kernel before: that one writes the rows, while the maps
 // and counts were complete before it let this kernel up (it waited for them itself).
 // ------------------------------------------------------------------------------------------------------------------
 constexpr int kF8MaxWorkers = 256;
+constexpr int kF8MostRanks = 8;   // CTAs of a cluster that share an item
 constexpr int kF8LeastSteps = 4;  // of a worker; with fewer, what the joining costs is more than the streaming
 
 // The work of one worker, item by item.
@@ -624,12 +630,18 @@ struct F8Part {
   bool shared;
   bool valid;
 };
-struct F8Split {
+template <bool CLUSTERED> struct F8Split {
   F8Walk<1> walk;             // decodes; its lanes 0 to 15 hold items of the shared run, 16 to 31 whole ones
   int64_t begin, end, steps;  // the shared run: this worker's part of it, and all of it
   int worker, all_workers, workers, kiters, item0, items, wholes, loose;
   __device__ __forceinline__ F8Split(const F8Args& a, int worker_, int all_workers_, int kiters_)
       : walk(a, 0, 1, 128, 0), worker(worker_), all_workers(all_workers_), kiters(kiters_) {
+    if (CLUSTERED) {
+      begin = end = steps = 0;
+      workers = item0 = items = loose = 0;
+      wholes = 1;
+      return;
+    }
     wholes = walk.count / all_workers;
     loose = walk.count - wholes * all_workers;  // items of the shared run
     steps = static_cast<int64_t>(loose) * kiters;
@@ -653,6 +665,15 @@ struct F8Split {
     F8Part p;
     p.valid = i < items + wholes;
     if (!p.valid) return p;
+    if (CLUSTERED) {
+      const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+      p.item = worker / ranks;
+      p.c = walk.decode(p.item, a, 128);
+      p.kb0 = kiters * rank / ranks;
+      p.kb1 = kiters * (rank + 1) / ranks;
+      p.shared = false;
+      return p;
+    }
     const bool is_shared = i < items;
     const int j = is_shared ? i : i - items;
     if ((j & 15) == 0 && (j > 0 || items > 16)) decode(is_shared ? j : 0, is_shared ? 0 : j, a);
@@ -674,7 +695,10 @@ struct F8Split {
   __device__ __forceinline__ int worker_of(int64_t step) const { return static_cast<int>(((step + 1) * workers - 1) / steps); }
 };
 
-template <int R, bool GLU> struct F8LanesPlan {
+constexpr int kF8LaneRows = 64;  // rows per pass (128: every step costs the epilogue what two of 64 do)
+
+template <bool GLU> struct F8LanesPlan {
+  static constexpr int R = kF8LaneRows;
   static constexpr int kWBytes = (GLU ? 2 : 1) * kF8Tile;
   static constexpr int kStageBytes = kWBytes + R * kF8K;
   static constexpr int kAccCols = (GLU ? 2 : 1) * R;
@@ -690,13 +714,17 @@ template <int R, bool GLU> struct F8LanesPlan {
   static constexpr int kStages = kBudget / kStageBytes > 10 ? 10 : kBudget / kStageBytes;
   static constexpr int kTotal = kStages * kStageBytes + kExtra + kBarrierBytes + 1024;
   static_assert(kTable >= 16 * R, "scales of 16 steps at least");
+  static_assert(kAccs == 4, "sums of two steps are fetched together");
+  // split over a cluster: the sums of all rows, where the ring was
+  static_assert(R * 128 * 4 <= kStages * kStageBytes, "room for the sums");
 };
 
-template <typename T, int OUT, int R>
+template <typename T, int OUT, bool CLUSTERED>
 __global__ void __launch_bounds__(kF8Threads, 1)
 f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const F8Args args) {
   constexpr bool kGlu = OUT == F8_GLU_QUANT;
-  using Plan = F8LanesPlan<R, kGlu>;
+  constexpr int R = kF8LaneRows;
+  using Plan = F8LanesPlan<kGlu>;
   constexpr int kStages = Plan::kStages, kAccs = Plan::kAccs;
   constexpr int kMats = kGlu ? 2 : 1;
   constexpr int kChunks = R / 32;  // groups of 16 rows whose results a warp sees to
@@ -748,7 +776,7 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int kiters = (args.k_dim + kF8K - 1) / kF8K;
-  F8Split split(args, blockIdx.x, gridDim.x, kiters);
+  F8Split<CLUSTERED> split(args, blockIdx.x, gridDim.x, kiters);
 
   if (warp >= 4) {
     more_registers<72>();
@@ -835,11 +863,11 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
               break;
             }
           }
-          if (!arrived && i >= split.items && kb - base >= 8) arrive();
+          if (!CLUSTERED && !arrived && i >= split.items && kb - base >= 8) arrive();
           // Two steps at a time where there are two: a step is a chain of waits (sums there, sums fetched) of about 350 ns, which is what
           // 16 KB of weights take to arrive.
-          constexpr int kTogether = kAccs >= 4 ? 2 : 1;
-          const int together = kTogether == 2 && kb + 1 < filled && (acc & 1) == 0 ? 2 : 1;
+          constexpr int kTogether = 2;
+          const int together = kb + 1 < filled && (acc & 1) == 0 ? 2 : 1;
 #pragma unroll
           for (int t = 0; t < kTogether; ++t)
             if (t < together && ok &&
@@ -889,6 +917,18 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
           if (acc == kAccs) { acc = 0; acc_phase ^= 1; }
         }
         if (!ok) break;
+        if constexpr (CLUSTERED) {
+          // (the last products have read the ring; its memory takes the sums, [row][column])
+          float* to = reinterpret_cast<float*>(tiles) + quad * 32 + lane;
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch) {
+            const int col = 16 * (2 * ch + half);
+            if (col >= rows) continue;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) to[(col + j) * 128] = sum[0][ch][j];
+          }
+          continue;
+        }
         if (part.shared) {
           // (R rows at most: one pass)
           constexpr int kSlot = kMats * R * 128;  // floats: [matrix][four rows][lane][row of the four]
@@ -977,7 +1017,7 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
           for (int rr = warp - 4; rr < live; rr += kEpilogueWarps) {
             const float4 v = *reinterpret_cast<const float4*>(staging + rr * 128 + 4 * lane);
             float f[4] = {v.x, v.y, v.z, v.w};
-            act_row(f, args.act);
+            act_row<4>(f, args.act);
             if (kGlu) {
               const float4 u = *reinterpret_cast<const float4*>(staging + (16 + rr) * 128 + 4 * lane);
               f[0] *= u.x;
@@ -1008,6 +1048,35 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
             break;
           }
         }
+      }
+    }
+    if constexpr (CLUSTERED) {
+      __syncwarp();
+      cluster_sync_all();  // every CTA's sums are there
+      // a part of the rows for each CTA, a row per warp; the sums are added in the order of K
+      const F8Part part = split.get(0, args, R);
+      const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+      const int end = part.c.rows * (rank + 1) / ranks;
+      const int col = part.c.n0 + 4 * lane;
+#pragma unroll 1
+      for (int rr = part.c.rows * rank / ranks + warp - 4; ok && rr < end; rr += kEpilogueWarps) {
+        float4 v[kF8MostRanks];
+#pragma unroll
+        for (int w = 0; w < kF8MostRanks; ++w)
+          if (w < ranks) v[w] = ld_cluster_v4(mapa_shared(tiles_addr + (rr * 128 + 4 * lane) * 4, static_cast<uint32_t>(w)));
+        float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kF8MostRanks; ++w)
+          if (w < ranks) {
+            f[0] += v[w].x;
+            f[1] += v[w].y;
+            f[2] += v[w].z;
+            f[3] += v[w].w;
+          }
+        act_row<4>(f, args.act);
+        if (col < args.n_dim)
+          *reinterpret_cast<uint2*>(static_cast<T*>(args.out) + static_cast<int64_t>(part.c.a_row + rr) * args.n_dim + col) =
+              make_uint2(Elem<T>::pack2(f[0], f[1]), Elem<T>::pack2(f[2], f[3]));
       }
     }
   } else {
@@ -1111,10 +1180,15 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         for (int i = 0; i < 2000; ++i) __nanosleep(1000);
       }
     }
+    if constexpr (CLUSTERED) {
+      __syncwarp();
+      cluster_sync_all();
+    }
   }
 
   tc_fence_before();
   __syncthreads();
+  if constexpr (CLUSTERED) cluster_sync_all();  // no CTA ends while another reads its sums
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();

@@ -90,10 +90,57 @@ template <typename V> __device__ __forceinline__ V score_of(float x, bool sigmoi
   return exp_of(static_cast<V>(x) - static_cast<V>(top)) / sum;
 }
 
+// p as the choice in fp32 takes it: a sigmoid of the quick exponential and division.  With errors of (2 + 1.2 |x|) and 1 units of 2^-23
+// and p (1 - p) |x| < 0.23 it is off by less than 3e-7, which `slack` covers.  (A softmax adds E such errors up: it does not use them.)
+__device__ __forceinline__ float key_score(float x, bool sigmoid, float top, float sum) {
+  return sigmoid ? __fdividef(1.0f, 1.0f + __expf(-x)) : score_of<float>(x, false, top, sum);
+}
+__device__ __forceinline__ double key_score(float x, bool sigmoid, float top, double sum) { return score_of<double>(x, sigmoid, top, sum); }
+
+// The logits of a lane.
+template <typename T, int PER>
+__device__ __forceinline__ void load_logits(const TopkArgs& a, const T* row, int first, int count, float (&x)[PER]) {
+  constexpr int kVec = 16 / sizeof(T);
+  // whole 16-byte pieces where every lane's experts begin on one (its address is a multiple of per_lane = PER elements)
+  if constexpr (PER % kVec == 0) {
+    if (a.per_lane == PER && a.group_size % kVec == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && count == PER) {
+#pragma unroll
+      for (int i = 0; i < PER; i += kVec) {
+        const uint4 u = *reinterpret_cast<const uint4*>(row + first + i);
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) x[i + j] = load_elem(e + j);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] = i < count ? load_elem(row + first + i) : 0.0f;
+}
+
+// The best two of a lane's keys that come after (last, last_at) in the order of the results: value descending, index ascending.
+template <typename Key, int PER>
+__device__ __forceinline__ void best_two(const Key (&key)[PER], Key last, int last_at, Key& m1, int& i1, Key& m2, int& i2) {
+  m1 = m2 = 0;
+  i1 = i2 = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const Key k = key[i] < last || (key[i] == last && i > last_at) ? key[i] : Key(0);
+    const bool first = k > m1, second = k > m2;
+    m2 = first ? m1 : second ? k : m2;
+    i2 = first ? i1 : second ? i : i2;
+    m1 = first ? k : m1;
+    i1 = first ? i : i1;
+  }
+}
+
 // The choice: lane s < topk gets the s-th expert and its p.  False (fp32 only): two values that decide are too close to tell.
+// Each lane holds its best two; a round takes the largest of the lanes' first ones, and a lane that has given both looks through
+// its keys again (with 8 of 256 about every fourth token has such a lane; looking through them in every round made half
+// of all instructions: 31 us for 16384 tokens, now XXX).
 template <typename T, typename V, int PER>
-__device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, const float (&x)[PER], int first, int count, float top,
-                                       int& my_expert, V& my_p) {
+__device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int first, int count, float top, int& my_expert, V& my_p,
+                                       const float (&x)[PER]) {
   typedef Order<V> O;
   typedef typename O::Key Key;
   const int lane = threadIdx.x & 31;
@@ -115,33 +162,30 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, const fl
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     key[i] = 0;
-    if (i < count) key[i] = O::key(biased ? score_of<V>(x[i], sigmoid, top, sum) + static_cast<V>(a.bias[first + i]) : static_cast<V>(x[i]));
+    if (i < count) key[i] = O::key(biased ? key_score(x[i], sigmoid, top, sum) + static_cast<V>(a.bias[first + i]) : static_cast<V>(x[i]));
   }
   bool sure = true;
+  Key m1, m2;
+  int i1, i2;
+  best_two(key, ~Key(0), 0, m1, i1, m2, i2);
   if (a.keep < a.num_groups) {
-    Key m1 = 0, m2 = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const Key lower = key[i] < m1 ? key[i] : m1;
-      m2 = lower > m2 ? lower : m2;
-      m1 = key[i] > m1 ? key[i] : m1;
-    }
+    Key g1 = m1, g2 = m2;
     for (int off = (1 << a.lanes_log2) >> 1; off > 0; off >>= 1) {
-      const Key o1 = __shfl_xor_sync(kAll, m1, off), o2 = __shfl_xor_sync(kAll, m2, off);
-      const Key lower = o1 < m1 ? o1 : m1;
-      m2 = m2 > o2 ? m2 : o2;
-      m2 = lower > m2 ? lower : m2;
-      m1 = o1 > m1 ? o1 : m1;
+      const Key o1 = __shfl_xor_sync(kAll, g1, off), o2 = __shfl_xor_sync(kAll, g2, off);
+      const Key lower = o1 < g1 ? o1 : g1;
+      g2 = g2 > o2 ? g2 : o2;
+      g2 = lower > g2 ? lower : g2;
+      g1 = o1 > g1 ? o1 : g1;
     }
     const int group = lane >> a.lanes_log2;
     Key mine = 0;
     if (group < a.num_groups) {
-      V v = O::value(m1);
+      V v = O::value(g1);
       if (a.best == 2) {
-        V w = O::value(m2);
+        V w = O::value(g2);
         if (!biased) {
-          v = score_of<V>(static_cast<float>(v), sigmoid, top, sum);
-          w = score_of<V>(static_cast<float>(w), sigmoid, top, sum);
+          v = key_score(static_cast<float>(v), sigmoid, top, sum);
+          w = key_score(static_cast<float>(w), sigmoid, top, sum);
         }
         v += w;
       }
@@ -158,41 +202,62 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, const fl
       const float next = static_cast<float>(O::value(O::warp_max(open ? Key(0) : mine)));
       if (worst - next <= 4.0f * slack + 4e-7f * (fabsf(worst) + fabsf(next))) sure = false;
     }
-    if (!open) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) key[i] = 0;
-    }
+    if (!open) m1 = m2 = 0;
   }
   // k rounds of the largest value left, and one more to see how close the next one came
-  Key last = 0;
+  Key mine = 0, last = 0;  // lane s: the s-th largest
+  int left = count;
   const int rounds = kFirst && biased ? a.topk + 1 : a.topk;
   for (int s = 0; s < rounds; ++s) {
-    Key best = 0;
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (key[i] > best) {
-        best = key[i];
-        at = i;
+    last = O::warp_max(m1);
+    const int winner = __ffs(__ballot_sync(kAll, m1 == last)) - 1;
+    const int expert = __shfl_sync(kAll, first + i1, winner);
+    if (lane == s) {
+      my_expert = expert;
+      mine = last;
+    }
+    const int at = i1;
+    bool again = false;
+    if (lane == winner && last != 0) {
+      m1 = m2;
+      i1 = i2;
+      m2 = 0;
+      again = --left > 0 && m1 == 0;
+    }
+    if (__any_sync(kAll, again)) {
+      Key n1, n2;
+      int j1, j2;
+      best_two(key, last, at, n1, j1, n2, j2);
+      if (again) {
+        m1 = n1;
+        m2 = n2;
+        i1 = j1;
+        i2 = j2;
       }
-    const Key m = O::warp_max(best);
-    const int winner = __ffs(__ballot_sync(kAll, best == m)) - 1;
-    const int expert = __shfl_sync(kAll, first + at, winner);
-    if (lane == winner) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i == at) key[i] = 0;
     }
-    if (kFirst && biased && s > 0) {
-      const float above = static_cast<float>(O::value(last)), below = static_cast<float>(O::value(m));
-      if (m != 0 && above - below <= 2.0f * slack + 1.2e-7f * (fabsf(above) + fabsf(below))) sure = false;
-    }
-    last = m;
-    if (lane == s && s < a.topk) my_expert = expert;
+  }
+  if (kFirst && biased) {
+    Key next = __shfl_down_sync(kAll, mine, 1);
+    if (lane == a.topk - 1) next = last;
+    const float above = static_cast<float>(O::value(mine)), below = static_cast<float>(O::value(next));
+    const bool close = lane < a.topk && next != 0 && above - below <= 2.0f * slack + 1.2e-7f * (fabsf(above) + fabsf(below));
+    sure = sure && !__any_sync(kAll, close);
   }
   my_p = V(0);
   if (lane < a.topk) my_p = score_of<V>(load_elem(row + my_expert), sigmoid, top, sum);
   return sure;
+}
+
+// The rare token again, in 64 bits; a function of its own, so that its registers are not everyone's.
+template <typename T, int PER>
+__device__ __noinline__ double choose_exactly(const TopkArgs& a, const T* row, int first, int count, float top, int* expert) {
+  float x[PER];
+  load_logits<T, PER>(a, row, first, count, x);
+  double p;
+  int e = 0;
+  choose<T, double, PER>(a, row, first, count, top, e, p, x);
+  *expert = e;
+  return p;
 }
 
 template <typename V>
@@ -209,7 +274,7 @@ __device__ __forceinline__ void store_weight(const TopkArgs& a, int64_t token, i
 }
 
 template <typename T, int PER>
-__global__ void __launch_bounds__(kTopkWarps * 32) grouped_topk_kernel(const TopkArgs a) {
+__global__ void __launch_bounds__(kTopkWarps * 32) grouped_topk_kernel(const __grid_constant__ TopkArgs a) {
   const int64_t token = static_cast<int64_t>(blockIdx.x) * kTopkWarps + (threadIdx.x >> 5);
   if (token >= a.num_tokens) return;
   const int lane = threadIdx.x & 31;
@@ -220,23 +285,7 @@ __global__ void __launch_bounds__(kTopkWarps * 32) grouped_topk_kernel(const Top
   const int count = left < 0 ? 0 : left < a.per_lane ? left : a.per_lane;
   const int first = count > 0 ? group * a.group_size + member : 0;
   float x[PER];
-  constexpr int kVec = 16 / sizeof(T);
-  // whole 16-byte pieces where every lane's experts begin on one (its address is a multiple of per_lane = PER elements)
-  const bool pieces = PER % kVec == 0 && a.per_lane == PER && a.group_size % kVec == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
-  if (pieces && count == PER) {
-    if constexpr (PER % kVec == 0) {
-#pragma unroll
-      for (int i = 0; i < PER; i += kVec) {
-        const uint4 u = *reinterpret_cast<const uint4*>(row + first + i);
-        const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) x[i + j] = load_elem(e + j);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = i < count ? load_elem(row + first + i) : 0.0f;
-  }
+  load_logits<T, PER>(a, row, first, count, x);
   float top = 0.0f;
   if (!a.sigmoid) {
     top = -CUDART_INF_F;
@@ -248,12 +297,12 @@ __global__ void __launch_bounds__(kTopkWarps * 32) grouped_topk_kernel(const Top
   }
   int expert = 0;
   float p;
-  if (choose<T, float, PER>(a, row, x, first, count, top, expert, p)) {
+  if (choose<T, float, PER>(a, row, first, count, top, expert, p, x)) {
     store_weight(a, token, expert, p);
   } else {
-    double q;
-    choose<T, double, PER>(a, row, x, first, count, top, expert, q);
-    store_weight(a, token, expert, q);
+    int exact = 0;
+    const double q = choose_exactly<T, PER>(a, row, first, count, top, &exact);
+    store_weight(a, token, exact, q);
   }
 }
 

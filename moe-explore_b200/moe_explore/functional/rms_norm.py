@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 
 from moe_explore import _native
-from moe_explore.functional.fp8 import BLOCK, Fp8Rows
+from moe_explore.functional.fp8 import BLOCK, DTYPE, Fp8Rows
 
 
 def _checked(x, weight, residual):
@@ -23,6 +23,8 @@ def _checked(x, weight, residual):
 
 def _rows(x):
     """[..., d] as rows [R, d] that the kernels can read: dense columns, 16-byte aligned rows."""
+    if x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x   # (a multiple of 8 columns is checked behind)
     x = x.reshape(-1, x.size(-1))
     if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.data_ptr() % 16 != 0:
         x = x.clone(memory_format=torch.contiguous_format)
@@ -34,21 +36,29 @@ def _aligned(weight):
     return weight if weight.data_ptr() % 16 == 0 else weight.clone()
 
 
+def _forward(x, weight, residual, eps, with_rstd):
+    """(y, h or None, 1 / root mean square of the rows or None)"""
+    rows = _rows(x)
+    y = torch.empty(rows.shape, dtype=x.dtype, device=x.device)
+    h = None if residual is None else torch.empty_like(y)
+    rstd = torch.empty(rows.size(0), dtype=torch.float32, device=x.device) if with_rstd else None
+    _native.rms_norm(rows, None if residual is None else _rows(residual), _aligned(weight), eps, h=h, y=y, rstd=rstd)
+    return _like(y, x), None if h is None else _like(h, x), rstd
+
+
+def _like(rows, x):
+    return rows if x.dim() == 2 else rows.view(x.shape)
+
+
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        rows, w = _rows(x), _aligned(weight)
-        y = torch.empty(rows.shape, dtype=x.dtype, device=x.device)
-        h = None if residual is None else torch.empty_like(y)
-        rstd = torch.empty(rows.size(0), dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
-        _native.rms_norm(rows, None if residual is None else _rows(residual), w, eps, h=h, y=y, rstd=rstd)
+        y, h, rstd = _forward(x, weight, residual, eps, any(ctx.needs_input_grad))
         ctx.set_materialize_grads(False)
-        ctx.shape, ctx.has_residual = x.shape, residual is not None
-        y = y.view(x.shape)
+        ctx.has_residual = residual is not None
         if residual is None:
             ctx.save_for_backward(x, weight, rstd)
             return y
-        h = h.view(x.shape)
         ctx.save_for_backward(h, weight, rstd)
         return y, h
 
@@ -58,9 +68,10 @@ class _RMSNorm(torch.autograd.Function):
         h, weight, rstd = ctx.saved_tensors
         if dy is None:   # only the sum was used
             return dh, None, dh if ctx.has_residual else None, None
-        dx, dw = _native.rms_norm_backward(_rows(dy).contiguous(), None if dh is None else _rows(dh).contiguous(), _rows(h),
-                                           _aligned(weight), rstd)
-        dx = dx.view(ctx.shape)
+        with _native.on_device_of(h):
+            dx, dw = _native.rms_norm_backward(_rows(dy).contiguous(), None if dh is None else _rows(dh).contiguous(), _rows(h),
+                                               _aligned(weight), rstd)
+        dx = _like(dx, h)
         return dx, dw, dx if ctx.has_residual else None, None
 
 
@@ -69,6 +80,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     all three; d a multiple of 8."""
     _checked(x, weight, residual)
     with _native.on_device_of(x):
+        if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or residual is not None and residual.requires_grad)):
+            y, h, _ = _forward(x, weight, residual, float(eps), False)
+            return y if residual is None else (y, h)
         return _RMSNorm.apply(x, weight, residual, float(eps))
 
 
@@ -82,12 +96,13 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     if d % 16 != 0:
         raise ValueError(f"8-bit rows have a multiple of 16 columns, got {d}")
     with _native.on_device_of(x):
-        rows = _rows(x.detach())
-        new = lambda dtype, cols: torch.empty(rows.size(0), cols, dtype=dtype, device=x.device)
-        q, scales = new(torch.float8_e4m3fn, d), new(torch.float32, -(-d // BLOCK))
-        y = new(x.dtype, d) if with_rows else None
-        h = new(x.dtype, d) if residual is not None else None
-        _native.rms_norm(rows, None if residual is None else _rows(residual.detach()), _aligned(weight.detach()), float(eps), h=h, y=y,
-                         q=q, scales=scales)
-    out = (Fp8Rows(q, scales, x.dtype),) + (() if y is None else (y.view(x.shape),)) + (() if h is None else (h.view(x.shape),))
-    return out if len(out) > 1 else out[0]
+        rows = _rows(x)
+        num_rows, device = rows.size(0), x.device
+        q = torch.empty(num_rows, d, dtype=DTYPE, device=device)
+        scales = torch.empty(num_rows, -(-d // BLOCK), dtype=torch.float32, device=device)
+        y = torch.empty(num_rows, d, dtype=x.dtype, device=device) if with_rows else None
+        h = torch.empty(num_rows, d, dtype=x.dtype, device=device) if residual is not None else None
+        _native.rms_norm(rows, None if residual is None else _rows(residual), _aligned(weight), float(eps), h=h, y=y, q=q, scales=scales)
+    if y is None and h is None:
+        return Fp8Rows(q, scales, x.dtype)
+    return (Fp8Rows(q, scales, x.dtype), *(_like(t, x) for t in (y, h) if t is not None))

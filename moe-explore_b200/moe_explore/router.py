@@ -146,16 +146,20 @@ def ernie_router(input: torch.Tensor, router_params: ErnieRouterParams):
         return picked.to(input.dtype), indices
 
 
+def _grouped_topk(logits, bias, p: GroupedTopkRouterParams, dtype):
+    best = p.group_best if p.num_groups > 1 else 1   # one group has no rank
+    return _native.grouped_topk(logits, bias, p.num_groups, p.topk_groups, best, p.topk, p.score_function == "sigmoid",
+                                bool(p.normalize_routing), float(p.scale), dtype)
+
+
 class _GroupedTopk(torch.autograd.Function):
     """scores, indices of ``logits``; differentiable with respect to the logits, given the selection."""
 
     @staticmethod
     def forward(ctx, logits, bias, p, dtype):
-        sigmoid = p.score_function == "sigmoid"
-        scores, indices = _native.grouped_topk(logits, bias, p.num_groups, p.topk_groups, _group_best(p), p.topk, sigmoid,
-                                               bool(p.normalize_routing), float(p.scale), dtype)
+        scores, indices = _grouped_topk(logits, bias, p, dtype)
         ctx.save_for_backward(logits, indices)
-        ctx.cfg = (sigmoid, bool(p.normalize_routing), float(p.scale))
+        ctx.cfg = (p.score_function == "sigmoid", bool(p.normalize_routing), float(p.scale))
         ctx.mark_non_differentiable(indices)
         return scores, indices
 
@@ -164,10 +168,6 @@ class _GroupedTopk(torch.autograd.Function):
     def backward(ctx, d_scores, _d_indices):
         logits, indices = ctx.saved_tensors
         return _native.grouped_topk_backward(logits, indices, d_scores.contiguous(), *ctx.cfg), None, None, None
-
-
-def _group_best(p: GroupedTopkRouterParams) -> int:
-    return p.group_best if p.num_groups > 1 else 1   # one group has no rank
 
 
 def grouped_topk_of_logits(logits: torch.Tensor, params: GroupedTopkRouterParams, dtype: torch.dtype = None):
@@ -186,6 +186,8 @@ def grouped_topk_of_logits(logits: torch.Tensor, params: GroupedTopkRouterParams
             raise ValueError("bias is fp32 [experts] on the device of the logits")
         bias = bias.detach().contiguous()
     with _native.on_device_of(logits):
+        if not (logits.requires_grad and torch.is_grad_enabled()):
+            return _grouped_topk(logits.contiguous(), bias, params, dtype)
         return _GroupedTopk.apply(logits.contiguous(), bias, params, dtype)
 
 
