@@ -10,7 +10,7 @@
 // lane, then the lowest register".
 //
 // THE CHOICE IS THAT OF EXACT ARITHMETIC.  Values whose fp32 images are closer than what the evaluation in fp32 can be off by
-// are decided again in 64 bits, by the warp that met them (about one token in 500 for 256 sigmoid scores with a bias): indices then
+// are decided again in 64 bits, by the warp that met them (about one token in 1500 for 256 sigmoid scores with a bias): indices then
 // depend neither on the order of a softmax's sum nor on the exponential's last bit.  Without a bias the logits
 // themselves are compared (p grows with l), and only sums over two members of a group can be that close.
 // Ties go to the lowest index, the k results come in descending order, NaN is taken after everything else.
@@ -90,20 +90,22 @@ template <typename V> __device__ __forceinline__ V score_of(float x, bool sigmoi
   return exp_of(static_cast<V>(x) - static_cast<V>(top)) / sum;
 }
 
-// p as the choice in fp32 takes it: a sigmoid of the quick exponential and division.  With errors of (2 + 1.2 |x|) and 1 units of 2^-23
-// and p (1 - p) |x| < 0.23 it is off by less than 3e-7, which `slack` covers.  (A softmax adds E such errors up: it does not use them.)
+// p as the choice in fp32 takes it: a sigmoid of the quick exponential and division.  Their errors are 2 + 1.2 |x| and 2 units of 2^-23,
+// that of the sum half a unit; the first counts with p (1 - p), and p (1 - p) (2 + 1.2 |x|) < 0.65: off by less than
+// (0.65 + 2.5) 2^-23 < 3.8e-7.  (A softmax would add E such errors up: it does not use them.)
+constexpr float kSigmoidSlack = 4e-7f;
 __device__ __forceinline__ float key_score(float x, bool sigmoid, float top, float sum) {
   return sigmoid ? __fdividef(1.0f, 1.0f + __expf(-x)) : score_of<float>(x, false, top, sum);
 }
 __device__ __forceinline__ double key_score(float x, bool sigmoid, float top, double sum) { return score_of<double>(x, sigmoid, top, sum); }
 
-// The logits of a lane.
+// The logits (or biases) of a lane.
 template <typename T, int PER>
 __device__ __forceinline__ void load_logits(const TopkArgs& a, const T* row, int first, int count, float (&x)[PER]) {
   constexpr int kVec = 16 / sizeof(T);
-  // whole 16-byte pieces where every lane's experts begin on one (its address is a multiple of per_lane = PER elements)
+  // whole 16-byte pieces where every lane's experts begin on one (a multiple of per_lane = PER elements from the row's beginning)
   if constexpr (PER % kVec == 0) {
-    if (a.per_lane == PER && a.group_size % kVec == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && count == PER) {
+    if (a.per_lane == PER && a.group_size % kVec == 0 && (reinterpret_cast<uintptr_t>(row) & 15) == 0 && count == PER) {
 #pragma unroll
       for (int i = 0; i < PER; i += kVec) {
         const uint4 u = *reinterpret_cast<const uint4*>(row + first + i);
@@ -136,11 +138,10 @@ __device__ __forceinline__ void best_two(const Key (&key)[PER], Key last, int la
 
 // The choice: lane s < topk gets the s-th expert and its p.  False (fp32 only): two values that decide are too close to tell.
 // Each lane holds its best two; a round takes the largest of the lanes' first ones, and a lane that has given both looks through
-// its keys again (with 8 of 256 about every fourth token has such a lane; looking through them in every round made half
-// of all instructions: 31 us for 16384 tokens, now XXX).
+// its keys again (with 8 of 256 about every fourth token has such a lane).
 template <typename T, typename V, int PER>
 __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int first, int count, float top, int& my_expert, V& my_p,
-                                       const float (&x)[PER]) {
+                                       const float (&x)[PER], int* taken) {
   typedef Order<V> O;
   typedef typename O::Key Key;
   const int lane = threadIdx.x & 31;
@@ -157,12 +158,16 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
   // how far p in fp32 may be off: exp, sum and division at a few units each, the sum of the softmax by one more per addition, and
   // the rounding of l - max, whose effect on p is largest (1/e) where l - max is -1
   const float p_top = sigmoid ? 1.0f : 1.0f / static_cast<float>(sum);
-  const float slack = p_top * (8e-7f + 1.2e-7f * PER) + 3e-8f;
+  const float slack = sigmoid ? kSigmoidSlack : p_top * (8e-7f + 1.2e-7f * PER) + 3e-8f;
   Key key[PER];
+  if (biased) {
+    float b[PER];
+    load_logits<float, PER>(a, a.bias, first, count, b);
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    key[i] = 0;
-    if (i < count) key[i] = O::key(biased ? key_score(x[i], sigmoid, top, sum) + static_cast<V>(a.bias[first + i]) : static_cast<V>(x[i]));
+    for (int i = 0; i < PER; ++i) key[i] = i < count ? O::key(key_score(x[i], sigmoid, top, sum) + static_cast<V>(b[i])) : Key(0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = i < count ? O::key(static_cast<V>(x[i])) : Key(0);
   }
   bool sure = true;
   Key m1, m2;
@@ -191,11 +196,15 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
       }
       mine = O::key(v);
     }
+    // groups before this one; the comparisons are shared out to its lanes
     int rank = 0;
-    for (int g = 0; g < a.num_groups; ++g) {
+    const int lanes = 1 << a.lanes_log2;
+    for (int g0 = 0; g0 < a.num_groups; g0 += lanes) {
+      const int g = g0 + (lane & (lanes - 1));
       const Key other = __shfl_sync(kAll, mine, g << a.lanes_log2);
-      rank += other > mine || (other == mine && g < group);
+      rank += g < a.num_groups && (other > mine || (other == mine && g < group));
     }
+    for (int off = lanes >> 1; off > 0; off >>= 1) rank += __shfl_xor_sync(kAll, rank, off);
     const bool open = group < a.num_groups && rank < a.keep;
     if (kFirst && (biased || a.best == 2)) {
       const float worst = static_cast<float>(O::value(O::warp_min(open ? mine : ~Key(0))));
@@ -207,22 +216,20 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
   // k rounds of the largest value left, and one more to see how close the next one came
   Key mine = 0, last = 0;  // lane s: the s-th largest
   int left = count;
+  const unsigned before = (1u << lane) - 1u;
   const int rounds = kFirst && biased ? a.topk + 1 : a.topk;
   for (int s = 0; s < rounds; ++s) {
     last = O::warp_max(m1);
-    const int winner = __ffs(__ballot_sync(kAll, m1 == last)) - 1;
-    const int expert = __shfl_sync(kAll, first + i1, winner);
-    if (lane == s) {
-      my_expert = expert;
-      mine = last;
-    }
+    const unsigned equal = __ballot_sync(kAll, m1 == last);
+    if (lane == s) mine = last;
     const int at = i1;
     bool again = false;
-    if (lane == winner && last != 0) {
+    if (m1 == last && (equal & before) == 0) {  // the first lane that has it
+      if (s < a.topk) taken[s] = first + i1;
       m1 = m2;
       i1 = i2;
       m2 = 0;
-      again = --left > 0 && m1 == 0;
+      again = --left > 0 && m1 == 0 && last != 0;
     }
     if (__any_sync(kAll, again)) {
       Key n1, n2;
@@ -236,6 +243,9 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
       }
     }
   }
+  __syncwarp();
+  if (lane < a.topk) my_expert = taken[lane];
+  __syncwarp();  // (it is written again by the choice in 64 bits)
   if (kFirst && biased) {
     Key next = __shfl_down_sync(kAll, mine, 1);
     if (lane == a.topk - 1) next = last;
@@ -250,12 +260,13 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
 
 // The rare token again, in 64 bits; a function of its own, so that its registers are not everyone's.
 template <typename T, int PER>
-__device__ __noinline__ double choose_exactly(const TopkArgs& a, const T* row, int first, int count, float top, int* expert) {
+__device__ __noinline__ double choose_exactly(const TopkArgs& a, const T* row, int first, int count, float top, int* expert,
+                                              int* taken) {
   float x[PER];
   load_logits<T, PER>(a, row, first, count, x);
   double p;
   int e = 0;
-  choose<T, double, PER>(a, row, first, count, top, e, p, x);
+  choose<T, double, PER>(a, row, first, count, top, e, p, x, taken);
   *expert = e;
   return p;
 }
@@ -275,9 +286,11 @@ __device__ __forceinline__ void store_weight(const TopkArgs& a, int64_t token, i
 
 template <typename T, int PER>
 __global__ void __launch_bounds__(kTopkWarps * 32) grouped_topk_kernel(const __grid_constant__ TopkArgs a) {
+  __shared__ int all_taken[kTopkWarps][32];
   const int64_t token = static_cast<int64_t>(blockIdx.x) * kTopkWarps + (threadIdx.x >> 5);
   if (token >= a.num_tokens) return;
   const int lane = threadIdx.x & 31;
+  int* taken = all_taken[threadIdx.x >> 5];
   const T* row = static_cast<const T*>(a.logits) + token * a.num_experts;
   const int group = lane >> a.lanes_log2;
   const int member = (lane & ((1 << a.lanes_log2) - 1)) * a.per_lane;
@@ -297,11 +310,11 @@ __global__ void __launch_bounds__(kTopkWarps * 32) grouped_topk_kernel(const __g
   }
   int expert = 0;
   float p;
-  if (choose<T, float, PER>(a, row, first, count, top, expert, p, x)) {
+  if (choose<T, float, PER>(a, row, first, count, top, expert, p, x, taken)) {
     store_weight(a, token, expert, p);
   } else {
     int exact = 0;
-    const double q = choose_exactly<T, PER>(a, row, first, count, top, &exact);
+    const double q = choose_exactly<T, PER>(a, row, first, count, top, &exact, taken);
     store_weight(a, token, exact, q);
   }
 }
