@@ -221,11 +221,18 @@ f8_rows_kernel(const T* x, const float* scales_in, const int32_t* dst_row, int c
       scale = live ? scales_in[t * blocks + b] : 0.0f;
     }
     if (!live) continue;
-    for (int s = 0; s < copies; ++s) {
-      const int64_t to = dst_row != nullptr ? dst_row[t * copies + s] : t;
-      if (to < 0) continue;
-      if (ok) out[to * vecs + v] = q;
-      if (lane16 == 0) scales[to * blocks + b] = scale;
+    // the rows it goes to, one per lane: asked for at once (one after the other their loads took as long as the copies)
+    const unsigned group = 0xFFFFu << (threadIdx.x & 16);
+    for (int s0 = 0; s0 < copies; s0 += 16) {
+      const int mine = dst_row == nullptr ? static_cast<int>(t) : s0 + lane16 < copies ? dst_row[t * copies + s0 + lane16] : -1;
+      const int some = min(copies - s0, 16);
+#pragma unroll 4
+      for (int s = 0; s < some; ++s) {
+        const int64_t to = __shfl_sync(group, mine, s, 16);
+        if (to < 0) continue;
+        if (ok) out[to * vecs + v] = q;
+        if (lane16 == 0) scales[to * blocks + b] = scale;
+      }
     }
   }
 }

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBa
     if (v < vecs) load_weight8<W>(static_cast<const W*>(a.weight), v * kNormVec, w[i]);
   }
   const uint4* dy = static_cast<const uint4*>(a.dy);
-  uint4 uy[VECS], uh[VECS];
+  uint4 uy[VECS], uh[VECS], ud[VECS];
   const auto load = [&](int64_t row) {
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBa
       const bool ok = v < vecs;
       uy[i] = ok ? dy[row * vecs + v] : make_uint4(0, 0, 0, 0);
       uh[i] = ok ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.h) + row * a.h_stride)[v] : make_uint4(0, 0, 0, 0);
+      ud[i] = ok && a.dh != nullptr ? static_cast<const uint4*>(a.dh)[row * vecs + v] : make_uint4(0, 0, 0, 0);
     }
   };
   int64_t row = blockIdx.x;
@@ -180,10 +181,9 @@ __global__ void __launch_bounds__(THREADS) rms_norm_backward_kernel(const NormBa
     uint4 cy[VECS], ch[VECS], cr[VECS];
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
-      const int v = i * THREADS + tid;
       cy[i] = uy[i];
       ch[i] = uh[i];
-      cr[i] = a.dh != nullptr && v < vecs ? static_cast<const uint4*>(a.dh)[row * vecs + v] : make_uint4(0, 0, 0, 0);
+      cr[i] = ud[i];
     }
     const float r = a.rstd[row];
     if (row + gridDim.x < a.rows) load(row + gridDim.x);
