@@ -185,53 +185,70 @@ template <typename T> __device__ __forceinline__ void to_floats(const uint4& u, 
 }
 
 // T: a 16-bit type (rows are converted) or uint8_t (8-bit rows with `scales_in` are copied).
+// A warp takes two blocks of a row at a time, so that the row and where it goes are the whole warp's; the next ones are on their way
+// meanwhile.  Bound by instructions rather than by HBM: everything that counts is 32 bits wide (the host keeps rows x blocks below
+// 2^31) and advances by additions.
+constexpr int kF8RowsCtas = 6;  // per SM
 template <typename T>
-__global__ void __launch_bounds__(256)
-f8_rows_kernel(const T* x, const float* scales_in, const int32_t* dst_row, int copies, uint2* out, float* scales, int64_t rows, int cols,
+__global__ void __launch_bounds__(256, kF8RowsCtas)
+f8_rows_kernel(const T* x, const float* scales_in, const int32_t* dst_row, int copies, uint2* out, float* scales, int rows, int cols,
                uint32_t* counters, int num_counters) {
   await_predecessor();  // before the release: what comes up next reads the routing metadata
   grid_release();
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < num_counters; i += 256) counters[i] = 0;
   const int blocks = (cols + kF8Block - 1) / kF8Block;
+  const int pairs = (blocks + 1) / 2;
   const int vecs = cols / 8;
-  const int lane16 = threadIdx.x & 15;
-  const int64_t total = rows * blocks;
-  // (a warp's two groups stay together: the block maximum is exchanged between 16 lanes of a whole warp)
-  for (int64_t g0 = (static_cast<int64_t>(blockIdx.x) * 256 + (threadIdx.x & ~31)) / 16; g0 < total; g0 += static_cast<int64_t>(gridDim.x) * 16) {
-    const int64_t g = g0 + ((threadIdx.x >> 4) & 1);
-    const bool live = g < total;
-    const int64_t t = live ? g / blocks : 0;
-    const int b = live ? static_cast<int>(g - t * blocks) : 0;
-    const int v = b * 16 + lane16;
-    const bool ok = live && v < vecs;
-    uint2 q = make_uint2(0, 0);
+  const int lane = threadIdx.x & 31;
+  const int stride = static_cast<int>(gridDim.x) * 8;
+  const int stride_rows = stride / pairs, stride_pairs = stride - stride_rows * pairs;
+  const int first = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  int row = first / pairs, pair = first - row * pairs;
+  typedef typename std::conditional<sizeof(T) == 2, uint4, uint2>::type Piece;
+  const auto load = [&](int r, int v) {
+    return r < rows && v < vecs ? reinterpret_cast<const Piece*>(x)[static_cast<int64_t>(r) * vecs + v] : Piece{};
+  };
+  Piece next = load(row, pair * 32 + lane);
+  while (row < rows) {
+    const Piece u = next;
+    const int this_row = row, v = pair * 32 + lane;
+    row += stride_rows;
+    if ((pair += stride_pairs) >= pairs) {
+      pair -= pairs;
+      ++row;
+    }
+    next = load(row, pair * 32 + lane);
+    const int block = v >> 4;
+    const bool ok = v < vecs, has_scale = (lane & 15) == 0 && block < blocks;
+    uint2 q;
     float scale;
     if constexpr (sizeof(T) == 2) {
-      const uint4 u = ok ? reinterpret_cast<const uint4*>(x)[t * vecs + v] : make_uint4(0, 0, 0, 0);
       float f[8];
       to_floats<T>(u, f);
       const float most = block_most(f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = f8_exact(f[i], most);
+      f8_quotients(f, most);
       q = make_uint2(f8x4(f[0], f[1], f[2], f[3]), f8x4(f[4], f[5], f[6], f[7]));
       scale = most / kF8Top;
     } else {
-      if (ok) q = reinterpret_cast<const uint2*>(x)[t * vecs + v];
-      scale = live ? scales_in[t * blocks + b] : 0.0f;
+      q = u;
+      scale = has_scale ? scales_in[static_cast<int64_t>(this_row) * blocks + block] : 0.0f;
     }
-    if (!live) continue;
-    // the rows it goes to, one per lane: asked for at once (one after the other their loads took as long as the copies)
-    const unsigned group = 0xFFFFu << (threadIdx.x & 16);
-    for (int s0 = 0; s0 < copies; s0 += 16) {
-      const int mine = dst_row == nullptr ? static_cast<int>(t) : s0 + lane16 < copies ? dst_row[t * copies + s0 + lane16] : -1;
-      const int some = min(copies - s0, 16);
-#pragma unroll 4
+    const auto put = [&](int to) {
+      if (ok) out[static_cast<int64_t>(to) * vecs + v] = q;
+      if (has_scale) scales[static_cast<int64_t>(to) * blocks + block] = scale;
+    };
+    if (dst_row == nullptr) {
+      put(this_row);
+      continue;
+    }
+    // the rows it goes to, one per lane: asked for at once
+    for (int s0 = 0; s0 < copies; s0 += 32) {
+      const int mine = s0 + lane < copies ? dst_row[static_cast<int64_t>(this_row) * copies + s0 + lane] : -1;
+      const int some = min(copies - s0, 32);
       for (int s = 0; s < some; ++s) {
-        const int64_t to = __shfl_sync(group, mine, s, 16);
-        if (to < 0) continue;
-        if (ok) out[to * vecs + v] = q;
-        if (lane16 == 0) scales[to * blocks + b] = scale;
+        const int to = __shfl_sync(0xFFFFFFFFu, mine, s);
+        if (to >= 0) put(to);
       }
     }
   }
@@ -260,7 +277,7 @@ f8_gather_kernel(const uint2* x, const float* scales_in, const int64_t* index, i
 
 static int f8_row_grid(int64_t rows, int cols) {
   const int64_t want = (rows * ((cols + kF8Block - 1) / kF8Block) + 15) / 16;
-  const int64_t most = 8ll * sm_count();
+  const int64_t most = static_cast<int64_t>(kF8RowsCtas) * sm_count();
   return static_cast<int>(want < most ? want : most);
 }
 
@@ -272,20 +289,24 @@ int f8_rows(const char* name, const void* x, const float* x_scales, const int32_
     return MOE_ERR_UNSUPPORTED;
   }
   if (rows == 0) return MOE_OK;
+  if (rows * ((cols + kF8Block - 1) / kF8Block) > 0x7FFFFFFF - kF8RowsCtas * 16ll * sm_count()) {
+    set_error("%s: at most 2^31 blocks of 128 columns are supported, got %lld rows of %d", name, static_cast<long long>(rows), cols);
+    return MOE_ERR_UNSUPPORTED;
+  }
   MOE_CHECK_ARG(x && out && scales, "%s: null pointer argument", name);
   MOE_CHECK_ARG(aligned16(x) && aligned16(out), "%s: pointers must be 16-byte aligned", name);
   MOE_CHECK_ARG(x_scales != nullptr || dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16, "%s: unknown dtype %d", name, dtype);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int grid = f8_row_grid(rows, cols);
+  const int grid = f8_row_grid(rows, cols);  // (16 blocks of 128 columns per CTA)
   uint2* o = static_cast<uint2*>(out);
   if (x_scales != nullptr)
-    MOE_CUDA(launch_kernel(f8_rows_kernel<uint8_t>, grid, 256, s, static_cast<const uint8_t*>(x), x_scales, dst_row, copies, o, scales, rows, cols,
+    MOE_CUDA(launch_kernel(f8_rows_kernel<uint8_t>, grid, 256, s, static_cast<const uint8_t*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols,
                            counters, num_counters));
   else if (dtype == MOE_DTYPE_BF16)
-    MOE_CUDA(launch_kernel(f8_rows_kernel<__nv_bfloat16>, grid, 256, s, static_cast<const __nv_bfloat16*>(x), x_scales, dst_row, copies, o, scales, rows, cols,
+    MOE_CUDA(launch_kernel(f8_rows_kernel<__nv_bfloat16>, grid, 256, s, static_cast<const __nv_bfloat16*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols,
                            counters, num_counters));
   else
-    MOE_CUDA(launch_kernel(f8_rows_kernel<__half>, grid, 256, s, static_cast<const __half*>(x), x_scales, dst_row, copies, o, scales, rows, cols,
+    MOE_CUDA(launch_kernel(f8_rows_kernel<__half>, grid, 256, s, static_cast<const __half*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols,
                            counters, num_counters));
   return MOE_OK;
 }

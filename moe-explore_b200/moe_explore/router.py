@@ -161,11 +161,14 @@ class _GroupedTopk(torch.autograd.Function):
         ctx.save_for_backward(logits, indices)
         ctx.cfg = (p.score_function == "sigmoid", bool(p.normalize_routing), float(p.scale))
         ctx.mark_non_differentiable(indices)
+        ctx.set_materialize_grads(False)   # (or zeros are made for the indices)
         return scores, indices
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_scores, _d_indices):
+        if d_scores is None:
+            return None, None, None, None
         logits, indices = ctx.saved_tensors
         return _native.grouped_topk_backward(logits, indices, d_scores.contiguous(), *ctx.cfg), None, None, None
 
