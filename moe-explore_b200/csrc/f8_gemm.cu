@@ -21,10 +21,14 @@ static int launch_f8(Kernel kernel, int threads, int smem, std::atomic<int> (&gr
   return MOE_OK;
 }
 
-template <typename T, int OUT>
-static int launch_f8_pair(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& to, const F8Args& args, cudaStream_t s) {
+template <typename T, int OUT, int CTAS>
+static int launch_f8_wide_on(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& to, const F8Args& args, cudaStream_t s) {
   static std::atomic<int> grids[64];
-  return launch_f8<2>(f8_pair_kernel<T, OUT>, kF8Threads, F8PairPlan::kTotal, grids, s, tx, tw, to, args);
+  return launch_f8<CTAS>(f8_wide_kernel<T, OUT, CTAS>, kF8Threads, F8WidePlan<CTAS>::kTotal, grids, s, tx, tw, to, args);
+}
+template <typename T, int OUT>
+static int launch_f8_wide(bool pairs, const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& to, const F8Args& args, cudaStream_t s) {
+  return pairs ? launch_f8_wide_on<T, OUT, 2>(tx, tw, to, args, s) : launch_f8_wide_on<T, OUT, 1>(tx, tw, to, args, s);
 }
 template <typename T, int OUT>
 static int launch_f8_lanes(const CUtensorMap& tx, const CUtensorMap& tw, const F8Args& args, cudaStream_t s) {
@@ -92,6 +96,9 @@ static int f8_ranks(int items, int kiters) {
     if (items * ranks * 8 <= sm_count() * 7 && kiters >= ranks * kF8LeastSteps) return ranks;
   return 1;
 }
+static bool f8_in_pairs(int64_t routed_rows, int num_experts) {
+  return routed_rows / num_experts > 640;
+}
 static int f8_workers() {
   const int n = sm_count();
   return n < kF8MaxWorkers ? n : kF8MaxWorkers;
@@ -138,11 +145,13 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
   a.status = p.status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool lanes = f8_on_lanes(p.routed_rows, p.num_experts);
+  const bool pairs = f8_in_pairs(p.routed_rows, p.num_experts);
   MOE_CHECK_ARG(!lanes || (p.counters != nullptr && aligned16(p.counters)), "%s: 16-byte aligned partials are needed", name);
   a.counters = p.counters;
   a.partials = p.partials;
   CUtensorMap tx, tw;
-  const int rc = f8_maps(&tx, &tw, p.x, p.x_rows, p.w, static_cast<int64_t>(p.num_experts) * (glu ? 2 : 1), p.N, p.K, lanes ? 16 : BM);
+  const int rc = f8_maps(&tx, &tw, p.x, p.x_rows, p.w, static_cast<int64_t>(p.num_experts) * (glu ? 2 : 1), p.N, p.K,
+                         lanes ? 16 : pairs ? BM : kF8RowBox);
   if (rc != MOE_OK) return rc;
   const bool bf16 = p.dtype == MOE_DTYPE_BF16;
   if (lanes && p.dense && p.kind == F8_ROWS && p.out_perm == nullptr && p.x_rows <= kF8LaneRows) {
@@ -162,9 +171,9 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
       const int rc2 = make_tmap(&to, p.dtype, p.out, 2, dims, box);
       if (rc2 != MOE_OK) return rc2;
     }
-    if (p.kind == F8_GLU_QUANT) return launch_f8_pair<__nv_bfloat16, F8_GLU_QUANT>(tx, tw, to, a, s);
-    if (p.kind == F8_QUANT) return launch_f8_pair<__nv_bfloat16, F8_QUANT>(tx, tw, to, a, s);
-    return bf16 ? launch_f8_pair<__nv_bfloat16, F8_ROWS>(tx, tw, to, a, s) : launch_f8_pair<__half, F8_ROWS>(tx, tw, to, a, s);
+    if (p.kind == F8_GLU_QUANT) return launch_f8_wide<__nv_bfloat16, F8_GLU_QUANT>(pairs, tx, tw, to, a, s);
+    if (p.kind == F8_QUANT) return launch_f8_wide<__nv_bfloat16, F8_QUANT>(pairs, tx, tw, to, a, s);
+    return bf16 ? launch_f8_wide<__nv_bfloat16, F8_ROWS>(pairs, tx, tw, to, a, s) : launch_f8_wide<__half, F8_ROWS>(pairs, tx, tw, to, a, s);
   }
   if (p.kind == F8_GLU_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_GLU_QUANT>(tx, tw, a, s);
   if (p.kind == F8_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_QUANT>(tx, tw, a, s);

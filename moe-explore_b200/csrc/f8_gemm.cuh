@@ -259,9 +259,10 @@ constexpr int kF8MmaK = 32;                  // K of one instruction
 // 32 at a time, the next 32 on their way while the last are added.  A thread's row is its lane, so a step's factor is one register
 // (two where gated).
 // ------------------------------------------------------------------------------------------------------------------
-struct F8PairPlan {
-  static constexpr int kStageBytes = 2 * kF8Tile;
-  static constexpr int kStages = 6;
+constexpr int kF8RowBox = 32;  // rows of one copy, for a CTA by itself
+template <int CTAS> struct F8WidePlan {
+  static constexpr int kStageBytes = (CTAS == 2 ? 2 : 3) * kF8Tile;
+  static constexpr int kStages = CTAS == 2 ? 6 : 4;
   static constexpr int kStagingTile = 32 * 128;
   static constexpr int kStagingBytes = kEpilogueWarps * kStagingTile;
   static constexpr int kBarrierBytes = 1024;
@@ -269,11 +270,11 @@ struct F8PairPlan {
   static_assert(kTotal <= 232448, "shared memory");
 };
 
-template <typename T, int OUT>
+template <typename T, int OUT, int CTAS>
 __global__ void __launch_bounds__(kF8Threads, 1)
-f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
+f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                const __grid_constant__ CUtensorMap tmap_out, const F8Args args) {
-  using Plan = F8PairPlan;
+  using Plan = F8WidePlan<CTAS>;
   constexpr int kStages = Plan::kStages;
   constexpr bool kGlu = OUT == F8_GLU_QUANT;
   constexpr int kCols = kGlu ? 128 : 256;  // result columns of a tile
@@ -293,20 +294,21 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(cluster_ctarank());
+  constexpr bool kPair = CTAS == 2;
+  const int rank = kPair ? static_cast<int>(cluster_ctarank()) : 0;
   WaitCtx wctx;
   wctx.abort_flag = abort_flag;
-  wctx.peer_abort = mapa_shared(smem_u32(const_cast<int*>(abort_flag)), static_cast<uint32_t>(rank ^ 1));
+  wctx.peer_abort = kPair ? mapa_shared(smem_u32(const_cast<int*>(abort_flag)), static_cast<uint32_t>(rank ^ 1)) : 0;
   wctx.status = args.status;
   wctx.limit = args.wait_limit;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(full_bar + 8 * s, 2);
+      mbar_init(full_bar + 8 * s, CTAS);
       mbar_init(empty_bar + 8 * s, 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar + 8 * a, 1);
-      mbar_init(tempty_bar + 8 * a, kEpilogueWarps * 2);
+      mbar_init(tempty_bar + 8 * a, kEpilogueWarps * CTAS);
     }
     for (int q = 0; q < 4; ++q) mbar_init(meet_bar + 8 * q, 2);
     *abort_flag = 0;
@@ -316,16 +318,21 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     if (OUT == F8_ROWS) tma_prefetch_desc(&tmap_out);
   }
   if (warp == 1) {
-    tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
-    tmem_relinquish_pair();
+    if constexpr (kPair) {
+      tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  if constexpr (kPair) cluster_sync_all();
   tc_fence_after();
   await_predecessor();
   const uint32_t tmem_base = *tmem_slot;
-  F8Walk<2> walk(args, blockIdx.x >> 1, gridDim.x >> 1, kCols, rank);
+  F8Walk<CTAS> walk(args, blockIdx.x / CTAS, gridDim.x / CTAS, kCols, rank);
   const int kiters = (args.k_dim + kF8K - 1) / kF8K;
 
   if (warp >= 4) {
@@ -516,12 +523,13 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       uint32_t phase = 0;
       bool ok = true;
       const uint64_t pol = l2_policy_evict_normal();
-      const uint32_t full_leader = mapa_shared(full_bar, 0);
+      const uint32_t full_leader = kPair ? mapa_shared(full_bar, 0) : full_bar;
       for (int i = 0; ok; ++i) {
         const F8Item c = walk.get(i, args, kCols);
         if (!c.valid) break;
         const int wz = kGlu ? 2 * c.expert + rank : c.expert;
         const int wrow = kGlu ? c.n0 : c.n0 + rank * BM;
+        const int groups = (c.rows + kF8RowBox - 1) / kF8RowBox;  // (what the products make of rows that are not there is not stored)
         for (int kb = 0; kb < kiters; ++kb) {
           if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, wctx, DS_TIMEOUT_PRODUCER))) {
             ok = false;
@@ -529,10 +537,19 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
           }
           if (elect_one()) {
             const uint32_t sx = tiles_addr + stage * Plan::kStageBytes;
-            const uint32_t fb = full_leader + 8 * stage;
-            mbar_arrive_expect_tx_cluster(fb, Plan::kStageBytes);
-            tma_load_2d_pair(sx, &tmap_x, kb * (kF8K / 2), c.a_row, fb, pol);
-            tma_load_3d_pair(sx + kF8Tile, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
+            if constexpr (kPair) {
+              const uint32_t fb = full_leader + 8 * stage;
+              mbar_arrive_expect_tx_cluster(fb, Plan::kStageBytes);
+              tma_load_2d_pair(sx, &tmap_x, kb * (kF8K / 2), c.a_row, fb, pol);
+              tma_load_3d_pair(sx + kF8Tile, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
+            } else {
+              const uint32_t fb = full_bar + 8 * stage;
+              mbar_arrive_expect_tx(fb, 2 * kF8Tile + groups * kF8RowBox * kF8K);
+              for (int g = 0; g < groups; ++g)
+                tma_load_2d(sx + g * kF8RowBox * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + g * kF8RowBox, fb, pol);
+              tma_load_3d(sx + kF8Tile, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
+              tma_load_3d(sx + 2 * kF8Tile, &tmap_w, kb * (kF8K / 2), kGlu ? wrow : wrow + BM, kGlu ? wz + 1 : wz, fb, pol);
+            }
           }
           __syncwarp();
           if (++stage == kStages) { stage = 0; phase ^= 1; }
@@ -545,7 +562,7 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     } else if (warp == 1) {
       // ------------------------------ MMA issuer (leader CTA only) --------------
       if (rank == 0) {
-        constexpr uint32_t idesc = f8_idesc(2 * BM, 256);
+        constexpr uint32_t idesc = f8_idesc(CTAS * BM, 256);
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
@@ -563,11 +580,18 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
             if (elect_one()) {
               const uint32_t sx = tiles_addr + stage * Plan::kStageBytes;
 #pragma unroll
-              for (int k = 0; k < kF8K / kF8MmaK; ++k)
-                umma_f8_pair(tmem_base + acc * 256, make_desc(sx + k * kF8MmaK, 16, 1024), make_desc(sx + kF8Tile + k * kF8MmaK, 16, 1024),
-                             idesc, k != 0 ? 1u : 0u);
-              umma_commit_pair_both(tfull_bar + 8 * acc);
-              umma_commit_pair_both(empty_bar + 8 * stage);
+              for (int k = 0; k < kF8K / kF8MmaK; ++k) {
+                const uint64_t dx = make_desc(sx + k * kF8MmaK, 16, 1024), dw = make_desc(sx + kF8Tile + k * kF8MmaK, 16, 1024);
+                if constexpr (kPair) umma_f8_pair(tmem_base + acc * 256, dx, dw, idesc, k != 0 ? 1u : 0u);
+                else umma_f8(tmem_base + acc * 256, dx, dw, idesc, k != 0 ? 1u : 0u);
+              }
+              if constexpr (kPair) {
+                umma_commit_pair_both(tfull_bar + 8 * acc);
+                umma_commit_pair_both(empty_bar + 8 * stage);
+              } else {
+                umma_commit(tfull_bar + 8 * acc);
+                umma_commit(empty_bar + 8 * stage);
+              }
             }
             __syncwarp();
             if (++stage == kStages) { stage = 0; phase ^= 1; }
@@ -584,11 +608,12 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
 
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();  // neither CTA may end while its peer can still touch its memory or barriers
+  if constexpr (kPair) cluster_sync_all();  // neither CTA may end while its peer can still touch its memory or barriers
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc_pair(tmem_base, kTmemCols);
+    if constexpr (kPair) tmem_dealloc_pair(tmem_base, kTmemCols);
+    else tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
