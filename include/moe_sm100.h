@@ -588,11 +588,7 @@ typedef struct moe_f8_pass {
   float* hidden_scales;
   void *ys, *out;
   const void* addend;
-  void* partials; /* moe_f8_partial_bytes(num_tokens * topk, num_experts, act) bytes; written by MOE_F8_DISPATCH and the products */
 } moe_f8_pass;
-
-/* Bytes that few rows need beside the results: sums of parts of K, which several workers of a product share (0: none). */
-size_t moe_f8_partial_bytes(int64_t num_rows, int num_experts, int act);
 
 size_t moe_f8_pass_size(void);
 
@@ -621,7 +617,6 @@ typedef struct moe_f8_rows_pass {
   int32_t *pad_offsets, *mtile_expert, *tile_pairs, *num_mtiles, *status;
   void* gathered;
   float* gathered_scales;
-  void* partials; /* moe_f8_partial_bytes(num_rows, num_experts, act) bytes */
 } moe_f8_rows_pass;
 
 size_t moe_f8_rows_pass_size(void);

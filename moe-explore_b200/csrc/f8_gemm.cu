@@ -11,7 +11,7 @@ template <int CTAS, typename Kernel, typename... Args>
 static int launch_f8(Kernel kernel, int threads, int smem, std::atomic<int> (&grids)[64], cudaStream_t s, const Args&... args) {
   LaunchParams lp;
   lp.stream = s;
-  lp.max_ctas = CTAS == 1 ? kF8MaxWorkers : 0;
+  lp.max_ctas = 0;
   lp.chained = chained_launches();
   PersistentLaunch l;
   const int rc = configure<CTAS>(l, kernel, smem, grids, lp);
@@ -30,16 +30,11 @@ template <typename T, int OUT>
 static int launch_f8_wide(bool pairs, const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& to, const F8Args& args, cudaStream_t s) {
   return pairs ? launch_f8_wide_on<T, OUT, 2>(tx, tw, to, args, s) : launch_f8_wide_on<T, OUT, 1>(tx, tw, to, args, s);
 }
-template <typename T, int OUT>
-static int launch_f8_lanes(const CUtensorMap& tx, const CUtensorMap& tw, const F8Args& args, cudaStream_t s) {
-  static std::atomic<int> grids[64];
-  return launch_f8<1>(f8_lanes_kernel<T, OUT, false>, kF8Threads, F8LanesPlan<OUT == F8_GLU_QUANT>::kTotal, grids, s, tx, tw, args);
-}
 // One cluster of `ranks` CTAs per item.
-template <typename T>
-static int launch_f8_clusters(const CUtensorMap& tx, const CUtensorMap& tw, const F8Args& args, int items, int ranks, cudaStream_t s) {
-  const auto kernel = f8_lanes_kernel<T, F8_ROWS, true>;
-  constexpr int smem = F8LanesPlan<false>::kTotal;
+template <typename T, int OUT>
+static int launch_f8_lanes(const CUtensorMap& tx, const CUtensorMap& tw, const F8Args& args, int items, int ranks, cudaStream_t s) {
+  const auto kernel = f8_lanes_kernel<T, OUT>;
+  constexpr int smem = F8LanesPlan<OUT == F8_GLU_QUANT>::kTotal;
   static std::atomic<bool> prepared[64];
   int dev = 0;
   MOE_CUDA(cudaGetDevice(&dev));
@@ -75,33 +70,33 @@ static int f8_maps(CUtensorMap* tx, CUtensorMap* tw, const void* x, int64_t rows
   return make_tmap(tw, MOE_DTYPE_BF16, w, 3, dw, bw);
 }
 
-__global__ void __launch_bounds__(256) f8_zero_kernel(uint32_t* counters, int num_counters) {
-  await_predecessor();
-  grid_release();
-  for (int i = threadIdx.x; i < num_counters; i += 256) counters[i] = 0;
+// The kernel with the weights on the lanes: how many items there can be (an expert each, in blocks of 128 columns) and how many
+// CTAs share one; none where it does not serve.  It does for 64 rows in all and no more items than SMs: 29 MB of one matrix
+// (7168 x 4096) take 11 to 15 us so and 29 with rows on the lanes; the 2 x 32 items of one token's down products (14336 x 4096) XX
+// us instead of YY.
+struct F8Lanes {
+  int items, ranks;
+};
+static F8Lanes f8_lanes(const F8Product& p) {
+  if (p.routed_rows > kF8LaneRows) return {0, 0};
+  const int64_t experts = p.dense ? 1 : p.routed_rows < p.num_experts ? p.routed_rows : p.num_experts;
+  const int64_t items = experts * ((p.N + 127) / 128);
+  if (items > sm_count()) return {0, 0};
+  const int kiters = (p.K + kF8K - 1) / kF8K;
+  // as many CTAs as leave every one an SM (a cluster lies within a processing cluster of 16 to 20 SMs, so that some stay without)
+  int ranks = kF8MostRanks;
+  while (ranks > 1 && (items * ranks * 8 > sm_count() * 7 || kiters < ranks * kF8LeastSteps)) ranks /= 2;
+  return {static_cast<int>(items), ranks};
 }
-
-// Rows per expert up to which the weights lie on the lanes.  us with the weights on the lanes / the rows, by rows per expert:
-//   64 experts of 7168 x 2048   16: 184 / 246   24: 203 / 259   32: 220 / 264   48: 336 / 274
-//   64 experts of 2048 x 1024   16:  50 /  49   24:  57 /  49   32:  64 /  50   48:  75 /  49
-//   60 experts of 2000 x 1416   16:  61 /  71   24:  69 /  69   32:  74 /  67   48:  92 /  67
-//   one matrix of 7168 x 4096   16:  XX /  34   32:  XX /  30   64:  XX /  31   96:  59 /  31
-bool f8_on_lanes(int64_t routed_rows, int num_experts) {
-  return routed_rows / num_experts <= (num_experts == 1 ? kF8LaneRows : 24);
-}
-// CTAs that share an item of one matrix: as many as leave every CTA an SM (a cluster lies within a processing cluster of 16 to 20 SMs,
-// so that some stay without) and steps enough.
-static int f8_ranks(int items, int kiters) {
-  for (int ranks = kF8MostRanks; ranks > 1; ranks /= 2)
-    if (items * ranks * 8 <= sm_count() * 7 && kiters >= ranks * kF8LeastSteps) return ranks;
-  return 1;
-}
-static bool f8_in_pairs(int64_t routed_rows, int num_experts) {
-  return routed_rows / num_experts > 640;
-}
-static int f8_workers() {
-  const int n = sm_count();
-  return n < kF8MaxWorkers ? n : kF8MaxWorkers;
+// Rows on the lanes: pairs of CTAs or single ones.  A pair's 256 rows are more often partly empty, a single CTA takes half as much again
+// from L2, and more where rows of K bytes begin inside a line of 128.  us with single CTAs / pairs by rows per expert (0.5 to 1.5 of it):
+//   64 experts of 7168 x 2048    64: 175 / 235   128: 229 / 250   384: 470 / 540   512: 645 / 607
+//   64 experts of 2048 x 1024    64:  36 /  50   128:  43 /  49   384:  78 /  76   512:  95 /  95
+//   60 experts of 2000 x 1416    64:  47 /  64   128:  68 /  64   384: 143 / 116
+//   one matrix of 7168 x 4096                    128:  33 /  29   512:  35 /  30
+static bool f8_in_pairs(const F8Product& p) {
+  const int64_t mean = p.routed_rows / p.num_experts;
+  return mean > (p.num_experts == 1 ? 64 : p.K % 128 == 0 ? 400 : 96);
 }
 
 int f8_product(const char* name, const F8Product& p, void* stream) {
@@ -144,26 +139,15 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
   a.wait_limit = wait_limit_cycles();
   a.status = p.status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool lanes = f8_on_lanes(p.routed_rows, p.num_experts);
-  const bool pairs = f8_in_pairs(p.routed_rows, p.num_experts);
-  MOE_CHECK_ARG(!lanes || (p.counters != nullptr && aligned16(p.counters)), "%s: 16-byte aligned partials are needed", name);
-  a.counters = p.counters;
-  a.partials = p.partials;
+  a.maps_before = p.dense || p.maps_before;
+  const F8Lanes lanes = f8_lanes(p);
+  const bool pairs = f8_in_pairs(p);
   CUtensorMap tx, tw;
   const int rc = f8_maps(&tx, &tw, p.x, p.x_rows, p.w, static_cast<int64_t>(p.num_experts) * (glu ? 2 : 1), p.N, p.K,
-                         lanes ? 16 : pairs ? BM : kF8RowBox);
+                         lanes.items > 0 ? 16 : pairs ? BM : kF8RowBox);
   if (rc != MOE_OK) return rc;
   const bool bf16 = p.dtype == MOE_DTYPE_BF16;
-  if (lanes && p.dense && p.kind == F8_ROWS && p.out_perm == nullptr && p.x_rows <= kF8LaneRows) {
-    const int items = (p.N + 127) / 128, ranks = f8_ranks(items, (p.K + kF8K - 1) / kF8K);
-    if (items <= sm_count())
-      return bf16 ? launch_f8_clusters<__nv_bfloat16>(tx, tw, a, items, ranks, s) : launch_f8_clusters<__half>(tx, tw, a, items, ranks, s);
-  }
-  if (lanes && p.zero_counters) {
-    MOE_CUDA(launch_kernel(f8_zero_kernel, 1, 256, s, p.counters, kF8MaxWorkers));
-    chained_launches() = true;
-  }
-  if (!lanes) {
+  if (lanes.items == 0) {
     CUtensorMap to = tx;
     if (p.kind == F8_ROWS && p.out_perm == nullptr) {
       const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.x_rows)};
@@ -175,9 +159,10 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
     if (p.kind == F8_QUANT) return launch_f8_wide<__nv_bfloat16, F8_QUANT>(pairs, tx, tw, to, a, s);
     return bf16 ? launch_f8_wide<__nv_bfloat16, F8_ROWS>(pairs, tx, tw, to, a, s) : launch_f8_wide<__half, F8_ROWS>(pairs, tx, tw, to, a, s);
   }
-  if (p.kind == F8_GLU_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_GLU_QUANT>(tx, tw, a, s);
-  if (p.kind == F8_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_QUANT>(tx, tw, a, s);
-  return bf16 ? launch_f8_lanes<__nv_bfloat16, F8_ROWS>(tx, tw, a, s) : launch_f8_lanes<__half, F8_ROWS>(tx, tw, a, s);
+  if (p.kind == F8_GLU_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_GLU_QUANT>(tx, tw, a, lanes.items, lanes.ranks, s);
+  if (p.kind == F8_QUANT) return launch_f8_lanes<__nv_bfloat16, F8_QUANT>(tx, tw, a, lanes.items, lanes.ranks, s);
+  return bf16 ? launch_f8_lanes<__nv_bfloat16, F8_ROWS>(tx, tw, a, lanes.items, lanes.ranks, s)
+              : launch_f8_lanes<__half, F8_ROWS>(tx, tw, a, lanes.items, lanes.ranks, s);
 }
 
 // ---- rows to 8 bits, and their way to the experts ----
@@ -200,12 +185,9 @@ template <typename T> __device__ __forceinline__ void to_floats(const uint4& u, 
 constexpr int kF8RowsCtas = 6;  // per SM
 template <typename T>
 __global__ void __launch_bounds__(256, kF8RowsCtas)
-f8_rows_kernel(const T* x, const float* scales_in, const int32_t* dst_row, int copies, uint2* out, float* scales, int rows, int cols,
-               uint32_t* counters, int num_counters) {
+f8_rows_kernel(const T* x, const float* scales_in, const int32_t* dst_row, int copies, uint2* out, float* scales, int rows, int cols) {
   await_predecessor();  // before the release: what comes up next reads the routing metadata
   grid_release();
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < num_counters; i += 256) counters[i] = 0;
   const int blocks = (cols + kF8Block - 1) / kF8Block;
   const int pairs = (blocks + 1) / 2;
   const int vecs = cols / 8;
@@ -291,7 +273,7 @@ static int f8_row_grid(int64_t rows, int cols) {
 }
 
 int f8_rows(const char* name, const void* x, const float* x_scales, const int32_t* dst_row, int copies, void* out, float* scales,
-            int64_t rows, int cols, int dtype, uint32_t* counters, int num_counters, void* stream) {
+            int64_t rows, int cols, int dtype, void* stream) {
   MOE_CHECK_ARG(rows >= 0 && cols > 0 && copies > 0, "%s: negative or zero size", name);
   if (cols % 16 != 0) {
     set_error("%s: 8-bit rows have a multiple of 16 columns, got %d", name, cols);
@@ -309,21 +291,15 @@ int f8_rows(const char* name, const void* x, const float* x_scales, const int32_
   const int grid = f8_row_grid(rows, cols);  // (16 blocks of 128 columns per CTA)
   uint2* o = static_cast<uint2*>(out);
   if (x_scales != nullptr)
-    MOE_CUDA(launch_kernel(f8_rows_kernel<uint8_t>, grid, 256, s, static_cast<const uint8_t*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols,
-                           counters, num_counters));
+    MOE_CUDA(launch_kernel(f8_rows_kernel<uint8_t>, grid, 256, s, static_cast<const uint8_t*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols));
   else if (dtype == MOE_DTYPE_BF16)
-    MOE_CUDA(launch_kernel(f8_rows_kernel<__nv_bfloat16>, grid, 256, s, static_cast<const __nv_bfloat16*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols,
-                           counters, num_counters));
+    MOE_CUDA(launch_kernel(f8_rows_kernel<__nv_bfloat16>, grid, 256, s, static_cast<const __nv_bfloat16*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols));
   else
-    MOE_CUDA(launch_kernel(f8_rows_kernel<__half>, grid, 256, s, static_cast<const __half*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols,
-                           counters, num_counters));
+    MOE_CUDA(launch_kernel(f8_rows_kernel<__half>, grid, 256, s, static_cast<const __half*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols));
   return MOE_OK;
 }
 
 // Floats of the workers' slots.
-static size_t f8_slot_floats(bool glu) {
-  return static_cast<size_t>(2 * f8_workers()) * (glu ? 2 : 1) * kF8LaneRows * 128;
-}
 
 static bool glu(int act) { return act == MOE_ACT_SWIGLU || act == MOE_ACT_GEGLU; }
 
@@ -332,7 +308,7 @@ static bool glu(int act) { return act == MOE_ACT_SWIGLU || act == MOE_ACT_GEGLU;
 using namespace moe;
 
 extern "C" int moe_f8_quantize_rows(const void* x, void* q, float* scales, int64_t num_rows, int cols, int dtype, void* stream) {
-  return f8_rows("moe_f8_quantize_rows", x, nullptr, nullptr, 1, q, scales, num_rows, cols, dtype, nullptr, 0, stream);
+  return f8_rows("moe_f8_quantize_rows", x, nullptr, nullptr, 1, q, scales, num_rows, cols, dtype, stream);
 }
 
 extern "C" size_t moe_f8_pass_size(void) { return sizeof(moe_f8_pass); }
@@ -351,12 +327,9 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
   if (steps & MOE_F8_ROUTE)
     MOE_STEP(routing_metadata(p->expert_idx, rows, p->num_experts, p->group_indices, nullptr, p->pad_offsets, p->row_src, p->dst_row,
                               p->mtile_expert, p->tile_pairs, p->num_mtiles, p->status, p->workspace, p->workspace_bytes, false, stream));
-  // counters of the two products, then the slots that both use in turn
-  uint32_t* const counters = static_cast<uint32_t*>(p->partials);
-  const bool lanes = f8_on_lanes(rows, p->num_experts);
   if (steps & MOE_F8_DISPATCH)
     MOE_STEP(f8_rows("moe_f8_expert_forward", p->x, p->x_scales, p->dst_row, p->topk, p->xs, p->xs_scales, p->num_tokens, p->d, p->dtype,
-                     counters, lanes && counters != nullptr ? 2 * kF8MaxWorkers : 0, stream));
+                     stream));
   F8Product g{};
   g.x_rows = p->padded_rows;
   g.routed_rows = rows;
@@ -368,10 +341,9 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
   g.pad_offsets = p->pad_offsets;
   g.group_indices = p->group_indices;
   g.status = p->status;
-  g.partials = reinterpret_cast<float*>(counters + 2 * kF8MaxWorkers);
   if (steps & MOE_F8_UP) {
     g.kind = glu(p->act) ? F8_GLU_QUANT : F8_QUANT;
-    g.counters = counters;
+    g.maps_before = !(steps & MOE_F8_ROUTE) || (steps & MOE_F8_DISPATCH);  // by an earlier call, or with a kernel between
     g.x = p->xs;
     g.x_scales = p->xs_scales;
     g.w = p->w1;
@@ -385,7 +357,7 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
   }
   if (steps & MOE_F8_DOWN) {
     g.kind = F8_ROWS;
-    g.counters = counters + kF8MaxWorkers;
+    g.maps_before = !(steps & MOE_F8_ROUTE) || (steps & (MOE_F8_DISPATCH | MOE_F8_UP));
     g.x = p->hidden;
     g.x_scales = p->hidden_scales;
     g.w = p->w2;
@@ -401,11 +373,6 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
     MOE_STEP(combine_topk(p->ys, p->scores, p->dst_row, p->out, p->num_tokens, p->topk, p->d, p->dtype, p->addend, nullptr, nullptr,
                           nullptr, stream));
   return MOE_OK;
-}
-
-extern "C" size_t moe_f8_partial_bytes(int64_t num_rows, int num_experts, int act) {
-  if (num_rows <= 0 || num_experts <= 0 || !f8_on_lanes(num_rows, num_experts)) return 0;
-  return 2 * kF8MaxWorkers * sizeof(uint32_t) + f8_slot_floats(glu(act)) * sizeof(float);
 }
 
 extern "C" size_t moe_f8_rows_pass_size(void) { return sizeof(moe_f8_rows_pass); }
@@ -439,9 +406,6 @@ extern "C" int moe_f8_rows_gemm(const moe_f8_rows_pass* p, int steps, void* stre
   }
   if (steps & MOE_ROWS_GEMM) {
     F8Product g{};
-    g.counters = static_cast<uint32_t*>(p->partials);
-    g.partials = reinterpret_cast<float*>(g.counters + 2 * kF8MaxWorkers);
-    g.zero_counters = true;
     g.kind = F8_ROWS;
     g.x = p->gather ? p->gathered : p->x;
     g.x_scales = p->gather ? p->gathered_scales : p->x_scales;

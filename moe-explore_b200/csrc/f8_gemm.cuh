@@ -7,10 +7,10 @@
 // epilogue warps fetch it, multiply by the two scales and add in fp32 registers while the tensor cores work on the next block.
 // (The scales are fp32, not powers of two, so the tensor cores' own block scaling cannot apply them.)
 //
-// Two kernels, chosen by how many rows an expert has (f8_gemm.cu):
-//   f8_pair_kernel   rows on the accumulator's lanes: a CTA pair covers 256 rows x 256 weight rows of one expert
-//   f8_lanes_kernel  weights on the lanes: a CTA covers 128 weight rows (of gate AND up where gated) and up to R rows of one
-//                    expert, so that few rows cost few columns and the weights stream at the rate of the memory
+// Two kernels, chosen by the sizes (f8_gemm.cu):
+//   f8_wide_kernel   rows on the accumulator's lanes: a CTA covers 128 rows x 256 weight rows of one expert, a CTA pair twice the rows
+//   f8_lanes_kernel  weights on the lanes: a cluster covers 128 weight rows (of gate AND up where gated) and up to 64 rows of
+//                    one expert, each of its CTAs a part of K; for calls with so few of these that SMs would be idle
 //
 // Operands are described to the copy engine as pairs of bytes (16-bit elements, 64 to a 128-byte swizzle row); loads past an edge
 // read zeros, which are zeros in e4m3 too.
@@ -42,9 +42,7 @@ struct F8Product {
   float* out_scales;
   int K, N, num_experts, act, dtype;
   int64_t routed_rows;      // about how many rows there are
-  float* partials;          // F8Args
-  uint32_t* counters;
-  bool zero_counters;       // by a launch of their own (else a kernel before has done it)
+  bool maps_before;         // F8Args
   bool dense;
   int compact;
   const int64_t* out_perm;
@@ -53,8 +51,6 @@ struct F8Product {
   int32_t* status;
 };
 int f8_product(const char* name, const F8Product& p, void* stream);
-// Whether the kernel with the weights on the lanes does it.
-bool f8_on_lanes(int64_t routed_rows, int num_experts);
 
 struct F8Args {
   // The rows of the experts: maps of the padded layout, or dense_rows >= 0: one expert, rows 0 .. dense_rows - 1, no maps.
@@ -73,8 +69,7 @@ struct F8Args {
   int32_t k_dim;
   int32_t act;
   int32_t group_m;
-  float* partials;        // f8_lanes_kernel: two slots per worker
-  uint32_t* counters;     // f8_lanes_kernel: kF8MaxWorkers words, zero
+  int32_t maps_before;    // the maps were complete when the kernel before began
   long long wait_limit;
   int32_t* status;
 };
@@ -251,13 +246,17 @@ constexpr int kF8Tile = BM * kF8K;           // 16 KB: 128 rows of an operand
 constexpr int kF8MmaK = 32;                  // K of one instruction
 
 // ------------------------------------------------------------------------------------------------------------------
-// Rows on the lanes, CTA pairs.
+// Rows on the lanes, CTA pairs or CTAs by themselves.
 //
 // A pair's tile is 256 rows x 256 weight rows (128 gate + 128 up rows where gated); per 128 of K each CTA loads 16 KB of rows and
-// 16 KB of weights, and the leader's four instructions (M 256, N 256, K 32) fill one of the two accumulator stages.  Each of
+// 16 KB of weights, and the leader's four instructions (M 256, N 256, K 32) fill one of the two accumulator stages.  A CTA by itself
+// has 128 rows x 256 weight rows: as many products, 32 KB of weights, and no more of the rows than there are.  Each of
 // the eight epilogue warps of a CTA owns 32 rows x 128 of the columns: 128 fp32 sums per thread, fetched from TMEM
 // 32 at a time, the next 32 on their way while the last are added.  A thread's row is its lane, so a step's factor is one register
 // (two where gated).
+//
+// Bound by TMEM, which the accumulators' writes and the epilogue's reads share, and between 24 and 400 rows per expert by what L2
+// hands out: pairs take 2.0 to 2.1 PFLOP/s at 8192 rows (a step of 256 x 256 x 128 in 0.55 us).
 // ------------------------------------------------------------------------------------------------------------------
 constexpr int kF8RowBox = 32;  // rows of one copy, for a CTA by itself
 template <int CTAS> struct F8WidePlan {
@@ -618,133 +617,44 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// Weights on the lanes.
+// Weights on the lanes, K split over a cluster.
 //
-// A tile is 128 result columns (weight rows on the lanes; gate and up rows where gated: two accumulators) x the rows of one row
-// tile, R at a time.  The instruction's N is the rows there are, in steps of 16, and so are the rows loaded per stage: with one
-// token a stage is 16 (32) KB of weights and 2 KB of rows.  The ring holds about 190 KB, what an SM needs in flight to stream
-// weights at the memory's rate.  Epilogue warp w owns the 32 lanes of quadrant w % 4 and every other group of 16 rows; a row's scale
-// is handed around by shuffles.  (CTA pairs bring nothing here: there is nothing to share but the few rows.)
+// An item is 128 result columns (weight rows on the lanes; gate and up rows where gated: two accumulators) x the rows of one expert,
+// kF8LaneRows of them at most.  The instruction's N is the rows there are, in steps of 16, and so are the rows loaded per stage:
+// with one token a stage is 16 (32) KB of weights and 2 KB of rows.  The CTAs of a cluster have equal parts of K; each leaves its sums
+// in its shared memory, and after a meeting of the cluster they share out the rows of the results, adding in the order of K.  Nothing
+// goes through global memory, and nobody waits but for its own cluster.
 //
-// SPLIT ALONG K.  As many items as there are workers, as often as that goes, are dealt out whole; what is left (everything, where
-// there are fewer items than workers) is one run of steps of 128 of K, of which every worker takes an equal part, wherever that
-// begins and ends.  An item that several workers share is summed by each over its own steps into a slot of its own in `partials`, and
-// whoever arrives last (a counter per first worker of a shared item) adds the slots in the order of the workers and goes on to
-// the results.  Nobody waits for anybody, and the sums do not depend on who was last.  The shared steps come first and are joined
-// last.  Bound by HBM: one token through 2 of 8 experts of 4096 x 14336 has 224 and 64 items
-// for 148 SMs, which dealt out whole left half of them idle.  (All items as one run of steps, 14 in a row per worker: 1.9 GB of
-// weights at 5.0 TB/s instead of 6.0; neighbours then no longer stream neighbouring weights.)
-// A product of one matrix whose items are fewer than half the SMs is split over clusters instead (CLUSTERED): each CTA of a
-// cluster has an equal part of K of one item and leaves its sums in its shared memory, and the CTAs share out the rows of the results.
-// 64 rows of 7168 by 4096 columns: XXX us instead of 30 with slots and counters (and a launch that zeroes them).
+// For the smallest calls: few items, which by themselves would leave most SMs without work.  64 rows of 7168 by 4096 columns (32
+// items, clusters of 4): 15 us, 29 MB of weights at 2 TB/s; of that 6 us are the launch, the first loads' way and the joining.
+// (Items cut wherever a worker's equal share of all steps ended, their parts joined through global memory and a counter: 30 us.)
 //
-// (An item with more than R rows takes more than one pass over its weights and is not shared: its first worker does all of it.)
-//
-// The weights of the first stages are asked for before the wait for the kernel before: that one writes the rows, while the maps
-// and counts were complete before it let this kernel up (it waited for them itself).
+// Epilogue warp w owns the 32 lanes of quadrant w % 4 and every other group of 16 rows.
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int kF8MaxWorkers = 256;
-constexpr int kF8MostRanks = 8;   // CTAs of a cluster that share an item
-constexpr int kF8LeastSteps = 4;  // of a worker; with fewer, what the joining costs is more than the streaming
-
-// The work of one worker, item by item.
-struct F8Part {
-  F8Item c;
-  int kb0, kb1;  // steps of this item (kb0 >= kb1: none)
-  int item;
-  bool shared;
-  bool valid;
-};
-template <bool CLUSTERED> struct F8Split {
-  F8Walk<1> walk;             // decodes; its lanes 0 to 15 hold items of the shared run, 16 to 31 whole ones
-  int64_t begin, end, steps;  // the shared run: this worker's part of it, and all of it
-  int worker, all_workers, workers, kiters, item0, items, wholes, loose;
-  __device__ __forceinline__ F8Split(const F8Args& a, int worker_, int all_workers_, int kiters_)
-      : walk(a, 0, 1, 128, 0), worker(worker_), all_workers(all_workers_), kiters(kiters_) {
-    if (CLUSTERED) {
-      begin = end = steps = 0;
-      workers = item0 = items = loose = 0;
-      wholes = 1;
-      return;
-    }
-    wholes = walk.count / all_workers;
-    loose = walk.count - wholes * all_workers;  // items of the shared run
-    steps = static_cast<int64_t>(loose) * kiters;
-    const int64_t most = steps / kF8LeastSteps;
-    workers = most < 1 ? 1 : most < all_workers ? static_cast<int>(most) : all_workers;
-    begin = worker < workers ? steps * worker / workers : steps;
-    end = worker < workers ? steps * (worker + 1) / workers : steps;
-    item0 = static_cast<int>(begin / kiters);
-    items = begin < end ? static_cast<int>((end - 1) / kiters) - item0 + 1 : 0;
-    decode(0, 0, a);
-  }
-  // Decodes shared items from `shared0` and whole ones from `whole0` on, 16 of each: one chain of dependent loads for both.
-  __device__ __forceinline__ void decode(int shared0, int whole0, const F8Args& a) {
-    const int lane = threadIdx.x & 31;
-    const int i = lane < 16 ? shared0 + lane : whole0 + lane - 16;
-    if (i < (lane < 16 ? items : wholes)) walk.mine = walk.decode(lane < 16 ? item0 + i : loose + worker + i * all_workers, a, 128);
-    __syncwarp();
-  }
-  // The i-th of this worker; i = 0, 1, 2, ... in this order, by all lanes of the warp (shared ones also again afterwards, from 0 on).
-  __device__ __forceinline__ F8Part get(int i, const F8Args& a, int most_rows) {
-    F8Part p;
-    p.valid = i < items + wholes;
-    if (!p.valid) return p;
-    if (CLUSTERED) {
-      const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-      p.item = worker / ranks;
-      p.c = walk.decode(p.item, a, 128);
-      p.kb0 = kiters * rank / ranks;
-      p.kb1 = kiters * (rank + 1) / ranks;
-      p.shared = false;
-      return p;
-    }
-    const bool is_shared = i < items;
-    const int j = is_shared ? i : i - items;
-    if ((j & 15) == 0 && (j > 0 || items > 16)) decode(is_shared ? j : 0, is_shared ? 0 : j, a);
-    p.item = is_shared ? item0 + i : loose + worker + j * all_workers;
-    p.c = walk.held((is_shared ? 0 : 16) + (j & 15));
-    p.kb0 = 0;
-    p.kb1 = kiters;
-    p.shared = false;
-    if (!is_shared) return p;
-    if (i == 0) p.kb0 = static_cast<int>(begin - static_cast<int64_t>(item0) * kiters);
-    if (i == items - 1) p.kb1 = static_cast<int>(end - static_cast<int64_t>(p.item) * kiters);
-    p.shared = p.kb0 > 0 || p.kb1 < kiters;
-    if (p.shared && p.c.rows > most_rows) {
-      p.shared = false;
-      p.kb1 = p.kb0 == 0 ? kiters : p.kb0;
-    }
-    return p;
-  }
-  __device__ __forceinline__ int worker_of(int64_t step) const { return static_cast<int>(((step + 1) * workers - 1) / steps); }
-};
-
-constexpr int kF8LaneRows = 64;  // rows per pass (128: every step costs the epilogue what two of 64 do)
+constexpr int kF8LaneRows = 64;
+constexpr int kF8MostRanks = 8;   // CTAs of a cluster
+constexpr int kF8LeastSteps = 4;  // of a CTA; with fewer, what the joining costs is more than the streaming
 
 template <bool GLU> struct F8LanesPlan {
   static constexpr int R = kF8LaneRows;
   static constexpr int kWBytes = (GLU ? 2 : 1) * kF8Tile;
   static constexpr int kStageBytes = kWBytes + R * kF8K;
   static constexpr int kAccCols = (GLU ? 2 : 1) * R;
-  static constexpr int kAccs = 512 / kAccCols > 4 ? 4 : 512 / kAccCols;
-  // the results' way from lanes to rows: 16 rows x 128 columns in fp32
-  static constexpr int kStaging = (GLU ? 2 : 1) * 16 * 128 * 4;
+  static constexpr int kAccs = 4;
   // the scales of as many steps as fit: [step][row], and [matrix][step] of the weights
   static constexpr int kTable = 2048;
   static constexpr int kTableSteps = 128;
-  static constexpr int kExtra = kStaging + (kTable + 2 * kTableSteps) * 4;
+  static constexpr int kExtra = (kTable + 2 * kTableSteps) * 4;
   static constexpr int kBarrierBytes = 1024;
   static constexpr int kBudget = 232448 - 1024 - kBarrierBytes - kExtra;
   static constexpr int kStages = kBudget / kStageBytes > 10 ? 10 : kBudget / kStageBytes;
   static constexpr int kTotal = kStages * kStageBytes + kExtra + kBarrierBytes + 1024;
+  static_assert(kAccs * kAccCols <= static_cast<int>(kTmemCols), "tensor memory");
   static_assert(kTable >= 16 * R, "scales of 16 steps at least");
-  static_assert(kAccs == 4, "sums of two steps are fetched together");
-  // split over a cluster: the sums of all rows, where the ring was
-  static_assert(R * 128 * 4 <= kStages * kStageBytes, "room for the sums");
+  static_assert((GLU ? 2 : 1) * R * 128 * 4 <= kStages * kStageBytes, "the sums lie where the ring was");
 };
 
-template <typename T, int OUT, bool CLUSTERED>
+template <typename T, int OUT>
 __global__ void __launch_bounds__(kF8Threads, 1)
 f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const F8Args args) {
   constexpr bool kGlu = OUT == F8_GLU_QUANT;
@@ -752,13 +662,12 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   using Plan = F8LanesPlan<kGlu>;
   constexpr int kStages = Plan::kStages, kAccs = Plan::kAccs;
   constexpr int kMats = kGlu ? 2 : 1;
-  constexpr int kChunks = R / 32;  // groups of 16 rows whose results a warp sees to
+  constexpr int kChunks = R / 32;  // groups of 16 rows whose sums a warp sees to
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t tiles_addr = (raw_addr + 1023u) & ~1023u;
   uint8_t* tiles = smem_raw + (tiles_addr - raw_addr);
-  float* const staging = reinterpret_cast<float*>(tiles + kStages * Plan::kStageBytes);
-  float* const table = staging + Plan::kStaging / 4;
+  float* const table = reinterpret_cast<float*>(tiles + kStages * Plan::kStageBytes);
   float* const weight_table = table + Plan::kTable;
   uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kStages * Plan::kStageBytes + Plan::kExtra);
   const uint32_t full_bar = smem_u32(bars);
@@ -768,7 +677,6 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   const uint32_t meet_bar = smem_u32(bars + 2 * kStages + 2 * kAccs);  // the epilogue warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kAccs + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* joined = reinterpret_cast<volatile int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -801,7 +709,17 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int kiters = (args.k_dim + kF8K - 1) / kF8K;
-  F8Split<CLUSTERED> split(args, blockIdx.x, gridDim.x, kiters);
+  const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+  const int kb0 = kiters * rank / ranks, kb1 = kiters * (rank + 1) / ranks;
+  // (the grid has a cluster for every item there could be)
+  const auto find_item = [&]() {
+    const F8Walk<1> walk(args, 0, 1, 128, 0);
+    const int item = static_cast<int>(blockIdx.x) / ranks;
+    F8Item c{};
+    if (item < walk.count) c = walk.decode(item, args, 128);
+    c.rows = min(c.rows, R);
+    return c;
+  };
 
   if (warp >= 4) {
     more_registers<72>();
@@ -809,7 +727,6 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     const int quad = warp & 3;
     const int half = (warp - 4) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const int kblocks = kiters;
     const int nblocks = (args.n_dim + kF8Block - 1) / kF8Block;
     int acc = 0, meets = 0;
     uint32_t acc_phase = 0;
@@ -819,351 +736,201 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       if (lane == 0) mbar_arrive(meet_bar);
       return __all_sync(0xFFFFFFFFu, mbar_wait(meet_bar, meets++ & 1, wctx, DS_TIMEOUT_EPILOGUE));
     };
-    // Shared items a second time, at the end: their parts are written on the way, and by then the writes are long complete (waiting for
-    // them, and for the counter, at once took 5 us under a saturated memory, twice per worker, and the weights' stream stood).
-    const int parts = split.items + split.wholes;
-    // One warp tells the counters that this worker's parts are written, and which shared items are left to this worker: in the middle of
-    // a whole item, where its waiting costs nothing, else at the end.  A meeting of the warps since the writes lies before.
-    bool arrived = false;
-    const auto arrive = [&]() {
-      arrived = true;
-      if (warp != 4) return;
-      for (int j = 0; j < split.items; ++j) {
-        const F8Part p = split.get(j, args, R);
-        if (!p.shared || p.kb0 >= p.kb1 || lane != 0) continue;
-        __threadfence();  // (what the others wrote before the meeting is covered)
-        const int first_worker = split.worker_of(static_cast<int64_t>(p.item) * kiters);
-        const int last_worker = split.worker_of(static_cast<int64_t>(p.item + 1) * kiters - 1);
-        joined[j] = atomicAdd(args.counters + first_worker, 1u) == static_cast<uint32_t>(last_worker - first_worker) ? 1 : 0;
-        __threadfence();
-      }
-      __syncwarp();
-    };
     await_predecessor();
-    for (int i = 0; ok && i < parts + split.items; ++i) {
-      const bool joining = i >= parts;
-      const F8Part part = split.get(joining ? i - parts : i, args, R);
-      if (part.kb0 >= part.kb1) continue;  // (done by the item's first worker)
-      if (joining) {
-        if (!part.shared) continue;
-        if (!arrived) {
-          if (!meet()) break;
-          arrive();
-        }
-        if (!meet()) break;
-        if (joined[i - parts] == 0) continue;  // someone else goes on with this item
-      }
-      const F8Item& c = part.c;
-      const float* ws = args.w_scales + (static_cast<int64_t>(c.expert) * kMats * nblocks + c.n0 / kF8Block) * kblocks;
-      for (int r0 = 0; r0 < c.rows && ok; r0 += R) {
-        const int rows = min(c.rows - r0, R);
-        const int rows16 = (rows + 15) & ~15;
-        const int64_t first = static_cast<int64_t>(c.a_row) + r0;
-        float sum[kMats][kChunks][16];
+    const F8Item c = find_item();
+    if (c.rows > 0) {
+      const float* ws = args.w_scales + (static_cast<int64_t>(c.expert) * kMats * nblocks + c.n0 / kF8Block) * kiters;
+      const int rows16 = (c.rows + 15) & ~15;
+      float sum[kMats][kChunks][16];
 #pragma unroll
-        for (int ch = 0; ch < kChunks; ++ch)
+      for (int ch = 0; ch < kChunks; ++ch)
 #pragma unroll
-          for (int m = 0; m < kMats; ++m)
+        for (int m = 0; m < kMats; ++m)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sum[m][ch][j] = 0.0f;
-        const int most = min(Plan::kTable / rows16, Plan::kTableSteps);
-        int filled = part.kb0, base = part.kb0;  // the table holds the scales of steps [base, filled)
-        for (int kb = joining ? part.kb1 : part.kb0; kb < part.kb1;) {
-          if (kb == filled) {
-            if (!meet()) {  // (everyone is done with what it held)
-              ok = false;
-              break;
-            }
-            base = kb;
-            const int steps = min(part.kb1 - kb, most);
-            filled = kb + steps;
+          for (int j = 0; j < 16; ++j) sum[m][ch][j] = 0.0f;
+      const int most = min(Plan::kTable / rows16, Plan::kTableSteps);
+      int filled = kb0, base = kb0;  // the table holds the scales of steps [base, filled)
+      for (int kb = kb0; kb < kb1;) {
+        if (kb == filled) {
+          if (!meet()) {  // (everyone is done with what it held)
+            ok = false;
+            break;
+          }
+          base = kb;
+          const int steps = min(kb1 - kb, most);
+          filled = kb + steps;
 #pragma unroll 1
-            for (int rr = warp - 4; rr < rows; rr += kEpilogueWarps)
-              for (int s = lane; s < steps; s += 32) table[s * rows16 + rr] = args.x_scales[(first + rr) * kblocks + kb + s];
-            if (warp < 4 + kMats)
-              for (int s = lane; s < steps; s += 32)
-                weight_table[(warp - 4) * Plan::kTableSteps + s] = ws[static_cast<int64_t>(warp - 4) * nblocks * kblocks + kb + s];
-            if (!meet()) {
-              ok = false;
-              break;
-            }
-          }
-          if (!CLUSTERED && !arrived && i >= split.items && kb - base >= 8) arrive();
-          // Two steps at a time where there are two: a step is a chain of waits (sums there, sums fetched) of about 350 ns, which is what
-          // 16 KB of weights take to arrive.
-          constexpr int kTogether = 2;
-          const int together = kb + 1 < filled && (acc & 1) == 0 ? 2 : 1;
-#pragma unroll
-          for (int t = 0; t < kTogether; ++t)
-            if (t < together && ok &&
-                !__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar + 8 * (acc + t), acc_phase, wctx, DS_TIMEOUT_EPILOGUE))) ok = false;
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int ch = 0; ch < kChunks; ++ch) {
-            const int col = 16 * (2 * ch + half);
-            if (col < rows) {
-              uint32_t v[kTogether][kMats][16];
-#pragma unroll
-              for (int t = 0; t < kTogether; ++t)
-                if (t < together) {
-#pragma unroll
-                  for (int m = 0; m < kMats; ++m) tmem_ld_32x16(tmem_base + lanes + (acc + t) * Plan::kAccCols + m * R + col, v[t][m]);
-                }
-#pragma unroll
-              for (int t = 0; t < kTogether; ++t)
-                if (t < together) {
-                  const float* xs = table + (kb + t - base) * rows16 + col;
-                  const float a0 = weight_table[kb + t - base], b0 = kGlu ? weight_table[Plan::kTableSteps + kb + t - base] : 0.0f;
-                  float x[16];
-#pragma unroll
-                  for (int j = 0; j < 16; j += 4) {
-                    const float4 q = *reinterpret_cast<const float4*>(xs + j);
-                    x[j] = q.x;
-                    x[j + 1] = q.y;
-                    x[j + 2] = q.z;
-                    x[j + 3] = q.w;
-                  }
-#pragma unroll
-                  for (int m = 0; m < kMats; ++m) tmem_ld_wait16(v[t][m]);
-#pragma unroll
-                  for (int j = 0; j < 16; ++j) {
-                    sum[0][ch][j] = fmaf(__uint_as_float(v[t][0][j]), x[j] * a0, sum[0][ch][j]);
-                    if (kGlu) sum[kMats - 1][ch][j] = fmaf(__uint_as_float(v[t][kMats - 1][j]), x[j] * b0, sum[kMats - 1][ch][j]);
-                  }
-                }
-            }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane < together) mbar_arrive(tempty_bar + 8 * (acc + lane));
-          kb += together;
-          acc += together;
-          if (acc == kAccs) { acc = 0; acc_phase ^= 1; }
-        }
-        if (!ok) break;
-        if constexpr (CLUSTERED) {
-          // (the last products have read the ring; its memory takes the sums, [row][column])
-          float* to = reinterpret_cast<float*>(tiles) + quad * 32 + lane;
-#pragma unroll
-          for (int ch = 0; ch < kChunks; ++ch) {
-            const int col = 16 * (2 * ch + half);
-            if (col >= rows) continue;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) to[(col + j) * 128] = sum[0][ch][j];
-          }
-          continue;
-        }
-        if (part.shared) {
-          // (R rows at most: one pass)
-          constexpr int kSlot = kMats * R * 128;  // floats: [matrix][four rows][lane][row of the four]
-          const int first_worker = split.worker_of(static_cast<int64_t>(part.item) * kiters);
-          const int last_worker = split.worker_of(static_cast<int64_t>(part.item + 1) * kiters - 1);
-          // a worker's slots: of the item it shares with those before it, and of the one it begins
-          const auto slot_of = [&](int worker) {
-            return reinterpret_cast<float4*>(args.partials + static_cast<int64_t>(2 * worker + (worker == first_worker ? 1 : 0)) * kSlot) +
-                   quad * 32 + lane;
-          };
-          if (!joining) {
-            float4* mine = slot_of(blockIdx.x);
-#pragma unroll
-            for (int ch = 0; ch < kChunks; ++ch) {
-              const int col = 16 * (2 * ch + half);
-              if (col >= rows) continue;
-#pragma unroll
-              for (int m = 0; m < kMats; ++m)
-#pragma unroll
-                for (int j = 0; j < 16; j += 4)
-                  __stcg(mine + (m * R + col + j) / 4 * 128,
-                         make_float4(sum[m][ch][j], sum[m][ch][j + 1], sum[m][ch][j + 2], sum[m][ch][j + 3]));
-            }
-            continue;
-          }
-#pragma unroll
-          for (int ch = 0; ch < kChunks; ++ch) {
-            const int col = 16 * (2 * ch + half);
-            if (col >= rows) continue;
-#pragma unroll
-            for (int m = 0; m < kMats; ++m)
-#pragma unroll
-              for (int j = 0; j < 16; ++j) sum[m][ch][j] = 0.0f;
-#pragma unroll 2
-            for (int w = first_worker; w <= last_worker; ++w) {
-              const float4* from = slot_of(w);
-              float4 v[kMats][4];
-#pragma unroll
-              for (int m = 0; m < kMats; ++m)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[m][j] = __ldcg(from + ((m * R + col) / 4 + j) * 128);
-#pragma unroll
-              for (int m = 0; m < kMats; ++m)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  sum[m][ch][4 * j] += v[m][j].x;
-                  sum[m][ch][4 * j + 1] += v[m][j].y;
-                  sum[m][ch][4 * j + 2] += v[m][j].z;
-                  sum[m][ch][4 * j + 3] += v[m][j].w;
-                }
-            }
-          }
-        }
-        // The results, 16 rows at a time: the warps that have them leave them in shared memory, then every warp takes rows, 128 columns
-        // (a block) over its lanes.  A loop of little code: the weights that stream through L2 throw instructions out of it, and
-        // each line that has to be fetched again behind them takes a microsecond (unrolled over rows and groups this took 5 us
-        // after the last step, at one token).
-#pragma unroll 1
-        for (int q = 0; 16 * q < rows; ++q) {
-          if ((q & 1) == half) {
-            // (constant indexes, group by group: an index that varies would put the sums into local memory)
-            float* to = staging + quad * 32 + lane;
-            const auto put = [&](auto group) {
-              constexpr int ch = decltype(group)::value;
-              if constexpr (ch < kChunks) {
-#pragma unroll
-                for (int m = 0; m < kMats; ++m)
-#pragma unroll
-                  for (int j = 0; j < 16; ++j) to[(m * 16 + j) * 128] = sum[m][ch][j];
-              }
-            };
-            switch (q >> 1) {
-              case 0: put(std::integral_constant<int, 0>()); break;
-              case 1: put(std::integral_constant<int, 1>()); break;
-              case 2: put(std::integral_constant<int, 2>()); break;
-              default: put(std::integral_constant<int, 3>()); break;
-            }
-          }
+          for (int rr = warp - 4; rr < c.rows; rr += kEpilogueWarps)
+            for (int s = lane; s < steps; s += 32) table[s * rows16 + rr] = args.x_scales[(static_cast<int64_t>(c.a_row) + rr) * kiters + kb + s];
+          if (warp < 4 + kMats)
+            for (int s = lane; s < steps; s += 32)
+              weight_table[(warp - 4) * Plan::kTableSteps + s] = ws[static_cast<int64_t>(warp - 4) * nblocks * kiters + kb + s];
           if (!meet()) {
             ok = false;
             break;
           }
-          const int live = min(rows - 16 * q, 16);
-          const int col = c.n0 + 4 * lane;
-#pragma unroll 1
-          for (int rr = warp - 4; rr < live; rr += kEpilogueWarps) {
-            const float4 v = *reinterpret_cast<const float4*>(staging + rr * 128 + 4 * lane);
-            float f[4] = {v.x, v.y, v.z, v.w};
-            act_row<4>(f, args.act);
-            if (kGlu) {
-              const float4 u = *reinterpret_cast<const float4*>(staging + (16 + rr) * 128 + 4 * lane);
-              f[0] *= u.x;
-              f[1] *= u.y;
-              f[2] *= u.z;
-              f[3] *= u.w;
-            }
-            int64_t row = first + 16 * q + rr;
-            if constexpr (OUT == F8_ROWS) {
-              if (args.out_perm != nullptr) row = args.out_perm[row];
-              if (row >= 0 && row < args.out_rows && col < args.n_dim)
-                *reinterpret_cast<uint2*>(static_cast<T*>(args.out) + row * args.n_dim + col) =
-                    make_uint2(Elem<T>::pack2(f[0], f[1]), Elem<T>::pack2(f[2], f[3]));
-            } else {
-              float most = kF8Least;
+        }
+        // Two steps at a time where there are two: a step is a chain of waits (sums there, sums fetched) of about 350 ns, which is what
+        // 16 KB of weights take to arrive.
+        const int together = kb + 1 < filled && (acc & 1) == 0 ? 2 : 1;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(f[j]));
-              most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));  // (non-negative: ordered as integers)
-              const float inv = kF8Top / most;
-              if (col < args.n_dim)
-                *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(args.out) + row * args.n_dim + col) =
-                    f8x4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-              if (lane == 0) args.out_scales[row * nblocks + c.n0 / kF8Block] = most / kF8Top;
-            }
-          }
-          if (!meet()) {  // (everyone is done with the staged rows)
+        for (int t = 0; t < 2; ++t)
+          if (t < together && ok && !__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar + 8 * (acc + t), acc_phase, wctx, DS_TIMEOUT_EPILOGUE)))
             ok = false;
-            break;
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+          const int col = 16 * (2 * ch + half);
+          if (col < c.rows) {
+            uint32_t v[2][kMats][16];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (t < together) {
+#pragma unroll
+                for (int m = 0; m < kMats; ++m) tmem_ld_32x16(tmem_base + lanes + (acc + t) * Plan::kAccCols + m * R + col, v[t][m]);
+              }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (t < together) {
+                const float* xs = table + (kb + t - base) * rows16 + col;
+                const float a0 = weight_table[kb + t - base], b0 = kGlu ? weight_table[Plan::kTableSteps + kb + t - base] : 0.0f;
+                float x[16];
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  const float4 q = *reinterpret_cast<const float4*>(xs + j);
+                  x[j] = q.x;
+                  x[j + 1] = q.y;
+                  x[j + 2] = q.z;
+                  x[j + 3] = q.w;
+                }
+#pragma unroll
+                for (int m = 0; m < kMats; ++m) tmem_ld_wait16(v[t][m]);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  sum[0][ch][j] = fmaf(__uint_as_float(v[t][0][j]), x[j] * a0, sum[0][ch][j]);
+                  if (kGlu) sum[kMats - 1][ch][j] = fmaf(__uint_as_float(v[t][kMats - 1][j]), x[j] * b0, sum[kMats - 1][ch][j]);
+                }
+              }
           }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane < together) mbar_arrive(tempty_bar + 8 * (acc + lane));
+        kb += together;
+        acc += together;
+        if (acc == kAccs) { acc = 0; acc_phase ^= 1; }
+      }
+      if (ok) {
+        // (every product that read the ring is complete; its memory takes the sums: [matrix][row][column])
+        float* to = reinterpret_cast<float*>(tiles) + quad * 32 + lane;
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+          const int col = 16 * (2 * ch + half);
+          if (col >= c.rows) continue;
+#pragma unroll
+          for (int m = 0; m < kMats; ++m)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) to[(m * R + col + j) * 128] = sum[m][ch][j];
         }
       }
     }
-    if constexpr (CLUSTERED) {
-      __syncwarp();
-      cluster_sync_all();  // every CTA's sums are there
-      // a part of the rows for each CTA, a row per warp; the sums are added in the order of K
-      const F8Part part = split.get(0, args, R);
-      const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-      const int end = part.c.rows * (rank + 1) / ranks;
-      const int col = part.c.n0 + 4 * lane;
+    __syncwarp();
+    cluster_sync_all();  // every CTA's sums are there
+    // a part of the rows for each CTA, a row (a block of 128 columns) per warp
+    const int end = c.rows * (rank + 1) / ranks;
+    const int col = c.n0 + 4 * lane;
 #pragma unroll 1
-      for (int rr = part.c.rows * rank / ranks + warp - 4; ok && rr < end; rr += kEpilogueWarps) {
+    for (int rr = c.rows * rank / ranks + warp - 4; ok && rr < end; rr += kEpilogueWarps) {
+      float f[kMats][4];
+#pragma unroll
+      for (int m = 0; m < kMats; ++m) {
         float4 v[kF8MostRanks];
 #pragma unroll
         for (int w = 0; w < kF8MostRanks; ++w)
-          if (w < ranks) v[w] = ld_cluster_v4(mapa_shared(tiles_addr + (rr * 128 + 4 * lane) * 4, static_cast<uint32_t>(w)));
-        float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (w < ranks) v[w] = ld_cluster_v4(mapa_shared(tiles_addr + ((m * R + rr) * 128 + 4 * lane) * 4, static_cast<uint32_t>(w)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[m][j] = 0.0f;
 #pragma unroll
         for (int w = 0; w < kF8MostRanks; ++w)
           if (w < ranks) {
-            f[0] += v[w].x;
-            f[1] += v[w].y;
-            f[2] += v[w].z;
-            f[3] += v[w].w;
+            f[m][0] += v[w].x;
+            f[m][1] += v[w].y;
+            f[m][2] += v[w].z;
+            f[m][3] += v[w].w;
           }
-        act_row<4>(f, args.act);
+      }
+      act_row<4>(f[0], args.act);
+      if (kGlu) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[0][j] *= f[kMats - 1][j];
+      }
+      int64_t row = static_cast<int64_t>(c.a_row) + rr;
+      if constexpr (OUT == F8_ROWS) {
+        if (args.out_perm != nullptr) row = args.out_perm[row];
+        if (row >= 0 && row < args.out_rows && col < args.n_dim)
+          *reinterpret_cast<uint2*>(static_cast<T*>(args.out) + row * args.n_dim + col) =
+              make_uint2(Elem<T>::pack2(f[0][0], f[0][1]), Elem<T>::pack2(f[0][2], f[0][3]));
+      } else {
+        float most = kF8Least;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(f[0][j]));
+        most = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(most)));  // (non-negative: ordered as integers)
+        const float inv = kF8Top / most;
         if (col < args.n_dim)
-          *reinterpret_cast<uint2*>(static_cast<T*>(args.out) + static_cast<int64_t>(part.c.a_row + rr) * args.n_dim + col) =
-              make_uint2(Elem<T>::pack2(f[0], f[1]), Elem<T>::pack2(f[2], f[3]));
+          *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(args.out) + row * args.n_dim + col) =
+              f8x4(f[0][0] * inv, f[0][1] * inv, f[0][2] * inv, f[0][3] * inv);
+        if (lane == 0) args.out_scales[row * nblocks + c.n0 / kF8Block] = most / kF8Top;
       }
     }
   } else {
     fewer_registers<72>();
     if (warp == 0) {
       // ------------------------------ TMA producer ------------------------------
-      int stage = 0;
-      uint32_t phase = 0;
       bool ok = true;
       const uint64_t pol = l2_policy_evict_normal();
-      const auto load_weights = [&](int st, int kb, const F8Item& c, int groups) {
+      // Where the maps are complete before the kernel before (which waited for them itself) lets this one up, the first weights are
+      // asked for before the wait for it: that one writes the rows.
+      if (!args.maps_before) await_predecessor();
+      const F8Item c = find_item();
+      const int groups = (c.rows + 15) >> 4;
+      const int ahead = c.rows > 0 ? min(kb1 - kb0, kStages) : 0;
+      const auto load_weights = [&](int st, int kb) {
         const uint32_t sw = tiles_addr + st * Plan::kStageBytes;
         mbar_arrive_expect_tx(full_bar + 8 * st, Plan::kWBytes + groups * 16 * kF8K);
 #pragma unroll
         for (int m = 0; m < kMats; ++m)
           tma_load_3d(sw + m * kF8Tile, &tmap_w, kb * (kF8K / 2), c.n0, kMats * c.expert + m, full_bar + 8 * st, pol);
       };
-      const auto load_rows = [&](int st, int kb, const F8Item& c, int r0, int groups) {
+      const auto load_rows = [&](int st, int kb) {
         const uint32_t sx = tiles_addr + st * Plan::kStageBytes + Plan::kWBytes;
-        for (int g = 0; g < groups; ++g)
-          tma_load_2d(sx + g * 16 * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + r0 + 16 * g, full_bar + 8 * st, pol);
+        for (int g = 0; g < groups; ++g) tma_load_2d(sx + g * 16 * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + 16 * g, full_bar + 8 * st, pol);
       };
-      bool waited = false;
-      for (int i = 0; ok; ++i) {
-        const F8Part part = split.get(i, args, R);
-        if (!part.valid) break;
-        const F8Item& c = part.c;
-        if (part.kb0 >= part.kb1) continue;
-        for (int r0 = 0; r0 < c.rows && ok; r0 += R) {
-          const int groups = (min(c.rows - r0, R) + 15) >> 4;
-          int kb = part.kb0;
-          if (!waited) {
-            const int ahead = min(part.kb1 - kb, kStages);
-            if (elect_one())
-              for (int st = 0; st < ahead; ++st) load_weights(st, kb + st, c, groups);
-            __syncwarp();
-            await_predecessor();
-            waited = true;
-            if (elect_one())
-              for (int st = 0; st < ahead; ++st) load_rows(st, kb + st, c, r0, groups);
-            __syncwarp();
-            kb += ahead;
-            if ((stage = ahead) == kStages) { stage = 0; phase = 1; }
+      if (elect_one())
+        for (int st = 0; st < ahead; ++st) load_weights(st, kb0 + st);
+      __syncwarp();
+      if (args.maps_before) await_predecessor();
+      if (elect_one())
+        for (int st = 0; st < ahead; ++st) load_rows(st, kb0 + st);
+      __syncwarp();
+      int stage = ahead == kStages ? 0 : ahead;
+      uint32_t phase = ahead == kStages ? 1 : 0;
+      if (c.rows > 0)
+        for (int kb = kb0 + ahead; kb < kb1; ++kb) {
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, wctx, DS_TIMEOUT_PRODUCER))) {
+            ok = false;
+            break;
           }
-          for (; kb < part.kb1; ++kb) {
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, wctx, DS_TIMEOUT_PRODUCER))) {
-              ok = false;
-              break;
-            }
-            if (elect_one()) {
-              load_weights(stage, kb, c, groups);
-              load_rows(stage, kb, c, r0, groups);
-            }
-            __syncwarp();
-            if (++stage == kStages) { stage = 0; phase ^= 1; }
+          if (elect_one()) {
+            load_weights(stage, kb);
+            load_rows(stage, kb);
           }
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
-      }
-      if (!waited) await_predecessor();
       grid_release();
       if (!ok || *abort_flag) {
-        for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+        for (int i = 0; i < 2000; ++i) __nanosleep(1000);  // copies already issued land before the CTA ends
       }
     } else if (warp == 1) {
       // ------------------------------ MMA issuer --------------------------------
@@ -1171,49 +938,42 @@ f8_lanes_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       await_predecessor();  // (the limits of the waits below are not to run out on the kernel before)
-      for (int i = 0; ok; ++i) {
-        const F8Part part = split.get(i, args, R);
-        if (!part.valid) break;
-        const F8Item& c = part.c;
-        for (int r0 = 0; r0 < c.rows && ok; r0 += R) {
-          const uint32_t idesc = f8_idesc(BM, (min(c.rows - r0, R) + 15) & ~15);
-          for (int kb = part.kb0; kb < part.kb1; ++kb) {
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1, wctx, DS_TIMEOUT_MMA)) ||
-                !__all_sync(0xFFFFFFFFu, mbar_wait(full_bar + 8 * stage, phase, wctx, DS_TIMEOUT_MMA))) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            if (elect_one()) {
-              const uint32_t sw = tiles_addr + stage * Plan::kStageBytes;
-#pragma unroll
-              for (int m = 0; m < kMats; ++m)
-#pragma unroll
-                for (int k = 0; k < kF8K / kF8MmaK; ++k)
-                  umma_f8(tmem_base + acc * Plan::kAccCols + m * R, make_desc(sw + m * kF8Tile + k * kF8MmaK, 16, 1024),
-                          make_desc(sw + Plan::kWBytes + k * kF8MmaK, 16, 1024), idesc, k != 0 ? 1u : 0u);
-              umma_commit(empty_bar + 8 * stage);
-              umma_commit(tfull_bar + 8 * acc);
-            }
-            __syncwarp();
-            if (++stage == kStages) { stage = 0; phase ^= 1; }
-            if (++acc == kAccs) { acc = 0; acc_phase ^= 1; }
+      const F8Item c = find_item();
+      const uint32_t idesc = f8_idesc(BM, (c.rows + 15) & ~15);
+      if (c.rows > 0)
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!__all_sync(0xFFFFFFFFu, mbar_wait(tempty_bar + 8 * acc, acc_phase ^ 1, wctx, DS_TIMEOUT_MMA)) ||
+              !__all_sync(0xFFFFFFFFu, mbar_wait(full_bar + 8 * stage, phase, wctx, DS_TIMEOUT_MMA))) {
+            ok = false;
+            break;
           }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t sw = tiles_addr + stage * Plan::kStageBytes;
+#pragma unroll
+            for (int m = 0; m < kMats; ++m)
+#pragma unroll
+              for (int k = 0; k < kF8K / kF8MmaK; ++k)
+                umma_f8(tmem_base + acc * Plan::kAccCols + m * R, make_desc(sw + m * kF8Tile + k * kF8MmaK, 16, 1024),
+                        make_desc(sw + Plan::kWBytes + k * kF8MmaK, 16, 1024), idesc, k != 0 ? 1u : 0u);
+            umma_commit(empty_bar + 8 * stage);
+            umma_commit(tfull_bar + 8 * acc);
+          }
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
+          if (++acc == kAccs) { acc = 0; acc_phase ^= 1; }
         }
-      }
       if (!ok || *abort_flag) {
         for (int i = 0; i < 2000; ++i) __nanosleep(1000);
       }
     }
-    if constexpr (CLUSTERED) {
-      __syncwarp();
-      cluster_sync_all();
-    }
+    __syncwarp();
+    cluster_sync_all();
   }
 
   tc_fence_before();
   __syncthreads();
-  if constexpr (CLUSTERED) cluster_sync_all();  // no CTA ends while another reads its sums
+  cluster_sync_all();  // no CTA ends while another reads its sums
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();

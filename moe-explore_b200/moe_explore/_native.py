@@ -67,7 +67,7 @@ class F8Pass(ctypes.Structure):
                                         "pad_offsets", "row_src", "dst_row", "mtile_expert", "tile_pairs", "num_mtiles", "status",
                                         "workspace")] + \
                [("workspace_bytes", c_size_t)] + \
-               [(f, c_void_p) for f in ("xs", "xs_scales", "hidden", "hidden_scales", "ys", "out", "addend", "partials")]
+               [(f, c_void_p) for f in ("xs", "xs_scales", "hidden", "hidden_scales", "ys", "out", "addend")]
 
 
 class F8RowsPass(ctypes.Structure):
@@ -75,8 +75,7 @@ class F8RowsPass(ctypes.Structure):
     _fields_ = [(f, c_int64) for f in ("num_rows", "x_rows")] + \
                [(f, c_int32) for f in ("num_experts", "k_dim", "n_dim", "topk", "act", "dtype", "gather", "scatter")] + \
                [(f, c_void_p) for f in ("x", "x_scales", "w", "w_scales", "out", "group_indices", "perm", "pad_offsets", "mtile_expert",
-                                        "tile_pairs", "num_mtiles", "status", "gathered", "gathered_scales",
-                                        "partials")]
+                                        "tile_pairs", "num_mtiles", "status", "gathered", "gathered_scales")]
 
 
 # name -> (restype, argtypes); the single source for both binding and the symbol-export test
@@ -123,7 +122,6 @@ SIGNATURES = {
     "moe_f8_quantize_rows": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p]),
     "moe_f8_pass_size": (c_size_t, []),
     "moe_f8_expert_forward": (c_int, [POINTER(F8Pass), c_int, c_void_p]),
-    "moe_f8_partial_bytes": (c_size_t, [c_int64, c_int, c_int]),
     "moe_f8_rows_pass_size": (c_size_t, []),
     "moe_f8_rows_gemm": (c_int, [POINTER(F8RowsPass), c_int, c_void_p]),
     "moe_rows_pass_size": (c_size_t, []),
@@ -462,11 +460,6 @@ def rms_norm_backward(dy, dh, h, weight, rstd):
     _check("moe_rms_norm_backward", rc)
     _count(2)
     return dx, dw
-
-
-@functools.lru_cache(maxsize=1024)
-def f8_partial_bytes(num_rows: int, num_experts: int, act_code: int) -> int:
-    return int(load().moe_f8_partial_bytes(num_rows, num_experts, act_code))
 
 
 def f8_quantize_rows(x, q, scales):

@@ -479,15 +479,14 @@ def fp8_expert_compute(x, scores, indices, params: Fp8ExpertParams, addend=None)
         workspace = None
         if launches > 1:
             workspace = torch.empty(max(_native.routing_workspace_bytes(num_rows, E), 16), dtype=torch.uint8, device=data.device)
-        held, (words, xs, xs_scales, hidden, hidden_scales, ys, partials) = _buffers(
-            (4 * num_words, rp * d, 4 * rp * blocks(d), rp * inter, 4 * rp * blocks(inter), 2 * rp * d,
-             _native.f8_partial_bytes(num_rows, E, _native.ACT_CODES[act])), data.device)
+        held, (words, xs, xs_scales, hidden, hidden_scales, ys) = _buffers(
+            (4 * num_words, rp * d, 4 * rp * blocks(d), rp * inter, 4 * rp * blocks(inter), 2 * rp * d), data.device)
         ptr = _native._ptr
         p = _native.F8Pass(T, rp, d, inter, E, topk, _native.ACT_CODES[act], _native.dtype_code(dtype), ids.data_ptr(), data.data_ptr(),
                            ptr(x_scales), scores.data_ptr(), up.data_ptr(), up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(),
                            *_packed_pointers(words, offsets, device_status(data.get_device())), ptr(workspace),
                            0 if workspace is None else workspace.numel(), xs, xs_scales, hidden, hidden_scales, ys, out.data_ptr(),
-                           ptr(addend), partials)
+                           ptr(addend))
         _native.run_pass("moe_f8_expert_forward", p, [
             (_native.F8_ROUTE, "routing", launches), (_native.F8_DISPATCH, "rows:gather", 1), (_native.F8_UP, "f8_gemm:up", 1),
             (_native.F8_DOWN, "f8_gemm:down", 1), (_native.F8_FOLD, "rows:combine", 1)], num_rows)

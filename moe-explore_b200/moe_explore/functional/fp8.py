@@ -170,9 +170,5 @@ def fp8_rows_gemm(rows: Fp8Rows, weight: Fp8Weight, group_indices, permute_indic
             gathered_scales = torch.empty(num_rows, blocks(k), dtype=torch.float32, device=device)
             p.gathered, p.gathered_scales = gathered.data_ptr(), gathered_scales.data_ptr()
             steps.insert(-1, (_native.ROWS_GATHER, "rows:f8", 1))
-        partial_bytes = _native.f8_partial_bytes(num_rows, E, _native.ACT_CODES[act])
-        if partial_bytes:
-            partials = torch.empty(partial_bytes, dtype=torch.uint8, device=device)
-            p.partials = partials.data_ptr()
         _native.run_pass("moe_f8_rows_gemm", p, steps, num_rows)
     return out
