@@ -156,9 +156,8 @@ int combine_bwd_tokens(const void* dout, const void* scores, const void* ys, con
                        void* stream, bool live_blocks_only, uint32_t* work_counters);
 
 // Tensor map of 16-bit elements (grouped_gemm.cu), kept for the next call that asks for the same.
-constexpr int kNoSwizzle = 0, kSwizzle128 = 1, kSwizzle64 = 2;
 int make_tmap(CUtensorMap* map, int dtype, const void* ptr, int rank, const uint64_t* dims, const uint32_t* box,
-              const uint64_t* strides = nullptr, int swizzle = kSwizzle128);
+              const uint64_t* strides = nullptr, bool swizzle = true);
 
 // Status codes written by kernels into the caller's device status word.
 enum DeviceStatus : int {

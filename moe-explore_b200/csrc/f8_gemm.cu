@@ -72,8 +72,8 @@ static int f8_maps(CUtensorMap* tx, CUtensorMap* tw, const void* x, int64_t rows
 
 // The kernel with the weights on the lanes: how many items there can be (an expert each, in blocks of 128 columns) and how many
 // CTAs share one; none where it does not serve.  It does for 64 rows in all and no more items than SMs: 29 MB of one matrix
-// (7168 x 4096) take 11 to 15 us so and 29 with rows on the lanes; the 2 x 32 items of one token's down products (14336 x 4096) XX
-// us instead of YY.
+// (7168 x 4096) take 11 to 15 us so and 29 with rows on the lanes; the 2 x 32 items of one token's down products (14336 x 4096) 31
+// instead of 63 (as a part of the pass, waiting for the up products included).
 struct F8Lanes {
   int items, ranks;
 };

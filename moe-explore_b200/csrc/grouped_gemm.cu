@@ -93,7 +93,7 @@ static int g_tmap_used = 0, g_tmap_next = 0;
 // Tensor map (by default with the 128-byte swizzle); dims[0] is the contiguous dimension.  `strides` (bytes, for dims 1..rank-1)
 // may be null for a dense row-major tensor.
 int make_tmap(CUtensorMap* map, int dtype, const void* ptr, int rank, const uint64_t* dims, const uint32_t* box,
-              const uint64_t* strides, int swizzle) {
+              const uint64_t* strides, bool swizzle) {
   TmapKey key{};
   key.ptr = ptr;
   key.dtype = dtype;
@@ -130,7 +130,7 @@ int make_tmap(CUtensorMap* map, int dtype, const void* ptr, int rank, const uint
   }
   CUresult r = fn(map, dtype == MOE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                   rank, const_cast<void*>(ptr), gdim, gstride, bdim, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle == kSwizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : swizzle == kSwizzle64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed with CUresult %d (rank %d, dims %llu x %llu x %llu)", (int)r, rank,
               (unsigned long long)dims[0], (unsigned long long)(rank > 1 ? dims[1] : 1),

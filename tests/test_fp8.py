@@ -304,6 +304,65 @@ def test_experts(T, E, k, d, inter, favour, act, native):
     check_experts(fp8_expert_compute(x, scores, ids, p, addend=addend), rows, scores, ids, p, addend)
 
 
+# few rows and deep products: K split over clusters of 2 to 8 CTAs; fewer experts hit than there could be; one row for each of many
+# experts; a wide result (more blocks than SMs); 64 rows of one expert, and 65
+DEEP = [(1, 8, 2, 2048, 1024, 0), (1, 4, 1, 8192, 256, 0), (9, 8, 3, 4096, 400, 30), (4, 300, 8, 1040, 128, 0), (2, 3, 3, 256, 7168, 0),
+        (21, 64, 3, 2064, 272, 0), (64, 2, 1, 1024, 1536, 30), (65, 2, 1, 1024, 1536, 30), (3, 16, 8, 128, 2560, 0)]
+
+
+@gpu
+@pytest.mark.parametrize("act", ["swiglu", "gelu"])
+@pytest.mark.parametrize("T,E,k,d,inter,favour", DEEP)
+def test_experts_of_few_rows(T, E, k, d, inter, favour, act, native):
+    from moe_explore.expert_compute import fp8_expert_compute
+
+    g = gen(T + E + d)
+    p = make_experts(g, E, d, inter, act)
+    x = torch.randn(T, d, generator=g, device="cuda").bfloat16()
+    scores, ids = routing(g, T, E, k, torch.bfloat16, favour)
+    out = fp8_expert_compute(x, scores, ids, p)
+    check_experts(out, quantize_rows(x), scores, ids, p)
+    ids[:] = ids[:, :1]                                   # one expert for all of a token's slots
+    out = fp8_expert_compute(x, scores, ids, p)
+    check_experts(out, quantize_rows(x), scores, ids, p)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = fp8_expert_compute(x, scores, ids, p)
+    for shift in (0, 1, 2):                               # the maps of every replay are its own
+        ids.add_(shift).remainder_(E)
+        graph.replay()
+        assert torch.equal(again, fp8_expert_compute(x, scores, ids, p))
+
+
+@gpu
+@pytest.mark.parametrize("counts", [[1, 0, 3], [0] * 30 + [7], [1] * 40, [64], [30, 34, 0], [10, 55, 0], [200, 90, 110, 80]], ids=str)
+@pytest.mark.parametrize("n,k", [(264, 4096), (2048, 1040)])
+def test_deep_grouped_product(n, k, counts, native):
+    """The product right behind the kernel that makes its maps, eager and replayed with other groups."""
+    g = gen(n)
+    groups, owner, w, rows = grouped_case(g, counts, k, n)
+    x = random_rows(g, rows, k)
+    perm = torch.randperm(rows, generator=g, device="cuda")
+    plain = MGroupedGEMMParams(w, groups, None, False, False, rows, 1)
+    moved = MGroupedGEMMParams(w, groups, perm, True, True, rows, 1)
+    graph = torch.cuda.CUDAGraph()
+    m_grouped_gemm(x, plain)
+    with torch.cuda.graph(graph):
+        out, there = m_grouped_gemm(x, plain), m_grouped_gemm(x, moved)
+    for turn in range(2):
+        if turn == 1:
+            counts = counts[::-1]
+            groups.copy_(torch.tensor([0] + counts, device="cuda").cumsum(0))
+            owner = torch.repeat_interleave(torch.arange(len(counts), device="cuda"), torch.tensor(counts, device="cuda"))
+        graph.replay()
+        assert torch.equal(out, m_grouped_gemm(x, plain))
+        for e in range(len(counts)):
+            if counts[e]:
+                check_product(out[owner == e], rows64(x)[owner == e], weight64(Fp8Weight(w.data[e], w.scales[e])), torch.bfloat16)
+                at = perm[owner == e]
+                check_product(there[at], rows64(x)[at], weight64(Fp8Weight(w.data[e], w.scales[e])), torch.bfloat16)
+
+
 @gpu
 def test_ids_out_of_range_add_nothing_and_are_reported(native):
     from moe_explore.expert_compute import fp8_expert_compute
