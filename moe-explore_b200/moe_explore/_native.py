@@ -12,6 +12,7 @@ import os
 from ctypes import c_float, c_int, c_int32, c_int64, c_size_t, c_void_p, c_char_p, POINTER
 
 import torch
+from torch.autograd import forward_ad
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 # MOE_SM100_LIBRARY points at another build of the same library (e.g. one compiled with instrumentation)
@@ -227,6 +228,13 @@ def _stream():
 def on_device_of(t: torch.Tensor):
     """Context in which the launches go to the current stream of the tensor's device."""
     return _NO_SECTION if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def needs_gradient(*tensors) -> bool:
+    """Whether a derivative with respect to one of the tensors is asked for, backwards or forwards."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def dtype_code(dtype: torch.dtype) -> int:

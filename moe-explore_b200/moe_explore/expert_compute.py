@@ -460,7 +460,7 @@ def fp8_expert_compute(x, scores, indices, params: Fp8ExpertParams, addend=None)
         raise ValueError("indices (int64) and scores are [tokens, k]")
     if any(t.device != data.device for t in (scores, indices, params.up.data, params.down.data) + (() if addend is None else (addend,))):
         raise ValueError("all tensors lie on the device of the input")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (data, scores, addend)):
+    if _native.needs_gradient(data, scores, addend):
         raise RuntimeError("experts in 8 bits have no backward pass: call this under torch.no_grad(), or train 16-bit experts")
     if addend is not None and (addend.shape != (T, d) or addend.dtype is not dtype):
         raise ValueError("addend is like the result")

@@ -70,7 +70,7 @@ def quantize_rows(x: torch.Tensor) -> Fp8Rows:
     _native.require_cuda(x)
     if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"quantize_rows takes bf16 or fp16 [R, K], got {x.dtype} {tuple(x.shape)}")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _native.needs_gradient(x):
         raise RuntimeError("8-bit rows have no backward pass: call this under torch.no_grad()")
     with _native.on_device_of(x):
         x = _dense(x.detach())

@@ -80,7 +80,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     all three; d a multiple of 8."""
     _checked(x, weight, residual)
     with _native.on_device_of(x):
-        if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or residual is not None and residual.requires_grad)):
+        if not _native.needs_gradient(x, weight, residual):
             y, h, _ = _forward(x, weight, residual, float(eps), False)
             return y if residual is None else (y, h)
         return _RMSNorm.apply(x, weight, residual, float(eps))
@@ -90,7 +90,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     """The norm's result in 8 bits (``Fp8Rows``), for the 8-bit products of a serving pass: ``rows``, then, with ``with_rows``, the
     same result in 16 bits (what a router reads), then, with ``residual``, ``x + residual``.  No gradient; d a multiple of 16."""
     _checked(x, weight, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    if _native.needs_gradient(x, weight, residual):
         raise RuntimeError("rms_norm_fp8 has no backward pass: call it under torch.no_grad(), or train with rms_norm")
     d = x.size(-1)
     if d % 16 != 0:

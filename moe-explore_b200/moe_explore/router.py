@@ -189,7 +189,7 @@ def grouped_topk_of_logits(logits: torch.Tensor, params: GroupedTopkRouterParams
             raise ValueError("bias is fp32 [experts] on the device of the logits")
         bias = bias.detach().contiguous()
     with _native.on_device_of(logits):
-        if not (logits.requires_grad and torch.is_grad_enabled()):
+        if not _native.needs_gradient(logits):
             return _grouped_topk(logits.contiguous(), bias, params, dtype)
         return _GroupedTopk.apply(logits.contiguous(), bias, params, dtype)
 

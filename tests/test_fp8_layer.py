@@ -110,3 +110,32 @@ def test_parameters_keep_their_positions():
     """Positional construction as before, the new fields last."""
     p = MOEParams("router", "experts", 8, 2, "shared")
     assert (p.router_params, p.expert_params, p.num_experts, p.topk, p.shared_expert_params, p.norm_params) == ("router", "experts", 8, 2, "shared", None)
+
+
+@gpu
+def test_offsets_past_32_bits(native):
+    """Rows, results and logits of more than 2^31 elements: the last rows are what they are by themselves."""
+    from moe_explore.functional.fp8 import Fp8Rows, Fp8Weight, fp8_matmul, quantize_rows
+    from moe_explore.router import grouped_topk_of_logits
+
+    tail = 300
+    rows, k = 270000, 8192
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    x[-tail:] = torch.randn(tail, k, device="cuda")
+    w = torch.ones(k, device="cuda")
+    q, y = rms_norm_fp8(x, w, with_rows=True)
+    q_tail, y_tail = rms_norm_fp8(x[-tail:].clone(), w, with_rows=True)
+    same = lambda a, b: torch.equal(a.data[-tail:].view(torch.uint8), b.data.view(torch.uint8)) and torch.equal(a.scales[-tail:], b.scales)
+    assert same(q, q_tail) and torch.equal(y[-tail:], y_tail) and same(quantize_rows(x), quantize_rows(x[-tail:].clone()))
+    del x, y
+    up = Fp8Weight((torch.randn(264, k, device="cuda") * 20).to(torch.float8_e4m3fn), torch.ones(3, 64, device="cuda"))
+    assert torch.equal(fp8_matmul(q, up)[-tail:], fp8_matmul(q_tail, up))                    # deep rows
+    wide = Fp8Weight((torch.randn(k, 128, device="cuda") * 20).to(torch.float8_e4m3fn), torch.ones(64, 1, device="cuda"))
+    narrow = Fp8Rows(q.data[:, :128].contiguous(), q.scales[:, :1].contiguous())
+    few = Fp8Rows(narrow.data[-tail:].clone(), narrow.scales[-tail:].clone())
+    assert torch.equal(fp8_matmul(narrow, wide)[-tail:], fp8_matmul(few, wide))              # wide results
+    del q, narrow
+    logits = torch.randn(2100000, 1024, device="cuda").bfloat16()
+    p = GroupedTopkRouterParams(None, 8, num_groups=8, topk_groups=4)
+    for a, b in zip(grouped_topk_of_logits(logits, p), grouped_topk_of_logits(logits[-tail:].clone(), p)):
+        assert torch.equal(a[-tail:], b)

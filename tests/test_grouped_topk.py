@@ -251,3 +251,17 @@ def test_refusals_of_tensors(native):
         grouped_topk_of_logits(x.double(), GroupedTopkRouterParams(None, 2))
     with pytest.raises(native.MoeNativeError, match="equal groups"):
         grouped_topk_of_logits(x, GroupedTopkRouterParams(None, 2, num_groups=3))
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(native):
+    from moe_explore.params import GroupedTopkRouterParams
+    from moe_explore.router import grouped_topk_of_logits
+
+    x = torch.randn(3, 16, device="cuda")
+    p = GroupedTopkRouterParams(None, 2)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(Exception, match="forward"):
+            grouped_topk_of_logits(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), p)
+        scores, indices = grouped_topk_of_logits(x, p)
+        assert scores.shape == indices.shape == (3, 2)

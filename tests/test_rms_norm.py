@@ -235,3 +235,16 @@ def test_refusals_of_tensors(native):
         rms_norm_fp8(x.detach()[:, :40].contiguous()[:, :24], w[:24])
     with pytest.raises(native.MoeNativeError, match="multiple of 8"):
         rms_norm(x.detach()[:, :60].contiguous(), w[:60].contiguous())
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(native):
+    """No derivative is lost in silence: a tangent is refused where there is no formula for it, and only there."""
+    x, r, w = make(4, 64, torch.bfloat16, torch.bfloat16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(Exception, match="forward"):
+            rms_norm(dual, w, residual=r)
+        with pytest.raises(RuntimeError, match="no backward"):
+            rms_norm_fp8(dual, w)
+        assert torch.equal(rms_norm(x, w), rms_norm(x.clone().requires_grad_(True), w))
