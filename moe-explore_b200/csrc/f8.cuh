@@ -40,16 +40,16 @@ __device__ __forceinline__ float block_most(const float (&v)[8]) {
 // "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).  Both sides are first brought by a power of two
 // to where reciprocal and remainder are normal numbers; a value that is not normal then is far below the least 8-bit one.
 // (Eight divisions of their own were 100 instructions per thread, and the kernel of the rows was bound by them.)
-__device__ __forceinline__ void f8_quotients(float (&f)[8], float most) {
+template <int N> __device__ __forceinline__ void f8_quotients(float (&f)[N], float most) {
   if (!(most <= 3.0e38f)) {  // infinite, or nothing is left to spare: as the formula says
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __fdiv_rn(f[i] * 0.875f, most) * 512.0f;
+    for (int i = 0; i < N; ++i) f[i] = __fdiv_rn(f[i] * 0.875f, most) * 512.0f;
     return;
   }
   const float near1 = most >= 1.0f ? 0x1p-60f : 0x1p60f;  // most: 2^-20 to 2^68
   const float d = most * near1, r = __frcp_rn(d);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < N; ++i) {
     const float v = f[i] * (0.875f * near1);
     const float q = v * r;
     f[i] = copysignf(fmaf(fmaf(-q, d, v), r, q) * 512.0f, v);  // (the correction makes -0 a 0)

@@ -166,9 +166,9 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
 }
 
 // ---- rows to 8 bits, and their way to the experts ----
-// Sixteen lanes share a block of 128 columns (8 each).  Every source block is read once and written to `copies` rows:
+// Eight lanes share a block of 128 columns (16 each).  Every source block is read once and written to `copies` rows:
 //   dst_row == nullptr: row t;  otherwise rows dst_row[t * copies + s] (negative: none).
-template <typename T> __device__ __forceinline__ void to_floats(const uint4& u, float (&f)[8]) {
+template <typename T> __device__ __forceinline__ void to_floats(const uint4& u, float* f) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -179,50 +179,68 @@ template <typename T> __device__ __forceinline__ void to_floats(const uint4& u, 
 }
 
 // T: a 16-bit type (rows are converted) or uint8_t (8-bit rows with `scales_in` are copied).
-// A warp takes two blocks of a row at a time, so that the row and where it goes are the whole warp's; the next ones are on their way
-// meanwhile.  Bound by instructions rather than by HBM: everything that counts is 32 bits wide (the host keeps rows x blocks below
-// 2^31) and advances by additions.
-constexpr int kF8RowsCtas = 6;  // per SM
+// A warp takes four blocks of a row at a time, 16 values per lane, so that the row and where it goes are the whole warp's; the next ones
+// are on their way meanwhile.  Everything that counts is 32 bits wide (the host keeps rows x blocks below 2^31) and advances by
+// additions.
+constexpr int kF8RowsCtas = 4;  // per SM
 template <typename T>
 __global__ void __launch_bounds__(256, kF8RowsCtas)
-f8_rows_kernel(const T* x, const float* scales_in, const int32_t* dst_row, int copies, uint2* out, float* scales, int rows, int cols) {
+f8_rows_kernel(const T* x, const float* scales_in, const int32_t* dst_row, int copies, uint4* out, float* scales, int rows, int cols) {
   await_predecessor();  // before the release: what comes up next reads the routing metadata
   grid_release();
   const int blocks = (cols + kF8Block - 1) / kF8Block;
-  const int pairs = (blocks + 1) / 2;
-  const int vecs = cols / 8;
+  const int units = (blocks + 3) / 4;
+  const int vecs = cols / 16;
   const int lane = threadIdx.x & 31;
   const int stride = static_cast<int>(gridDim.x) * 8;
-  const int stride_rows = stride / pairs, stride_pairs = stride - stride_rows * pairs;
+  const int stride_rows = stride / units, stride_units = stride - stride_rows * units;
   const int first = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  int row = first / pairs, pair = first - row * pairs;
-  typedef typename std::conditional<sizeof(T) == 2, uint4, uint2>::type Piece;
-  const auto load = [&](int r, int v) {
-    return r < rows && v < vecs ? reinterpret_cast<const Piece*>(x)[static_cast<int64_t>(r) * vecs + v] : Piece{};
+  int row = first / units, unit = first - row * units;
+  struct Piece {
+    uint4 a, b;
   };
-  Piece next = load(row, pair * 32 + lane);
+  const auto load = [&](int r, int v) {
+    Piece p{};
+    if (r < rows && v < vecs) {
+      const int64_t at = static_cast<int64_t>(r) * vecs + v;
+      if constexpr (sizeof(T) == 2) {
+        p.a = reinterpret_cast<const uint4*>(x)[2 * at];
+        p.b = reinterpret_cast<const uint4*>(x)[2 * at + 1];
+      } else {
+        p.a = reinterpret_cast<const uint4*>(x)[at];
+      }
+    }
+    return p;
+  };
+  Piece next = load(row, unit * 32 + lane);
   while (row < rows) {
     const Piece u = next;
-    const int this_row = row, v = pair * 32 + lane;
+    const int this_row = row, v = unit * 32 + lane;
     row += stride_rows;
-    if ((pair += stride_pairs) >= pairs) {
-      pair -= pairs;
+    if ((unit += stride_units) >= units) {
+      unit -= units;
       ++row;
     }
-    next = load(row, pair * 32 + lane);
-    const int block = v >> 4;
-    const bool ok = v < vecs, has_scale = (lane & 15) == 0 && block < blocks;
-    uint2 q;
+    next = load(row, unit * 32 + lane);
+    const int block = v >> 3;
+    const bool ok = v < vecs, has_scale = (lane & 7) == 0 && block < blocks;
+    uint4 q;
     float scale;
     if constexpr (sizeof(T) == 2) {
-      float f[8];
-      to_floats<T>(u, f);
-      const float most = block_most(f);
+      float f[16];
+      to_floats<T>(u.a, f);
+      to_floats<T>(u.b, f + 8);
+      float most = kF8Least;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(f[i]));
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
       f8_quotients(f, most);
-      q = make_uint2(f8x4(f[0], f[1], f[2], f[3]), f8x4(f[4], f[5], f[6], f[7]));
+      q = make_uint4(f8x4(f[0], f[1], f[2], f[3]), f8x4(f[4], f[5], f[6], f[7]), f8x4(f[8], f[9], f[10], f[11]),
+                     f8x4(f[12], f[13], f[14], f[15]));
       scale = most / kF8Top;
     } else {
-      q = u;
+      q = u.a;
       scale = has_scale ? scales_in[static_cast<int64_t>(this_row) * blocks + block] : 0.0f;
     }
     const auto put = [&](int to) {
@@ -268,7 +286,7 @@ f8_gather_kernel(const uint2* x, const float* scales_in, const int64_t* index, i
 
 static int f8_row_grid(int64_t rows, int cols) {
   const int64_t want = (rows * ((cols + kF8Block - 1) / kF8Block) + 15) / 16;
-  const int64_t most = static_cast<int64_t>(kF8RowsCtas) * sm_count();
+  const int64_t most = 8ll * sm_count();
   return static_cast<int>(want < most ? want : most);
 }
 
@@ -288,8 +306,9 @@ int f8_rows(const char* name, const void* x, const float* x_scales, const int32_
   MOE_CHECK_ARG(aligned16(x) && aligned16(out), "%s: pointers must be 16-byte aligned", name);
   MOE_CHECK_ARG(x_scales != nullptr || dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16, "%s: unknown dtype %d", name, dtype);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int grid = f8_row_grid(rows, cols);  // (16 blocks of 128 columns per CTA)
-  uint2* o = static_cast<uint2*>(out);
+  const int64_t want = (rows * ((cols + 4 * kF8Block - 1) / (4 * kF8Block)) + 7) / 8, most = static_cast<int64_t>(kF8RowsCtas) * sm_count();
+  const int grid = static_cast<int>(want < most ? want : most);
+  uint4* o = static_cast<uint4*>(out);
   if (x_scales != nullptr)
     MOE_CUDA(launch_kernel(f8_rows_kernel<uint8_t>, grid, 256, s, static_cast<const uint8_t*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols));
   else if (dtype == MOE_DTYPE_BF16)
