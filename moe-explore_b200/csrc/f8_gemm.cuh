@@ -329,13 +329,13 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   __syncthreads();
   if constexpr (kPair) cluster_sync_all();
   tc_fence_after();
-  await_predecessor();
   const uint32_t tmem_base = *tmem_slot;
-  F8Walk<CTAS> walk(args, blockIdx.x / CTAS, gridDim.x / CTAS, kCols, rank);
   const int kiters = (args.k_dim + kF8K - 1) / kF8K;
 
   if (warp >= 4) {
     more_registers<40>();
+    await_predecessor();
+    F8Walk<CTAS> walk(args, blockIdx.x / CTAS, gridDim.x / CTAS, kCols, rank);
     // ------------------------------ epilogue ----------------------------------
     const int quad = warp & 3;
     const int half = (warp - 4) >> 2;
@@ -518,37 +518,62 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     fewer_registers<40>();
     if (warp == 0) {
       // ------------------------------ TMA producer ------------------------------
+      // Where the maps are complete before the kernel before (which waited for them itself) lets this one up, the first weights are
+      // asked for before the wait for it: that one writes the rows.
+      if (!args.maps_before) await_predecessor();
+      F8Walk<CTAS> walk(args, blockIdx.x / CTAS, gridDim.x / CTAS, kCols, rank);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       const uint64_t pol = l2_policy_evict_normal();
       const uint32_t full_leader = kPair ? mapa_shared(full_bar, 0) : full_bar;
-      for (int i = 0; ok; ++i) {
-        const F8Item c = walk.get(i, args, kCols);
-        if (!c.valid) break;
+      const auto groups_of = [](const F8Item& c) { return (c.rows + kF8RowBox - 1) / kF8RowBox; };
+      const auto load_weights = [&](int st, int kb, const F8Item& c) {
+        const uint32_t sw = tiles_addr + st * Plan::kStageBytes + kF8Tile, fb = full_leader + 8 * st;
         const int wz = kGlu ? 2 * c.expert + rank : c.expert;
         const int wrow = kGlu ? c.n0 : c.n0 + rank * BM;
-        const int groups = (c.rows + kF8RowBox - 1) / kF8RowBox;  // (what the products make of rows that are not there is not stored)
-        for (int kb = 0; kb < kiters; ++kb) {
+        if constexpr (kPair) {
+          mbar_arrive_expect_tx_cluster(fb, Plan::kStageBytes);
+          tma_load_3d_pair(sw, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
+        } else {
+          mbar_arrive_expect_tx(fb, 2 * kF8Tile + groups_of(c) * kF8RowBox * kF8K);
+          tma_load_3d(sw, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
+          tma_load_3d(sw + kF8Tile, &tmap_w, kb * (kF8K / 2), kGlu ? wrow : wrow + BM, kGlu ? wz + 1 : wz, fb, pol);
+        }
+      };
+      const auto load_rows = [&](int st, int kb, const F8Item& c) {
+        const uint32_t sx = tiles_addr + st * Plan::kStageBytes, fb = full_leader + 8 * st;
+        if constexpr (kPair) {
+          tma_load_2d_pair(sx, &tmap_x, kb * (kF8K / 2), c.a_row, fb, pol);
+        } else {  // (what the products make of rows that are not there is not stored)
+          for (int g = 0; g < groups_of(c); ++g)
+            tma_load_2d(sx + g * kF8RowBox * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + g * kF8RowBox, fb, pol);
+        }
+      };
+      for (int i = 0; ok; ++i) {
+        const F8Item c = walk.get(i, args, kCols);
+        int kb = 0;
+        if (i == 0) {
+          const int ahead = c.valid ? min(kiters, kStages) : 0;
+          if (elect_one())
+            for (int st = 0; st < ahead; ++st) load_weights(st, st, c);
+          __syncwarp();
+          if (args.maps_before) await_predecessor();
+          if (elect_one())
+            for (int st = 0; st < ahead; ++st) load_rows(st, st, c);
+          __syncwarp();
+          kb = ahead;
+          if ((stage = ahead) == kStages) { stage = 0; phase = 1; }
+        }
+        if (!c.valid) break;
+        for (; kb < kiters; ++kb) {
           if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty_bar + 8 * stage, phase ^ 1, wctx, DS_TIMEOUT_PRODUCER))) {
             ok = false;
             break;
           }
           if (elect_one()) {
-            const uint32_t sx = tiles_addr + stage * Plan::kStageBytes;
-            if constexpr (kPair) {
-              const uint32_t fb = full_leader + 8 * stage;
-              mbar_arrive_expect_tx_cluster(fb, Plan::kStageBytes);
-              tma_load_2d_pair(sx, &tmap_x, kb * (kF8K / 2), c.a_row, fb, pol);
-              tma_load_3d_pair(sx + kF8Tile, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
-            } else {
-              const uint32_t fb = full_bar + 8 * stage;
-              mbar_arrive_expect_tx(fb, 2 * kF8Tile + groups * kF8RowBox * kF8K);
-              for (int g = 0; g < groups; ++g)
-                tma_load_2d(sx + g * kF8RowBox * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + g * kF8RowBox, fb, pol);
-              tma_load_3d(sx + kF8Tile, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
-              tma_load_3d(sx + 2 * kF8Tile, &tmap_w, kb * (kF8K / 2), kGlu ? wrow : wrow + BM, kGlu ? wz + 1 : wz, fb, pol);
-            }
+            load_weights(stage, kb, c);
+            load_rows(stage, kb, c);
           }
           __syncwarp();
           if (++stage == kStages) { stage = 0; phase ^= 1; }
@@ -561,6 +586,8 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     } else if (warp == 1) {
       // ------------------------------ MMA issuer (leader CTA only) --------------
       if (rank == 0) {
+        await_predecessor();
+        F8Walk<CTAS> walk(args, blockIdx.x / CTAS, gridDim.x / CTAS, kCols, rank);
         constexpr uint32_t idesc = f8_idesc(CTAS * BM, 256);
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;

@@ -114,11 +114,9 @@ def quantize_experts(params):
 
 def fp8_matmul(rows: Fp8Rows, weight: Fp8Weight) -> torch.Tensor:
     """``rows @ weight^T`` [R, N] in ``rows.dtype``; ``weight`` [N, K] or [1, N, K].  K a multiple of 16, N of 8."""
-    rows.checked()
-    data, scales = weight.data, weight.scales
-    if data.dim() == 2:
-        data, scales = data[None], scales[None]
-    return fp8_rows_gemm(rows, Fp8Weight(data, scales), None, None, False, False, rows.data.size(0), 1, None)
+    if weight.data.dim() == 2:
+        weight = Fp8Weight(weight.data[None], weight.scales[None])
+    return fp8_rows_gemm(rows, weight, None, None, False, False, rows.data.size(0), 1, None)
 
 
 @functools.lru_cache(maxsize=256)
