@@ -127,19 +127,32 @@ __device__ __forceinline__ void load_logits(const TopkArgs& a, const T* row, int
   for (int i = 0; i < PER; ++i) x[i] = i < count ? load_elem(row + first + i) : 0.0f;
 }
 
-// The best two of a lane's keys that come after (last, last_at) in the order of the results: value descending, index ascending.
+// The best two of a lane's keys, the lower index first where they are equal.
 template <typename Key, int PER>
-__device__ __forceinline__ void best_two(const Key (&key)[PER], Key last, int last_at, Key& m1, int& i1, Key& m2, int& i2) {
+__device__ __forceinline__ void best_two(const Key (&key)[PER], Key& m1, int& i1, Key& m2, int& i2) {
   m1 = m2 = 0;
   i1 = i2 = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const Key k = key[i] < last || (key[i] == last && i > last_at) ? key[i] : Key(0);
-    const bool first = k > m1, second = k > m2;
-    m2 = first ? m1 : second ? k : m2;
+    const bool first = key[i] > m1, second = key[i] > m2;
+    m2 = first ? m1 : second ? key[i] : m2;
     i2 = first ? i1 : second ? i : i2;
-    m1 = first ? k : m1;
+    m1 = first ? key[i] : m1;
     i1 = first ? i : i1;
+  }
+}
+// The key after (last, last_at) in the order of the results: value descending, index ascending.
+template <typename Key, int PER>
+__device__ __forceinline__ void best_after(const Key (&key)[PER], Key last, int last_at, Key& m, int& at) {
+  m = 0;
+  at = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const Key below = last + (i > last_at ? 1 : 0);  // (no key is the type's largest number)
+    if (key[i] < below && key[i] > m) {
+      m = key[i];
+      at = i;
+    }
   }
 }
 
@@ -179,7 +192,7 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
   bool sure = true;
   Key m1, m2;
   int i1, i2;
-  best_two(key, ~Key(0), 0, m1, i1, m2, i2);
+  best_two(key, m1, i1, m2, i2);
   if (a.keep < a.num_groups) {
     Key g1 = m1, g2 = m2;
     for (int off = (1 << a.lanes_log2) >> 1; off > 0; off >>= 1) {
@@ -239,14 +252,12 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
       again = --left > 0 && m1 == 0 && last != 0;
     }
     if (__any_sync(kAll, again)) {
-      Key n1, n2;
-      int j1, j2;
-      best_two(key, last, at, n1, j1, n2, j2);
+      Key next;
+      int next_at;
+      best_after(key, last, at, next, next_at);
       if (again) {
-        m1 = n1;
-        m2 = n2;
-        i1 = j1;
-        i2 = j2;
+        m1 = next;
+        i1 = next_at;
       }
     }
   }
