@@ -258,7 +258,7 @@ constexpr int kF8MmaK = 32;                  // K of one instruction
 // Bound by TMEM, which the accumulators' writes and the epilogue's reads share, and between 24 and 400 rows per expert by what L2
 // hands out: pairs take 2.0 to 2.1 PFLOP/s at 8192 rows (a step of 256 x 256 x 128 in 0.55 us).
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int kF8RowBox = 32;  // rows of one copy, for a CTA by itself
+constexpr int kF8RowBox = 16;  // rows of one copy, for a CTA by itself
 template <int CTAS> struct F8WidePlan {
   static constexpr int kStageBytes = (CTAS == 2 ? 2 : 3) * kF8Tile;
   static constexpr int kStages = CTAS == 2 ? 6 : 4;
@@ -316,6 +316,15 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     tma_prefetch_desc(&tmap_w);
     if (OUT == F8_ROWS) tma_prefetch_desc(&tmap_out);
   }
+  if constexpr (!kPair) {
+    // Rows that are not there are multiplied too.  As zeros they cost the least power, which is what a long run of products that stream
+    // their weights is short of (XXX us instead of YYY per pass).
+    for (int i = threadIdx.x; i < kStages * kF8Tile / 16; i += kF8Threads) {
+      const int st = i / (kF8Tile / 16), at = i % (kF8Tile / 16);
+      reinterpret_cast<uint4*>(tiles + st * Plan::kStageBytes)[at] = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
+  }
   if (warp == 1) {
     if constexpr (kPair) {
       tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
@@ -351,11 +360,21 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     uint32_t acc_phase = 0;
     bool ok = true;
     F8Item c = walk.get(0, args, kCols);
-    const int r = quad * 32 + lane;
+    // The thread's row of the tile.  Products of at most 64 rows leave rows 16 q to 16 q + 15 on the first 16 lanes of quadrant q.
+    const auto is_small = [&]() { return !kPair && c.rows <= 64; };
+    int r = 0;
+    bool here = false, live = false;  // the row exists; some of this warp's rows do
+    const auto place = [&]() {
+      r = is_small() ? quad * 16 + (lane & 15) : quad * 32 + lane;
+      here = r < c.rows && (!is_small() || lane < 16);
+      live = (is_small() ? quad * 16 : quad * 32) < c.rows;
+    };
     const float *xs = args.x_scales, *wa = args.w_scales, *wb = args.w_scales;
     float x0 = 0.0f, a0 = 0.0f, b0 = 0.0f, x1 = 0.0f, a1 = 0.0f, b1 = 0.0f;
     const auto begin = [&]() {  // the scales of the first two steps of item c
-      if (!c.valid || quad * 32 >= c.rows) return;
+      if (!c.valid) return;
+      place();
+      if (!live) return;
       const int64_t row = static_cast<int64_t>(c.a_row) + (r < c.rows ? r : c.rows - 1);
       xs = args.x_scales + row * kblocks;
       // (a tile's second block of columns may lie past the last one: its products are zeros, any scale serves)
@@ -374,7 +393,7 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     begin();
     F8Item next;
     for (int i = 0; ok && c.valid; ++i, c = next) {
-      const bool live = quad * 32 < c.rows;  // some of this warp's rows exist
+      place();
       float sum[128];
 #pragma unroll
       for (int j = 0; j < 128; ++j) sum[j] = 0.0f;
@@ -425,13 +444,14 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       c = next;
       begin();
       c = done;
+      place();
       if constexpr (OUT == F8_ROWS) {
         if (!live) continue;
         // 64 columns at a time through the warp's staging tile: a tensor copy where all 32 rows are this expert's own (in the padded
         // layout they always are), else, or by a row map, stores of whole 128-byte row segments
-        const bool whole = args.out_perm == nullptr && (args.padded || quad * 32 + 32 <= c.rows);
+        const bool whole = !is_small() && args.out_perm == nullptr && (args.padded || quad * 32 + 32 <= c.rows);
         long long out_row = -1;
-        if (!whole && r < c.rows) {
+        if (!whole && here) {
           out_row = args.out_perm != nullptr ? args.out_perm[c.a_row + r] : c.a_row + r;
           if (out_row >= args.out_rows) out_row = -1;
         }
@@ -489,13 +509,13 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         if (kGlu) {
           // two places used in turn, so that one meeting of the quadrant's warps is enough
           float* mine = reinterpret_cast<float*>(tiles + kStages * Plan::kStageBytes) + (i & 1) * 256;
-          mine[half * 128 + r] = most;
+          mine[half * 128 + quad * 32 + lane] = most;
           __syncwarp();
           if (lane == 0) mbar_arrive(meet_bar + 8 * quad);
           if (!__all_sync(0xFFFFFFFFu, mbar_wait(meet_bar + 8 * quad, i & 1, wctx, DS_TIMEOUT_EPILOGUE))) break;
-          most = fmaxf(most, mine[(half ^ 1) * 128 + r]);
+          most = fmaxf(most, mine[(half ^ 1) * 128 + quad * 32 + lane]);
         }
-        if (r < c.rows) {
+        if (here) {
           const float inv = kF8Top / most;
           const int col0 = kGlu ? c.n0 + 64 * half : c.n0 + 128 * half;
           const int64_t to = static_cast<int64_t>(c.a_row) + r;
@@ -588,13 +608,13 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       if (rank == 0) {
         await_predecessor();
         F8Walk<CTAS> walk(args, blockIdx.x / CTAS, gridDim.x / CTAS, kCols, rank);
-        constexpr uint32_t idesc = f8_idesc(CTAS * BM, 256);
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
         for (int i = 0; ok; ++i) {
           const F8Item c = walk.get(i, args, kCols);
           if (!c.valid) break;
+          const uint32_t idesc = f8_idesc(!kPair && c.rows <= 64 ? 64 : CTAS * BM, 256);  // (half the work where half will do)
           for (int kb = 0; kb < kiters; ++kb) {
             // (the operands first: they are there before the accumulator stage is, and a wait that passes takes its 100 cycles too)
             if (!__all_sync(0xFFFFFFFFu, mbar_wait(full_bar + 8 * stage, phase, wctx, DS_TIMEOUT_MMA)) ||
