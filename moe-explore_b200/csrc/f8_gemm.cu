@@ -144,7 +144,7 @@ int f8_product(const char* name, const F8Product& p, void* stream) {
   const bool pairs = f8_in_pairs(p);
   CUtensorMap tx, tw;
   const int rc = f8_maps(&tx, &tw, p.x, p.x_rows, p.w, static_cast<int64_t>(p.num_experts) * (glu ? 2 : 1), p.N, p.K,
-                         lanes.items > 0 ? 16 : pairs ? BM : kF8RowBox);
+                         lanes.items > 0 ? 16 : f8_row_box(pairs ? 2 : 1));
   if (rc != MOE_OK) return rc;
   const bool bf16 = p.dtype == MOE_DTYPE_BF16;
   if (lanes.items == 0) {

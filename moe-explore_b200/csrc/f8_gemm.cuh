@@ -118,7 +118,7 @@ template <int CTAS> struct F8Walk {
       c.expert = static_cast<int>((info >> 20) & 0x7FFu);
       if (rank == 1) {
         if (info >> 31) ++tile;
-        else active = false;  // re-reads the first tile and stores nothing
+        else active = false;  // reads no rows and stores nothing
       }
     } else {
       c.expert = map_word(a.mtile_expert + unit);
@@ -250,7 +250,8 @@ constexpr int kF8MmaK = 32;                  // K of one instruction
 //
 // A pair's tile is 256 rows x 256 weight rows (128 gate + 128 up rows where gated); per 128 of K each CTA loads 16 KB of rows and
 // 16 KB of weights, and the leader's four instructions (M 256, N 256, K 32) fill one of the two accumulator stages.  A CTA by itself
-// has 128 rows x 256 weight rows: as many products, 32 KB of weights, and no more of the rows than there are.  Each of
+// has 128 rows x 256 weight rows: as many products and 32 KB of weights; 64 rows or fewer take instructions of M 64.  Either loads no
+// more of the rows than there are.  Each of
 // the eight epilogue warps of a CTA owns 32 rows x 128 of the columns: 128 fp32 sums per thread, fetched from TMEM
 // 32 at a time, the next 32 on their way while the last are added.  A thread's row is its lane, so a step's factor is one register
 // (two where gated).
@@ -258,7 +259,7 @@ constexpr int kF8MmaK = 32;                  // K of one instruction
 // Bound by TMEM, which the accumulators' writes and the epilogue's reads share, and between 24 and 400 rows per expert by what L2
 // hands out: pairs take 2.0 to 2.1 PFLOP/s at 8192 rows (a step of 256 x 256 x 128 in 0.55 us).
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int kF8RowBox = 16;  // rows of one copy, for a CTA by itself
+__host__ __device__ constexpr int f8_row_box(int ctas) { return ctas == 2 ? 32 : 16; }  // rows of one copy
 template <int CTAS> struct F8WidePlan {
   static constexpr int kStageBytes = (CTAS == 2 ? 2 : 3) * kF8Tile;
   static constexpr int kStages = CTAS == 2 ? 6 : 4;
@@ -318,7 +319,8 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
   }
   if constexpr (!kPair) {
     // Rows that are not there are multiplied too.  As zeros they cost the least power, which is what a long run of products that stream
-    // their weights is short of (XXX us instead of YYY per pass).
+    // their weights is short of: 128 tokens x 8 on 64 experts of 7168 x 2048 at the 1000 W limit 558 us per pass at 1.25 GHz with what
+    // the memory held, 543 with zeros, 536 with copies of 16 rows instead of 32, 522 at 1.59 GHz with products of 64 rows.
     for (int i = threadIdx.x; i < kStages * kF8Tile / 16; i += kF8Threads) {
       const int st = i / (kF8Tile / 16), at = i % (kF8Tile / 16);
       reinterpret_cast<uint4*>(tiles + st * Plan::kStageBytes)[at] = make_uint4(0, 0, 0, 0);
@@ -547,27 +549,27 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
       bool ok = true;
       const uint64_t pol = l2_policy_evict_normal();
       const uint32_t full_leader = kPair ? mapa_shared(full_bar, 0) : full_bar;
-      const auto groups_of = [](const F8Item& c) { return (c.rows + kF8RowBox - 1) / kF8RowBox; };
+      constexpr int kBox = f8_row_box(CTAS);
+      const auto groups_of = [](const F8Item& c) { return (c.rows + kBox - 1) / kBox; };
       const auto load_weights = [&](int st, int kb, const F8Item& c) {
         const uint32_t sw = tiles_addr + st * Plan::kStageBytes + kF8Tile, fb = full_leader + 8 * st;
         const int wz = kGlu ? 2 * c.expert + rank : c.expert;
         const int wrow = kGlu ? c.n0 : c.n0 + rank * BM;
         if constexpr (kPair) {
-          mbar_arrive_expect_tx_cluster(fb, Plan::kStageBytes);
+          mbar_arrive_expect_tx_cluster(fb, kF8Tile + groups_of(c) * kBox * kF8K);
           tma_load_3d_pair(sw, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
         } else {
-          mbar_arrive_expect_tx(fb, 2 * kF8Tile + groups_of(c) * kF8RowBox * kF8K);
+          mbar_arrive_expect_tx(fb, 2 * kF8Tile + groups_of(c) * kBox * kF8K);
           tma_load_3d(sw, &tmap_w, kb * (kF8K / 2), wrow, wz, fb, pol);
           tma_load_3d(sw + kF8Tile, &tmap_w, kb * (kF8K / 2), kGlu ? wrow : wrow + BM, kGlu ? wz + 1 : wz, fb, pol);
         }
       };
       const auto load_rows = [&](int st, int kb, const F8Item& c) {
         const uint32_t sx = tiles_addr + st * Plan::kStageBytes, fb = full_leader + 8 * st;
-        if constexpr (kPair) {
-          tma_load_2d_pair(sx, &tmap_x, kb * (kF8K / 2), c.a_row, fb, pol);
-        } else {  // (what the products make of rows that are not there is not stored)
-          for (int g = 0; g < groups_of(c); ++g)
-            tma_load_2d(sx + g * kF8RowBox * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + g * kF8RowBox, fb, pol);
+        // (what the products make of rows that are not there is not stored)
+        for (int g = 0; g < groups_of(c); ++g) {
+          if constexpr (kPair) tma_load_2d_pair(sx + g * kBox * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + g * kBox, fb, pol);
+          else tma_load_2d(sx + g * kBox * kF8K, &tmap_x, kb * (kF8K / 2), c.a_row + g * kBox, fb, pol);
         }
       };
       for (int i = 0; ok; ++i) {
