@@ -89,11 +89,14 @@ static F8Lanes f8_lanes(const F8Product& p) {
   return {static_cast<int>(items), ranks};
 }
 // Rows on the lanes: pairs of CTAs or single ones.  A pair's 256 rows are more often partly empty, a single CTA takes half as much again
-// from L2, and more where rows of K bytes begin inside a line of 128.  us with single CTAs / pairs by rows per expert (0.5 to 1.5 of it):
-//   64 experts of 7168 x 2048    64: 175 / 235   128: 229 / 250   384: 470 / 540   512: 645 / 607
-//   64 experts of 2048 x 1024    64:  36 /  50   128:  43 /  49   384:  78 /  76   512:  95 /  95
-//   60 experts of 2000 x 1416    64:  47 /  64   128:  68 /  64   384: 143 / 116
-//   one matrix of 7168 x 4096                    128:  33 /  29   512:  35 /  30
+// from L2, and more where rows of K bytes begin inside a line of 128.  us with single CTAs / pairs by rows per expert, experts having
+// 0.5 to 1.5 times that:
+//   64 experts of 7168 x 2048    64: 175 / 234   128: 230 / 238   256: 356 / 370   384: 514 / 466   512: 637 / 655
+//   64 experts of 2048 x 1024    64:  35 /  45   128:  43 /  47   256:  60 /  63   384:  80 /  77   512:  96 /  96
+//   60 experts of 2000 x 1416    64:  49 /  55   128:  66 /  59   256: 104 /  89   384: 143 / 113
+//   one matrix of 7168 x 4096                    128:  35 /  29                    512:  36 /  31
+// Routers are less even than that: 375 rows per expert of which a quarter of the experts have none to 20 (3001 tokens x 8 on 64 experts
+// of 2048 x 1024) take 289 / 317 for the whole pass, which is why the bound lies at 400.
 static bool f8_in_pairs(const F8Product& p) {
   const int64_t mean = p.routed_rows / p.num_experts;
   return mean > (p.num_experts == 1 ? 64 : p.K % 128 == 0 ? 400 : 96);
