@@ -251,13 +251,12 @@ constexpr int kF8MmaK = 32;                  // K of one instruction
 // A pair's tile is 256 rows x 256 weight rows (128 gate + 128 up rows where gated); per 128 of K each CTA loads 16 KB of rows and
 // 16 KB of weights, and the leader's four instructions (M 256, N 256, K 32) fill one of the two accumulator stages.  A CTA by itself
 // has 128 rows x 256 weight rows: as many products and 32 KB of weights; 64 rows or fewer take instructions of M 64.  Either loads no
-// more of the rows than there are.  Each of
-// the eight epilogue warps of a CTA owns 32 rows x 128 of the columns: 128 fp32 sums per thread, fetched from TMEM
-// 32 at a time, the next 32 on their way while the last are added.  A thread's row is its lane, so a step's factor is one register
-// (two where gated).
+// more of the rows than there are.  Each of the eight epilogue warps of a CTA owns 32 rows x 128 of the columns: 128 fp32 sums per
+// thread, fetched from TMEM 32 at a time, the next 32 on their way while the last are added.  A thread's row is its lane, so a step's
+// factor is one register (two where gated).
 //
 // Bound by TMEM, which the accumulators' writes and the epilogue's reads share, and between 24 and 400 rows per expert by what L2
-// hands out: pairs take 2.0 to 2.1 PFLOP/s at 8192 rows (a step of 256 x 256 x 128 in 0.55 us).
+// hands out: pairs take 2.0 to 2.1 PFLOP/s at 8192 rows (a step of 256 x 256 x 128 in 0.55 us), 1.7 in long runs under the power limit.
 // ------------------------------------------------------------------------------------------------------------------
 __host__ __device__ constexpr int f8_row_box(int ctas) { return ctas == 2 ? 32 : 16; }  // rows of one copy
 template <int CTAS> struct F8WidePlan {
