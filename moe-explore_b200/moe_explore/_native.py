@@ -232,8 +232,10 @@ def on_device_of(t: torch.Tensor):
 
 def needs_gradient(*tensors) -> bool:
     """Whether a derivative with respect to one of the tensors is asked for, backwards or forwards."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
     return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 

@@ -100,9 +100,12 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
         num_rows, device = rows.size(0), x.device
         q = torch.empty(num_rows, d, dtype=DTYPE, device=device)
         scales = torch.empty(num_rows, -(-d // BLOCK), dtype=torch.float32, device=device)
-        y = torch.empty(num_rows, d, dtype=x.dtype, device=device) if with_rows else None
-        h = torch.empty(num_rows, d, dtype=x.dtype, device=device) if residual is not None else None
+        y = torch.empty_like(rows, memory_format=torch.contiguous_format) if with_rows else None
+        h = torch.empty_like(rows, memory_format=torch.contiguous_format) if residual is not None else None
         _native.rms_norm(rows, None if residual is None else _rows(residual), _aligned(weight), float(eps), h=h, y=y, q=q, scales=scales)
     if y is None and h is None:
         return Fp8Rows(q, scales, x.dtype)
-    return (Fp8Rows(q, scales, x.dtype), *(_like(t, x) for t in (y, h) if t is not None))
+    out = (Fp8Rows(q, scales, x.dtype),)
+    if y is not None:
+        out += (_like(y, x),)
+    return out if h is None else out + (_like(h, x),)
