@@ -204,6 +204,7 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
     }
     const int group = lane >> a.lanes_log2;
     Key mine = 0;
+    float off_by = 0.0f;  // what the group's score in fp32 may be off by
     if (group < a.num_groups) {
       V v = O::value(g1);
       if (a.best == 2) {
@@ -212,7 +213,19 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
           v = key_score(static_cast<float>(v), sigmoid, top, sum);
           w = key_score(static_cast<float>(w), sigmoid, top, sum);
         }
+        // (half the sum ranks as the sum does, and does not overflow)
+        v = V(0.5) * v;
+        w = V(0.5) * w;
+        if (kFirst) {
+          // each member's slack and its rounding to fp32 by 2^-24 of ITS size, the addition's and that of the bounds below by 2^-24 of
+          // the sum: members that cancel leave a small sum with the large ones' roundings.  (An infinite member is exact.)
+          const float size = fabsf(static_cast<float>(v)) + fabsf(static_cast<float>(w));
+          off_by = size < CUDART_INF_F ? slack + 2.4e-7f * size : 0.0f;
+        }
         v += w;
+      } else if (kFirst) {
+        const float size = fabsf(static_cast<float>(v));
+        off_by = size < CUDART_INF_F ? slack + 2.4e-7f * size : 0.0f;
       }
       mine = O::key(v);
     }
@@ -227,9 +240,11 @@ __device__ __forceinline__ bool choose(const TopkArgs& a, const T* row, int firs
     for (int off = lanes >> 1; off > 0; off >>= 1) rank += __shfl_xor_sync(kAll, rank, off);
     const bool open = group < a.num_groups && rank < a.keep;
     if (kFirst && (biased || a.best == 2)) {
-      const float worst = static_cast<float>(O::value(O::warp_min(open ? mine : ~Key(0))));
-      const float next = static_cast<float>(O::value(O::warp_max(open ? Key(0) : mine)));
-      if (worst - next <= 4.0f * slack + 4e-7f * (fabsf(worst) + fabsf(next))) sure = false;
+      // the least that an open group can have, and the most that a closed one can; closed ones of minus infinity (masked) or NaN
+      // are exact: what they are compared with is larger, or equal and decided by index
+      const Key worst = O::warp_min(open ? O::key(static_cast<V>(static_cast<float>(O::value(mine)) - off_by)) : ~Key(0));
+      const Key next = O::warp_max(open || group >= a.num_groups ? Key(0) : O::key(static_cast<V>(static_cast<float>(O::value(mine)) + off_by)));
+      if (worst <= next && next > O::key(static_cast<V>(-CUDART_INF_F))) sure = false;
     }
     if (!open) m1 = m2 = 0;
   }

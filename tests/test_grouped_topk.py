@@ -83,6 +83,25 @@ def test_values_too_close_for_32_bits_are_told_apart(native):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("large", [64.0, 3.0e4, 3.0e38])
+def test_members_that_cancel_rank_their_group_exactly(large, native):
+    """A group's two members of +large and about -large leave a small sum with the large ones' roundings to fp32 (64 + p is rounded to
+    2^-18 steps).  At 3e38 two members of one sign would leave the range of fp32, and p is below the bias's steps in 64 bits too."""
+    g = torch.Generator().manual_seed(7)
+    T, G = 4096, 16
+    bias = torch.empty(G, 2)
+    bias[:, 0], bias[:, 1] = large, -large + (0.5 if large < 1e5 else 0.0)
+    if large > 1e5:
+        bias[::2] = -large
+    spread = 10.0 ** (-5.0 * torch.rand(T, 1, generator=g))      # 1e-5 to 1: around the steps of each of the sizes
+    logits = spread * torch.randn(T, 2 * G, generator=g) + torch.randn(1, 2, generator=g).repeat(1, G)
+    params = GroupedTopkRouterParams(None, 6, bias=bias.flatten().cuda(), num_groups=G, topk_groups=5, group_best=2)
+    _, indices = grouped_topk_of_logits(logits.cuda(), params)
+    _, want = plain(logits.cuda(), params)
+    assert torch.equal(indices, want)
+
+
+@pytest.mark.gpu
 def test_ties_take_the_lowest_index(native):
     logits = torch.zeros(3, 24, device="cuda")
     logits[1, 20] = 1.0
