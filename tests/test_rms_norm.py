@@ -198,6 +198,43 @@ def test_leading_axes_strides_empty_streams_and_capture(native):
     assert torch.equal(out, y2) and torch.equal(rows.data.view(torch.uint8), again.data.view(torch.uint8)) and torch.equal(rows.scales, again.scales)
 
 
+def test_one_row_has_no_stride(native):
+    """Torch calls a single row contiguous whatever its stride; the kernels get one that they can read."""
+    from moe_explore.functional.rms_norm import _rows
+
+    for cut in (lambda b: b[:1, :64], lambda b: b[5:6, 3:67], lambda b: b[2:3, 1:2].expand(1, 64), lambda b: b.t()[:1, :64],
+                lambda b: b[:1, None, :64], lambda b: b[0, :64]):
+        x = cut(torch.arange(80 * 77, dtype=torch.float32).view(80, 77).bfloat16())
+        rows = _rows(x)
+        assert torch.equal(rows, x.reshape(1, 64)) and rows.stride(1) == 1 and rows.stride(0) % 8 == 0 and rows.data_ptr() % 16 == 0
+    dense = torch.zeros(3, 64)
+    assert _rows(dense) is dense
+    wide = torch.zeros(4, 512, dtype=torch.bfloat16)
+    assert _rows(wide[:1, 256:]).data_ptr() == wide[:1, 256:].data_ptr()      # read in place
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 256, 4096])
+def test_one_row_of_a_wider_matrix(d, native):
+    """One token's row, cut out of rows whose length is no multiple of 8, as x and as the residual, forward and backward."""
+    x, r, w = make(1, d, torch.bfloat16, torch.bfloat16)
+    wide = torch.zeros(2, 60, d + 13, device="cuda", dtype=torch.bfloat16)
+    wide[0, :1, :d], wide[1, :1, :d] = x, r
+    xs, rs = wide[0, :1, :d], wide[1, :1, :d]
+    assert xs.stride(0) == d + 13 and xs.is_contiguous()
+    for a, b in zip(rms_norm(xs, w, residual=rs), rms_norm(x, w, residual=r)):
+        assert torch.equal(a, b)
+    one, two = rms_norm_fp8(xs, w, residual=rs), rms_norm_fp8(x, w, residual=r)
+    assert torch.equal(one[0].data.view(torch.uint8), two[0].data.view(torch.uint8)) and torch.equal(one[1], two[1])
+    dy = torch.randn(1, 60, d + 13, device="cuda").bfloat16()[0, :1, :d]
+    leaf, dense = wide.requires_grad_(True), x.clone().requires_grad_(True)
+    got, = torch.autograd.grad(rms_norm(leaf[0, :1, :d], w), leaf, dy)
+    want, = torch.autograd.grad(rms_norm(dense, w), dense, dy.contiguous())
+    assert torch.equal(got[0, :1, :d], want)
+    got[0, :1, :d] = 0
+    assert got.abs().max() == 0
+
+
 def test_refusals(native):
     lib = native.load()
     p = 4096
