@@ -145,6 +145,8 @@ def fp8_rows_gemm(rows: Fp8Rows, weight: Fp8Weight, group_indices, permute_indic
     if is_glu(act) or act not in _native.ACT_CODES:
         raise ValueError(f"products of 8-bit rows take no or an element-wise activation, got {act!r} "
                          "(gated experts: moe_explore.expert_compute.fp8_expert_compute)")
+    if _native.needs_gradient(rows.data, rows.scales, weight.data, weight.scales):
+        raise RuntimeError("products in 8 bits have no backward pass, of rows, weights or scales: call this under torch.no_grad()")
     device = rows.data.device
     with _native.on_device_of(rows.data):
         out = torch.empty(num_rows, n, dtype=rows.dtype, device=device)

@@ -510,6 +510,35 @@ def test_refusals_of_tensors(native):
         fp8_expert_compute(x.float(), scores, ids, p)
 
 
+@gpu
+def test_no_gradient_is_lost_in_silence(native):
+    """Rows, weights or scales that ask for a gradient are refused, by every product; without gradients they are taken."""
+    from moe_explore.expert_compute import fp8_expert_compute
+
+    g = gen(8)
+    rows, w = random_rows(g, 4, 128), random_weight(g, 1, 64, 128)
+    groups = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    p = make_experts(g, 2, 128, 64, "swiglu")
+    scores, ids = routing(g, 4, 2, 1, torch.bfloat16)
+    products = (lambda: fp8_matmul(rows, w),
+                lambda: m_grouped_gemm(rows, MGroupedGEMMParams(w, groups, None, False, False, 4, 1)))
+    experts = (lambda: fp8_expert_compute(rows, scores, ids, p),)
+    for held, calls in ((rows.scales, products + experts), (w.scales, products), (rows.data, products + experts), (w.data, products),
+                        (p.up.scales, experts), (p.down.scales, experts), (p.up.data, experts), (p.down.data, experts), (scores, experts)):
+        for call in calls:
+            want = call()
+            held.requires_grad_(True)
+            with pytest.raises(RuntimeError, match="no backward"):
+                call()
+            with torch.no_grad():
+                assert torch.equal(call(), want)
+            held.requires_grad_(False)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(rows.scales, torch.ones_like(rows.scales))
+        with pytest.raises(RuntimeError, match="no backward"):
+            fp8_matmul(Fp8Rows(rows.data, dual), w)
+
+
 def test_chained_kernels_promise_no_constant_memory():
     """The kernels that wait for the one before through await_predecessor(): see tests/test_chained_kernels.py."""
     found = 0
