@@ -253,6 +253,13 @@ def require_cuda(*tensors):
             raise RuntimeError("libmoe_sm100 runs on CUDA tensors only (no CPU path); got a tensor on " + str(t.device))
 
 
+def require_one_device(first, **others):
+    """Kernels run on the device of ``first`` and cannot read another one's memory."""
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, the rows are on {first.device}: one device is expected")
+
+
 def padded_rows_bound(num_rows: int, num_experts: int) -> int:
     return int(load().moe_padded_rows_bound(num_rows, num_experts))
 

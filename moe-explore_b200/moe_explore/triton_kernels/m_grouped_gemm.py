@@ -53,6 +53,8 @@ def m_grouped_gemm(token: torch.Tensor, params: MGroupedGEMMParams, autotune_mod
     if params.gather or params.scatter:
         assert params.permute_indices is not None
     _native.require_cuda(token, params.weight, params.group_indices)
+    _native.require_one_device(token, weight=params.weight, group_indices=params.group_indices,
+                               permute_indices=params.permute_indices if params.gather or params.scatter else None)
 
     num_experts, k_dim, n_dim = params.weight.shape
     rows = params.num_tokens * params.topk if (params.gather or params.scatter) else params.num_tokens
@@ -96,7 +98,9 @@ def _m_grouped_gemm_fp8(token: Fp8Rows, params: MGroupedGEMMParams) -> torch.Ten
         raise TypeError("8-bit rows are multiplied with 8-bit weights: both of Fp8Rows and Fp8Weight, or neither")
     moved = params.gather or params.scatter
     assert not moved or params.permute_indices is not None
-    _native.require_cuda(params.group_indices)
+    _native.require_cuda(token.data, params.group_indices)
+    _native.require_one_device(token.data, scales=token.scales, weight=params.weight.data, group_indices=params.group_indices,
+                               permute_indices=params.permute_indices if moved else None)
     rows = params.num_tokens * params.topk if moved else params.num_tokens
     num_experts = params.weight.data.size(0)
     assert params.group_indices.dim() == 1 and params.group_indices.numel() == num_experts + 1

@@ -325,3 +325,34 @@ def test_a_default_device_does_not_watch(monkeypatch):
         pass
     with Watching(torch.device("cpu")):
         assert not R.nothing_watches(t)
+
+
+class _On(torch.Tensor):
+    """A tensor that says it lies on a given CUDA device (nothing of it is read)."""
+    is_cuda = True
+    device = property(lambda self: torch.device("cuda", self.index))
+
+    @staticmethod
+    def of(t, index):
+        t = torch.Tensor._make_subclass(_On, t)
+        t.index = index
+        return t
+
+
+@pytest.mark.parametrize("away", ["weight", "group_indices", "permute_indices"])
+@pytest.mark.parametrize("eight", [False, True])
+def test_grouped_products_take_one_device(eight, away):
+    """Maps or weights on another device than the rows are refused before anything is launched: a kernel could not read them."""
+    from moe_explore.functional.fp8 import Fp8Rows, Fp8Weight
+    from moe_explore.triton_kernels.m_grouped_gemm import MGroupedGEMMParams, m_grouped_gemm
+
+    at = lambda name, t: _On.of(t, int(name == away))
+    groups, perm = at("group_indices", torch.tensor([0, 4, 8], dtype=torch.int32)), at("permute_indices", torch.arange(8))
+    if eight:
+        f8 = torch.float8_e4m3fn
+        token = Fp8Rows(at("token", torch.zeros(8, 128).to(f8)), at("token", torch.ones(8, 1)))
+        weight = Fp8Weight(at("weight", torch.zeros(2, 64, 128).to(f8)), at("weight", torch.ones(2, 1, 1)))
+    else:
+        token, weight = at("token", torch.zeros(8, 128).bfloat16()), at("weight", torch.zeros(2, 128, 64).bfloat16())
+    with pytest.raises(ValueError, match=f"{away} is on cuda:1"):
+        m_grouped_gemm(token, MGroupedGEMMParams(weight, groups, perm, True, False, 8, 1))
