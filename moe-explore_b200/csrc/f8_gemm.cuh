@@ -214,11 +214,6 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t cluster_addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr) : "memory");
   return v;
 }
-// An arrival in either CTA of the pair that publishes no memory (TMEM reads are ordered by the tcgen05 fence before it): a releasing
-// one would wait for the loads of the scales that are under way.
-__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
 // The element-wise activation of N registers of a row; the choice is made once, so that the elements interleave.
 template <int N, int M> __device__ __forceinline__ void act_row(float (&v)[M], int act, int from = 0) {
   if (act == MOE_ACT_SILU || act == MOE_ACT_SWIGLU) {
@@ -349,7 +344,13 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
     // ------------------------------ epilogue ----------------------------------
     const int quad = warp & 3;
     const int half = (warp - 4) >> 2;
-    const uint32_t tempty_leader = mapa_shared(tempty_bar, 0);
+    const uint32_t tempty_leader = kPair ? mapa_shared(tempty_bar, 0) : tempty_bar;
+    // An accumulator stage goes back when this warp has fetched its sums: by an arrival that releases, the same as in the 16-bit
+    // kernels, so that the reads before it are over for whoever the barrier lets on.
+    const auto give_back = [&](int stage) {
+      if constexpr (kPair) mbar_arrive_cluster(tempty_leader + 8 * stage);
+      else mbar_arrive(tempty_leader + 8 * stage);
+    };
     const uint32_t stage_base = staging_addr + (warp - 4) * Plan::kStagingTile;
     const int kblocks = kiters;
     // first accumulator column of the thread's two groups of 64
@@ -403,11 +404,6 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
         x0 = x1;
         a0 = a1;
         b0 = b1;
-        if (live && kb + 2 < kiters) {
-          x1 = xs[kb + 2];
-          a1 = wa[kb + 2];
-          if (kGlu) b1 = wb[kb + 2];
-        }
         if (!__all_sync(0xFFFFFFFFu, mbar_wait(tfull_bar + 8 * acc, acc_phase, wctx, DS_TIMEOUT_EPILOGUE))) {
           ok = false;
           break;
@@ -426,14 +422,21 @@ f8_wide_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant
               // before the last additions: the stage is in registers
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
+              if (lane == 0) give_back(acc);
+              // (loads behind the arrival, which would wait for them: they are not needed before the step after the next.  8192 rows of
+              // 4096 by 14336 columns take 489 us, as with an arrival that releases nothing)
+              if (kb + 2 < kiters) {
+                x1 = xs[kb + 2];
+                a1 = wa[kb + 2];
+                if (kGlu) b1 = wb[kb + 2];
+              }
             }
 #pragma unroll
             for (int j = 0; j < 32; ++j) sum[ch * 32 + j] = fmaf(__uint_as_float(v[ch & 1][j]), ch < 2 ? fa : fb, sum[ch * 32 + j]);
             if (ch < 3) tmem_ld_wait32(v[(ch + 1) & 1]);
           }
         } else {
-          if (lane == 0) mbar_arrive_cluster_relaxed(tempty_leader + 8 * acc);
+          if (lane == 0) give_back(acc);
         }
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
