@@ -95,6 +95,40 @@ def test_empty_blocks_zeros_and_what_is_not_finite(native):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,d", [(1, 64), (5, 1024), (400, 776), (3, 4096), (700, 4104), (2, 16384)])
+def test_rows_whose_squares_leave_fp32(T, d, native):
+    """Finite bf16 rows up to the type's largest value have a finite norm, forward and backward, beside ordinary rows."""
+    g = torch.Generator(device="cuda").manual_seed(d)
+    size = 10.0 ** (17 + 21.4 * torch.rand(T, 1, generator=g, device="cuda", dtype=torch.float64))
+    if T > 1:
+        size[1] = 1.0
+    x = ((2 * torch.rand(T, d, generator=g, device="cuda", dtype=torch.float64) - 1) * size).to(torch.bfloat16)
+    x[0, 5] = torch.finfo(torch.bfloat16).max
+    assert torch.isfinite(x).all()
+    w = 1.0 + 0.2 * torch.randn(d, generator=g, device="cuda")
+    want, _ = plain(x, w)
+    y = rms_norm(x, w)
+    # 1 / root mean square is at least 2^-128 and held in fp32: 21 bits where it is the least
+    assert bool(((y.double() - want).abs() <= (half_step(torch.bfloat16) + EVAL + 2.0 ** -21) * want.abs() + 2.0 ** -25).all())
+    rows, y2 = rms_norm_fp8(x, w, with_rows=True) if d % 16 == 0 else (None, y)
+    assert torch.equal(y, y2)
+    if rows is not None:
+        check_fp8(rows, want, d)
+    dy = torch.randn(T, d, generator=g, device="cuda").bfloat16()
+    leaves = x.requires_grad_(True), w.requires_grad_(True)
+    dx, dw = torch.autograd.grad(rms_norm(*leaves), leaves, dy)
+    wide = [t.detach().double().requires_grad_(True) for t in leaves]
+    want_x, want_w = torch.autograd.grad(plain(*wide)[0], wide, dy.double())
+    r = torch.rsqrt(wide[0].detach().square().mean(-1, keepdim=True) + 1e-6)
+    terms = dy.double().abs() * wide[1].detach().abs()
+    bound = half_step(torch.bfloat16) * want_x.abs() + 4 * (EVAL + 2.0 ** -21) * r * (terms + wide[0].detach().abs() * r * terms.mean(-1, keepdim=True) * 4)
+    bound = bound + torch.finfo(torch.bfloat16).tiny * torch.finfo(torch.bfloat16).eps
+    assert bool(((dx.double() - want_x).abs() <= bound).all())
+    total = (dy.double() * wide[0].detach() * r).abs().sum(0)
+    assert bool(((dw.double() - want_w).abs() <= 2 * (EVAL + 2.0 ** -21) * total + 1e-30).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,d", [(1, 8), (5, 248), (700, 256), (333, 1032), (1500, 2048), (601, 4104), (64, 7168), (9, 16384)])
 def test_gradients(T, d, dtype, native):
