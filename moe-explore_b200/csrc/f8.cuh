@@ -14,8 +14,9 @@ constexpr int kF8Block = 128;
 constexpr float kF8Top = 448.0f;
 constexpr float kF8Least = 8.271806125530277e-25f;  // 2^-80
 
-// The wait of the kernels in this family for the one they are chained to: nothing before it touches global memory, and what was
-// said about such kernels at grid_wait() holds for them (no __restrict__, no __ldg).
+// grid_wait() of the kernels in this family.  They may read the maps before it where a kernel before their predecessor wrote them
+// (F8Args::maps_before), past L1; otherwise what is said at grid_wait() holds for them, no __restrict__ and no __ldg included.
+// (tests/test_synchronisation_sources.py finds the kernels that wait by what they call, not by the name.)
 __device__ __forceinline__ void await_predecessor() { grid_wait(); }
 
 __device__ __forceinline__ uint32_t f8x4(float a, float b, float c, float d) {
