@@ -202,6 +202,48 @@ def test_gather_and_scatter(T, E, topk, gather, scatter, native):
 
 
 @gpu
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("T,E,k", [(25, 4, 272), (500, 4, 256), (1000, 3, 272), (4096, 16, 1024)], ids=["few", "single", "pairs", "prompt"])
+def test_scattered_rows_go_nowhere_else(T, E, k, gather, native):
+    """Rows behind a scatter: each lies at its place, a dropped position (-1) is stored nowhere, and what lay there is left as it was.
+    The sizes reach the kernel of few rows, single CTAs, pairs, and a prompt's gather and scatter."""
+    import ctypes
+
+    from moe_explore.functional.fp8 import _maps_layout
+    from moe_explore.routing_plan import device_status
+
+    g, n, topk = gen(T), 136, 2
+    ids = torch.stack([torch.randperm(E, generator=g, device="cuda")[:topk] for _ in range(min(T, 64))]).repeat(-(-T // 64), 1)[:T].reshape(-1)
+    rows = T * topk
+    order = torch.sort(ids, stable=True).indices
+    groups = torch.cat((torch.zeros(1, dtype=torch.int64, device="cuda"), torch.bincount(ids, minlength=E).cumsum(0))).to(torch.int32)
+    w, x = random_weight(g, E, n, k), random_rows(g, T if gather else rows, k)
+    data = x.data.view(torch.uint8)[order // topk if gather else slice(None)].view(DTYPE)
+    sorted_rows = Fp8Rows(data, x.scales[order // topk] if gather else x.scales, x.dtype)
+    want = m_grouped_gemm(sorted_rows, MGroupedGEMMParams(w, groups, None, False, False, rows, 1))
+    for e in range(E):
+        at = slice(int(groups[e]), int(groups[e + 1]))
+        check_product(want[at], rows64(sorted_rows)[at], weight64(Fp8Weight(w.data[e], w.scales[e])), torch.bfloat16)
+    drop = torch.tensor([0, 3, rows // 2, rows - 1], device="cuda")
+    perm = order.clone()
+    perm[drop] = -1
+    keep = perm >= 0
+    there = torch.full_like(want, 7.0)
+    there[order[keep]] = want[keep]
+    out = torch.full_like(want, 7.0)
+    offsets, words = _maps_layout(rows, E)
+    maps = torch.empty(words, dtype=torch.int32, device="cuda")
+    gathered, gathered_scales = torch.empty(rows, k, dtype=DTYPE, device="cuda"), torch.empty(rows, -(-k // BLOCK), device="cuda")
+    p = native.F8RowsPass(rows, x.data.size(0), E, k, n, topk if gather else 1, 0, 0, gather, True, x.data.data_ptr(), x.scales.data_ptr(),
+                          w.data.data_ptr(), w.scales.data_ptr(), out.data_ptr(), groups.data_ptr(), perm.data_ptr(),
+                          *[maps.data_ptr() + o for o in offsets], device_status(0).data_ptr(), gathered.data_ptr(), gathered_scales.data_ptr())
+    steps = native.ROWS_LAYOUT | native.ROWS_GEMM | (native.ROWS_GATHER if gather else 0)
+    assert native.load().moe_f8_rows_gemm(ctypes.byref(p), steps, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, there)
+    assert torch.equal(m_grouped_gemm(x, MGroupedGEMMParams(w, groups, perm, gather, True, T, topk))[order[keep]], want[keep])
+
+
+@gpu
 def test_a_prefix_that_is_none_is_reported(native):
     from moe_explore.routing_plan import check_device_status
 
@@ -276,6 +318,32 @@ def routing(g, T, E, k, dtype, favour=0.0):
     logits[:, 0] += favour
     top = torch.topk(logits, k, dim=-1)
     return torch.softmax(top.values, -1).to(dtype), top.indices
+
+
+@gpu
+@pytest.mark.parametrize("T,E,k,d,inter", [(1, 4, 2, 256, 512), (300, 4, 2, 272, 208), (1100, 3, 2, 512, 656)])
+def test_experts_with_the_tanh_form_of_gelu(T, E, k, d, inter, native, monkeypatch):
+    from moe_explore.expert_compute import fp8_expert_compute
+
+    g = gen(T)
+    p = make_experts(g, E, d, inter, "approx_gelu")
+    x = torch.randn(T, d, generator=g, device="cuda").bfloat16()
+    scores, ids = routing(g, T, E, k, torch.bfloat16)
+    out = fp8_expert_compute(x, scores, ids, p)
+    # the plain form with the tanh form in the distribution function's place; its slope, too, is below 1.2
+    monkeypatch.setattr(torch.special, "ndtr", lambda v: 0.5 * (1 + torch.tanh((2 / math.pi) ** 0.5 * (v + 0.044715 * v ** 3))))
+    check_experts(out, quantize_rows(x), scores, ids, Fp8ExpertParams(p.up, p.down, "gelu"))
+    # and the product by itself
+    groups, owner, w, rows = grouped_case(g, [5, 0, 300], 272, 40)
+    xr = random_rows(g, rows, 272)
+    got = m_grouped_gemm(xr, MGroupedGEMMParams(w, groups, None, False, False, rows, 1, activation="approx_gelu"))
+    for e in (0, 2):
+        r64, w64 = rows64(xr)[owner == e], weight64(Fp8Weight(w.data[e], w.scales[e]))
+        z, terms = r64 @ w64.T, r64.abs() @ w64.abs().T
+        want = z * torch.special.ndtr(z)
+        # tanh to 2^-22 of 1 (its error bound is 2 units), multiplied by z / 2
+        assert bool(((got[owner == e].double() - want).abs() <= (half_step(torch.bfloat16) + 2.0 ** -20) * want.abs() + 2.0 ** -21 * z.abs()
+                     + 1.2 * sum_error(272) * terms).all())
 
 
 # tokens, experts, slots, d, I, pull towards expert 0: one token; a batch; many rows for one of many experts; odd widths; many rows

@@ -115,6 +115,22 @@ def test_ties_take_the_lowest_index(native):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_equal_values_of_a_whole_prompt(score, native):
+    """A bias of zeros, as training begins with it, and 16-bit logits: a third of the tokens have equal values among their best."""
+    T, E = 16384, 256
+    logits = (1.5 * torch.randn(T, E, generator=torch.Generator(device="cuda").manual_seed(11), device="cuda")).bfloat16()
+    p = GroupedTopkRouterParams(None, 8, bias=torch.zeros(E, device="cuda"), num_groups=8, topk_groups=4, score_function=score)
+    scores, indices = grouped_topk_of_logits(logits, p, torch.float32)
+    best = logits.sort(-1, descending=True).values[:, :9]
+    assert float((best[:, 1:] == best[:, :-1]).any(-1).float().mean()) > 0.25
+    want, chosen = plain(logits, p)
+    assert torch.equal(indices, chosen) and close(scores, want, torch.float32)
+    p.bias = None
+    assert torch.equal(grouped_topk_of_logits(logits, p)[1], chosen)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.float32).min])
 def test_masked_experts(low, native):
     """Logits or biases of minus infinity, or the type's lowest value, leave an expert for last; rows with nothing left still get k
