@@ -89,17 +89,17 @@ static F8Lanes f8_lanes(const F8Product& p) {
   return {static_cast<int>(items), ranks};
 }
 // Rows on the lanes: pairs of CTAs or single ones.  A pair's 256 rows are more often partly empty, a single CTA takes half as much again
-// from L2, and more where rows of K bytes begin inside a line of 128.  us with single CTAs / pairs by rows per expert, experts having
-// 0.5 to 1.5 times that:
-//   64 experts of 7168 x 2048    64: 175 / 234   128: 230 / 238   256: 356 / 370   384: 514 / 466   512: 637 / 655
-//   64 experts of 2048 x 1024    64:  35 /  45   128:  43 /  47   256:  60 /  63   384:  80 /  77   512:  96 /  96
-//   60 experts of 2000 x 1416    64:  49 /  55   128:  66 /  59   256: 104 /  89   384: 143 / 113
-//   one matrix of 7168 x 4096                    128:  35 /  29                    512:  36 /  31
-// Routers are less even than that: 375 rows per expert of which a quarter of the experts have none to 20 (3001 tokens x 8 on 64 experts
-// of 2048 x 1024) take 289 / 317 for the whole pass, which is why the bound lies at 400.
+// from L2, and more where rows of K bytes begin inside a line of 128.  Time of single CTAs over that of pairs by rows per expert, the
+// geometric mean over shapes (8 to 64 experts, K 720 to 14336, N 1024 to 14336); loads: all the same / 0.5 to 1.5 of the mean /
+// exponential, as an unbalanced router leaves them:
+//                                   64              128              192              256              384              448              768
+//   8 shapes of K % 128 == 0   .78 .74 .76     .79 .91 .84    1.06 .92 .86    1.08 .94 .92     .88 .96 .96    1.07 .97 .99    1.09 1.00 .97
+//   6 others                   .81 .77 .82     .85 1.06 .98   1.25 1.11 1.03  1.24 1.16 1.14   1.09 1.19 1.16 1.29 1.21 1.23  1.34 1.31 1.29
+// Over the three loads they meet at about 430 (.94 at 384, 1.01 at 448) and 144 (.96 at 128, 1.13 at 192) rows per expert.  One matrix
+// of 7168 x 4096 takes 35 / 29 us with 128 rows and 36 / 31 with 512.
 static bool f8_in_pairs(const F8Product& p) {
   const int64_t mean = p.routed_rows / p.num_experts;
-  return mean > (p.num_experts == 1 ? 64 : p.K % 128 == 0 ? 400 : 96);
+  return mean > (p.num_experts == 1 ? 64 : p.K % 128 == 0 ? 432 : 144);
 }
 
 int f8_product(const char* name, const F8Product& p, void* stream) {
