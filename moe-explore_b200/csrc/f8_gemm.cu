@@ -345,6 +345,8 @@ extern "C" int moe_f8_expert_forward(const moe_f8_pass* p, int steps, void* stre
     set_error("moe_f8_expert_forward: d=%d and inter=%d must be multiples of 16", p->d, p->inter);
     return MOE_ERR_UNSUPPORTED;
   }
+  // (the steps by themselves take a null map for "rows stay where they are")
+  MOE_CHECK_ARG(p->dst_row != nullptr || !(steps & (MOE_F8_ROUTE | MOE_F8_DISPATCH | MOE_F8_FOLD)), "moe_f8_expert_forward: null pointer argument");
   const Chain chain;
   if (steps & MOE_F8_ROUTE)
     MOE_STEP(routing_metadata(p->expert_idx, rows, p->num_experts, p->group_indices, nullptr, p->pad_offsets, p->row_src, p->dst_row,

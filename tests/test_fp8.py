@@ -578,6 +578,20 @@ def test_refusals_of_tensors(native):
         fp8_expert_compute(x.float(), scores, ids, p)
 
 
+def test_a_pass_without_its_row_map_is_refused(native):
+    """Without dst_row the dispatch would leave the rows unsorted and the fold would take them so."""
+    import ctypes
+
+    lib = native.load()
+    for step in (native.F8_ROUTE, native.F8_DISPATCH, native.F8_FOLD):
+        s = native.F8Pass(0, native.padded_rows_bound(4, 2), 64, 64, 2, 1, 3, 0)
+        s.num_tokens = 0
+        s.xs = s.xs_scales = s.x = s.ys = s.out = s.scores = 4096
+        assert lib.moe_f8_expert_forward(ctypes.byref(s), step, None) == -1 and b"bad sizes" in lib.moe_last_error()
+        s.num_tokens = 4
+        assert lib.moe_f8_expert_forward(ctypes.byref(s), step, None) == -1 and b"null" in lib.moe_last_error()
+
+
 @gpu
 def test_no_gradient_is_lost_in_silence(native):
     """Rows, weights or scales that ask for a gradient are refused, by every product; without gradients they are taken."""
