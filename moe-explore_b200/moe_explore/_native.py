@@ -230,6 +230,20 @@ def on_device_of(t: torch.Tensor):
     return _NO_SECTION if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+# (names private to torch: where one is missing, such traces cannot be told)
+_jit_traces = getattr(torch._C, "_is_tracing", lambda: False)
+_dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
+
+
+def refuse_tracing():
+    """A trace does not see a kernel of this library: it would hold its results of the traced input for constants.  (torch.compile
+    breaks its graph at the call, and runs it.)"""
+    if not _dispatch_modes() and not _jit_traces():
+        return
+    if _jit_traces() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("this operator is a kernel that torch.jit.trace and make_fx cannot record: call it outside the trace")
+
+
 def needs_gradient(*tensors) -> bool:
     """Whether a derivative with respect to one of the tensors is asked for, backwards or forwards."""
     if torch.is_grad_enabled():

@@ -460,6 +460,7 @@ def fp8_expert_compute(x, scores, indices, params: Fp8ExpertParams, addend=None)
         raise ValueError("indices (int64) and scores are [tokens, k]")
     if any(t.device != data.device for t in (scores, indices, params.up.data, params.down.data) + (() if addend is None else (addend,))):
         raise ValueError("all tensors lie on the device of the input")
+    _native.refuse_tracing()
     if _native.needs_gradient(data, x.scales if rows else None, scores, addend, params.up.data, params.up.scales, params.down.data,
                               params.down.scales):
         raise RuntimeError("experts in 8 bits have no backward pass: call this under torch.no_grad(), or train 16-bit experts")

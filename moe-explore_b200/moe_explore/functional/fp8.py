@@ -70,6 +70,7 @@ def quantize_rows(x: torch.Tensor) -> Fp8Rows:
     _native.require_cuda(x)
     if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"quantize_rows takes bf16 or fp16 [R, K], got {x.dtype} {tuple(x.shape)}")
+    _native.refuse_tracing()
     if _native.needs_gradient(x):
         raise RuntimeError("8-bit rows have no backward pass: call this under torch.no_grad()")
     with _native.on_device_of(x):
@@ -145,6 +146,7 @@ def fp8_rows_gemm(rows: Fp8Rows, weight: Fp8Weight, group_indices, permute_indic
     if is_glu(act) or act not in _native.ACT_CODES:
         raise ValueError(f"products of 8-bit rows take no or an element-wise activation, got {act!r} "
                          "(gated experts: moe_explore.expert_compute.fp8_expert_compute)")
+    _native.refuse_tracing()
     if _native.needs_gradient(rows.data, rows.scales, weight.data, weight.scales):
         raise RuntimeError("products in 8 bits have no backward pass, of rows, weights or scales: call this under torch.no_grad()")
     device = rows.data.device

@@ -81,6 +81,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     """``y`` like ``x`` [..., d]; with ``residual``: (y, x + residual).  ``weight`` [d] in the rows' dtype or fp32.  Differentiable in
     all three; d a multiple of 8."""
     _checked(x, weight, residual)
+    _native.refuse_tracing()
     with _native.on_device_of(x):
         if not _native.needs_gradient(x, weight, residual):
             y, h, _ = _forward(x, weight, residual, float(eps), False)
@@ -92,6 +93,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     """The norm's result in 8 bits (``Fp8Rows``), for the 8-bit products of a serving pass: ``rows``, then, with ``with_rows``, the
     same result in 16 bits (what a router reads), then, with ``residual``, ``x + residual``.  No gradient; d a multiple of 16."""
     _checked(x, weight, residual)
+    _native.refuse_tracing()
     if _native.needs_gradient(x, weight, residual):
         raise RuntimeError("rms_norm_fp8 has no backward pass: call it under torch.no_grad(), or train with rms_norm")
     d = x.size(-1)

@@ -179,6 +179,7 @@ def grouped_topk_of_logits(logits: torch.Tensor, params: GroupedTopkRouterParams
     exact arithmetic, equal values by ascending index, NaN last.  Differentiable with respect to the logits."""
     dtype = logits.dtype if dtype is None else dtype
     _native.require_cuda(logits, params.bias)
+    _native.refuse_tracing()
     if logits.dim() != 2:
         raise ValueError(f"logits are [tokens, experts], got {tuple(logits.shape)}")
     if params.score_function not in ("sigmoid", "softmax"):

@@ -106,6 +106,38 @@ def test_refusals(native):
         topk_moe_forward(x.requires_grad_(True), p8)
 
 
+@gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning", "ignore::UserWarning")
+def test_traces_are_refused(native):
+    """A trace would hold the results of the traced input for constants; torch.compile runs the operators between its graphs."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from moe_explore.functional.fp8 import fp8_matmul, quantize_rows, quantize_weight
+    from moe_explore.router import grouped_topk_of_logits
+
+    p, new = make()
+    experts = quantize_experts(p.expert_params)
+    x, w = new(5, 256).bfloat16(), quantize_weight(new(64, 256))
+    rows, scores = quantize_rows(x), torch.rand(5, 4, device="cuda").bfloat16()
+    ids = torch.arange(4, device="cuda").expand(5, 4).contiguous()
+    calls = [lambda x: rms_norm(x, p.norm_params.weight), lambda x: rms_norm_fp8(x, p.norm_params.weight).data.float(),
+             lambda x: quantize_rows(x).data.float(), lambda x: fp8_matmul(rows, w) + x[:, :64],
+             lambda x: fp8_expert_compute(x, scores, ids, experts),
+             lambda x: grouped_topk_of_logits(x[:, :16], p.router_params)[0]]
+    with torch.no_grad():
+        for call in calls:
+            want = call(x)
+            with pytest.raises(RuntimeError, match="trace"):
+                make_fx(call)(x)
+            with pytest.raises(RuntimeError, match="trace"):
+                torch.jit.trace(call, (x,), check_trace=False)
+            assert torch.equal(call(x), want)
+        torch._dynamo.reset()
+        both = lambda x: rms_norm(x * 2, p.norm_params.weight) + 1
+        assert torch.equal(torch.compile(both, backend="eager")(x), both(x))
+        torch._dynamo.reset()
+
+
 def test_parameters_keep_their_positions():
     """Positional construction as before, the new fields last."""
     p = MOEParams("router", "experts", 8, 2, "shared")
