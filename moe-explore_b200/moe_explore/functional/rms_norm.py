@@ -23,7 +23,7 @@ def _checked(x, weight, residual):
 
 def _rows(x):
     """[..., d] as rows [R, d] that the kernels can read: dense columns, 16-byte aligned rows."""
-    if x.dim() == 2 and x.is_contiguous() and x.stride(0) == x.size(1) and x.data_ptr() % 16 == 0:
+    if x.dim() == 2 and x.stride() == (x.size(1), 1) and x.data_ptr() % 16 == 0:
         return x   # (a multiple of 8 columns is checked behind)
     x = x.reshape(-1, x.size(-1))
     if x.size(0) == 1 and x.stride(1) == 1:   # one row is contiguous whatever its stride, which counts for nothing
