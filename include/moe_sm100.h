@@ -126,7 +126,7 @@ int moe_grouped_topk_backward(const void* logits, const int64_t* indices, const 
  * Root-mean-square norm of rows x [num_rows, cols] (row stride x_stride elements), with the residual's addition:
  *   h = x + residual (rounded to `dtype`; x itself without a residual);  r = 1 / sqrt(mean h^2 + eps);  y = h * r * weight
  * y [num_rows, cols] in `dtype` and / or in 8 bits: q (e4m3) and scales fp32 [num_rows, ceil(cols / 128)], where a
- * block's scale is max(max |y|, 2^-80) / 448 and q = y / scale.  h (may be NULL), y, q and rstd (fp32 [num_rows], may
+ * block's scale is max(max |y|, 2^-80) / 448 and q = y / scale, by a product with the rounded 448 / max.  h (may be NULL), y, q and rstd (fp32 [num_rows], may
  * be NULL) are dense.  weight [cols]: `dtype`, or fp32.  cols a multiple of 8, at most 16384; pointers and row strides 16-byte
  * aligned.
  * Backward: dx = dh + r (g - h r mean(g h r)) with g = dy * weight (dh may be NULL; dx is also the residual's gradient), dw =

@@ -71,8 +71,9 @@ static int f8_maps(CUtensorMap* tx, CUtensorMap* tw, const void* x, int64_t rows
 }
 
 // The kernel with the weights on the lanes: how many items there can be (an expert each, in blocks of 128 columns) and how many
-// CTAs share one; none where it does not serve.  It does for 64 rows in all and no more items than SMs: 29 MB of one matrix
-// (7168 x 4096) take 11 to 15 us so and 29 with rows on the lanes; the 2 x 32 items of one token's down products (14336 x 4096) 31
+// CTAs share one; none where it does not serve.  It does for 64 rows in all (what its accumulators hold beside the ring) and no more
+// items than SMs: 29 MB of one matrix (7168 x 4096) take 12 us with 1 to 16 rows, 13 with 32 and 16 with 64, and 31 to 32 with rows on
+// the lanes, 65 of them or 600; the 2 x 32 items of one token's down products (14336 x 4096) 31
 // instead of 63 (as a part of the pass, waiting for the up products included).
 struct F8Lanes {
   int items, ranks;
@@ -320,8 +321,6 @@ int f8_rows(const char* name, const void* x, const float* x_scales, const int32_
     MOE_CUDA(launch_kernel(f8_rows_kernel<__half>, grid, 256, s, static_cast<const __half*>(x), x_scales, dst_row, copies, o, scales, static_cast<int>(rows), cols));
   return MOE_OK;
 }
-
-// Floats of the workers' slots.
 
 static bool glu(int act) { return act == MOE_ACT_SWIGLU || act == MOE_ACT_GEGLU; }
 

@@ -10,14 +10,15 @@
 // lane, then the lowest register".
 //
 // THE CHOICE IS THAT OF EXACT ARITHMETIC.  Values whose fp32 images are closer than what the evaluation in fp32 can be off by
-// are decided again in 64 bits, by the warp that met them (about one token in 1500 for 256 sigmoid scores with a bias): indices then
+// are decided again in 64 bits, by the warp that met them: about one token in 1500 for 256 sigmoid scores with a bias, but every
+// token that has equal values among those that decide, as a third have with 16-bit logits and a bias of zeros.  Indices then
 // depend neither on the order of a softmax's sum nor on the exponential's last bit.  Without a bias the logits
 // themselves are compared (p grows with l), and only sums over two members of a group can be that close.
 // Ties go to the lowest index, the k results come in descending order, NaN is taken after everything else.
 //
 // Bound by the instructions, about 1100 per token: 16384 tokens with 256 experts in 8 groups and a bias take 24 to 28 us (the logits
 // pass HBM in 3), one token 5 us, most of which are the launch and the chain of the rounds.  A token that is decided again in 64
-// bits takes 5 us more, beside the others.
+// bits takes 5 us more, beside the others: 16384 tokens with 16-bit logits 27 us, 45 where the bias is zeros, 22 without one.
 #include "common.cuh"
 
 #include <math_constants.h>

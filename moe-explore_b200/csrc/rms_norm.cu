@@ -173,8 +173,10 @@ struct NormBackArgs {
 
 // A CTA takes every gridDim.x-th row (a warp of the 32-thread form every row of its own stride) and keeps the weight gradient of
 // its columns in registers; the partial sums are joined by the next kernel in a fixed order.  The next row's loads are issued before
-// the row's one reduction.  8191 rows of 2048 with a residual: 28 us, 4.8 TB/s, with the sums of dw (42 us with the residual's
-// gradient fetched in the row's own turn); the launch bounds make all CTAs resident at once.
+// the row's one reduction.  8191 rows of 2048 with a residual: 28 to 31 us, 4.3 to 4.8 TB/s, with the sums of dw (42 us with the
+// residual's gradient fetched in the row's own turn).  Up to 2048 columns all CTAs are resident at once; wider rows leave room for two
+// or one per SM, so that they come in two to four waves and begin anew in each: 8192 x 4096 51 us (5.2 TB/s), 4096 x 7168 56 (4.2),
+// 4096 x 16384 143 (3.8; two pieces per thread in 64 registers spill).
 template <typename T, typename W, int THREADS, int VECS>
 __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : VECS == 1 ? 4 : 512 / THREADS)
     rms_norm_backward_kernel(const NormBackArgs a) {
@@ -294,7 +296,7 @@ static int launch_norm(const NormArgs& a, cudaStream_t s) {
     const int block = THREADS == 32 ? 128 : THREADS;                                                     \
     MOE_CUDA(launch_kernel(rms_norm_kernel<T, W, THREADS, VECS, QUANT>, static_cast<int>(grid), block, s, a)); \
   } while (0)
-  // few rows: as many threads per row as have a piece of it (one row of 8 KB: see below); many rows: a few pieces per thread
+  // few rows: as many threads per row as have a piece of it; many rows: a few pieces per thread
   const bool few = a.rows < 2 * sm_count();
   if (vecs <= 32) MOE_NORM(32, 1);
   else if (vecs <= 128 && !few) MOE_NORM(32, 4);
@@ -309,7 +311,7 @@ static int launch_norm(const NormArgs& a, cudaStream_t s) {
 }
 
 constexpr int kNormMaxCols = 16384;
-constexpr int kNormPartials = 592;  // four CTAs on each of 148 SMs
+constexpr int kNormPartials = 592;  // four CTAs on each of 148 SMs, at every width
 
 template <typename T, typename W>
 static int launch_norm_backward(const NormBackArgs& a, W* dw, cudaStream_t s) {

@@ -439,7 +439,7 @@ def fp8_expert_compute(x, scores, indices, params: Fp8ExpertParams, addend=None)
     """out[t] = sum_s scores[t, s] * (act(x[t] @ up[e]^T) @ down[e]^T) with e = indices[t, s], the products in 8 bits: rows (unless
     they are ``Fp8Rows`` already) and the activated products get a scale per 128 columns; everything is added in fp32 and
     each expert's row is rounded to the 16-bit result type before the fold.  ``x`` [T, d] in bf16 / fp16 or ``Fp8Rows`` (result in
-    their ``dtype``), ``scores`` and ``indices`` (int64) [T, k]; slots with an expert id out of range add nothing (and are
+    their ``dtype``), ``scores`` (rounded to the result's type, like the 16-bit experts') and ``indices`` (int64) [T, k]; slots with an expert id out of range add nothing (and are
     reported by the status word).  ``addend`` [T, d] is added by the fold.  For serving: no gradients.  d and I multiples of 16."""
     rows = isinstance(x, Fp8Rows)
     data = x.checked().data if rows else x

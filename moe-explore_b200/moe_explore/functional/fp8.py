@@ -1,8 +1,10 @@
 """Matrices in 8 bits -- e4m3 values with one fp32 scale per block of 128 -- and their products, for serving.
 
 Rows have a scale per row and 128 columns, weights one per 128 x 128 block and lie as [N, K] (K contiguous, as checkpoints store a
-linear layer).  ``scale = max(max |v|, 2^-80) / 448`` and ``q = v / scale`` rounded once, to nearest even.  Nothing here has a
-backward pass.  No reference counterpart.
+linear layer).  ``scale = max(max |v|, 2^-80) / 448`` and ``q = v / scale``, to nearest even; ``quantize_rows`` (and the experts'
+dispatch) round the quotient once to fp32 before, results that are made in fp32 (the norm's, the activated products) by one unit
+of fp32 more.  Nothing here has a backward pass: a product that is asked for a gradient, of rows, weights or scales, raises
+``RuntimeError``.  No reference counterpart.
 """
 from __future__ import annotations
 
@@ -82,7 +84,7 @@ def quantize_rows(x: torch.Tensor) -> Fp8Rows:
 
 
 def quantize_weight(weight: torch.Tensor) -> Fp8Weight:
-    """Weights [..., N, K] (16 or 32 bits) in 8 bits.  Torch operations: done once, when a model is loaded."""
+    """Weights [..., N, K] (16 or 32 bits) in 8 bits, detached.  Torch operations in fp32: done once, when a model is loaded."""
     w = weight.detach().float()
     n, k = w.shape[-2:]
     w = torch.nn.functional.pad(w, (0, blocks(k) * BLOCK - k, 0, blocks(n) * BLOCK - n))
