@@ -470,10 +470,13 @@ def grouped_topk_backward(logits, indices, d_scores, sigmoid: bool, normalize: b
 
 def rms_norm(x, residual, weight, eps: float, h=None, y=None, q=None, scales=None, rstd=None):
     """Rows ``x`` [R, d] (row stride allowed) into the outputs that are given (see moe_rms_norm)."""
+    rows, cols = x.shape
+    # (torch calls a single row contiguous whatever its stride, and the kernels read 16-byte pieces: it goes as a dense one)
+    x_stride = x.stride(0) if rows > 1 else cols
+    residual_stride = 0 if residual is None else residual.stride(0) if rows > 1 else cols
     with timed("rows:norm"):
-        rc = load().moe_rms_norm(x.data_ptr(), x.stride(0), _ptr(residual), 0 if residual is None else residual.stride(0),
-                                 weight.data_ptr(), float_code(weight.dtype), _ptr(h), _ptr(y), _ptr(q), _ptr(scales), _ptr(rstd),
-                                 x.size(0), x.size(1), eps, dtype_code(x.dtype), _stream())
+        rc = load().moe_rms_norm(x.data_ptr(), x_stride, _ptr(residual), residual_stride, weight.data_ptr(), float_code(weight.dtype),
+                                 _ptr(h), _ptr(y), _ptr(q), _ptr(scales), _ptr(rstd), rows, cols, eps, dtype_code(x.dtype), _stream())
     _check("moe_rms_norm", rc)
     _count(1)
 
@@ -485,7 +488,7 @@ def rms_norm_backward(dy, dh, h, weight, rstd):
     dw = torch.empty_like(weight)
     partials = torch.empty(int(load().moe_rms_norm_partials(rows)), cols, dtype=torch.float32, device=h.device)
     with timed("rows:norm_bwd"):
-        rc = load().moe_rms_norm_backward(dy.data_ptr(), _ptr(dh), h.data_ptr(), h.stride(0), weight.data_ptr(), float_code(weight.dtype),
+        rc = load().moe_rms_norm_backward(dy.data_ptr(), _ptr(dh), h.data_ptr(), h.stride(0) if rows > 1 else cols, weight.data_ptr(), float_code(weight.dtype),
                                           rstd.data_ptr(), dx.data_ptr(), dw.data_ptr(), partials.data_ptr(), rows, cols,
                                           dtype_code(h.dtype), _stream())
     _check("moe_rms_norm_backward", rc)

@@ -23,12 +23,10 @@ def _checked(x, weight, residual):
 
 def _rows(x):
     """[..., d] as rows [R, d] that the kernels can read: dense columns, 16-byte aligned rows."""
-    if x.dim() == 2 and x.stride() == (x.size(1), 1) and x.data_ptr() % 16 == 0:
-        return x   # (a multiple of 8 columns is checked behind)
+    if x.dim() == 2 and x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x   # (a multiple of 8 columns is checked behind; a single row's stride, whatever it is, is not looked at)
     x = x.reshape(-1, x.size(-1))
-    if x.size(0) == 1 and x.stride(1) == 1:   # one row is contiguous whatever its stride, which counts for nothing
-        x = x.as_strided(x.shape, (x.size(1), 1))
-    if x.stride(1) != 1 or x.stride(0) % 8 != 0 or x.data_ptr() % 16 != 0:
+    if x.stride(1) != 1 or x.size(0) != 1 and x.stride(0) % 8 != 0 or x.data_ptr() % 16 != 0:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 

@@ -232,15 +232,35 @@ def test_leading_axes_strides_empty_streams_and_capture(native):
     assert torch.equal(out, y2) and torch.equal(rows.data.view(torch.uint8), again.data.view(torch.uint8)) and torch.equal(rows.scales, again.scales)
 
 
-def test_one_row_has_no_stride(native):
+def test_one_row_has_no_stride(native, monkeypatch):
     """Torch calls a single row contiguous whatever its stride; the kernels get one that they can read."""
-    from moe_explore.functional.rms_norm import _rows
+    from moe_explore.functional.rms_norm import _forward, _rows
 
+    class Library:   # takes down the strides that the kernels would get
+        def moe_rms_norm(self, x, x_stride, residual, residual_stride, *rest):
+            self.got = x, x_stride, residual, residual_stride
+            return 0
+
+        def moe_rms_norm_backward(self, dy, dh, h, h_stride, *rest):
+            self.got = dy, 0, h, h_stride
+            return 0
+
+        moe_rms_norm_partials = staticmethod(lambda rows: rows)
+
+    library = Library()
+    monkeypatch.setattr(native, "load", lambda: library)
+    monkeypatch.setattr(native, "_stream", lambda: None)
+    w = torch.ones(64, dtype=torch.bfloat16)
     for cut in (lambda b: b[:1, :64], lambda b: b[5:6, 3:67], lambda b: b[2:3, 1:2].expand(1, 64), lambda b: b.t()[:1, :64],
                 lambda b: b[:1, None, :64], lambda b: b[0, :64]):
         x = cut(torch.arange(80 * 77, dtype=torch.float32).view(80, 77).bfloat16())
         rows = _rows(x)
-        assert torch.equal(rows, x.reshape(1, 64)) and rows.stride(1) == 1 and rows.stride(0) % 8 == 0 and rows.data_ptr() % 16 == 0
+        assert torch.equal(rows, x.reshape(1, 64)) and rows.stride(1) == 1
+        y, h, _ = _forward(x, w, x, 1e-6, False)
+        assert y.shape == h.shape == x.shape
+        assert all(v % 8 == 0 for v in library.got[1::2]) and all(v % 16 == 0 for v in library.got[::2])
+        native.rms_norm_backward(_rows(x).contiguous(), None, rows, w, torch.ones(1))
+        assert all(v % 8 == 0 for v in library.got[1::2]) and library.got[2] % 16 == 0
     dense = torch.zeros(3, 64)
     assert _rows(dense) is dense
     wide = torch.zeros(4, 512, dtype=torch.bfloat16)
