@@ -499,6 +499,15 @@ typedef struct moe_expert_pass {
   const float* router_bias; /* MOE_FWD_TAIL: see moe_router_tail */
   int32_t logits_dtype;
   int32_t own_tie_rule; /* MOE_FWD_TAIL by moe_router_topk instead */
+  /* The un-activated product kept in 8 bits (NULL: in 16, in pre_act): e4m3 [padded_rows, columns rounded up to 16] with fp32 scales
+   * [padded_rows, ceil(columns / 128)], columns = 2 inter (gated) or inter; rows of the padding are left as they are.  Not with
+   * `gather`, `fused_combine`, `identity` or MOE_BWD_ROUTER.  Forward: MOE_FWD_UP leaves the plain product in pre_act (scratch),
+   * MOE_FWD_ACT (part of every such pass) the activated one in hidden and the kept one here.  Backward: x holds the tokens' rows;
+   * MOE_BWD_FOLD copies the rows of grad_out to gs and those of x to xs (scratch), MOE_BWD_DOWN leaves gs W2^T in dh (scratch
+   * [padded_rows, inter]), MOE_BWD_ACT writes d_pre, d_scores and the weighted activated rows that MOE_BWD_DW2 reads (hidden, scratch). */
+  void* pre_q;
+  float* pre_scales;
+  void* dh;
 } moe_expert_pass;
 
 /* sizeof(moe_expert_pass), for bindings that declare the struct themselves. */
@@ -511,6 +520,7 @@ size_t moe_expert_pass_size(void);
 #define MOE_FWD_FOLD 16
 #define MOE_FWD_ALL 31
 #define MOE_FWD_TAIL 32 /* first: moe_router_tail (moe_router_topk) of `logits` into `scores` and `expert_idx` */
+#define MOE_FWD_ACT 64  /* after MOE_FWD_UP: with pre_q */
 int moe_expert_forward(const moe_expert_pass* pass, int steps, void* stream);
 
 #define MOE_BWD_FOLD 1    /* gs, d_scores */
@@ -521,6 +531,7 @@ int moe_expert_forward(const moe_expert_pass* pass, int steps, void* stream);
 #define MOE_BWD_DW2 32
 #define MOE_BWD_ROUTER 64 /* dl, dlogits, router_t */
 #define MOE_BWD_ALL 127
+#define MOE_BWD_ACT 128   /* after MOE_BWD_DOWN: with pre_q */
 int moe_expert_backward(const moe_expert_pass* pass, int steps, void* stream);
 
 /* The functional grouped GEMM in one call, rows grouped by `group_indices` [num_experts + 1]:
@@ -621,6 +632,16 @@ typedef struct moe_f8_rows_pass {
 
 size_t moe_f8_rows_pass_size(void);
 int moe_f8_rows_gemm(const moe_f8_rows_pass* pass, int steps, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Activations that keep their input in 8 bits for the backward pass.  No counterpart in the reference.
+ * z [rows, columns] in `dtype`, columns = 2 inter with gate and up in turn (gated) or inter; h, dh [rows, inter]; q e4m3 [rows, columns
+ * rounded up to 16] and scales [rows, ceil(columns / 128)] as moe_f8_quantize_rows makes them; inter a multiple of 8.
+ * forward: h = act(z) (from z itself), q and scales (both NULL: not kept).  backward: dz = gradient at q * scales of dh.
+ * --------------------------------------------------------------------------------- */
+int moe_act_f8_forward(const void* z, void* h, void* q, float* scales, int64_t rows, int inter, int act, int dtype, void* stream);
+int moe_act_f8_backward(const void* q, const float* scales, const void* dh, void* dz, int64_t rows, int inter, int act, int dtype,
+                        void* stream);
 
 #ifdef __cplusplus
 }

@@ -155,6 +155,10 @@ int combine_bwd_tokens(const void* dout, const void* scores, const void* ys, con
                        const int32_t* num_mtiles, void* gs, void* dscores, int64_t num_tokens, int topk, int cols, int dtype,
                        void* stream, bool live_blocks_only, uint32_t* work_counters);
 
+// The steps of an experts' pass that keeps the un-activated product in 8 bits (act_f8.cu).
+int act_f8_layer_forward(const moe_expert_pass* p, void* stream);
+int act_f8_layer_backward(const moe_expert_pass* p, void* stream);
+
 // Tensor map of 16-bit elements (grouped_gemm.cu), kept for the next call that asks for the same.
 int make_tmap(CUtensorMap* map, int dtype, const void* ptr, int rank, const uint64_t* dims, const uint32_t* box,
               const uint64_t* strides = nullptr, bool swizzle = true);

@@ -44,6 +44,9 @@ extern "C" int moe_expert_forward(const moe_expert_pass* p, int steps, void* str
                              p->inter, p->d, 1, 0, MOE_ACT_NONE, p->dtype, 0, 1, nullptr, p->status, stream, out));
     return MOE_OK;
   }
+  const bool kept8 = p->pre_q != nullptr;  // the un-activated product is kept in 8 bits
+  MOE_CHECK_ARG(!kept8 || (!p->gather && !p->fused_combine && p->pre_scales && p->pre_act && p->hidden),
+                "moe_expert_forward: pre_q goes with pre_scales, pre_act and hidden, without gather and fused_combine");
   RowCounts counts{p->pad_offsets, p->group_indices};
   counts.routed_rows = rows;
   uint32_t* const counters = p->gather ? nullptr : reinterpret_cast<uint32_t*>(p->counters);
@@ -68,7 +71,7 @@ extern "C" int moe_expert_forward(const moe_expert_pass* p, int steps, void* str
   const bool cleared = p->fused_combine && !p->keep && !p->gather && (steps & MOE_FWD_DISPATCH) != 0;
   if ((steps & MOE_FWD_DISPATCH) && !p->gather) {
     // rows do not mix in a forward pass, and only a weight gradient contracts over the padding rows
-    if (p->keep)
+    if (p->keep && !kept8)
       MOE_STEP(dispatch_rows(p->x, p->dst_row, p->row_src, p->num_mtiles, p->xs, p->num_tokens, p->topk, p->padded_rows, p->d,
                                  p->dtype, stream, true, counters));
     else
@@ -81,10 +84,11 @@ extern "C" int moe_expert_forward(const moe_expert_pass* p, int steps, void* str
                                         p->tile_pairs, p->num_mtiles, p->padded_rows, p->d, up_cols, p->num_experts, p->act,
                                         p->dtype, nullptr, p->status, stream, counts));
     else
-      MOE_STEP(mgrouped_gemm(p->xs, p->w1, p->hidden, p->pre_act, p->mtile_expert, p->tile_pairs, p->num_mtiles,
-                                 p->padded_rows, p->d, up_cols, p->num_experts, 0, p->act, p->dtype, 0, 1, nullptr, p->status,
-                                 stream, claiming(counts, counters, 0)));
+      MOE_STEP(mgrouped_gemm(p->xs, p->w1, kept8 ? p->pre_act : p->hidden, kept8 ? nullptr : p->pre_act, p->mtile_expert, p->tile_pairs,
+                                 p->num_mtiles, p->padded_rows, p->d, up_cols, p->num_experts, 0, kept8 ? MOE_ACT_NONE : p->act,
+                                 p->dtype, 0, 1, nullptr, p->status, stream, claiming(counts, counters, 0)));
   }
+  if ((steps & MOE_FWD_ACT) && kept8) MOE_STEP(act_f8_layer_forward(p, stream));
   if (steps & MOE_FWD_DOWN) {
     if (p->fused_combine) {
       if (!cleared) {
@@ -138,21 +142,30 @@ extern "C" int moe_expert_backward(const moe_expert_pass* p, int steps, void* st
   counts.routed_rows = p->num_tokens * p->topk;
   counts.settled = true;  // nothing of a backward pass writes the metadata or the weights
   uint32_t* const counters = reinterpret_cast<uint32_t*>(p->counters);
-  if (steps & MOE_BWD_FOLD)
+  const bool kept8 = p->pre_q != nullptr;  // d_scores and what dW2 contracts then come behind the product of the rows of grad_out
+  MOE_CHECK_ARG(!kept8 || (!p->gather && p->dl == nullptr && p->pre_scales && p->dh && p->xs && p->hidden),
+                "moe_expert_backward: pre_q goes with pre_scales, dh, xs and hidden, without gather and the router's gradient");
+  if ((steps & MOE_BWD_FOLD) && kept8) {
+    MOE_STEP(dispatch_rows(p->grad_out, p->dst_row, p->row_src, p->num_mtiles, p->gs, p->num_tokens, p->topk, p->padded_rows, p->d,
+                           p->dtype, stream, true, counters));
+    MOE_STEP(dispatch_rows(p->x, p->dst_row, p->row_src, p->num_mtiles, p->xs, p->num_tokens, p->topk, p->padded_rows, p->d, p->dtype,
+                           stream, true, nullptr));
+  } else if (steps & MOE_BWD_FOLD)
     MOE_STEP(combine_bwd_tokens(p->grad_out, p->scores, p->ys, p->dst_row, p->row_src, p->num_mtiles, p->gs, p->d_scores,
                                     p->num_tokens, p->topk, p->d, p->dtype, stream, true, counters));
   if ((steps & MOE_BWD_ROUTER) && p->dl != nullptr)
     MOE_STEP(router_backward(p->logits, p->expert_idx, p->d_scores, p->router_w, p->dl, p->dlogits, p->router_t, p->num_tokens,
                              p->num_experts, p->topk, p->d, p->dtype, stream));
   if (steps & MOE_BWD_DOWN) {
-    if (p->act == MOE_ACT_NONE)  // linear "activation": d_pre = gs @ W2^T
-      MOE_STEP(mgrouped_gemm(p->gs, p->w2, p->d_pre, nullptr, p->mtile_expert, p->tile_pairs, p->num_mtiles, p->padded_rows,
+    if (p->act == MOE_ACT_NONE || kept8)  // linear "activation": d_pre = gs @ W2^T
+      MOE_STEP(mgrouped_gemm(p->gs, p->w2, kept8 ? p->dh : p->d_pre, nullptr, p->mtile_expert, p->tile_pairs, p->num_mtiles, p->padded_rows,
                                  p->d, p->inter, p->num_experts, 1, MOE_ACT_NONE, p->dtype, 0, 1, nullptr, p->status, stream, claiming(counts, counters, 0)));
     else
       MOE_STEP(mgrouped_gemm_dglu(p->gs, p->w2, p->pre_act, p->d_pre, p->mtile_expert, p->tile_pairs, p->num_mtiles,
                                       p->padded_rows, p->d, p->inter, p->num_experts, p->act, p->dtype, 0, 1, nullptr, p->status,
                                       stream, claiming(counts, counters, 0)));
   }
+  if ((steps & MOE_BWD_ACT) && kept8) MOE_STEP(act_f8_layer_backward(p, stream));
   if (steps & MOE_BWD_UP)
     MOE_STEP(mgrouped_gemm(p->d_pre, p->w1, p->dxs, nullptr, p->mtile_expert, p->tile_pairs, p->num_mtiles, p->padded_rows,
                                up_cols, p->d, p->num_experts, 1, MOE_ACT_NONE, p->dtype, 0, 1, nullptr, p->status, stream, claiming(counts, counters, 1)));

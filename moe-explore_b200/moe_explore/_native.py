@@ -49,7 +49,8 @@ class ExpertPass(ctypes.Structure):
                [(f, c_void_p) for f in ("xs", "pre_act", "hidden", "ys", "out", "grad_out", "gs", "d_scores", "d_pre", "dxs", "dx",
                                         "d_w1", "d_w2", "addend", "logits", "router_w", "dl", "dlogits", "router_t")] + \
                [(f, c_int32) for f in ("softmax_before_topk", "normalize")] + [("counters", c_void_p)] + \
-               [("router_bias", c_void_p), ("logits_dtype", c_int32), ("own_tie_rule", c_int32)]
+               [("router_bias", c_void_p), ("logits_dtype", c_int32), ("own_tie_rule", c_int32)] + \
+               [(f, c_void_p) for f in ("pre_q", "pre_scales", "dh")]
 
 
 class RowsPass(ctypes.Structure):
@@ -120,6 +121,8 @@ SIGNATURES = {
     "moe_expert_pass_size": (c_size_t, []),
     "moe_expert_forward": (c_int, [POINTER(ExpertPass), c_int, c_void_p]),
     "moe_expert_backward": (c_int, [POINTER(ExpertPass), c_int, c_void_p]),
+    "moe_act_f8_forward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
+    "moe_act_f8_backward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
     "moe_f8_quantize_rows": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p]),
     "moe_f8_pass_size": (c_size_t, []),
     "moe_f8_expert_forward": (c_int, [POINTER(F8Pass), c_int, c_void_p]),
@@ -322,8 +325,8 @@ def _opt(options):
 
 ROWS_LAYOUT, ROWS_GATHER, ROWS_GEMM = 1, 2, 4
 F8_ROUTE, F8_DISPATCH, F8_UP, F8_DOWN, F8_FOLD = 1, 2, 4, 8, 16
-FWD_ROUTE, FWD_DISPATCH, FWD_UP, FWD_DOWN, FWD_FOLD, FWD_TAIL = 1, 2, 4, 8, 16, 32
-BWD_FOLD, BWD_DOWN, BWD_UP, BWD_FOLD_DX, BWD_DW1, BWD_DW2, BWD_ROUTER = 1, 2, 4, 8, 16, 32, 64
+FWD_ROUTE, FWD_DISPATCH, FWD_UP, FWD_DOWN, FWD_FOLD, FWD_TAIL, FWD_ACT = 1, 2, 4, 8, 16, 32, 64
+BWD_FOLD, BWD_DOWN, BWD_UP, BWD_FOLD_DX, BWD_DW1, BWD_DW2, BWD_ROUTER, BWD_ACT = 1, 2, 4, 8, 16, 32, 64, 128
 
 
 def run_pass(name: str, p, steps, rows: int) -> None:
@@ -502,6 +505,24 @@ def f8_quantize_rows(x, q, scales):
         rc = load().moe_f8_quantize_rows(x.data_ptr(), q.data_ptr(), scales.data_ptr(), x.size(0), x.size(1), dtype_code(x.dtype),
                                          _stream())
     _check("moe_f8_quantize_rows", rc)
+    _count(1)
+
+
+def act_f8_forward(z, h, q, scales, act):
+    """Activated rows of ``z`` [R, columns] and, with ``q``, what is kept of them (see moe_act_f8_forward)."""
+    with timed("rows:act"):
+        rc = load().moe_act_f8_forward(z.data_ptr(), h.data_ptr(), _ptr(q), _ptr(scales), h.size(0), h.size(1), ACT_CODES[act],
+                                       dtype_code(z.dtype), _stream())
+    _check("moe_act_f8_forward", rc)
+    _count(1)
+
+
+def act_f8_backward(q, scales, dh, dz, act):
+    """Gradient of ``act_f8_forward``'s rows from what was kept (see moe_act_f8_backward)."""
+    with timed("rows:act"):
+        rc = load().moe_act_f8_backward(q.data_ptr(), scales.data_ptr(), dh.data_ptr(), dz.data_ptr(), dh.size(0), dh.size(1),
+                                        ACT_CODES[act], dtype_code(dh.dtype), _stream())
+    _check("moe_act_f8_backward", rc)
     _count(1)
 
 

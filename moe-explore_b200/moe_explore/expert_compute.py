@@ -19,6 +19,7 @@ import torch
 
 from moe_explore import _native
 from moe_explore.functional.activation import is_glu
+from moe_explore.functional.activation_fp8 import kept_columns
 from moe_explore.functional.fp8 import Fp8Rows, _dense, blocks
 from moe_explore.params import ErnieRouterParams, Fp8ExpertParams, TopkRouterParams
 from moe_explore.router import ernie_router, fused_topk_of_logits, nothing_watches, tail_in_one_kernel, topk_of_logits
@@ -234,6 +235,76 @@ class ExpertCompute(torch.autograd.Function):
         return _backward(ctx.info, ctx.saved_tensors, grad_out)[:4] + (None,) * 4 + (grad_out if ctx.needs_input_grad[8] else None,)
 
 
+class ExpertComputeFp8(torch.autograd.Function):
+    """The routed experts with the un-activated product kept in 8 bits (``moe_explore.functional.activation_fp8``) and nothing else of
+    their rows: the backward pass gathers the tokens' rows again, and computes the activation, the weighted rows of weight2's
+    gradient and the router weights' gradient from the kept product.  Of a row (a token's slot) it holds 1.03 bytes per column of
+    weight1 instead of two bytes for each of these columns, the activated ones and twice the hidden size."""
+
+    @staticmethod
+    def forward(ctx, x, scores, weight1, weight2, routing, act, addend):
+        indices, E, topk = routing
+        T, d, inter, n1 = x.size(0), x.size(1), weight2.size(1), weight1.size(2)
+        x, weight1, weight2 = x.contiguous(), weight1.contiguous(), weight2.contiguous()
+        flat, scores = indices.reshape(-1).contiguous(), scores.to(x.dtype).contiguous()
+        addend = None if addend is None else addend.contiguous()
+        rows = T * topk
+        ctx.sizes, ctx.act = (T, d, inter, E, topk, 0, n1), act
+        if T == 0:
+            ctx.save_for_backward(x, scores, weight1, weight2)
+            return torch.empty_like(x)
+        rp, offsets, num_words = packed_layout(rows, E)
+        ctx.kept = (4 * num_words, rp * kept_columns(n1), 4 * rp * blocks(n1))
+        ctx.sizes = (T, d, inter, E, topk, rp, n1)
+        kept, (words, pre_q, pre_scales) = _buffers(ctx.kept, x.device)
+        scratch, (xs, pre, hidden, ys, counters) = _buffers(
+            (2 * rp * d, 2 * rp * n1, 2 * rp * inter, 2 * rp * d, 4 * _native.WORK_COUNTERS), x.device)
+        launches = _native.routing_launches(rows, E)
+        workspace = None
+        if launches > 1:
+            workspace = torch.empty(max(_native.routing_workspace_bytes(rows, E), 16), dtype=torch.uint8, device=x.device)
+        out = torch.empty(T, d, dtype=x.dtype, device=x.device)
+        ptr = _native._ptr
+        p = _native.ExpertPass(
+            T, rp, d, inter, E, topk, _native.ACT_CODES[act], _native.dtype_code(x.dtype), 0, 0, 1, 0, flat.data_ptr(), x.data_ptr(),
+            scores.data_ptr(), weight1.data_ptr(), weight2.data_ptr(), *_packed_pointers(words, offsets, device_status(x.get_device())),
+            ptr(workspace), 0 if workspace is None else workspace.numel(), xs, pre, hidden, ys, out.data_ptr())
+        p.addend, p.counters, p.pre_q, p.pre_scales = ptr(addend), counters, pre_q, pre_scales
+        _native.run_pass("moe_expert_forward", p, [
+            (_native.FWD_ROUTE, "routing", launches), (_native.FWD_DISPATCH, "rows:gather", 1), (_native.FWD_UP, "mgrouped_gemm:plain", 1),
+            (_native.FWD_ACT, "rows:act", 1), (_native.FWD_DOWN, "mgrouped_gemm:plain", 1), (_native.FWD_FOLD, "rows:combine", 1)], rows)
+        ctx.save_for_backward(x, scores, weight1, weight2, *kept)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        x, scores, weight1, weight2, *kept = ctx.saved_tensors
+        T, d, inter, E, topk, rp, n1 = ctx.sizes
+        rows = T * topk
+        if T == 0:
+            return (*(torch.zeros_like(t) for t in (x, scores, weight1, weight2)), None, None, grad_out if ctx.needs_input_grad[6] else None)
+        with _native.on_device_of(x):
+            grad = grad_out.contiguous()
+            words, pre_q, pre_scales = _addresses(ctx.kept, kept)
+            scratch, (xs, gs, dh, d_pre, hidden, dxs, counters) = _buffers(
+                (2 * rp * d, 2 * rp * d, 2 * rp * inter, 2 * rp * n1, 2 * rp * inter, 2 * rp * d, 4 * _native.WORK_COUNTERS), x.device)
+            d_scores, dx = torch.empty_like(scores), torch.empty_like(x)
+            d_w1, d_w2 = torch.empty_like(weight1), torch.empty_like(weight2)
+            p = _native.ExpertPass(
+                T, rp, d, inter, E, topk, _native.ACT_CODES[ctx.act], _native.dtype_code(x.dtype), 0, 0, 1, 0, None, x.data_ptr(),
+                scores.data_ptr(), weight1.data_ptr(), weight2.data_ptr(),
+                *_packed_pointers(words, packed_layout(rows, E)[1], device_status(x.get_device())), None, 0,
+                xs, None, hidden, None, None, grad.data_ptr(), gs, d_scores.data_ptr(), d_pre, dxs, dx.data_ptr(), d_w1.data_ptr(),
+                d_w2.data_ptr())
+            p.counters, p.pre_q, p.pre_scales, p.dh = counters, pre_q, pre_scales, dh
+            _native.run_pass("moe_expert_backward", p, [
+                (_native.BWD_FOLD, "rows:gather", 2), (_native.BWD_DOWN, "mgrouped_gemm:wt", 1), (_native.BWD_ACT, "rows:act", 1),
+                (_native.BWD_UP, "mgrouped_gemm:wt", 1), (_native.BWD_FOLD_DX, "rows:combine", 1), (_native.BWD_DW1, "kgrouped_gemm:dw1", 1),
+                (_native.BWD_DW2, "kgrouped_gemm:dw2", 1)], rows)
+        return dx, d_scores, d_w1, d_w2, None, None, grad_out if ctx.needs_input_grad[6] else None
+
+
 class RoutedLayer(torch.autograd.Function):
     """The layer with a router whose softmax runs over the selected logits: scores and indices with the bits of ``topk_router`` (the
     router's tail as part of the pass, or its torch ops), their backward as part of the experts' backward pass.  The gradient of such
@@ -350,15 +421,44 @@ def dense_expert(x, weight1, weight2, act) -> torch.Tensor:
 
 
 def routed_expert_compute(x, scores, weight1, weight2, indices, num_experts: int, topk: int, act, gather_in_gemm=None,
-                          fused_combine: bool = False, addend=None) -> torch.Tensor:
+                          fused_combine: bool = False, addend=None, save_fp8: bool = False) -> torch.Tensor:
     """``expert_compute`` of a routing decision given as expert indices (int64 [T, topk]) instead of a plan; ``addend`` (like the
-    output, not with ``fused_combine``) is added to the result."""
+    output, not with ``fused_combine``) is added to the result.  ``save_fp8``: where a gradient is wanted, the pass keeps the
+    un-activated product in 8 bits instead of its 16-bit rows (``ExpertComputeFp8``); the activation is then taken of the product
+    rounded to 16 bits, and the gradients at the kept values.  Not with ``gather_in_gemm``."""
     _native.require_cuda(indices)
     assert indices.dtype is torch.int64, "expert indices must be int64 (what torch.topk returns)"
+    if save_fp8 and torch.is_grad_enabled() and any(t.requires_grad for t in (x, scores, weight1, weight2)):
+        return _experts_kept_in_8_bits(x, scores, weight1, weight2, indices, num_experts, topk, act, gather_in_gemm, addend)
     if gather_in_gemm is None:
         gather_in_gemm = GATHER_IN_GEMM_DEFAULT
     return ExpertCompute.apply(x, scores, weight1, weight2, (indices, num_experts, topk), None if act is None else str(act),
                                bool(gather_in_gemm), bool(fused_combine), addend)
+
+
+def _experts_kept_in_8_bits(x, scores, weight1, weight2, indices, num_experts: int, topk: int, act, gather_in_gemm, addend):
+    _native.require_cuda(x, scores, weight1, weight2, addend)
+    _native.refuse_tracing()
+    act = None if act is None else str(act)
+    if act not in _native.ACT_CODES:
+        raise ValueError(f"Unsupported activation: {act!r}")
+    if gather_in_gemm:
+        raise ValueError("save_fp8 keeps the rows' product instead of gathering rows twice: not with gather_in_gemm")
+    if x.dtype not in (torch.bfloat16, torch.float16) or any(t.dtype is not x.dtype for t in (weight1, weight2)):
+        raise TypeError(f"save_fp8 takes bf16 or fp16 rows and weights of one type, got {x.dtype}, {weight1.dtype}, {weight2.dtype}")
+    if x.dim() != 2 or weight1.dim() != 3 or weight2.dim() != 3 or weight1.shape[:2] != (num_experts, x.size(1)) or \
+            weight2.shape != (num_experts, weight1.size(2) // (2 if is_glu(act) else 1), x.size(1)) or \
+            weight1.size(2) != weight2.size(1) * (2 if is_glu(act) else 1):
+        raise ValueError(f"shapes do not match: input {tuple(x.shape)}, weight1 {tuple(weight1.shape)}, weight2 {tuple(weight2.shape)}")
+    if indices.numel() != x.size(0) * topk or scores.numel() != indices.numel():
+        raise ValueError("indices (int64) and scores are [tokens, k]")
+    if any(t.device != x.device for t in (scores, weight1, weight2, indices) + (() if addend is None else (addend,))):
+        raise ValueError("all tensors lie on the device of the input")
+    if addend is not None and (addend.shape != x.shape or addend.dtype is not x.dtype):
+        raise ValueError("addend is like the result")
+    with _native.on_device_of(x):
+        # (a scores tensor of another type or shape is brought to the result's in sight of autograd)
+        return ExpertComputeFp8.apply(x, scores.to(x.dtype).reshape(-1, topk), weight1, weight2, (indices, num_experts, topk), act, addend)
 
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)

@@ -42,10 +42,11 @@ def _shared_expert(input: torch.Tensor, shared) -> torch.Tensor:
 
 
 def topk_moe_forward(input: torch.Tensor, params: MOEParams, autotune_mode=None, *, fused_router: bool = False,
-                     gather_in_gemm=None, fused_combine: bool = False, residual: torch.Tensor = None):
+                     gather_in_gemm=None, fused_combine: bool = False, residual: torch.Tensor = None, save_fp8: bool = False):
     """The layer (functional/topk_moe.py:10-64).  ``autotune_mode`` is accepted and ignored.  Keyword-only additions:
     ``fused_router`` runs the router tail in one kernel with its own declared tie rule (see
-    ``moe_explore.router.fused_topk_router``); ``gather_in_gemm`` / ``fused_combine`` as in ``expert_compute``.
+    ``moe_explore.router.fused_topk_router``); ``gather_in_gemm`` / ``fused_combine`` as in ``expert_compute``; ``save_fp8`` as in
+    ``routed_expert_compute``: a training pass keeps its experts' un-activated product in 8 bits and nothing else of their rows.
 
     With ``params.norm_params`` the layer begins with its norm: router, experts and shared expert see ``rms_norm(input)``, or, with
     ``residual``, ``rms_norm(input + residual)``, and the result is the pair (layer's output, ``input + residual``) that the next
@@ -55,7 +56,7 @@ def topk_moe_forward(input: torch.Tensor, params: MOEParams, autotune_mode=None,
     if norm is None:
         if residual is not None:
             raise ValueError("residual is added by the layer's norm: params.norm_params is None")
-        return _layer(input, None, params, fused_router, gather_in_gemm, fused_combine)
+        return _layer(input, None, params, fused_router, gather_in_gemm, fused_combine, save_fp8)
     rows = stream = None
     if isinstance(params.expert_params, Fp8ExpertParams):
         rows, normed, *rest = rms_norm_fp8(input, norm.weight, norm.eps, residual, with_rows=True)
@@ -64,11 +65,12 @@ def topk_moe_forward(input: torch.Tensor, params: MOEParams, autotune_mode=None,
         normed = rms_norm(input, norm.weight, norm.eps)
     else:
         normed, stream = rms_norm(input, norm.weight, norm.eps, residual)
-    out = _layer(normed, rows, params, fused_router, gather_in_gemm, fused_combine)
+    out = _layer(normed, rows, params, fused_router, gather_in_gemm, fused_combine, save_fp8)
     return out if residual is None else (out, stream)
 
 
-def _layer(input: torch.Tensor, rows: Fp8Rows, params: MOEParams, fused_router: bool, gather_in_gemm, fused_combine: bool) -> torch.Tensor:
+def _layer(input: torch.Tensor, rows: Fp8Rows, params: MOEParams, fused_router: bool, gather_in_gemm, fused_combine: bool,
+           save_fp8: bool) -> torch.Tensor:
     """Router, experts and shared expert; ``rows``: the input in 8 bits where it is there already."""
     ep: MLPParams = params.expert_params
     shared = getattr(params, "shared_expert_params", None)
@@ -83,7 +85,7 @@ def _layer(input: torch.Tensor, rows: Fp8Rows, params: MOEParams, fused_router: 
         else:
             scores, indices = router(input, params.router_params)
         out = fp8_expert_compute(input if rows is None else rows, scores, indices, ep, addend=addend)
-    elif not fused_router and router_joins_the_pass(input, params.router_params, params.num_experts, params.topk):
+    elif not save_fp8 and not fused_router and router_joins_the_pass(input, params.router_params, params.num_experts, params.topk):
         out = routed_layer(input, params.router_params, ep.weight1, ep.weight2, params.num_experts, ep.activation,
                            gather_in_gemm=gather_in_gemm, addend=addend)
     elif router_and_experts_at_once(input, params.router_params, ep.weight1, ep.weight2, params.num_experts, params.topk, addend):
@@ -95,7 +97,8 @@ def _layer(input: torch.Tensor, rows: Fp8Rows, params: MOEParams, fused_router: 
         else:
             scores, indices = router(input, params.router_params)
         out = routed_expert_compute(input, scores, ep.weight1, ep.weight2, indices, params.num_experts, params.topk,
-                                    ep.activation, gather_in_gemm=gather_in_gemm, fused_combine=fused_combine, addend=addend)
+                                    ep.activation, gather_in_gemm=gather_in_gemm, fused_combine=fused_combine, addend=addend,
+                                    save_fp8=save_fp8)
     if shared_out is not None and addend is None:
         out = out + shared_out
     return out
