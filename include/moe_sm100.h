@@ -643,6 +643,18 @@ int moe_act_f8_forward(const void* z, void* h, void* q, float* scales, int64_t r
 int moe_act_f8_backward(const void* q, const float* scales, const void* dh, void* dz, int64_t rows, int inter, int act, int dtype,
                         void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Products of a few 16-bit rows with weights in 4 bits (for serving: forward only).  No counterpart in the reference.
+ * Element [n, k] of w [n_dim, k_dim] is (value - zero) * scale: a value of 0 to 15, scale (`dtype`) and zero (uint8; `zeros` NULL: 8) per row
+ * and `group` of 32, 64 or 128 columns.  Laid out in tiles of 16 rows and steps of 128 columns, ceil(n_dim / 16) tiles of ceil(k_dim /
+ * 128) steps:  data: 1024 bytes per step, byte (half * 32 + 4 r + t) * 16 + 4 i + b holds row r + 8 half, columns 32 i + 8 t + 4 (b % 2) +
+ * b / 2 (low four bits) and two behind (high);  scales, zeros: [16 rows][128 / group] per step.  Rows behind n_dim and columns behind
+ * k_dim hold zeros.  All pointers 16-byte aligned, k_dim and n_dim multiples of 8.
+ * out [rows, n_dim] = x [rows, k_dim] @ w^T.
+ * --------------------------------------------------------------------------------- */
+int moe_int4_matmul(const void* x, const void* data, const void* scales, const void* zeros, void* out, int64_t rows, int k_dim, int n_dim,
+                    int group, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

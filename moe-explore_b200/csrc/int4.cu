@@ -1,0 +1,163 @@
+// A few 16-bit rows by one matrix of 4-bit weights (int4.cuh): out [rows, N] = x [rows, K] @ w [N, K]^T.
+//
+// A CTA takes one tile of 16 weight rows and up to 8 MT rows of x; its eight warps share the steps of K, and where there are few tiles,
+// so do the CTAs of a cluster.  Their sums are joined in a fixed order, through shared memory and then the cluster's.
+#include "int4.cuh"
+
+#include <atomic>
+
+namespace moe {
+
+constexpr int kQ4Warps = 8;
+constexpr int kQ4Depth = 5;   // steps that a warp has room for: 3 CTAs per SM ask for 100 KB at a time
+template <int NG, bool ZEROS> constexpr int kQ4Ring = kQ4Depth * Q4Stage<NG, ZEROS>::kBytes;
+
+struct Q4Args {
+  Q4Matrix w;
+  const uint16_t* x;
+  uint16_t* out;
+  int rows, K, N, ranks;
+};
+
+__device__ __forceinline__ float load_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <typename T, int NG, bool ZEROS, int MT>
+__global__ void __launch_bounds__(kQ4Warps * 32, MT <= 2 ? 3 : 2) q4_rows_kernel(const Q4Args a) {
+  constexpr int TOKENS = 8 * MT;
+  extern __shared__ __align__(128) uint8_t rings[];
+  __shared__ float parts[kQ4Warps][TOKENS][kQ4Rows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = a.ranks > 1 ? static_cast<int>(blockIdx.x) % a.ranks : 0;
+  const int64_t tile = blockIdx.x / a.ranks;
+  const int row0 = blockIdx.y * TOKENS;
+  const uint16_t* x[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int row = row0 + 8 * m + (lane >> 2);
+    x[m] = row < a.rows ? a.x + static_cast<int64_t>(row) * a.K : nullptr;
+  }
+  float acc[MT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.0f;
+  q4_tile<T, NG, ZEROS, MT, kQ4Depth>(acc, a.w, tile, x, a.K, rank * kQ4Warps + warp, a.ranks * kQ4Warps,
+                                          smem_u32(rings) + warp * kQ4Ring<NG, ZEROS>, lane);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) parts[warp][8 * m + 2 * (lane & 3) + (c & 1)][(lane >> 2) + 8 * (c >> 1)] = acc[m][c];
+  __syncthreads();
+  constexpr int PER = TOKENS * kQ4Rows / (kQ4Warps * 32) > 0 ? TOKENS * kQ4Rows / (kQ4Warps * 32) : 1;
+  float sum[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = threadIdx.x + i * kQ4Warps * 32;
+    sum[i] = 0.0f;
+    if (at < TOKENS * kQ4Rows)
+      for (int v = 0; v < kQ4Warps; ++v) sum[i] += (&parts[v][0][0])[at];
+  }
+  if (a.ranks > 1) {  // the same for the whole grid
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (threadIdx.x + i * kQ4Warps * 32 < TOKENS * kQ4Rows) (&parts[0][0][0])[threadIdx.x + i * kQ4Warps * 32] = sum[i];
+    cluster_sync_all();
+    if (rank == 0) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int at = threadIdx.x + i * kQ4Warps * 32;
+        if (at < TOKENS * kQ4Rows)
+          for (int r = 1; r < a.ranks; ++r) sum[i] += load_cluster(mapa_shared(smem_u32(&(&parts[0][0][0])[at]), r));
+      }
+    }
+    cluster_sync_all();  // the others' shared memory lives until it has been read
+    if (rank != 0) return;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = threadIdx.x + i * kQ4Warps * 32;
+    const int row = row0 + at / kQ4Rows, n = static_cast<int>(tile) * kQ4Rows + at % kQ4Rows;
+    if (at < TOKENS * kQ4Rows && row < a.rows && n < a.N) {
+      const T v = Elem<T>::from_float(sum[i]);
+      a.out[static_cast<int64_t>(row) * a.N + n] = *reinterpret_cast<const uint16_t*>(&v);
+    }
+  }
+}
+
+template <typename T, int NG, bool ZEROS, int MT> static int launch_q4(const Q4Args& a, cudaStream_t s) {
+  const auto kernel = q4_rows_kernel<T, NG, ZEROS, MT>;
+  constexpr int smem = kQ4Warps * kQ4Ring<NG, ZEROS>;
+  static std::atomic<bool> prepared[64];
+  int dev = 0;
+  MOE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !prepared[dev].load(std::memory_order_acquire)) {
+    MOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev < 64) prepared[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.w.tiles * a.ranks), static_cast<unsigned>((a.rows + 8 * MT - 1) / (8 * MT)), 1);
+  cfg.blockDim = dim3(kQ4Warps * 32, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(a.ranks);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.ranks > 1 ? 1 : 0;
+  MOE_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+  return MOE_OK;
+}
+template <typename T, int NG, bool ZEROS> static int launch_q4_rows(const Q4Args& a, cudaStream_t s) {
+  if (a.rows <= 8) return launch_q4<T, NG, ZEROS, 1>(a, s);
+  if (a.rows <= 16) return launch_q4<T, NG, ZEROS, 2>(a, s);
+  return launch_q4<T, NG, ZEROS, 4>(a, s);
+}
+template <typename T> static int launch_q4_groups(const Q4Args& a, int group, cudaStream_t s) {
+  const bool z = a.w.zeros != nullptr;
+  if (group == 128) return z ? launch_q4_rows<T, 1, true>(a, s) : launch_q4_rows<T, 1, false>(a, s);
+  if (group == 64) return z ? launch_q4_rows<T, 2, true>(a, s) : launch_q4_rows<T, 2, false>(a, s);
+  return z ? launch_q4_rows<T, 4, true>(a, s) : launch_q4_rows<T, 4, false>(a, s);
+}
+
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" int moe_int4_matmul(const void* x, const void* data, const void* scales, const void* zeros, void* out, int64_t rows, int k_dim, int n_dim,
+                               int group, int dtype, void* stream) {
+  MOE_CHECK_ARG(rows >= 0 && rows <= (1 << 20) && k_dim > 0 && n_dim > 0, "moe_int4_matmul: %lld rows (at most 2^20), K=%d, N=%d",
+                static_cast<long long>(rows), k_dim, n_dim);
+  MOE_CHECK_ARG(group == 32 || group == 64 || group == 128, "moe_int4_matmul: groups of 32, 64 or 128 columns, got %d", group);
+  MOE_CHECK_ARG(dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16, "moe_int4_matmul: unknown dtype %d", dtype);
+  if (k_dim % 8 != 0 || n_dim % 8 != 0 || k_dim > (1 << 27) || n_dim > (1 << 27)) {
+    set_error("moe_int4_matmul: K=%d and N=%d must be multiples of 8 up to 2^27", k_dim, n_dim);
+    return MOE_ERR_UNSUPPORTED;
+  }
+  if (rows == 0) return MOE_OK;
+  MOE_CHECK_ARG(x && data && scales && out, "moe_int4_matmul: null pointer argument");
+  MOE_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales) |
+                  reinterpret_cast<uintptr_t>(zeros)) & 15) == 0,
+                "moe_int4_matmul: pointers must be 16-byte aligned");
+  Q4Args a{};
+  a.w.data = static_cast<const uint4*>(data);
+  a.w.scales = scales;
+  a.w.zeros = static_cast<const uint8_t*>(zeros);
+  a.w.tiles = (n_dim + kQ4Rows - 1) / kQ4Rows;
+  a.w.steps = (k_dim + kQ4Step - 1) / kQ4Step;
+  a.x = static_cast<const uint16_t*>(x);
+  a.out = static_cast<uint16_t*>(out);
+  a.rows = static_cast<int>(rows);
+  a.K = k_dim;
+  a.N = n_dim;
+  // CTAs share a tile's steps while SMs would stay idle and each of their warps has two steps
+  const int64_t row_blocks = rows <= 16 ? 1 : (rows + 31) / 32;
+  a.ranks = 1;
+  while (a.ranks < 8 && a.w.tiles * row_blocks * a.ranks < 2ll * sm_count() && a.w.steps >= 4 * kQ4Warps * a.ranks) a.ranks *= 2;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == MOE_DTYPE_BF16 ? launch_q4_groups<__nv_bfloat16>(a, group, s) : launch_q4_groups<__half>(a, group, s);
+}

@@ -123,6 +123,7 @@ SIGNATURES = {
     "moe_expert_backward": (c_int, [POINTER(ExpertPass), c_int, c_void_p]),
     "moe_act_f8_forward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
     "moe_act_f8_backward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
+    "moe_int4_matmul": (c_int, [c_void_p] * 5 + [c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "moe_f8_quantize_rows": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p]),
     "moe_f8_pass_size": (c_size_t, []),
     "moe_f8_expert_forward": (c_int, [POINTER(F8Pass), c_int, c_void_p]),
@@ -523,6 +524,15 @@ def act_f8_backward(q, scales, dh, dz, act):
         rc = load().moe_act_f8_backward(q.data_ptr(), scales.data_ptr(), dh.data_ptr(), dz.data_ptr(), dh.size(0), dh.size(1),
                                         ACT_CODES[act], dtype_code(dh.dtype), _stream())
     _check("moe_act_f8_backward", rc)
+    _count(1)
+
+
+def int4_matmul(x, weight, out):
+    """out [R, N] = x [R, K] @ weight^T for an ``Int4Weight`` (see moe_int4_matmul)."""
+    with timed("int4:rows"):
+        rc = load().moe_int4_matmul(x.data_ptr(), weight.data.data_ptr(), weight.scales.data_ptr(), _ptr(weight.zeros), out.data_ptr(),
+                                    x.size(0), weight.k, weight.n, weight.group, dtype_code(x.dtype), _stream())
+    _check("moe_int4_matmul", rc)
     _count(1)
 
 

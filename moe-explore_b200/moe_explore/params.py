@@ -14,6 +14,7 @@ import torch
 
 from moe_explore.functional.activation import Activation
 from moe_explore.functional.fp8 import Fp8Weight
+from moe_explore.functional.int4 import Int4Weight
 
 
 @dataclass
@@ -63,6 +64,16 @@ class Fp8ExpertParams(FFNParams):
     (gate, up) for swiglu / geglu, else [E, 1, I, d]; ``down`` [E, d, I].  No reference counterpart."""
     up: Fp8Weight
     down: Fp8Weight
+    activation: Activation
+
+
+@dataclass
+class Int4ExpertParams(FFNParams):
+    """Experts in 4 bits, for serving (``moe_explore.functional.int4.pack_experts_int4`` and ``quantize_experts_int4`` make them): ``up``
+    [E, 2I, d] with eight rows of the gate and eight of the up matrix in turn for swiglu / geglu, else [E, I, d]; ``down`` [E, d, I].
+    No reference counterpart."""
+    up: Int4Weight
+    down: Int4Weight
     activation: Activation
 
 
