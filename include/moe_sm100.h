@@ -655,6 +655,40 @@ int moe_act_f8_backward(const void* q, const float* scales, const void* dh, void
 int moe_int4_matmul(const void* x, const void* data, const void* scales, const void* zeros, void* out, int64_t rows, int k_dim, int n_dim,
                     int group, int dtype, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * A whole layer for a few tokens (at most 16; 512 slots, 1024 experts) in two kernels, forward only.  No counterpart in the reference.
+ *   h = round(x + residual), y = round(h / sqrt(mean h^2 + eps) * norm_w)  (norm_w NULL: y = x);  stream_out receives h
+ *   logits = y router_w in fp32 (of y before its rounding);  scores and experts as in moe_router_tail / moe_grouped_topk with equal values
+ *   by ascending index, or, with router_w NULL, as given (expert_idx, scores [num_tokens, topk])
+ *   out = sum over the slots of score * (round(act(y w1[e])) w2[e]) + addend, summed in fp32, rounded once
+ * bits 16: w1 [num_experts, d, 2 inter] (gated: gate and up columns in turn) or [num_experts, d, inter], w2 [num_experts, inter, d].
+ * bits 4: the layout of moe_int4_matmul, a matrix per expert: w1 [2 inter, d] (gated: eight rows of the gate, eight of the up matrix in
+ * turn) or [inter, d], w2 [d, inter].  d and inter multiples of 8.  score_function: 0 softmax, 1 sigmoid, 2 softmax over the selected
+ * logits; normalize: 0 no, 1 by the sum, 2 by the sum or 1e-12.  Slots with an expert out of range add nothing (status).  The second
+ * kernel's CTAs wait for one another, a bounded time (status); it is launched cooperatively, one wave.  workspace: this call's own until
+ * its kernels are done, moe_few_workspace_bytes large.  Two kernels (without norm and router a memset and one).
+ * --------------------------------------------------------------------------------- */
+typedef struct moe_few_pass {
+  int32_t num_tokens, d, inter, num_experts, topk, act, dtype, bits, group;
+  int32_t norm_dtype, router_dtype; /* 2: fp32, else `dtype` */
+  int32_t score_function, normalize, num_groups, topk_groups, group_best;
+  float scale, eps;
+  const void *x, *residual, *norm_w, *router_w;
+  const float* router_bias;
+  const int64_t* expert_idx;
+  const void* scores;
+  const void *w1, *w1_scales, *w1_zeros, *w2, *w2_scales, *w2_zeros;
+  const void* addend;
+  void *out, *stream_out;
+  int32_t* status;
+  void* workspace;
+  size_t workspace_bytes;
+} moe_few_pass;
+
+size_t moe_few_pass_size(void);
+size_t moe_few_workspace_bytes(int num_tokens, int d, int inter, int num_experts, int topk);
+int moe_few_tokens(const moe_few_pass* pass, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

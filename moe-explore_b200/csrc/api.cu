@@ -88,7 +88,7 @@ extern "C" int moe_check_status(const int32_t* status, void* stream) {
               "with unsynchronised scheduling and its results are valid");
     return MOE_ERR_TIMEOUT;
   }
-  set_error("a device-side bounded wait ran out (code %d: 1 = TMA producer, 2 = MMA issuer, 3 = epilogue); the outputs "
+  set_error("a device-side bounded wait ran out (code %d: 1 = TMA producer, 2 = MMA issuer, 3 = epilogue, 6 = CTAs of a layer for a few tokens); the outputs "
             "of that launch are incomplete", host);
   return MOE_ERR_TIMEOUT;
 }

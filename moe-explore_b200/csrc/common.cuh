@@ -172,6 +172,7 @@ enum DeviceStatus : int {
   DS_WAVE_FALLBACK = 4,     // the wave barrier of the persistent workers ran out; the launch finished with the static
                             // stride instead (its results are valid)
   DS_BAD_LAYOUT = 5,        // the routing metadata handed to a kernel was built for another padded row count
+  DS_TIMEOUT_GRID = 6,      // a CTA of a layer for a few tokens gave up waiting for the others
   DS_BAD_EXPERT_ID = 100,   // routing metadata saw an expert id outside [0, num_experts); the row was dropped
 };
 

@@ -80,6 +80,16 @@ class F8RowsPass(ctypes.Structure):
                                         "tile_pairs", "num_mtiles", "status", "gathered", "gathered_scales")]
 
 
+class FewPass(ctypes.Structure):
+    """``moe_few_pass``: a whole layer for a few tokens."""
+    _fields_ = [(f, c_int32) for f in ("num_tokens", "d", "inter", "num_experts", "topk", "act", "dtype", "bits", "group", "norm_dtype",
+                                       "router_dtype", "score_function", "normalize", "num_groups", "topk_groups", "group_best")] + \
+               [("scale", c_float), ("eps", c_float)] + \
+               [(f, c_void_p) for f in ("x", "residual", "norm_w", "router_w", "router_bias", "expert_idx", "scores", "w1", "w1_scales",
+                                        "w1_zeros", "w2", "w2_scales", "w2_zeros", "addend", "out", "stream_out", "status", "workspace")] + \
+               [("workspace_bytes", c_size_t)]
+
+
 # name -> (restype, argtypes); the single source for both binding and the symbol-export test
 _OPT = POINTER(GemmOptions)
 SIGNATURES = {
@@ -124,6 +134,9 @@ SIGNATURES = {
     "moe_act_f8_forward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
     "moe_act_f8_backward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
     "moe_int4_matmul": (c_int, [c_void_p] * 5 + [c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "moe_few_pass_size": (c_size_t, []),
+    "moe_few_workspace_bytes": (c_size_t, [c_int] * 5),
+    "moe_few_tokens": (c_int, [POINTER(FewPass), c_void_p]),
     "moe_f8_quantize_rows": (c_int, [c_void_p] * 3 + [c_int64, c_int, c_int, c_void_p]),
     "moe_f8_pass_size": (c_size_t, []),
     "moe_f8_expert_forward": (c_int, [POINTER(F8Pass), c_int, c_void_p]),
@@ -211,6 +224,8 @@ def load() -> ctypes.CDLL:
             raise ImportError(f"{LIB_PATH} was built with another layout of moe_rows_pass: rebuild it")
         if lib.moe_f8_pass_size() != ctypes.sizeof(F8Pass) or lib.moe_f8_rows_pass_size() != ctypes.sizeof(F8RowsPass):
             raise ImportError(f"{LIB_PATH} was built with another layout of moe_f8_pass or moe_f8_rows_pass: rebuild it")
+        if lib.moe_few_pass_size() != ctypes.sizeof(FewPass):
+            raise ImportError(f"{LIB_PATH} was built with another layout of moe_few_pass: rebuild it")
         _lib = lib
     return _lib
 
@@ -534,6 +549,22 @@ def int4_matmul(x, weight, out):
                                     x.size(0), weight.k, weight.n, weight.group, dtype_code(x.dtype), _stream())
     _check("moe_int4_matmul", rc)
     _count(1)
+
+
+FEW_TOKENS, FEW_SLOTS, FEW_EXPERTS, FEW_GROUPS, FEW_COLUMNS = 16, 512, 1024, 64, 1 << 20   # what moe_few_tokens takes
+
+
+@functools.lru_cache(maxsize=256)
+def few_workspace_bytes(num_tokens: int, d: int, inter: int, num_experts: int, topk: int) -> int:
+    return int(load().moe_few_workspace_bytes(num_tokens, d, inter, num_experts, topk))
+
+
+def few_tokens(p) -> None:
+    """The two kernels of a ``FewPass`` on the current stream."""
+    with timed("few:layer"):
+        rc = load().moe_few_tokens(ctypes.byref(p), _stream())
+    _check("moe_few_tokens", rc)
+    _count(2 if p.router_w or p.norm_w else 1)
 
 
 _PINNED = {}

@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from moe_explore import _native
-from moe_explore.functional.activation import Activation, is_glu
+from moe_explore.functional.activation import is_glu
 from moe_explore.functional.fp8 import _dense
 
 TILE = 16      # rows
@@ -138,6 +138,9 @@ def pack_experts_int4(up, down, activation, *, group: int = 128):
     activations, else [E, 1, I, d]; ``down`` [E, d, I]."""
     from moe_explore.params import Int4ExpertParams
 
+    activation = None if activation is None else str(activation)
+    if activation not in _native.ACT_CODES:
+        raise ValueError(f"Unsupported activation: {activation!r}")
     gates = 2 if is_glu(activation) else 1
     if up[0].dim() != 4 or up[0].size(1) != gates or down[0].dim() != 3 or up[0].size(2) % 8 != 0:
         raise ValueError(f"up is [E, {gates}, I, d] and down [E, d, I] for {activation!r} with I a multiple of 8, got {tuple(up[0].shape)}, "
@@ -148,7 +151,8 @@ def pack_experts_int4(up, down, activation, *, group: int = 128):
             return None
         e, _, inter, cols = t.shape
         return t.view(e, gates, inter // 8, 8, cols).transpose(1, 2).reshape(e, gates * inter, cols)
-    return Int4ExpertParams(pack_int4(*(rows(t) for t in up), group=group), pack_int4(*down, group=group), Activation(activation))
+    return Int4ExpertParams(pack_int4(*(rows(t) for t in up), group=group), pack_int4(*down, group=group),
+                            activation)
 
 
 def quantize_experts_int4(params, group: int = 128, zeros: bool = False):

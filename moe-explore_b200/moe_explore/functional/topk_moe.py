@@ -12,10 +12,11 @@ import torch
 
 from moe_explore.expert_compute import (dense_expert, fp8_expert_compute, inference_pass, routed_expert_compute, routed_layer,
                                         router_and_experts_at_once, router_joins_the_pass)
+from moe_explore.few_tokens import few_token_layer, int4_expert_compute
 from moe_explore.functional.activation import activation
 from moe_explore.functional.fp8 import Fp8Rows
 from moe_explore.functional.rms_norm import rms_norm, rms_norm_fp8
-from moe_explore.params import Fp8ExpertParams, MLPParams, MOEParams, TopkRouterParams
+from moe_explore.params import Fp8ExpertParams, Int4ExpertParams, MLPParams, MOEParams, TopkRouterParams
 from moe_explore.router import fused_topk_router, router
 
 
@@ -42,7 +43,8 @@ def _shared_expert(input: torch.Tensor, shared) -> torch.Tensor:
 
 
 def topk_moe_forward(input: torch.Tensor, params: MOEParams, autotune_mode=None, *, fused_router: bool = False,
-                     gather_in_gemm=None, fused_combine: bool = False, residual: torch.Tensor = None, save_fp8: bool = False):
+                     gather_in_gemm=None, fused_combine: bool = False, residual: torch.Tensor = None, save_fp8: bool = False,
+                     few_tokens: bool = False):
     """The layer (functional/topk_moe.py:10-64).  ``autotune_mode`` is accepted and ignored.  Keyword-only additions:
     ``fused_router`` runs the router tail in one kernel with its own declared tie rule (see
     ``moe_explore.router.fused_topk_router``); ``gather_in_gemm`` / ``fused_combine`` as in ``expert_compute``; ``save_fp8`` as in
@@ -51,12 +53,21 @@ def topk_moe_forward(input: torch.Tensor, params: MOEParams, autotune_mode=None,
     With ``params.norm_params`` the layer begins with its norm: router, experts and shared expert see ``rms_norm(input)``, or, with
     ``residual``, ``rms_norm(input + residual)``, and the result is the pair (layer's output, ``input + residual``) that the next
     layer's norm takes.  Experts in 8 bits (``Fp8ExpertParams``) serve without gradients: the norm then gives their rows in 8 bits at
-    once, and the router reads its 16-bit result."""
+    once, and the router reads its 16-bit result.
+
+    ``few_tokens``: where there are at most 16 tokens and no gradient is wanted, the layer runs in two kernels (see
+    ``moe_explore.few_tokens.few_token_layer``, also for what it does not take and leaves to the ordinary pass; a shared expert is a pass
+    of its own, as ever).  Its logits are fp32 sums that are not rounded to 16 bits, so that tokens whose logits nearly agree may go to
+    other experts than in the ordinary pass.  Experts in 4 bits (``Int4ExpertParams``) serve without gradients, with or without it."""
     norm = getattr(params, "norm_params", None)
     if norm is None:
         if residual is not None:
             raise ValueError("residual is added by the layer's norm: params.norm_params is None")
-        return _layer(input, None, params, fused_router, gather_in_gemm, fused_combine, save_fp8)
+        return _layer(input, None, params, fused_router, gather_in_gemm, fused_combine, save_fp8, few_tokens)
+    if few_tokens and getattr(params, "shared_expert_params", None) is None:
+        done = few_token_layer(input, params, residual, None, norm)
+        if done is not None:
+            return done
     rows = stream = None
     if isinstance(params.expert_params, Fp8ExpertParams):
         rows, normed, *rest = rms_norm_fp8(input, norm.weight, norm.eps, residual, with_rows=True)
@@ -65,21 +76,30 @@ def topk_moe_forward(input: torch.Tensor, params: MOEParams, autotune_mode=None,
         normed = rms_norm(input, norm.weight, norm.eps)
     else:
         normed, stream = rms_norm(input, norm.weight, norm.eps, residual)
-    out = _layer(normed, rows, params, fused_router, gather_in_gemm, fused_combine, save_fp8)
+    out = _layer(normed, rows, params, fused_router, gather_in_gemm, fused_combine, save_fp8, few_tokens)
     return out if residual is None else (out, stream)
 
 
 def _layer(input: torch.Tensor, rows: Fp8Rows, params: MOEParams, fused_router: bool, gather_in_gemm, fused_combine: bool,
-           save_fp8: bool) -> torch.Tensor:
+           save_fp8: bool, few_tokens: bool) -> torch.Tensor:
     """Router, experts and shared expert; ``rows``: the input in 8 bits where it is there already."""
     ep: MLPParams = params.expert_params
     shared = getattr(params, "shared_expert_params", None)
     shared_out = None if shared is None else _shared_expert(input, shared)
-    # a [T, d] shared branch is added by the fold of the routed experts; the fused fold has no such place (experts in 8 bits have
-    # no fused fold), and 2-D shared weights give a broadcast vector
-    in_fold = not fused_combine or isinstance(ep, Fp8ExpertParams)
+    # a [T, d] shared branch is added by the fold of the routed experts; the fused fold has no such place (experts in 8 or 4 bits
+    # have no fused fold), and 2-D shared weights give a broadcast vector
+    in_fold = not fused_combine or isinstance(ep, (Fp8ExpertParams, Int4ExpertParams))
     addend = shared_out if shared_out is not None and shared.up_weight.dim() == 3 and in_fold else None
-    if isinstance(ep, Fp8ExpertParams):
+    out = few_token_layer(input, params, None, addend) if few_tokens else None
+    if out is not None:
+        pass
+    elif isinstance(ep, Int4ExpertParams):
+        if fused_router and isinstance(params.router_params, TopkRouterParams):
+            scores, indices = fused_topk_router(input, params.router_params)
+        else:
+            scores, indices = router(input, params.router_params)
+        out = int4_expert_compute(input, scores, indices, ep, addend=addend)
+    elif isinstance(ep, Fp8ExpertParams):
         if fused_router and isinstance(params.router_params, TopkRouterParams):
             scores, indices = fused_topk_router(input, params.router_params)
         else:

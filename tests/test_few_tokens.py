@@ -1,0 +1,404 @@
+"""The layer for a few tokens in two kernels, and experts in 4 bits, against the formulas in 64 bits; refusals and what is left to the
+ordinary pass."""
+import math
+
+import pytest
+import torch
+
+from moe_explore.few_tokens import few_token_layer, int4_expert_compute
+from moe_explore.functional.int4 import pack_experts_int4, quantize_experts_int4
+from moe_explore.functional.topk_moe import topk_moe_forward
+from moe_explore.params import (ErnieRouterParams, GroupedTopkRouterParams, Int4ExpertParams, MLPParams, MOEParams, RMSNormParams,
+                                SharedExpertParams, TopkRouterParams)
+from moe_explore.routing_plan import device_status
+from test_activation_fp8 import act64, gated
+from test_int4 import raw, weight64
+
+gpu = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def make_router(g, kind, d, E, k, dtype):
+    w = 1.5 * d ** -0.5 * torch.randn(d, E, generator=g, device="cuda")
+    bias = 0.1 * torch.randn(E, generator=g, device="cuda")
+    if kind == "ernie":
+        return ErnieRouterParams(w, bias, k)
+    if kind.startswith("groups"):
+        return GroupedTopkRouterParams(w if "fp32" in kind else w.to(dtype), k, bias=None if "plain" in kind else bias, num_groups=4, topk_groups=3,
+                                       group_best=1 if "one" in kind else 2, score_function="softmax" if "softmax" in kind else "sigmoid",
+                                       normalize_routing="raw" not in kind, scale=2.5)
+    return TopkRouterParams(w.to(dtype), k, "after" not in kind, "norm" in kind)
+
+
+def route64(rp, logits):
+    """(weights, experts), best first, equal values by ascending index."""
+    def best(v, n):
+        return torch.sort(v, dim=-1, descending=True, stable=True).indices[:, :n]
+    E, k = logits.size(1), rp.topk
+    if isinstance(rp, TopkRouterParams):
+        i = best(logits, k)
+        if not rp.softmax_before_topk:
+            return torch.softmax(logits.gather(1, i), -1), i
+        w = torch.softmax(logits, -1).gather(1, i)
+        return w / w.sum(-1, keepdim=True) if rp.normalize_routing else w, i
+    if isinstance(rp, ErnieRouterParams):
+        p = torch.softmax(logits, -1)
+        i = best(p + rp.bias, k)
+        w = p.gather(1, i)
+        return w / w.sum(-1, keepdim=True).clamp_min(1e-12), i
+    p = torch.sigmoid(logits) if rp.score_function == "sigmoid" else torch.softmax(logits, -1)
+    key = p if rp.bias is None else p + rp.bias
+    value = key.view(-1, rp.num_groups, E // rp.num_groups).topk(min(rp.group_best, E // rp.num_groups)).values.sum(-1)
+    open_ = torch.zeros_like(value, dtype=torch.bool).scatter_(1, best(value, rp.topk_groups), True).repeat_interleave(E // rp.num_groups, 1)
+    i = best(torch.where(open_, key, -math.inf), k)
+    w = p.gather(1, i)
+    return (w / w.sum(-1, keepdim=True) if rp.normalize_routing else w) * rp.scale, i
+
+
+def experts64(x, weights, indices, w1, w2, act):
+    """x [T, d], matrices [E, d, N] and [E, I, d] in 64 bits, gate and up columns in turn."""
+    out = torch.zeros_like(x)
+    for e in indices.unique().tolist():
+        token, slot = (indices == e).nonzero(as_tuple=True)
+        out.index_add_(0, token, weights[token, slot, None] * (act64(x[token] @ w1[e], act) @ w2[e]))
+    return out
+
+
+def make_experts(g, bits, E, d, inter, act, dtype, group=128, zeros=False):
+    """(parameters, w1 and w2 in 64 bits as ``experts64`` takes them)"""
+    gates = 2 if gated(act) else 1
+    if bits == 16:
+        w1 = (torch.randn(E, d, gates * inter, generator=g, device="cuda") * d ** -0.5).to(dtype)
+        w2 = (torch.randn(E, inter, d, generator=g, device="cuda") * inter ** -0.5).to(dtype)
+        return MLPParams(w1, w2, act), w1.double(), w2.double()
+    up, down = raw(g, E, gates, inter, d, group=group, zeros=zeros, dtype=dtype), raw(g, E, d, inter, group=group, zeros=zeros, dtype=dtype)
+    w1 = weight64(*up, group).permute(0, 3, 2, 1).reshape(E, d, inter * gates)
+    return pack_experts_int4(up, down, act, group=group), w1, weight64(*down, group).mT
+
+
+def near(got, want, dtype, roundings):
+    """At the root of the mean square each rounding to 16 bits is off by eps / 2 / sqrt(3) at most, of the activated product, the result, and
+    of the normed rows, which the gate and the up matrix both read; the factor sqrt(3) is left for the activation's slope and fp32 sums."""
+    assert got.dtype is dtype and got.shape == want.shape
+    return float((got.double() - want).norm()) <= roundings * torch.finfo(dtype).eps / 2 * float(want.norm()) + 1e-30
+
+
+CASES = [
+    # T, d, E, k, I, act, dtype, bits, group, zeros, router, norm
+    (1, 64, 4, 1, 8, "swiglu", torch.bfloat16, 16, 128, False, "topk", False),
+    (1, 2048, 60, 4, 1408, "swiglu", torch.bfloat16, 16, 128, False, "topk", True),
+    (16, 512, 64, 8, 264, "swiglu", torch.bfloat16, 16, 128, False, "topk norm", False),
+    (7, 776, 12, 3, 1544, "geglu", torch.float16, 16, 128, False, "topk after", True),
+    (16, 136, 2, 2, 200, "gelu", torch.bfloat16, 16, 128, False, "topk after", False),
+    (5, 264, 7, 2, 40, "silu", torch.float16, 16, 128, False, "ernie", True),
+    (3, 8, 8, 8, 8, "approx_gelu", torch.bfloat16, 16, 128, False, "topk", False),
+    (11, 256, 32, 4, 96, None, torch.bfloat16, 16, 128, False, "groups fp32", False),
+    (1, 1024, 8, 2, 4096, "swiglu", torch.bfloat16, 4, 128, False, "topk after", True),
+    (7, 776, 12, 3, 1544, "geglu", torch.float16, 4, 32, True, "topk", False),
+    (16, 520, 64, 8, 136, "swiglu", torch.bfloat16, 4, 64, False, "groups fp32", True),
+    (13, 384, 16, 4, 264, "silu", torch.bfloat16, 4, 64, True, "groups softmax one", False),
+    (2, 72, 3, 2, 24, "gelu", torch.float16, 4, 32, False, "ernie", False),
+    (16, 256, 2, 1, 512, "swiglu", torch.float16, 4, 128, True, "topk", True),
+    (9, 2048, 128, 8, 256, "swiglu", torch.bfloat16, 4, 128, False, "groups plain raw", True),
+    (4, 128, 512, 16, 64, "swiglu", torch.bfloat16, 16, 128, False, "groups fp32 raw", True),
+]
+
+
+@gpu
+@pytest.mark.parametrize("T,d,E,k,inter,act,dtype,bits,group,zeros,kind,normed", CASES)
+def test_layer(T, d, E, k, inter, act, dtype, bits, group, zeros, kind, normed, native):
+    g = gen(T * d + E)
+    rp = make_router(g, kind, d, E, k, dtype)
+    experts, w1, w2 = make_experts(g, bits, E, d, inter, act, dtype, group, zeros)
+    norm = RMSNormParams((1 + 0.1 * torch.randn(d, generator=g, device="cuda")).to(dtype if T % 2 else torch.float32), 1e-5) if normed else None
+    p = MOEParams(rp, experts, E, k, None, norm)
+    x = torch.randn(T, d, generator=g, device="cuda").to(dtype)
+    for residual in (None, torch.randn(T, d, generator=g, device="cuda").to(dtype)) if normed else (None,):
+        h = x if residual is None else x + residual
+        y = h.double()
+        if normed:
+            y = y / (y.square().mean(-1, keepdim=True) + 1e-5).sqrt() * norm.weight.double()
+        want = experts64(y, *route64(rp, y @ rp.router_weight.double()), w1, w2, act)
+        with torch.no_grad():
+            assert few_token_layer(x, p, residual, None, norm) is not None, "the kernels serve this"
+            out = topk_moe_forward(x, p, residual=residual, few_tokens=True)
+        if residual is not None:
+            out, stream = out
+            assert torch.equal(stream, h)
+        assert near(out, want, dtype, 4 if normed else 2)
+    native.check_status(device_status(0))
+
+
+@gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_whole_numbers_are_exact(bits, native):
+    """Sums of small whole numbers without an activation: every step is exact in whatever order and share, so every index is right."""
+    g = gen(4)
+    for T, d, E, k, inter in ((1, 264, 4, 2, 200), (16, 136, 5, 5, 72), (6, 520, 3, 2, 1032)):
+        ints = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g, device="cuda")
+        sparse = lambda t, share: t * (torch.rand(t.shape, generator=g, device="cuda") < share)
+        w1, w2 = sparse(ints(-1, 2, E, d, inter), 0.05), sparse(ints(-1, 2, E, inter, d), 0.05)
+        if bits == 16:
+            experts = MLPParams(w1.half(), w2.half(), None)
+        else:
+            def four(w):   # [E, K, N] -> values + 8 of [E, N, K]
+                v = (w.mT + 8).to(torch.uint8)
+                return v[..., 0::2] | (v[..., 1::2] << 4), torch.ones(E, w.size(2), -(-w.size(1) // 32), device="cuda").half(), None
+            up = four(w1)
+            experts = pack_experts_int4(tuple(None if t is None else t[:, None] for t in up), four(w2), None, group=32)
+        x = ints(-2, 3, T, d).half()
+        indices = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(t))[:k] for t in range(T)]).cuda()
+        scores = torch.ones(T, k, device="cuda").half()
+        want = experts64(x.double(), scores.double(), indices, w1.double(), w2.double(), None)
+        assert float(want.abs().max()) < 2048
+        if bits == 4:
+            assert bool((int4_expert_compute(x, scores, indices, experts).double() == want).all())
+        # the same choice by the layer's own router: a logit of 1 + slot for the chosen experts (one more column of x), weights a half or one
+        wide = torch.zeros(T, d + 8, device="cuda").half()
+        wide[:, :d] = x
+        if T == 1:   # one token can be given any logits
+            wide[0, d] = 1
+            rw = torch.zeros(d + 8, E, device="cuda").half()
+            rw[d, indices[0]] = 20.0
+            w1w = torch.zeros(E, d + 8, inter, device="cuda")
+            w1w[:, :d] = w1
+            w2w = torch.zeros(E, inter, d + 8, device="cuda")
+            w2w[:, :, :d] = w2
+            if bits == 16:
+                p = MOEParams(TopkRouterParams(rw, k, False), MLPParams(w1w.half(), w2w.half(), None), E, k)
+                with torch.no_grad():
+                    got = topk_moe_forward(wide, p, few_tokens=True)
+                assert bool((got[:, :d].double() * k == want).all())
+
+
+@gpu
+def test_same_bits_in_any_company(native):
+    """A token's result does not depend on the other tokens of the call as long as the work is shared out alike, nor on the call."""
+    g = gen(8)
+    experts, _, _ = make_experts(g, 4, 8, 256, 128, "swiglu", torch.bfloat16)
+    x = torch.randn(16, 256, generator=g, device="cuda").bfloat16()
+    indices = torch.arange(2, device="cuda").repeat(16, 1)
+    scores = torch.full((16, 2), 0.5, device="cuda").bfloat16()
+    whole = int4_expert_compute(x, scores, indices, experts)
+    assert all(torch.equal(whole, int4_expert_compute(x, scores, indices, experts)) for _ in range(20))
+    assert torch.equal(int4_expert_compute(x[:5], scores[:5], indices[:5], experts), whole[:5])
+    many = int4_expert_compute(x.repeat(3, 1)[:41], scores.repeat(3, 1)[:41], indices.repeat(3, 1)[:41], experts)
+    assert torch.equal(many, whole.repeat(3, 1)[:41])
+    assert int4_expert_compute(x[:0], scores[:0], indices[:0], experts).shape == (0, 256)
+
+
+@gpu
+def test_equal_logits_duplicates_and_bad_experts(native):
+    g = gen(9)
+    d, E, inter = 128, 8, 64
+    w16, w1, w2 = make_experts(g, 16, E, d, inter, "swiglu", torch.bfloat16)
+    x = torch.randn(3, d, generator=g, device="cuda").bfloat16()
+    rw = torch.zeros(d, E, device="cuda").bfloat16()        # all logits are equal: the lowest experts
+    with torch.no_grad():
+        out = topk_moe_forward(x, MOEParams(TopkRouterParams(rw, 3, False), w16, E, 3), few_tokens=True)
+    want = experts64(x.double(), torch.full((3, 3), 1 / 3, device="cuda", dtype=torch.float64), torch.arange(3, device="cuda").repeat(3, 1), w1, w2, "swiglu")
+    assert near(out, want, torch.bfloat16, 2)
+    q, w1, w2 = make_experts(g, 4, E, d, inter, "swiglu", torch.bfloat16)
+    x = torch.randn(16, d, generator=g, device="cuda").bfloat16()
+    scores = torch.rand(16, 4, generator=g, device="cuda").bfloat16()
+    twice = torch.zeros(16, 4, dtype=torch.int64, device="cuda")    # one expert four times for each of 16 tokens
+    twice[3] = 5
+    want = torch.zeros(16, d, dtype=torch.float64, device="cuda")
+    for s in range(4):
+        want += experts64(x.double(), scores[:, s:s + 1].double(), twice[:, s:s + 1], w1, w2, "swiglu")
+    assert near(int4_expert_compute(x, scores, twice, q), want, torch.bfloat16, 2)
+    native.check_status(device_status(0))
+    bad = torch.randint(0, E, (16, 4), generator=g, device="cuda")
+    bad[2, 1], bad[7, 0], bad[9] = -1, E, 1 << 40
+    want = torch.zeros(16, d, dtype=torch.float64, device="cuda")
+    for s in range(4):
+        ok = (bad[:, s] >= 0) & (bad[:, s] < E)
+        want[ok] += experts64(x[ok].double(), scores[ok, s:s + 1].double(), bad[ok, s:s + 1], w1, w2, "swiglu")
+    out = int4_expert_compute(x, scores, bad, q)
+    assert near(out, want, torch.bfloat16, 2) and not out[9].any()
+    assert native.read_status(device_status(0), reset=True) == native.STATUS_BAD_EXPERT_ID
+
+
+@gpu
+def test_values_that_are_not_finite(native):
+    """A token that holds NaN or an infinity spoils its own row only."""
+    g = gen(10)
+    d, E, k = 256, 16, 4
+    experts, _, _ = make_experts(g, 16, E, d, 64, "swiglu", torch.bfloat16)
+    p = MOEParams(make_router(g, "topk", d, E, k, torch.bfloat16), experts, E, k)
+    x = torch.randn(6, d, generator=g, device="cuda").bfloat16()
+    with torch.no_grad():
+        clean = topk_moe_forward(x, p, few_tokens=True)
+        x[1, 3], x[4, 200] = math.nan, math.inf
+        out = topk_moe_forward(x, p, few_tokens=True)
+    assert torch.isnan(out[1]).all() and not torch.isfinite(out[4]).any()
+    rest = [0, 2, 3, 5]
+    assert float((out[rest].float() - clean[rest].float()).abs().max()) <= 2 * 2.0 ** -8 * float(clean.float().abs().max())
+
+
+@gpu
+def test_large_rows_get_their_norm(native):
+    """bf16 rows whose squares leave fp32."""
+    d = 512
+    experts, w1, w2 = make_experts(gen(1), 16, 4, d, 64, "swiglu", torch.bfloat16)
+    norm = RMSNormParams(torch.ones(d, device="cuda"), 1e-6)
+    p = MOEParams(make_router(gen(2), "topk after", d, 4, 2, torch.bfloat16), experts, 4, 2, None, norm)
+    x = torch.randn(2, d, generator=gen(3), device="cuda").bfloat16()
+    with torch.no_grad():
+        a, b = topk_moe_forward(x * 2.0 ** 100, p, few_tokens=True), topk_moe_forward(x * 2.0 ** 90, p, few_tokens=True)
+    assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_serving_with_a_shared_expert_in_a_graph_and_on_two_streams(bits, native):
+    """Layers that hand the stream on, captured together and replayed with other inputs while an eager call runs on another stream."""
+    g = gen(11)
+    d, E, k, inter = 256, 16, 4, 96
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    layers = []
+    for i in range(3):
+        experts, _, _ = make_experts(g, bits, E, d, inter, "swiglu", torch.bfloat16)
+        sp = SharedExpertParams((new(1, d, 2 * inter) * d ** -0.5).bfloat16(), (new(1, inter, d) * inter ** -0.5).bfloat16(), "swiglu") if i == 1 else None
+        layers.append(MOEParams(make_router(g, "groups fp32", d, E, k, torch.bfloat16), experts, E, k, sp, RMSNormParams((1 + 0.1 * new(d)).bfloat16())))
+
+    def model(x, residual):
+        for p in layers:
+            x, residual = topk_moe_forward(x, p, residual=residual, few_tokens=True)
+        return x, residual
+    with torch.no_grad():
+        x, residual = new(8, d).bfloat16(), new(8, d).bfloat16()
+        other = new(5, d).bfloat16(), new(5, d).bfloat16()
+        want = model(*other)
+        model(x, residual)
+        torch.cuda.synchronize()
+        graphs, outs = [], []
+        for _ in range(2):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                outs.append(model(x, residual))
+        x.copy_(new(8, d))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(20):
+            with torch.cuda.stream(side):
+                got = model(*other)
+            graphs[0].replay()
+            graphs[1].replay()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        eager = model(x, residual)
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, eager))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        # the shared expert's branch is in it
+        one = MOEParams(layers[1].router_params, layers[1].expert_params, E, k, layers[1].shared_expert_params)
+        bare = MOEParams(layers[1].router_params, layers[1].expert_params, E, k)
+        from moe_explore.expert_compute import dense_expert
+        both = topk_moe_forward(x, one, few_tokens=True).float()
+        sp = layers[1].shared_expert_params
+        apart = topk_moe_forward(x, bare, few_tokens=True).float() + dense_expert(x, sp.up_weight, sp.down_weight, "swiglu").float()
+        # three results rounded once each
+        assert bool(((both - apart).abs() <= 3 * 2.0 ** -8 * (both.abs() + dense_expert(x, sp.up_weight, sp.down_weight, "swiglu").float().abs()) + 1e-6).all())
+    native.check_status(device_status(0))
+
+
+@gpu
+def test_what_is_left_to_the_ordinary_pass(native):
+    g = gen(12)
+    d, E, k = 128, 8, 2
+    experts, _, _ = make_experts(g, 16, E, d, 64, "swiglu", torch.bfloat16)
+    p = MOEParams(make_router(g, "topk", d, E, k, torch.bfloat16), experts, E, k)
+    x = torch.randn(17, d, generator=g, device="cuda").bfloat16()
+    with torch.no_grad():
+        assert few_token_layer(x, p) is None
+        assert torch.equal(topk_moe_forward(x, p, few_tokens=True), topk_moe_forward(x, p))
+        assert few_token_layer(x[:16].float(), p) is None and few_token_layer(x[:0], p) is None
+        # rows that are neither dense nor aligned, weights that are not either
+        part = torch.randn(4, d + 5, generator=g, device="cuda").bfloat16()[:, 3:3 + d]
+        assert torch.equal(topk_moe_forward(part, p, few_tokens=True), topk_moe_forward(part.contiguous(), p, few_tokens=True))
+        turned = MOEParams(p.router_params, MLPParams(experts.weight1.mT.contiguous().mT, experts.weight2, "swiglu"), E, k)
+        assert few_token_layer(x[:4], turned) is None
+        assert torch.equal(topk_moe_forward(x[:4], turned, few_tokens=True), topk_moe_forward(x[:4], turned))
+    leaf = x[:4].clone().requires_grad_(True)
+    y = topk_moe_forward(leaf, p, few_tokens=True)
+    assert y.requires_grad and torch.equal(y, topk_moe_forward(leaf, p))
+    q = MOEParams(p.router_params, quantize_experts_int4(experts, 32), E, k)
+    with pytest.raises(RuntimeError, match="no backward"):
+        topk_moe_forward(leaf, q, few_tokens=True)
+    with torch.no_grad():   # 4 bits behind the ordinary router, more tokens than a pass takes
+        from moe_explore.router import router
+        out = topk_moe_forward(x, q)
+        scores, indices = router(x, p.router_params)
+        assert torch.equal(out, int4_expert_compute(x, scores, indices, q.expert_params))
+        assert float((out.float() - topk_moe_forward(x, p).float()).norm() / topk_moe_forward(x, p).float().norm()) < 0.3
+
+
+@gpu
+def test_a_wait_that_runs_out_is_reported(native):
+    """With a limit of one cycle some CTA gives up before the last one comes: the status word says so, and the next call is right."""
+    g = gen(13)
+    experts, _, _ = make_experts(g, 16, 8, 256, 512, "swiglu", torch.bfloat16)
+    p = MOEParams(make_router(g, "topk", 256, 8, 2, torch.bfloat16), experts, 8, 2)
+    x = torch.randn(4, 256, generator=g, device="cuda").bfloat16()
+    with torch.no_grad():
+        want = topk_moe_forward(x, p, few_tokens=True)
+        native.set_wait_limit_cycles(1)
+        try:
+            topk_moe_forward(x, p, few_tokens=True)
+        finally:
+            native.set_wait_limit_cycles(0)
+        with pytest.raises(native.MoeNativeError, match="bounded wait"):
+            native.check_status(device_status(0))
+        assert native.read_status(device_status(0), reset=True) == 6
+        assert torch.equal(topk_moe_forward(x, p, few_tokens=True), want)
+
+
+# ------------------------------------------------------------------------------------------------------- refusals
+def test_refusals_of_the_library(native):
+    import ctypes
+    lib = native.load()
+    assert native.few_workspace_bytes(16, 256, 128, 8, 2) >= 16 * 2 * 256 * 4 and lib.moe_few_workspace_bytes(-1, 8, 8, 8, 1) == 0
+    call = lambda p: (lib.moe_few_tokens(ctypes.byref(p), None), lib.moe_last_error())
+    def base(**kw):
+        p = native.FewPass(num_tokens=1, d=64, inter=64, num_experts=8, topk=2, act=3, dtype=0, bits=16, num_groups=1, topk_groups=1, group_best=1)
+        p.expert_idx = p.scores = 16
+        for name, v in kw.items():
+            setattr(p, name, v)
+        return p
+    assert lib.moe_few_tokens(None, None) == -1
+    for kw, rc, text in [(dict(num_tokens=17), -2, b"at most"), (dict(topk=0), -1, b"k=0"), (dict(num_experts=2000), -2, b"at most"), (dict(d=60), -2, b"multiples of 8"),
+                         (dict(dtype=5), -1, b"dtype"), (dict(act=9), -1, b"activation"), (dict(bits=4, group=16), -1, b"groups"), (dict(bits=8), -1, b"16 bits"),
+                         (dict(scores=None), -1, b"router, or"), (dict(router_w=16, num_groups=3), -1, b"groups"), (dict(router_w=16, router_dtype=7), -1, b"router options"),
+                         (dict(router_w=16, score_function=2, router_bias=16), -1, b"without bias"), (dict(), -1, b"null"),
+                         (dict(x=16, w1=16, w2=16, out=16, workspace=16), -1, b"workspace has"), (dict(x=8, w1=16, w2=16, out=16, workspace=16), -1, b"aligned"),
+                         (dict(x=16, w1=16, w2=16, out=16, workspace=16, bits=4, group=32), -1, b"have scales"),
+                         (dict(x=16, w1=16, w2=16, out=16, workspace=16, residual=16), -1, b"residual")]:
+        got = call(base(**kw))
+        assert got[0] == rc and text in got[1], (kw, got)
+    assert call(base(num_tokens=0))[0] == 0
+
+
+@gpu
+def test_refusals(native):
+    g = gen(14)
+    q, _, _ = make_experts(g, 4, 8, 64, 32, "swiglu", torch.bfloat16, 32)
+    x = torch.randn(2, 64, device="cuda").bfloat16()
+    s, i = torch.rand(2, 2, device="cuda").bfloat16(), torch.zeros(2, 2, dtype=torch.int64, device="cuda")
+    with pytest.raises(TypeError, match="type of the scales"):
+        int4_expert_compute(x.half(), s, i, q)
+    with pytest.raises(ValueError, match="tokens, k"):
+        int4_expert_compute(x, s, i.int(), q)
+    with pytest.raises(ValueError, match="fit together"):
+        int4_expert_compute(x[:, :56], s, i, q)
+    with pytest.raises(ValueError, match="fit together"):
+        int4_expert_compute(x, s, i, Int4ExpertParams(q.up, q.down, "silu"))
+    with pytest.raises(ValueError, match="addend"):
+        int4_expert_compute(x, s, i, q, addend=x[:1])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        int4_expert_compute(x, s.cpu(), i, q)
+    with pytest.raises(RuntimeError, match="trace"):
+        torch.jit.trace(lambda t: int4_expert_compute(t, s, i, q), (x,), check_trace=False)
