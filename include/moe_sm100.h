@@ -645,18 +645,18 @@ int moe_act_f8_backward(const void* q, const float* scales, const void* dh, void
 
 /* ---------------------------------------------------------------------------------
  * Products of a few 16-bit rows with weights in 4 bits (for serving: forward only).  No counterpart in the reference.
- * Element [n, k] of w [n_dim, k_dim] is (value - zero) * scale: a value of 0 to 15, scale (`dtype`) and zero (uint8; `zeros` NULL: 8) per row
- * and `group` of 32, 64 or 128 columns.  Laid out in tiles of 16 rows and steps of 128 columns, ceil(n_dim / 16) tiles of ceil(k_dim /
- * 128) steps:  data: 1024 bytes per step, byte (half * 32 + 4 r + t) * 16 + 4 i + b holds row r + 8 half, columns 32 i + 8 t + 4 (b % 2) +
- * b / 2 (low four bits) and two behind (high);  scales, zeros: [16 rows][128 / group] per step.  Rows behind n_dim and columns behind
- * k_dim hold zeros.  All pointers 16-byte aligned, k_dim and n_dim multiples of 8.
+ * Element [n, k] of w [n_dim, k_dim] is (value - zero) * scale: a value of 0 to 15, scale (`dtype`) and zero (uint8; without `zeros`: 8) per
+ * row and `group` of 32, 64 or 128 columns.  Laid out in tiles of 16 rows and steps of 128 columns, [ceil(n_dim / 16)][ceil(k_dim / 128)]
+ * blocks of 1024 bytes of values, 16 * (128 / group) scales and, with `zeros`, as many zeros:
+ *   values: byte (half * 32 + 4 r + t) * 16 + 4 i + b holds row r + 8 half, columns 32 i + 8 t + 4 (b % 2) + b / 2 (low four bits) and two
+ *   behind (high);  scales, zeros: [16 rows][128 / group].  Rows behind n_dim and columns behind k_dim hold zeros.
+ * x and data 16-byte aligned, k_dim and n_dim multiples of 8.
  * out [rows, n_dim] = x [rows, k_dim] @ w^T.
  * --------------------------------------------------------------------------------- */
-int moe_int4_matmul(const void* x, const void* data, const void* scales, const void* zeros, void* out, int64_t rows, int k_dim, int n_dim,
-                    int group, int dtype, void* stream);
+int moe_int4_matmul(const void* x, const void* data, void* out, int64_t rows, int k_dim, int n_dim, int group, int zeros, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------
- * A whole layer for a few tokens (at most 16; 512 slots, 1024 experts) in two kernels, forward only.  No counterpart in the reference.
+ * A whole layer for a few tokens (at most 16; 256 slots, 1024 experts) in two kernels, forward only.  No counterpart in the reference.
  *   h = round(x + residual), y = round(h / sqrt(mean h^2 + eps) * norm_w)  (norm_w NULL: y = x);  stream_out receives h
  *   logits = y router_w in fp32 (of y before its rounding);  scores and experts as in moe_router_tail / moe_grouped_topk with equal values
  *   by ascending index, or, with router_w NULL, as given (expert_idx, scores [num_tokens, topk])
@@ -669,7 +669,7 @@ int moe_int4_matmul(const void* x, const void* data, const void* scales, const v
  * its kernels are done, moe_few_workspace_bytes large.  Two kernels (without norm and router a memset and one).
  * --------------------------------------------------------------------------------- */
 typedef struct moe_few_pass {
-  int32_t num_tokens, d, inter, num_experts, topk, act, dtype, bits, group;
+  int32_t num_tokens, d, inter, num_experts, topk, act, dtype, bits, group, zeros;
   int32_t norm_dtype, router_dtype; /* 2: fp32, else `dtype` */
   int32_t score_function, normalize, num_groups, topk_groups, group_best;
   float scale, eps;
@@ -677,7 +677,7 @@ typedef struct moe_few_pass {
   const float* router_bias;
   const int64_t* expert_idx;
   const void* scores;
-  const void *w1, *w1_scales, *w1_zeros, *w2, *w2_scales, *w2_zeros;
+  const void *w1, *w2;
   const void* addend;
   void *out, *stream_out;
   int32_t* status;

@@ -18,15 +18,17 @@ namespace moe {
 
 constexpr int kFewTokens = 16;
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
-constexpr int kFewSlots = 512;      // tokens x slots
+constexpr int kFewSlots = 256;      // tokens x slots
+constexpr int kFewRows = 8;         // of an entry: slots of one expert that share its weights
 constexpr int kFewExperts = 1024, kFewGroups = 64;
 constexpr int kFewCtas = 2;         // per SM
 constexpr int kFewParts = 4;        // shares of the down product's depth, at most
 
 // ---------------------------------------------------------------------------------------------------- norm and logits
-constexpr int kHeadRanks = 8;       // CTAs of a cluster share the hidden size
-constexpr int kHeadCols = 32;       // experts of a cluster
-constexpr int kHeadRows = 256;      // hidden columns at a time
+constexpr int kHeadRanks = 8;           // CTAs of a cluster share the hidden size
+constexpr int kHeadCols = 16;           // experts of a cluster
+constexpr int kHeadMost = 16384;        // hidden size: a CTA keeps its eighth of all rows in fp32
+constexpr int kHeadLanes = kFewThreads / (kHeadCols / 4);
 
 struct HeadArgs {
   const void *x, *residual, *norm;  // residual, norm: or null
@@ -43,11 +45,8 @@ __device__ __forceinline__ float cluster_load(uint32_t addr) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ double cluster_load_double(uint32_t addr) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
-  return v;
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 template <typename T> __device__ __forceinline__ float to_f32(T v) { return Elem<T>::to_float(v); }
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
@@ -68,130 +67,183 @@ template <typename W> __device__ __forceinline__ void router_row(const W* p, int
     for (int c = 0; c < 4; ++c) f[c] = c < left ? to_f32<W>(p[c]) : 0.0f;
   }
 }
+template <typename T> __device__ __forceinline__ void eight(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = Elem<T>::unpack2(w[i]);
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
 
-// A cluster takes 32 experts' columns, its CTAs an eighth of the hidden size each; a thread four columns and every 32nd hidden row.
-// Norm and logits in one pass over x: the logits are linear in r, which is known when all have met.
+// A cluster takes 16 experts' columns, its CTAs an eighth of the hidden size each; a thread four columns and every 64th hidden row.  One
+// look at x: the logits are linear in r, which is known when the sums of squares have met, while the products are computed.
 template <typename T, typename W, int TT>
 __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a) {
-  __shared__ float rows[TT][kHeadRows];
+  extern __shared__ __align__(16) float rows[];  // [TT][share]: h w
   __shared__ float parts[kFewWarps][TT][kHeadCols];
   __shared__ float joined[TT][kHeadCols];
-  __shared__ double squares[kFewTokens], square_parts[kFewWarps][TT];
+  __shared__ float2 squares[kFewTokens];  // sum of squares, and whether it is in units of 2^144
   __shared__ float scale[kFewTokens];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = static_cast<int>(cluster_ctarank());
-  const int col0 = static_cast<int>(blockIdx.x / kHeadRanks) * kHeadCols;
-  const bool first = blockIdx.x < kHeadRanks;  // the cluster that writes stream and y
+  const int group = static_cast<int>(blockIdx.x / kHeadRanks), groups = static_cast<int>(gridDim.x / kHeadRanks);
+  const int col0 = group * kHeadCols;
   if (blockIdx.x == 0 && tid < 2) a.meeting[tid] = 0;
   const int share = (a.d + kHeadRanks * 8 - 1) / (kHeadRanks * 8) * 8;
-  const int k_begin = min(rank * share, a.d), k_end = min(k_begin + share, a.d);
-  const T* x = static_cast<const T*>(a.x);
-  const T* residual = static_cast<const T*>(a.residual);
-  const int cv = tid & 7, kl = tid >> 3;  // columns col0 + 4 cv + 0..3, hidden rows kl + 32 i
+  const int k_begin = min(rank * share, a.d), count = min(share, a.d - k_begin);
+  const int cv = tid % (kHeadCols / 4), kl = tid / (kHeadCols / 4);  // columns col0 + 4 cv + 0..3, hidden rows kl + 64 i
   const int left = a.E - (col0 + 4 * cv);
-  const bool whole = left >= 4 && (a.E & 3) == 0;
-  const auto norm_weight = [&](int k) {
-    return a.norm == nullptr ? 1.0f : a.norm_fp32 ? static_cast<const float*>(a.norm)[k] : to_f32<T>(static_cast<const T*>(a.norm)[k]);
+  const bool whole = left >= 4 && (a.E & 3) == 0, mine = a.router != nullptr && left > 0;
+  const W* router = static_cast<const W*>(a.router) + static_cast<int64_t>(k_begin) * a.E + col0 + 4 * cv;
+  constexpr int AHEAD = 4;
+  float w[AHEAD][4];
+  const auto ask = [&](int i, float (&f)[4]) {
+    if (mine && i < count) router_row<W>(router + static_cast<int64_t>(i) * a.E, left, whole, f);
+    else f[0] = f[1] = f[2] = f[3] = 0.0f;
   };
-  float acc[TT][4];
-  double sq[TT];
 #pragma unroll
-  for (int t = 0; t < TT; ++t) {
-    acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
-    sq[t] = 0.0;
-  }
-  for (int k0 = k_begin; k0 < k_end; k0 += kHeadRows) {
-    float w[kHeadRows / 32][4];
-#pragma unroll
-    for (int i = 0; i < kHeadRows / 32; ++i) {
-      const int k = k0 + kl + 32 * i;
-      if (a.router != nullptr && k < k_end && left > 0) router_row<W>(static_cast<const W*>(a.router) + static_cast<int64_t>(k) * a.E + col0 + 4 * cv, left, whole, w[i]);
-      else w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0.0f;
+  for (int i = 0; i < AHEAD; ++i) ask(kl + i * kHeadLanes, w[i]);  // on their way while the rows are made
+
+  // rows: a warp per token, eight columns per lane at a time
+  for (int t = warp; t < TT; t += kFewWarps) {
+    if (t >= a.T) {
+      for (int i = lane; i < share; i += 32) rows[t * share + i] = 0.0f;
+      if (lane == 0) squares[t] = make_float2(0.0f, 0.0f);
+      continue;
     }
-    const int k = k0 + tid;
-    const float g = k < k_end ? norm_weight(k) : 0.0f;
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      float h = 0.0f;
-      if (t < a.T && k < k_end) {
-        h = to_f32<T>(x[static_cast<int64_t>(t) * a.d + k]);
+    const T* x = static_cast<const T*>(a.x) + static_cast<int64_t>(t) * a.d + k_begin;
+    const T* residual = a.residual == nullptr ? nullptr : static_cast<const T*>(a.residual) + static_cast<int64_t>(t) * a.d + k_begin;
+    float sum = 0.0f, large = 0.0f, most = 0.0f;
+#pragma unroll 2
+    for (int i = lane * 8; i < share; i += 256) {
+      float h[8] = {}, g[8];
+      if (i < count) {
+        eight<T>(*reinterpret_cast<const uint4*>(x + i), h);
         if (residual != nullptr) {
-          const T v = Elem<T>::from_float(h + to_f32<T>(residual[static_cast<int64_t>(t) * a.d + k]));
-          if (first) static_cast<T*>(a.stream)[static_cast<int64_t>(t) * a.d + k] = v;
-          h = to_f32<T>(v);
+          float o[8];
+          eight<T>(*reinterpret_cast<const uint4*>(residual + i), o);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[j] += o[j];
+          const uint4 v = make_uint4(Elem<T>::pack2(h[0], h[1]), Elem<T>::pack2(h[2], h[3]), Elem<T>::pack2(h[4], h[5]), Elem<T>::pack2(h[6], h[7]));
+          if (t % groups == group) *reinterpret_cast<uint4*>(static_cast<T*>(a.stream) + static_cast<int64_t>(t) * a.d + k_begin + i) = v;
+          eight<T>(v, h);
         }
-        sq[t] += static_cast<double>(h) * h;  // (bf16 values' squares may leave fp32)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          sum = fmaf(h[j], h[j], sum);
+          large = fmaf(h[j] * 0x1p-72f, h[j] * 0x1p-72f, large);  // bf16 values from 2^57 on have squares whose sum may leave fp32
+          most = fmaxf(most, fabsf(h[j]));
+          g[j] = a.norm == nullptr ? 1.0f : a.norm_fp32 ? static_cast<const float*>(a.norm)[k_begin + i + j] : 0.0f;
+        }
+        if (a.norm != nullptr && !a.norm_fp32) eight<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.norm) + k_begin + i), g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] *= g[j];
       }
-      rows[t][tid] = h * g;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kHeadRows / 32; ++i) {
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const float h = rows[t][kl + 32 * i];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[t][c] = fmaf(h, w[i][c], acc[t][c]);
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int t = 0; t < TT; ++t) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      acc[t][c] += __shfl_xor_sync(0xFFFFFFFFu, acc[t][c], 8);
-      acc[t][c] += __shfl_xor_sync(0xFFFFFFFFu, acc[t][c], 16);
-      if (lane < 8) parts[warp][t][4 * cv + c] = acc[t][c];
+      float4* out = reinterpret_cast<float4*>(rows + t * share + i);
+      out[0] = make_float4(h[0], h[1], h[2], h[3]);
+      out[1] = make_float4(h[4], h[5], h[6], h[7]);
     }
     if (a.norm != nullptr) {
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) sq[t] += __shfl_xor_sync(0xFFFFFFFFu, sq[t], off);
-      if (lane == 0) square_parts[warp][t] = sq[t];
+      for (int off = 16; off > 0; off >>= 1) {
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+        large += __shfl_xor_sync(0xFFFFFFFFu, large, off);
+        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
+      }
+      if (lane == 0) squares[t] = most > 0x1p50f ? make_float2(large, 1.0f) : make_float2(sum, 0.0f);
     }
   }
   __syncthreads();
-  for (int at = tid; at < TT * kHeadCols; at += kFewThreads) {
-    float v = 0.0f;
-    for (int w = 0; w < kFewWarps; ++w) v += (&parts[w][0][0])[at];
-    (&joined[0][0])[at] = v;
+  cluster_arrive();  // the squares
+  float acc[TT][4];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
+  if (a.router != nullptr) {
+    for (int i0 = kl; i0 < count; i0 += AHEAD * kHeadLanes) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int k = i0 + i * kHeadLanes;
+        float f[4] = {w[i][0], w[i][1], w[i][2], w[i][3]};
+        ask(k + AHEAD * kHeadLanes, w[i]);
+        if (k < count) {
+#pragma unroll
+          for (int t = 0; t < TT; ++t) {
+            const float h = rows[t * share + k];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[t][c] = fmaf(h, f[c], acc[t][c]);
+          }
+        }
+      }
+    }
   }
-  if (a.norm != nullptr && tid < TT) {
-    double v = 0.0;
-    for (int w = 0; w < kFewWarps; ++w) v += square_parts[w][tid];
-    squares[tid] = v;
-  }
-  __syncthreads();
-  cluster_sync_all();
+  __syncwarp();
+  cluster_wait();
   if (tid < TT) {
     float r = 1.0f;
     if (a.norm != nullptr) {
-      double v = 0.0;
-      for (int q = 0; q < kHeadRanks; ++q) v += cluster_load_double(mapa_shared(smem_u32(&squares[tid]), q));
-      r = static_cast<float>(1.0 / sqrt(v / a.d + static_cast<double>(a.eps)));
+      float2 all[kHeadRanks];
+#pragma unroll
+      for (int q = 0; q < kHeadRanks; ++q) {
+        const uint32_t at = mapa_shared(smem_u32(&squares[tid]), q);
+        all[q] = make_float2(cluster_load(at), cluster_load(at + 4));
+      }
+      bool wide = false;
+#pragma unroll
+      for (int q = 0; q < kHeadRanks; ++q) wide |= all[q].y != 0.0f;
+      float v = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kHeadRanks; ++q) v += all[q].y == 0.0f && wide ? all[q].x * 0x1p-72f * 0x1p-72f : all[q].x;
+      v /= static_cast<float>(a.d);
+      r = wide ? rsqrtf(v) * 0x1p-72f : rsqrtf(v + a.eps);  // (beside such squares eps is nothing)
     }
     scale[tid] = r;
   }
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int off = kHeadCols / 4; off < 32; off <<= 1) acc[t][c] += __shfl_xor_sync(0xFFFFFFFFu, acc[t][c], off);
+      if (lane < kHeadCols / 4) parts[warp][t][4 * cv + c] = acc[t][c];
+    }
   __syncthreads();
-  if (rank == 0 && a.router != nullptr) {
-    for (int at = tid; at < TT * kHeadCols; at += kFewThreads) {
+  for (int at = tid; at < TT * kHeadCols; at += kFewThreads) {
+    float v = 0.0f;
+#pragma unroll
+    for (int w8 = 0; w8 < kFewWarps; ++w8) v += (&parts[w8][0][0])[at];
+    (&joined[0][0])[at] = v;
+  }
+  __syncthreads();
+  cluster_arrive();  // the logits
+  if (a.norm != nullptr) {
+    for (int t = group; t < a.T; t += groups) {
+      for (int i = tid * 8; i < count; i += kFewThreads * 8) {
+        const float4 u = *reinterpret_cast<const float4*>(rows + t * share + i), v = *reinterpret_cast<const float4*>(rows + t * share + i + 4);
+        const float r = scale[t];
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.y) + static_cast<int64_t>(t) * a.d + k_begin + i) =
+            make_uint4(Elem<T>::pack2(u.x * r, u.y * r), Elem<T>::pack2(u.z * r, u.w * r), Elem<T>::pack2(v.x * r, v.y * r), Elem<T>::pack2(v.z * r, v.w * r));
+      }
+    }
+  }
+  __syncwarp();
+  cluster_wait();
+  if (a.router != nullptr) {
+    // each CTA joins its share of the cluster's logits
+    for (int at = tid * kHeadRanks + rank; at < TT * kHeadCols; at += kFewThreads * kHeadRanks) {
       const int t = at / kHeadCols, e = col0 + at % kHeadCols;
       if (t >= a.T || e >= a.E) continue;
-      float v = 0.0f;
-      for (int q = 0; q < kHeadRanks; ++q) v += cluster_load(mapa_shared(smem_u32(&(&joined[0][0])[at]), q));
+      float part[kHeadRanks], v = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kHeadRanks; ++q) part[q] = cluster_load(mapa_shared(smem_u32(&(&joined[0][0])[at]), q));
+#pragma unroll
+      for (int q = 0; q < kHeadRanks; ++q) v += part[q];
       a.logits[static_cast<int64_t>(t) * a.E + e] = v * scale[t];
     }
   }
   __syncthreads();
   cluster_sync_all();  // the others' shared memory lives until it has been read
-  if (!first || a.norm == nullptr) return;
-  for (int t = 0; t < a.T; ++t) {
-    for (int k = k_begin + tid; k < k_end; k += kFewThreads) {
-      float h = to_f32<T>(x[static_cast<int64_t>(t) * a.d + k]);
-      if (residual != nullptr) h = to_f32<T>(Elem<T>::from_float(h + to_f32<T>(residual[static_cast<int64_t>(t) * a.d + k])));
-      static_cast<T*>(a.y)[static_cast<int64_t>(t) * a.d + k] = Elem<T>::from_float(h * scale[t] * norm_weight(k));
-    }
-  }
 }
 
 // -------------------------------------------------------------------------------------------------------- the experts
@@ -219,9 +271,10 @@ struct FewArgs {
 struct FewRouting {
   float score[kFewSlots];
   int16_t id[kFewSlots];
-  int16_t expert[kFewSlots];       // of an entry: up to 16 slots of one expert
+  int16_t expert[kFewSlots], first[kFewSlots];  // of an entry: its slots are slot[first] .. slot[first + count - 1]
+  int16_t slot[kFewSlots], token[kFewSlots];    // and these slots' tokens
   uint8_t count[kFewSlots];
-  int16_t slot[kFewSlots][kFewTokens];
+  int starts[kFewSlots / 32];
   int entries;
   int go_on;
 };
@@ -230,8 +283,8 @@ struct FewRouting {
 __device__ __forceinline__ bool meet(const FewArgs& a, int turn, int* go_on) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    __threadfence();
-    atomicAdd(a.meeting, 1u);
+    // what this CTA has written is published by the barrier above and this addition, what the others have is acquired by the last load
+    asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(a.meeting) : "memory");
     const uint32_t all = static_cast<uint32_t>(turn) * gridDim.x;
     const long long t0 = clock64();
     int ok = 1;
@@ -245,41 +298,67 @@ __device__ __forceinline__ bool meet(const FewArgs& a, int turn, int* go_on) {
         break;
       }
     }
-    __threadfence();
     *go_on = ok;
   }
   __syncthreads();
   return *go_on != 0;
 }
 
-// One warp, one token: keys [E] is scratch of this warp's own.
-__device__ __forceinline__ void choose(const FewArgs& a, int t, float* keys, FewRouting& r, int lane) {
-  const float* logits = a.logits + static_cast<int64_t>(t) * a.E;
-  const bool by_probability = a.bias != nullptr || a.groups > 1;
-  float most = -INFINITY, sum = 0.0f;
-  for (int e = lane; e < a.E; e += 32) most = fmaxf(most, logits[e]);
+// A number's bits in an order that whole numbers have.
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+}
+
+// One warp, one token; expert lane + 32 i is the lane's i-th of up to EACH.  `keys`: scratch of this warp's own, [E] and [groups].
+template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int t, float* keys, FewRouting& r, int lane) {
+  constexpr uint32_t kAll = 0xFFFFFFFFu;
+  const float* from = a.logits + static_cast<int64_t>(t) * a.E;
+  float p[EACH];        // logit, then its share before normalisation
+  float bias[EACH];
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
-  const bool softmax = !a.sigmoid && !a.softmax_after;
-  if (softmax) {
-    for (int e = lane; e < a.E; e += 32) sum += expf(logits[e] - most);
+  for (int i = 0; i < EACH; ++i) {
+    const int e = lane + 32 * i;
+    p[i] = e < a.E ? from[e] : -INFINITY;
+    bias[i] = e < a.E && a.bias != nullptr ? a.bias[e] : 0.0f;
+  }
+  // open experts' keys are 2 and above (NaN and -inf 2: they come last, lowest index first), taken and closed ones below
+  uint32_t key[EACH];
+  const auto key_of = [](float v) { return v > -3.402823466e38f ? ordered(v) : 2u; };
+  float most = -3.402823466e38f, sum = 0.0f;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+  for (int i = 0; i < EACH; ++i) {
+    most = fmaxf(most, p[i]);
+    key[i] = lane + 32 * i < a.E ? key_of(p[i]) : 0u;
   }
-  const auto probability = [&](float l) { return a.sigmoid ? 1.0f / (1.0f + expf(-l)) : softmax ? expf(l - most) / sum : l; };
-  // open experts' keys stay above -inf (NaN and -inf come last, lowest index first); taken and closed ones are -inf
-  constexpr float kLast = -3.402823466e38f;
-  for (int e = lane; e < a.E; e += 32) {
-    float key = logits[e];
-    if (by_probability) key = probability(key) + (a.bias != nullptr ? a.bias[e] : 0.0f);
-    keys[e] = key > kLast ? key : kLast;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kAll, most, off));
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    p[i] = a.sigmoid ? 1.0f / (1.0f + expf(-p[i])) : expf(p[i] - most);
+    if (lane + 32 * i < a.E) sum += p[i];
   }
-  __syncwarp();
+  if (!a.sigmoid && !a.softmax_after) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kAll, sum, off);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) p[i] /= sum;
+  }
+  if (a.bias != nullptr || a.groups > 1) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (lane + 32 * i < a.E) key[i] = key_of(p[i] + bias[i]);
+  }
   if (a.groups > 1) {
     const int width = a.E / a.groups;
-    float* worth = keys + a.E;  // [groups]
+    float* const worth = keys + a.E;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (lane + 32 * i < a.E) keys[lane + 32 * i] = key[i] > 2u ? p[i] + bias[i] : -3.402823466e38f;
+    __syncwarp();
     for (int g = lane; g < a.groups; g += 32) {
       float b0 = -INFINITY, b1 = -INFINITY;
+#pragma unroll 4
       for (int i = 0; i < width; ++i) {
         const float v = keys[g * width + i];
         b1 = fmaxf(b1, fminf(b0, v));
@@ -288,112 +367,125 @@ __device__ __forceinline__ void choose(const FewArgs& a, int t, float* keys, Few
       worth[g] = a.best == 2 && width > 1 ? b0 + b1 : b0;
     }
     __syncwarp();
-    for (int g = lane; g < a.groups; g += 32) {
-      const float mine = worth[g];
-      int before = 0;
-      for (int o = 0; o < a.groups; ++o) before += worth[o] > mine || (worth[o] == mine && o < g);
-      if (before >= a.keep)
-        for (int i = 0; i < width; ++i) keys[g * width + i] = -INFINITY;
+    uint32_t open0 = 0, open1 = 0;  // groups 0..31, 32..63
+    for (int g0 = 0; g0 < a.groups; g0 += 32) {
+      const int g = g0 + lane;
+      int before = a.keep;
+      if (g < a.groups) {
+        before = 0;
+        for (int o = 0; o < a.groups; ++o) before += worth[o] > worth[g] || (worth[o] == worth[g] && o < g);
+      }
+      (g0 == 0 ? open0 : open1) = __ballot_sync(kAll, before < a.keep);
     }
-    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int g = (lane + 32 * i) / width;
+      if (((g < 32 ? open0 : open1) >> (g & 31) & 1) == 0) key[i] = 0u;
+    }
   }
-  // k times the best; a lane looks again only when its own best was taken
-  float best = -INFINITY;
-  int at = a.E;
+  // k times the best of the lanes' best; only the lane that had it looks again
+  uint32_t best;
+  int at;
+  float share;
   const auto look = [&]() {
-    best = -INFINITY;
-    at = a.E;
-    for (int e = lane; e < a.E; e += 32)
-      if (keys[e] > best) best = keys[e], at = e;
+    best = key[0], at = lane, share = p[0];
+#pragma unroll
+    for (int i = 1; i < EACH; ++i)
+      if (key[i] > best) best = key[i], at = lane + 32 * i, share = p[i];
   };
   look();
-  float total = 0.0f, top = 0.0f;
+  float total = 0.0f;
   for (int s = 0; s < a.k; ++s) {
-    float v = best;
-    int e = at;
+    const uint32_t v = __reduce_max_sync(kAll, best);
+    const uint32_t e = __reduce_min_sync(kAll, best == v ? static_cast<uint32_t>(at) : 0xFFFFu);
+    if (e == static_cast<uint32_t>(at)) {
+      r.id[t * a.k + s] = static_cast<int16_t>(e);
+      r.score[t * a.k + s] = share;
+      total += share;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      const float ov = __shfl_xor_sync(0xFFFFFFFFu, v, off);
-      const int oe = __shfl_xor_sync(0xFFFFFFFFu, e, off);
-      if (ov > v || (ov == v && oe < e)) v = ov, e = oe;
-    }
-    if (e == at && e < a.E) {
-      keys[e] = -INFINITY;
+      for (int i = 0; i < EACH; ++i)
+        if (at == lane + 32 * i) key[i] = 0u;
       look();
     }
-    float p = e < a.E ? logits[e] : 0.0f;
-    if (a.softmax_after) {
-      if (s == 0) top = p;  // the largest selected logit comes first (no bias, no groups)
-      p = expf(p - top);
-    } else {
-      p = probability(p);
-    }
-    total += p;
-    if (lane == 0) {
-      r.id[t * a.k + s] = static_cast<int16_t>(e < a.E ? e : -1);
-      r.score[t * a.k + s] = p;
-    }
   }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(kAll, total, off);
   __syncwarp();
-  if (a.softmax_after) {
-    for (int s = lane; s < a.k; s += 32) r.score[t * a.k + s] /= total;
-  } else if (a.normalize) {
-    const float by = a.normalize == 2 ? fmaxf(total, 1e-12f) : total + 1e-20f;
-    for (int s = lane; s < a.k; s += 32) r.score[t * a.k + s] = r.score[t * a.k + s] / by * a.scale;
-  } else {
-    for (int s = lane; s < a.k; s += 32) r.score[t * a.k + s] *= a.scale;
-  }
+  const float by = a.softmax_after ? total : a.normalize == 2 ? fmaxf(total, 1e-12f) : a.normalize == 1 ? total + 1e-20f : 1.0f;
+  for (int s = lane; s < a.k; s += 32) r.score[t * a.k + s] = r.score[t * a.k + s] / by * (a.softmax_after ? 1.0f : a.scale);
+  __syncwarp();
 }
 
-// Scores, experts, and the list of entries: up to 16 slots of one expert each, in the order of their first slots.
+// Scores, experts, and the list of entries: up to eight slots of one expert each.  Entries of one expert follow one another (they read
+// the same weights at the same time), experts by their first slots.
 template <typename T> __device__ __forceinline__ void route(const FewArgs& a, FewRouting& r, float* scratch) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int slots = a.T * a.k;
   if (a.logits != nullptr) {
-    for (int t = warp; t < a.T; t += kFewWarps) choose(a, t, scratch + warp * (a.E + a.groups), r, lane);
-  } else {
-    for (int j = tid; j < slots; j += kFewThreads) {
-      const int64_t e = a.ids[j];
-      const bool ok = e >= 0 && e < a.E;
-      if (!ok && a.status != nullptr) atomicCAS(a.status, 0, DS_BAD_EXPERT_ID);
-      r.id[j] = static_cast<int16_t>(ok ? e : -1);
-      r.score[j] = to_f32<T>(static_cast<const T*>(a.given)[j]);
+    float* const keys = scratch + warp * (a.E + a.groups);
+    for (int t = warp; t < a.T; t += kFewWarps) {
+      if (a.E <= 64) choose<2>(a, t, keys, r, lane);
+      else if (a.E <= 256) choose<8>(a, t, keys, r, lane);
+      else choose<32>(a, t, keys, r, lane);
     }
+  } else if (tid < slots) {
+    const int64_t e = a.ids[tid];
+    const bool ok = e >= 0 && e < a.E;
+    if (!ok && a.status != nullptr) atomicCAS(a.status, 0, DS_BAD_EXPERT_ID);
+    r.id[tid] = static_cast<int16_t>(ok ? e : -1);
+    r.score[tid] = to_f32<T>(static_cast<const T*>(a.given)[tid]);
   }
   __syncthreads();
-  __shared__ int starts[kFewSlots / 32];
-  int rank[kFewSlots / kFewThreads];
-  bool begins[kFewSlots / kFewThreads];
-#pragma unroll
-  for (int i = 0; i < kFewSlots / kFewThreads; ++i) {
-    const int j = tid + i * kFewThreads;
-    const int e = j < slots ? r.id[j] : -1;
-    rank[i] = 0;
-    if (e >= 0)
-      for (int o = 0; o < j; ++o) rank[i] += r.id[o] == e;
-    begins[i] = e >= 0 && rank[i] % kFewTokens == 0;
-    const unsigned mine = __ballot_sync(0xFFFFFFFFu, begins[i]);
-    if (lane == 0) starts[i * kFewWarps + warp] = static_cast<int>(mine);
-  }
+  // slots of an expert per warp, then where its slots and entries begin
+  static_assert(kFewSlots == kFewThreads, "a slot per thread");
+  uint8_t* const counts = reinterpret_cast<uint8_t*>(scratch);                               // [warp][E]
+  int* const begins = reinterpret_cast<int*>(counts + kFewWarps * ((a.E + 15) / 16 * 16));   // [E]
+  const int pitch = (a.E + 15) / 16 * 16;
+  for (int i = tid; i < kFewWarps * pitch / 4; i += kFewThreads) reinterpret_cast<uint32_t*>(counts)[i] = 0;
   __syncthreads();
+  const int e = tid < slots ? r.id[tid] : -1;
+  const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
+  const int before = __popc(same & ((1u << lane) - 1));
+  if (e >= 0 && before == 0) counts[warp * pitch + e] = static_cast<uint8_t>(__popc(same));
+  __syncthreads();
+  int rank = before, all = 0;  // among the slots of its expert
+  if (e >= 0) {
 #pragma unroll
-  for (int i = 0; i < kFewSlots / kFewThreads; ++i) {
-    const int j = tid + i * kFewThreads;
-    if (begins[i]) {
-      int n = __popc(static_cast<unsigned>(starts[i * kFewWarps + warp]) & ((1u << lane) - 1));
-      for (int w = 0; w < i * kFewWarps + warp; ++w) n += __popc(static_cast<unsigned>(starts[w]));
-      int left = 0;
-      for (int o = j; o < slots; ++o) left += r.id[o] == r.id[j];
-      r.expert[n] = r.id[j];
-      r.count[n] = static_cast<uint8_t>(min(left, kFewTokens));
-      for (int o = j, c = 0; o < slots && c < kFewTokens; ++o)
-        if (r.id[o] == r.id[j]) r.slot[n][c++] = static_cast<int16_t>(o);
+    for (int w = 0; w < kFewWarps; ++w) {
+      const int n = counts[w * pitch + e];
+      all += n;
+      if (w < warp) rank += n;
     }
   }
-  if (tid == 0) {
-    int n = 0;
-    for (int w = 0; w < kFewSlots / 32; ++w) n += __popc(static_cast<unsigned>(starts[w]));
-    r.entries = n;
+  const bool first = e >= 0 && rank == 0;
+  int sum = first ? (all + kFewRows - 1) / kFewRows << 16 | all : 0;  // entries and slots up to here, then before
+  const int own = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xFFFFFFFFu, sum, off);
+    if (lane >= off) sum += o;
+  }
+  if (lane == 31) r.starts[warp] = sum;
+  __syncthreads();
+  int base = 0, everything = 0;
+#pragma unroll
+  for (int w = 0; w < kFewWarps; ++w) {
+    if (w < warp) base += r.starts[w];
+    everything += r.starts[w];
+  }
+  if (first) begins[e] = base + sum - own;
+  if (tid == 0) r.entries = everything >> 16;
+  __syncthreads();
+  if (e >= 0) {
+    const int entry = begins[e] >> 16, at = begins[e] & 0xFFFF;
+    r.slot[at + rank] = static_cast<int16_t>(tid);
+    r.token[at + rank] = static_cast<int16_t>(tid / a.k);
+    if (rank % kFewRows == 0) {
+      const int n = entry + rank / kFewRows;
+      r.expert[n] = static_cast<int16_t>(e);
+      r.first[n] = static_cast<int16_t>(at + rank);
+      r.count[n] = static_cast<uint8_t>(min(all - rank, kFewRows));
+    }
   }
   __syncthreads();
 }
@@ -409,201 +501,361 @@ __device__ __forceinline__ float few_act(float x, int act) {
   }
 }
 
-// ---- 16-bit weights [K, N] (N contiguous) by up to 16 rows: a warp's step is 16 rows of K by 64 columns ----
-// Tokens are the 16 rows of m16n8k16 and column 8 g + j of the tile is column g of its j-th product, so that a lane's 16-byte pieces are
-// eight products' columns; slots (2 t, 2 t + 1) and (2 t + 8, 2 t + 9) of K stand for rows 4 t .. 4 t + 3.
-constexpr int kWideCols = 64, kWideStep = 16;
-constexpr int kWideStage = kWideStep * kWideCols * 2;
-constexpr int kWideDepth = 5;
-
-template <typename T>
-__device__ __forceinline__ void wide_tile(float (&acc)[8][4], const uint16_t* w, int K, int N, int col0, const uint16_t* x0, const uint16_t* x1, int first,
-                                          int end, int stride, uint32_t ring, int lane) {
-  const int g = lane >> 2, t = lane & 3;
-  const bool inside = col0 + 8 * g < N;
-  const uint16_t* from = w + static_cast<int64_t>(4 * t) * N + col0 + 8 * g;
-  const auto copy = [&](uint32_t stage, int step) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int k = step * kWideStep + 4 * t + j;
-      if (inside && k < K) copy_16(stage + j * 512 + lane * 16, from + (static_cast<int64_t>(step) * kWideStep + j) * N);
-    }
-  };
-  int ahead = first;
-#pragma unroll
-  for (int s = 0; s < kWideDepth - 1; ++s, ahead += stride) {
-    if (ahead < end) copy(ring + s * kWideStage, ahead);
-    copies_commit();
-  }
-  uint32_t stage = ring, free_stage = ring + (kWideDepth - 1) * kWideStage;
-  for (int step = first; step < end; step += stride, ahead += stride) {
-    copies_wait<kWideDepth - 2>();
-    if (ahead < end) copy(free_stage, ahead);  // (a lane reads what it has copied itself, and has read what this replaces)
-    copies_commit();
-    const int k = step * kWideStep + 4 * t;
-    uint2 a0 = make_uint2(0, 0), a1 = a0;
-    if (k < K) {
-      if (x0 != nullptr) a0 = *reinterpret_cast<const uint2*>(x0 + k);
-      if (x1 != nullptr) a1 = *reinterpret_cast<const uint2*>(x1 + k);
-    }
-    const uint32_t a[4] = {a0.x, a1.x, a0.y, a1.y};
-    uint4 r[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = inside && k < K ? lds_128(stage + j * 512 + lane * 16) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t pick = j & 1 ? 0x7632u : 0x5410u;
-      mma_16x8x16<T>(acc[j], a, __byte_perm(word_of(r[0], j >> 1), word_of(r[1], j >> 1), pick),
-                     __byte_perm(word_of(r[2], j >> 1), word_of(r[3], j >> 1), pick));
-    }
-    free_stage = stage;
-    stage = stage == ring + (kWideDepth - 1) * kWideStage ? ring : stage + kWideStage;
-  }
-  copies_wait<0>();
-  __syncwarp();  // the ring is free again, for other lanes' words too
-}
-
-template <int BITS, int NG, bool ZEROS> struct FewPlan {
-  static constexpr int kDepth = BITS == 4 ? 6 : kWideDepth;
-  static constexpr int kStage = BITS == 4 ? Q4Stage<NG, ZEROS>::kBytes : kWideStage;
-  static constexpr int kRing = kDepth * kStage;
-  static constexpr int kCols = BITS == 4 ? kQ4Rows : kWideCols;       // of a tile of a product
-  static constexpr int kTotal = kFewWarps * kRing;
-  // a warp's ring also holds its sums of a unit, when the copies are through, and before all that the router's keys
-  static_assert(kFewTokens * kCols * 4 <= kRing && kFewWarps * (kFewExperts + kFewGroups) * 4 <= kTotal, "the rings are large enough");
+// A format of weights: how a warp copies one step of a tile with the same columns of an entry's rows to shared memory, and multiplies them.
+// A unit is an entry's rows by a few tiles of its expert's matrix over steps [begin, end).  Its tiles are shared out to the warps, `team` of
+// them to a tile (1, 2, 4 or 8, so that a unit has 8 / team tiles); warp w of a team takes steps begin + w, begin + w + team, ...
+struct FewMatrix {
+  const void* w16;
+  Q4Matrix w4;
+  int K, N, steps, cols;  // cols: of a tile
+  int team, shares;       // of the depth, see below
 };
 
-template <typename T, int BITS, int NG, bool ZEROS>
+// Team and shares of a product: the fullest CTA has `rounds` units, each of the steps of a warp and what the joining costs (about as much as
+// `cost` steps).  More shares, up to `most`, give more units of fewer steps, and partial sums for the fold.
+__device__ __forceinline__ void share_out(FewMatrix& m, int entries, int most, int cost) {
+  const int tiles = (m.N + m.cols - 1) / m.cols;
+  int least = 0x7FFFFFFF;
+  for (int shares = 1; shares <= most; shares *= 2)
+    for (int team = kFewWarps; team >= 1; team /= 2) {
+      const int units = entries * ((tiles * team + kFewWarps - 1) / kFewWarps) * shares;
+      const int rounds = (units + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+      const int steps = (m.steps + shares * team - 1) / (shares * team) + cost + (shares > 1);
+      if (rounds * steps < least) least = rounds * steps, m.team = team, m.shares = shares;
+    }
+}
+
+// 16 bits, [K, N] with N contiguous: 16 rows of K by up to 64 columns.  The weights are the 16 rows of m16n8k16, transposed on their way from
+// shared memory (ldmatrix); product q has columns 16 q .. 16 q + 15.  Eight lanes copy 128 bytes of one row (lanes in the order of the
+// products, four rows to a quarter of a warp, made a request of every 16 bytes: 2.2 TB/s); in shared memory the 16-byte pieces of a row
+// are turned by its number, so that the eight rows of a matrix lie in different banks.
+template <typename T> struct FewWide {
+  static constexpr int kCols = 64, kStep = 16, kDepth = 5, kProducts = 4, kCost = 4;
+  static constexpr int kRowsAt = kStep * kCols * 2, kStage = kRowsAt + kFewRows * kStep * 2;
+  const uint16_t* w;   // the copy's: this lane's piece of the step's first row
+  const uint16_t* x;   // this lane's piece of its row
+  int64_t row;
+  int K;
+  bool inside;
+  // the product's
+  uint32_t weight_at, row_at;
+  __device__ __forceinline__ void read(int count, int lane) {
+    const int mine = lane & 7, k = mine + 8 * (lane >> 4);
+    weight_at = k * 128 + ((((lane >> 3) & 1) ^ mine) << 4);   // product q: ^ 32 q
+    const int g = lane >> 2;
+    row_at = kRowsAt + (g < count ? g : 0) * 32 + (lane & 3) * 4;  // (rows behind the last give products that are nobody's)
+  }
+  template <typename Row> __device__ __forceinline__ void set(const FewMatrix& m, int expert, int tile, int step, Row rows, int count, int lane) {
+    const int piece = lane & 7, col = tile * m.cols + 8 * piece;
+    inside = 8 * piece < m.cols && col < m.N;
+    row = m.N;
+    K = m.K;
+    w = static_cast<const uint16_t*>(m.w16) + (static_cast<int64_t>(expert) * K + step * kStep + (lane >> 3)) * row + col;
+    x = (lane >> 1) < count ? rows(lane >> 1) : nullptr;
+  }
+  __device__ __forceinline__ void copy(uint32_t stage, int step, int lane) const {
+    if (!inside) return;
+    const int r = lane >> 3;
+    const uint32_t to = stage + r * 128;
+    if (step * kStep + kStep <= K) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) copy_16(to + j * 512 + (((lane & 7) ^ ((r + 4 * j) & 7)) << 4), w + 4 * j * row);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool real = step * kStep + r + 4 * j < K;
+        copy_16_or_zeros(to + j * 512 + (((lane & 7) ^ ((r + 4 * j) & 7)) << 4), real ? w + 4 * j * row : w, real);
+      }
+    }
+  }
+  __device__ __forceinline__ void copy_rows(uint32_t stage, int, int step, int lane) const {
+    const int k = step * kStep + 8 * (lane & 1);
+    if (x != nullptr) copy_16_or_zeros(stage + kRowsAt + lane * 16, k < K ? x + k : x, k < K);
+  }
+  __device__ __forceinline__ void next(int team) { w += team * kStep * row; }
+  __device__ __forceinline__ void multiply(float (&acc)[kProducts][4], uint32_t stage, int) const {
+    const uint32_t b0 = lds_32(stage + row_at), b1 = lds_32(stage + row_at + 16);
+#pragma unroll
+    for (int q = 0; q < kProducts; ++q) {
+      uint32_t a[4];
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                   : "r"(stage + (weight_at ^ (32 * q)))
+                   : "memory");
+      mma_16x8x16<T>(acc[q], a, b0, b1);
+    }
+  }
+  // column of the tile that value c of product q belongs to
+  __device__ static __forceinline__ int column(int q, int c, int lane) { return 16 * q + (lane >> 2) + 8 * (c >> 1); }
+  // Columns of a tile: as many, in eights, as leave the fullest CTA with the least (a unit's own costs count as eight columns).
+  __device__ static __forceinline__ int width(int entries, int N) {
+    int best = kCols, least = 0x7FFFFFFF;
+    for (int c = kCols; c >= 16; c -= 8) {
+      const int rounds = (entries * ((N + c - 1) / c) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+      if (rounds * (c + 8) < least) least = rounds * (c + 8), best = c;
+    }
+    return best;
+  }
+};
+
+// 4 bits (int4.cuh): 16 rows of the weight by 128 columns.
+template <typename T, int NG, bool ZEROS> struct FewFour {
+  static constexpr int kCols = kQ4Rows, kStep = kQ4Step, kDepth = 4, kProducts = 1, kCost = 4;
+  static constexpr int kStage = Q4Stage<NG, ZEROS>::kBytes, kBlock = Q4Stage<NG, ZEROS>::kBlock;
+  const uint8_t* block;
+  const uint16_t* x[4];
+  int K;
+  uint32_t row_at;
+  __device__ __forceinline__ void read(int count, int lane) { row_at = q4_row_at(count, lane); }
+  template <typename Row> __device__ __forceinline__ void set(const FewMatrix& m, int expert, int tile, int step, Row rows, int count, int lane) {
+    block = m.w4.data + ((expert * m.w4.tiles + tile) * m.w4.steps + step) * kBlock;
+    K = m.K;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 2 * i + (lane >> 4);
+      if (r < count) x[i] = rows(r);
+    }
+  }
+  __device__ __forceinline__ void copy(uint32_t stage, int, int lane) const { q4_copy<NG, ZEROS>(stage, block, lane); }
+  __device__ __forceinline__ void copy_rows(uint32_t stage, int count, int step, int lane) const {
+    q4_copy_rows<NG, ZEROS>(stage, [&](int i) { return x[i]; }, count, K, step, lane);
+  }
+  __device__ __forceinline__ void next(int team) { block += team * kBlock; }
+  __device__ __forceinline__ void multiply(float (&acc)[1][4], uint32_t stage, int lane) const { q4_step<T, NG, ZEROS>(acc[0], stage, row_at, lane); }
+  __device__ static __forceinline__ int column(int, int c, int lane) { return (lane >> 2) + 8 * (c >> 1); }
+  __device__ static __forceinline__ int width(int, int) { return kCols; }
+};
+
+template <typename F> struct FewPlan {
+  static constexpr int kRing = F::kDepth * F::kStage;
+  static constexpr int kParts = kFewWarps * kRing;                                   // the warps' sums of a unit: [warp][row][column]
+  static constexpr int kTotal = kParts + kFewWarps * kFewRows * F::kCols * 4;
+  static_assert(kFewWarps * (kFewExperts + kFewGroups) * 4 <= kParts && kFewWarps * kFewExperts + 4 * kFewExperts <= kParts, "the router's keys lie where the rings will be");
+};
+
+// The units of one product.  A warp's copies run ahead of its products by up to kDepth - 1 steps, into the next units, so that nothing
+// waits for memory while a unit's sums are joined.
+template <typename F> struct FewWalk {
+  const FewMatrix m;
+  const FewRouting& r;
+  const uint16_t* source;  // the rows, and which of them belong to the entries' slots
+  const int16_t* which;
+  int bundles, units;  // a bundle: the tiles of a unit
+  uint32_t ring;
+  int warp, lane;
+  // where the copies are
+  F f;
+  int unit, step, end, count;
+  uint32_t to;
+
+  // the entry, this warp's tile (maybe behind the last) and its steps [begin, stop)
+  __device__ __forceinline__ void place(int u, int& entry, int& bundle, int& share) const {
+    entry = u / (bundles * m.shares);
+    const int rest = u - entry * bundles * m.shares;
+    share = rest / bundles;
+    bundle = rest - share * bundles;
+  }
+  __device__ __forceinline__ int tile_of(int bundle) const { return bundle * (kFewWarps / m.team) + warp / m.team; }
+  __device__ __forceinline__ void steps_of(int tile, int share, int& begin, int& stop) const {
+    begin = m.steps * share / m.shares + warp % m.team;
+    stop = tile * m.cols < m.N ? m.steps * (share + 1) / m.shares : 0;
+  }
+  __device__ __forceinline__ void seek() {  // the unit's first step of this warp's, or the next unit that has one
+    while (unit < units) {
+      int n, bundle, share;
+      place(unit, n, bundle, share);
+      const int tile = tile_of(bundle);
+      steps_of(tile, share, step, end);
+      if (step < end) {
+        count = r.count[n];
+        const int first = r.first[n];
+        f.set(m, r.expert[n], tile, step, [&](int i) { return source + static_cast<int64_t>(which[first + i]) * m.K; }, count, lane);
+        return;
+      }
+      unit += gridDim.x;
+    }
+  }
+  __device__ __forceinline__ void start() {
+    unit = blockIdx.x;
+    to = ring;
+    seek();
+  }
+  __device__ __forceinline__ void advance() {
+    step += m.team;
+    if (step < end) {
+      f.next(m.team);
+    } else {
+      unit += gridDim.x;
+      seek();
+    }
+    to = to == ring + (F::kDepth - 1) * F::kStage ? ring : to + F::kStage;
+  }
+  __device__ __forceinline__ void copy_weights() const { if (unit < units) f.copy(to, step, lane); }
+  __device__ __forceinline__ void copy_rows() const { if (unit < units) f.copy_rows(to, count, step, lane); }
+};
+
+template <typename T, typename F>
 __global__ void __launch_bounds__(kFewThreads, kFewCtas) few_experts_kernel(const FewArgs a) {
-  using P = FewPlan<BITS, NG, ZEROS>;
+  using P = FewPlan<F>;
+  constexpr bool WIDE = F::kCols == 64;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ FewRouting r;
+  float* const parts = reinterpret_cast<float*>(smem + P::kParts);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, t4 = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * P::kRing;
-  const auto part = [&](int w, int row, int col) -> float& { return reinterpret_cast<float*>(smem + w * P::kRing)[row * P::kCols + col]; };
   route<T>(a, r, reinterpret_cast<float*>(smem));
   const bool gated = a.act == MOE_ACT_SWIGLU || a.act == MOE_ACT_GEGLU;
   const int slots = a.T * a.k;
-
-  // One unit: entry n's rows by a tile of its expert's matrix over steps [begin, end); `source` gives the row of a slot.  Leaves the
-  // warps' sums in their rings.
-  const auto product = [&](int n, int tile, const void* w16, const Q4Matrix& w4, int64_t tiles4, int K, int N, int begin, int end, auto source) {
-    const int count = r.count[n];
-    const int e = r.expert[n];
-    const uint16_t* x0 = g < count ? source(r.slot[n][g]) : nullptr;
-    const uint16_t* x1 = g + 8 < count ? source(r.slot[n][g + 8]) : nullptr;
-    if constexpr (BITS == 4) {
-      Q4Matrix w = w4;
-      w.steps = end;
-      const int64_t at = e * tiles4 + tile;
-      const uint4* data = w4.data + at * w4.steps * kQ4Words;
-      w.data = data;
-      w.scales = static_cast<const uint16_t*>(w4.scales) + at * w4.steps * (kQ4Rows * NG);
-      w.zeros = ZEROS ? w4.zeros + at * w4.steps * (kQ4Rows * NG) : nullptr;
-      const auto leave = [&](const auto& acc, int m) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int row = 8 * m + 2 * t4 + (c & 1);
-          if (row < count) part(warp, row, g + 8 * (c >> 1)) = acc[c];
-        }
-      };
-      if (count <= 8) {
-        float acc[1][4] = {};
-        const uint16_t* const x[1] = {x0};
-        q4_tile<T, NG, ZEROS, 1, P::kDepth>(acc, w, 0, x, K, begin + warp, kFewWarps, ring, lane);
-        leave(acc[0], 0);
-      } else {
-        float acc[2][4] = {};
-        const uint16_t* const x[2] = {x0, x1};
-        q4_tile<T, NG, ZEROS, 2, P::kDepth>(acc, w, 0, x, K, begin + warp, kFewWarps, ring, lane);
-        leave(acc[0], 0);
-        leave(acc[1], 1);
+  // All units of a product whose first copies are under way; `give` takes the sums of a unit's tiles: (entry, tile, its place in the
+  // bundle, share, total(row, column)).
+  const auto walk = [&](FewWalk<F>& c, auto give) {
+    F f;
+    uint32_t from = ring;
+    const int team = c.m.team;
+    for (int unit = blockIdx.x; unit < c.units; unit += gridDim.x) {
+      int n, bundle, share, step, end;
+      c.place(unit, n, bundle, share);
+      c.steps_of(c.tile_of(bundle), share, step, end);
+      const int count = r.count[n];
+      f.read(count, lane);
+      float acc[F::kProducts][4] = {};
+      for (; step < end; step += team) {
+        copies_wait<F::kDepth - 2>();
+        __syncwarp();  // every lane's copies of this step, and every lane is through with the stage that is filled next
+        c.copy_weights();
+        c.copy_rows();
+        copies_commit();
+        c.advance();
+        f.multiply(acc, from, lane);
+        from = from == ring + (F::kDepth - 1) * F::kStage ? ring : from + F::kStage;
       }
-    } else {
-      float acc[8][4] = {};
-      wide_tile<T>(acc, static_cast<const uint16_t*>(w16) + static_cast<int64_t>(e) * K * N, K, N, tile * kWideCols, x0, x1, begin + warp, end, kFewWarps, ring,
-                   lane);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int q = 0; q < F::kProducts; ++q)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int row = g + 8 * (c >> 1);
-          if (row < count) part(warp, row, 8 * (2 * t4 + (c & 1)) + j) = acc[j][c];
+        for (int i = 0; i < 4; ++i) {
+          const int row = 2 * (lane & 3) + (i & 1);
+          if (row < count) parts[(warp * kFewRows + row) * F::kCols + F::column(q, i, lane)] = acc[q][i];
         }
+      __syncthreads();
+      give(n, bundle * (kFewWarps / team), kFewWarps / team, share, [&](int place, int row, int col) {
+        float v = 0.0f;
+        const float* p = parts + (place * team * kFewRows + row) * F::kCols + col;
+        for (int w = 0; w < team; ++w) v += p[w * kFewRows * F::kCols];
+        return v;
+      });
+      __syncthreads();
     }
-    __syncthreads();
+    copies_wait<0>();
+    __syncwarp();
   };
-  const auto total = [&](int row, int col) {
-    float v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) v += part(w, row, col);
-    return v;
+  const auto open = [&](const FewMatrix& m, const uint16_t* source, const int16_t* which) {
+    const int tiles = (m.N + m.cols - 1) / m.cols;
+    const int bundles = (tiles * m.team + kFewWarps - 1) / kFewWarps;
+    FewWalk<F> c{m, r, source, which, bundles, r.entries * bundles * m.shares, ring, warp, lane};
+    c.start();
+    return c;
   };
 
-  {  // up: units (entry, tile)
+  {
     const int N = gated ? 2 * a.I : a.I;
-    const int tiles = (N + P::kCols - 1) / P::kCols;
-    const int steps = BITS == 4 ? a.up.steps : (a.d + kWideStep - 1) / kWideStep;
-    for (int unit = blockIdx.x; unit < r.entries * tiles; unit += gridDim.x) {
-      const int n = unit / tiles, tile = unit - n * tiles;
-      product(n, tile, a.w1, a.up, a.up.tiles, a.d, N, 0, steps,
-              [&](int slot) { return static_cast<const uint16_t*>(a.x) + static_cast<int64_t>(slot / a.k) * a.d; });
-      const int cols = gated ? P::kCols / 2 : P::kCols;
-      for (int at = tid; at < r.count[n] * cols; at += kFewThreads) {
-        const int row = at / cols, c = at - row * cols;
-        const int i = tile * cols + c;
+    FewMatrix up{a.w1, a.up, a.d, N, (a.d + F::kStep - 1) / F::kStep, F::width(r.entries, N), kFewWarps, 1};
+    if (!WIDE) share_out(up, r.entries, 1, F::kCost);
+    auto c = open(up, static_cast<const uint16_t*>(a.x), r.token);
+#pragma unroll
+    for (int s = 0; s < F::kDepth - 1; ++s) {
+      c.copy_weights();
+      c.copy_rows();
+      copies_commit();
+      c.advance();
+    }
+    const int cols = gated ? up.cols / 2 : up.cols;
+    walk(c, [&](int n, int tile, int tiles, int, auto total) {
+      const int count = r.count[n];
+      for (int at = tid; at < count * cols * tiles; at += kFewThreads) {
+        const int row = at / (cols * tiles), rest = at - row * cols * tiles;
+        const int place = rest / cols, col = rest - place * cols;
+        const int i = tile * cols + rest;
         if (i >= a.I) continue;
         float v;
-        if (gated) v = BITS == 4 ? few_act(total(row, c), a.act) * total(row, c + 8) : few_act(total(row, 2 * c), a.act) * total(row, 2 * c + 1);
-        else v = few_act(total(row, c), a.act);
+        if (gated) v = WIDE ? few_act(total(place, row, 2 * col), a.act) * total(place, row, 2 * col + 1) : few_act(total(place, row, col), a.act) * total(place, row, col + 8);
+        else v = few_act(total(place, row, col), a.act);
         const T h = Elem<T>::from_float(v);
-        a.hidden[static_cast<int64_t>(r.slot[n][row]) * a.I + i] = *reinterpret_cast<const uint16_t*>(&h);
+        a.hidden[static_cast<int64_t>(r.slot[r.first[n] + row]) * a.I + i] = *reinterpret_cast<const uint16_t*>(&h);
       }
-      __syncthreads();
-    }
+    });
   }
-  if (!meet(a, 1, &r.go_on)) return;
 
-  int shares = 1;  // of the depth of the down product: enough units for every CTA to have some
+  FewMatrix down{a.w2, a.down, a.I, a.d, (a.I + F::kStep - 1) / F::kStep, F::kCols, kFewWarps, 1};
+  share_out(down, r.entries, kFewParts, F::kCost);
+  const int shares = down.shares;
   {
-    const int tiles = (a.d + P::kCols - 1) / P::kCols;
-    const int steps = BITS == 4 ? a.down.steps : (a.I + kWideStep - 1) / kWideStep;
-    while (shares < kFewParts && r.entries * tiles * shares < 2 * static_cast<int>(gridDim.x) && steps >= 2 * kFewWarps * shares) shares *= 2;
-    for (int unit = blockIdx.x; unit < r.entries * tiles * shares; unit += gridDim.x) {
-      const int n = unit / (tiles * shares), rest = unit - n * tiles * shares;
-      const int share = rest / tiles, tile = rest - share * tiles;
-      product(n, tile, a.w2, a.down, a.down.tiles, a.I, a.d, steps * share / shares, steps * (share + 1) / shares,
-              [&](int slot) { return a.hidden + static_cast<int64_t>(slot) * a.I; });
-      for (int at = tid; at < r.count[n] * P::kCols; at += kFewThreads) {
-        const int row = at / P::kCols, c = at - row * P::kCols;
-        const int i = tile * P::kCols + c;
-        if (i < a.d) a.rows[(static_cast<int64_t>(share) * slots + r.slot[n][row]) * a.d + i] = total(row, c);
-      }
-      __syncthreads();
+    // the first weights of the down product are asked for before the wait for the rows that they multiply
+    auto ahead = open(down, a.hidden, r.slot);
+    auto c = ahead;
+#pragma unroll
+    for (int s = 0; s < F::kDepth - 1; ++s) {
+      ahead.copy_weights();
+      ahead.advance();
     }
+    if (!meet(a, 1, &r.go_on)) {
+      copies_wait<0>();
+      return;
+    }
+#pragma unroll
+    for (int s = 0; s < F::kDepth - 1; ++s) {
+      c.copy_rows();
+      copies_commit();
+      c.advance();
+    }
+    walk(c, [&](int n, int tile, int tiles, int share, auto total) {
+      const int count = r.count[n], cols = F::kCols * tiles;
+      for (int at = tid; at < count * cols; at += kFewThreads) {
+        const int row = at / cols, rest = at - row * cols;
+        const int i = tile * F::kCols + rest;
+        if (i < a.d) a.rows[(static_cast<int64_t>(share) * slots + r.slot[r.first[n] + row]) * a.d + i] = total(rest / F::kCols, row, rest % F::kCols);
+      }
+    });
   }
   if (!meet(a, 2, &r.go_on)) return;
 
   for (int at = blockIdx.x * kFewThreads + tid; at < a.T * a.d; at += gridDim.x * kFewThreads) {
     const int t = at / a.d, i = at - t * a.d;
     float v = a.addend != nullptr ? to_f32<T>(static_cast<const T*>(a.addend)[at]) : 0.0f;
-    for (int s = 0; s < a.k; ++s) {
-      const int slot = t * a.k + s;
-      if (r.id[slot] < 0) continue;
-      float row = 0.0f;
-      for (int p = 0; p < shares; ++p) row += a.rows[(static_cast<int64_t>(p) * slots + slot) * a.d + i];
-      v = fmaf(r.score[slot], row, v);
+    const float* from = a.rows + static_cast<int64_t>(t) * a.k * a.d + i;
+    const int64_t share = static_cast<int64_t>(slots) * a.d;
+    for (int s0 = 0; s0 < a.k; s0 += 4) {  // four slots' loads at once
+      float part[4][kFewParts];
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int p = 0; p < kFewParts; ++p)
+          part[s][p] = s0 + s < a.k && p < shares && r.id[t * a.k + s0 + s] >= 0 ? from[(s0 + s) * static_cast<int64_t>(a.d) + p * share] : 0.0f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        float row = part[s][0];
+#pragma unroll
+        for (int p = 1; p < kFewParts; ++p) row += part[s][p];
+        if (s0 + s < a.k && r.id[t * a.k + s0 + s] >= 0) v = fmaf(r.score[t * a.k + s0 + s], row, v);
+      }
     }
     static_cast<T*>(a.out)[at] = Elem<T>::from_float(v);
   }
 }
 
 template <typename T, typename W, int TT> static int launch_head(const HeadArgs& a, cudaStream_t s) {
+  const auto kernel = few_head_kernel<T, W, TT>;
+  static std::atomic<bool> prepared[64];
+  int dev = 0;
+  MOE_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !prepared[dev].load(std::memory_order_acquire)) {
+    MOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TT * kHeadMost / kHeadRanks * 4));
+    if (dev < 64) prepared[dev].store(true, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   const int tiles = a.router == nullptr ? 1 : (a.E + kHeadCols - 1) / kHeadCols;
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * kHeadRanks), 1, 1);
   cfg.blockDim = dim3(kFewThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(TT) * ((a.d + kHeadRanks * 8 - 1) / (kHeadRanks * 8) * 8) * 4;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -612,7 +864,7 @@ template <typename T, typename W, int TT> static int launch_head(const HeadArgs&
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  MOE_CUDA(cudaLaunchKernelEx(&cfg, few_head_kernel<T, W, TT>, a));
+  MOE_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   return MOE_OK;
 }
 template <typename T, typename W> static int launch_head_tokens(const HeadArgs& a, cudaStream_t s) {
@@ -622,16 +874,16 @@ template <typename T, typename W> static int launch_head_tokens(const HeadArgs& 
 }
 
 // One wave: what of the grid's CTAs fit at once, at most kFewCtas per SM.
-template <typename T, int BITS, int NG, bool ZEROS> static int launch_experts(const FewArgs& a, cudaStream_t s) {
-  using P = FewPlan<BITS, NG, ZEROS>;
-  const auto kernel = few_experts_kernel<T, BITS, NG, ZEROS>;
+template <typename T, typename F> static int launch_experts(const FewArgs& a, cudaStream_t s) {
+  constexpr int smem = FewPlan<F>::kTotal;
+  const auto kernel = few_experts_kernel<T, F>;
   static std::atomic<int> resident[64];
   int dev = 0;
   MOE_CUDA(cudaGetDevice(&dev));
   int ctas = dev < 64 ? resident[dev].load(std::memory_order_acquire) : 0;
   if (ctas == 0) {
-    MOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kTotal));
-    MOE_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, kFewThreads, P::kTotal));
+    MOE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    MOE_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, kFewThreads, smem));
     MOE_CHECK_ARG(ctas > 0, "moe_few_tokens: the kernel does not fit on an SM");
     if (ctas > kFewCtas) ctas = kFewCtas;
     if (dev < 64) resident[dev].store(ctas, std::memory_order_release);
@@ -639,7 +891,7 @@ template <typename T, int BITS, int NG, bool ZEROS> static int launch_experts(co
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas * sm_count()), 1, 1);
   cfg.blockDim = dim3(kFewThreads, 1, 1);
-  cfg.dynamicSmemBytes = P::kTotal;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeCooperative;
@@ -649,12 +901,11 @@ template <typename T, int BITS, int NG, bool ZEROS> static int launch_experts(co
   MOE_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   return MOE_OK;
 }
-template <typename T> static int launch_experts_of(const FewArgs& a, int bits, int group, cudaStream_t s) {
-  if (bits == 16) return launch_experts<T, 16, 1, false>(a, s);
-  const bool z = a.up.zeros != nullptr;
-  if (group == 128) return z ? launch_experts<T, 4, 1, true>(a, s) : launch_experts<T, 4, 1, false>(a, s);
-  if (group == 64) return z ? launch_experts<T, 4, 2, true>(a, s) : launch_experts<T, 4, 2, false>(a, s);
-  return z ? launch_experts<T, 4, 4, true>(a, s) : launch_experts<T, 4, 4, false>(a, s);
+template <typename T> static int launch_experts_of(const FewArgs& a, int bits, int group, bool z, cudaStream_t s) {
+  if (bits == 16) return launch_experts<T, FewWide<T>>(a, s);
+  if (group == 128) return z ? launch_experts<T, FewFour<T, 1, true>>(a, s) : launch_experts<T, FewFour<T, 1, false>>(a, s);
+  if (group == 64) return z ? launch_experts<T, FewFour<T, 2, true>>(a, s) : launch_experts<T, FewFour<T, 2, false>>(a, s);
+  return z ? launch_experts<T, FewFour<T, 4, true>>(a, s) : launch_experts<T, FewFour<T, 4, false>>(a, s);
 }
 
 static int64_t few_up(int64_t n) { return (n + 255) / 256 * 256; }
@@ -697,6 +948,10 @@ extern "C" int moe_few_tokens(const moe_few_pass* p, void* stream) {
     set_error("moe_few_tokens: d=%d and inter=%d must be multiples of 8", p->d, p->inter);
     return MOE_ERR_UNSUPPORTED;
   }
+  if ((p->router_w != nullptr || p->norm_w != nullptr) && p->d > kHeadMost) {
+    set_error("moe_few_tokens: norm and router take rows of at most %d, got %d", kHeadMost, p->d);
+    return MOE_ERR_UNSUPPORTED;
+  }
   MOE_CHECK_ARG(p->dtype == MOE_DTYPE_BF16 || p->dtype == MOE_DTYPE_F16, "moe_few_tokens: unknown dtype %d", p->dtype);
   MOE_CHECK_ARG(p->act >= MOE_ACT_NONE && p->act <= MOE_ACT_GELU_TANH, "moe_few_tokens: unknown activation %d", p->act);
   MOE_CHECK_ARG(p->bits == 16 || (p->bits == 4 && (p->group == 32 || p->group == 64 || p->group == 128)),
@@ -715,11 +970,9 @@ extern "C" int moe_few_tokens(const moe_few_pass* p, void* stream) {
                 "moe_few_tokens: unknown router options");
   if (p->num_tokens == 0) return MOE_OK;
   MOE_CHECK_ARG(p->x && p->w1 && p->w2 && p->out && p->workspace, "moe_few_tokens: null pointer argument");
-  MOE_CHECK_ARG(p->bits == 16 || (p->w1_scales && p->w2_scales && (p->w1_zeros == nullptr) == (p->w2_zeros == nullptr)),
-                "moe_few_tokens: 4-bit weights have scales, and both zero points or none");
   MOE_CHECK_ARG(p->residual == nullptr || (p->norm_w != nullptr && p->stream_out != nullptr), "moe_few_tokens: a residual goes with a norm and the stream");
   uintptr_t all = 0;
-  for (const void* q : {p->x, p->residual, p->norm_w, p->w1, p->w1_scales, p->w1_zeros, p->w2, p->w2_scales, p->w2_zeros, p->router_w, p->addend,
+  for (const void* q : {p->x, p->residual, p->norm_w, p->w1, p->w2, p->router_w, p->addend,
                         static_cast<const void*>(p->out), static_cast<const void*>(p->stream_out), static_cast<const void*>(p->workspace)})
     all |= reinterpret_cast<uintptr_t>(q);
   MOE_CHECK_ARG((all & 15) == 0, "moe_few_tokens: pointers must be 16-byte aligned");
@@ -763,11 +1016,11 @@ extern "C" int moe_few_tokens(const moe_few_pass* p, void* stream) {
   a.w2 = p->w2;
   if (p->bits == 4) {
     const bool glu = p->act == MOE_ACT_SWIGLU || p->act == MOE_ACT_GEGLU;
-    const auto matrix = [&](const void* data, const void* scales, const void* zeros, int n, int k) {
-      return Q4Matrix{static_cast<const uint4*>(data), scales, static_cast<const uint8_t*>(zeros), (n + kQ4Rows - 1) / kQ4Rows, (k + kQ4Step - 1) / kQ4Step};
+    const auto matrix = [&](const void* data, int n, int k) {
+      return Q4Matrix{static_cast<const uint8_t*>(data), (n + kQ4Rows - 1) / kQ4Rows, (k + kQ4Step - 1) / kQ4Step};
     };
-    a.up = matrix(p->w1, p->w1_scales, p->w1_zeros, glu ? 2 * p->inter : p->inter, p->d);
-    a.down = matrix(p->w2, p->w2_scales, p->w2_zeros, p->d, p->inter);
+    a.up = matrix(p->w1, glu ? 2 * p->inter : p->inter, p->d);
+    a.down = matrix(p->w2, p->d, p->inter);
   }
   a.hidden = reinterpret_cast<uint16_t*>(ws + sp.hidden);
   a.rows = reinterpret_cast<float*>(ws + sp.rows);
@@ -788,5 +1041,6 @@ extern "C" int moe_few_tokens(const moe_few_pass* p, void* stream) {
   a.keep = p->topk_groups;
   a.best = p->group_best;
   a.scale = p->scale;
-  return bf16 ? launch_experts_of<__nv_bfloat16>(a, p->bits, p->group, s) : launch_experts_of<__half>(a, p->bits, p->group, s);
+  return bf16 ? launch_experts_of<__nv_bfloat16>(a, p->bits, p->group, p->zeros != 0, s)
+              : launch_experts_of<__half>(a, p->bits, p->group, p->zeros != 0, s);
 }

@@ -1,6 +1,6 @@
 // A few 16-bit rows by one matrix of 4-bit weights (int4.cuh): out [rows, N] = x [rows, K] @ w [N, K]^T.
 //
-// A CTA takes one tile of 16 weight rows and up to 8 MT rows of x; its eight warps share the steps of K, and where there are few tiles,
+// A CTA takes one tile of 16 weight rows and up to eight rows of x; its eight warps share the steps of K, and where there are few tiles,
 // so do the CTAs of a cluster.  Their sums are joined in a fixed order, through shared memory and then the cluster's.
 #include "int4.cuh"
 
@@ -9,7 +9,7 @@
 namespace moe {
 
 constexpr int kQ4Warps = 8;
-constexpr int kQ4Depth = 5;   // steps that a warp has room for: 3 CTAs per SM ask for 100 KB at a time
+constexpr int kQ4Depth = 4;   // steps that a warp has room for: 2 CTAs per SM ask for 50 KB of weights at a time
 template <int NG, bool ZEROS> constexpr int kQ4Ring = kQ4Depth * Q4Stage<NG, ZEROS>::kBytes;
 
 struct Q4Args {
@@ -25,70 +25,69 @@ __device__ __forceinline__ float load_cluster(uint32_t addr) {
   return v;
 }
 
-template <typename T, int NG, bool ZEROS, int MT>
-__global__ void __launch_bounds__(kQ4Warps * 32, MT <= 2 ? 3 : 2) q4_rows_kernel(const Q4Args a) {
-  constexpr int TOKENS = 8 * MT;
+template <typename T, int NG, bool ZEROS>
+__global__ void __launch_bounds__(kQ4Warps * 32, 2) q4_rows_kernel(const Q4Args a) {
+  constexpr int kStage = Q4Stage<NG, ZEROS>::kBytes, TOKENS = 8;
   extern __shared__ __align__(128) uint8_t rings[];
   __shared__ float parts[kQ4Warps][TOKENS][kQ4Rows];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = a.ranks > 1 ? static_cast<int>(blockIdx.x) % a.ranks : 0;
   const int64_t tile = blockIdx.x / a.ranks;
-  const int row0 = blockIdx.y * TOKENS;
-  const uint16_t* x[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int row = row0 + 8 * m + (lane >> 2);
-    x[m] = row < a.rows ? a.x + static_cast<int64_t>(row) * a.K : nullptr;
-  }
-  float acc[MT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.0f;
-  q4_tile<T, NG, ZEROS, MT, kQ4Depth>(acc, a.w, tile, x, a.K, rank * kQ4Warps + warp, a.ranks * kQ4Warps,
-                                          smem_u32(rings) + warp * kQ4Ring<NG, ZEROS>, lane);
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) parts[warp][8 * m + 2 * (lane & 3) + (c & 1)][(lane >> 2) + 8 * (c >> 1)] = acc[m][c];
-  __syncthreads();
-  constexpr int PER = TOKENS * kQ4Rows / (kQ4Warps * 32) > 0 ? TOKENS * kQ4Rows / (kQ4Warps * 32) : 1;
-  float sum[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int at = threadIdx.x + i * kQ4Warps * 32;
-    sum[i] = 0.0f;
-    if (at < TOKENS * kQ4Rows)
-      for (int v = 0; v < kQ4Warps; ++v) sum[i] += (&parts[v][0][0])[at];
-  }
-  if (a.ranks > 1) {  // the same for the whole grid
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (threadIdx.x + i * kQ4Warps * 32 < TOKENS * kQ4Rows) (&parts[0][0][0])[threadIdx.x + i * kQ4Warps * 32] = sum[i];
-    cluster_sync_all();
-    if (rank == 0) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int at = threadIdx.x + i * kQ4Warps * 32;
-        if (at < TOKENS * kQ4Rows)
-          for (int r = 1; r < a.ranks; ++r) sum[i] += load_cluster(mapa_shared(smem_u32(&(&parts[0][0][0])[at]), r));
-      }
+  const int row0 = blockIdx.y * TOKENS, count = min(a.rows - row0, TOKENS);
+  constexpr int kBlock = Q4Stage<NG, ZEROS>::kBlock;
+  const uint8_t* data = a.w.data + tile * a.w.steps * kBlock;
+  const auto row = [&](int i) { return a.x + static_cast<int64_t>(row0 + 2 * i + (lane >> 4)) * a.K; };
+  const uint32_t row_at = q4_row_at(count, lane);
+  const int stride = a.ranks * kQ4Warps;
+  int step = rank * kQ4Warps + warp, ahead = step;
+  const uint32_t ring = smem_u32(rings) + warp * kQ4Ring<NG, ZEROS>;
+  uint32_t to = ring, from = ring;
+  const auto copy = [&]() {
+    if (ahead < a.w.steps) {
+      q4_copy<NG, ZEROS>(to, data + static_cast<int64_t>(ahead) * kBlock, lane);
+      q4_copy_rows<NG, ZEROS>(to, row, count, a.K, ahead, lane);
     }
+    copies_commit();
+    ahead += stride;
+    to = to == ring + (kQ4Depth - 1) * kStage ? ring : to + kStage;
+  };
+#pragma unroll
+  for (int s = 0; s < kQ4Depth - 1; ++s) copy();
+  float acc[4] = {};
+  for (; step < a.w.steps; step += stride) {
+    copies_wait<kQ4Depth - 2>();
+    __syncwarp();  // every lane's copies of this step, and every lane is through with the stage that is filled next
+    copy();
+    q4_step<T, NG, ZEROS>(acc, from, row_at, lane);
+    from = from == ring + (kQ4Depth - 1) * kStage ? ring : from + kStage;
+  }
+  copies_wait<0>();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) parts[warp][2 * (lane & 3) + (c & 1)][(lane >> 2) + 8 * (c >> 1)] = acc[c];
+  __syncthreads();
+  float sum = 0.0f;
+  float* const mine = &parts[0][0][0] + tid;
+  if (tid < TOKENS * kQ4Rows)
+    for (int v = 0; v < kQ4Warps; ++v) sum += mine[v * TOKENS * kQ4Rows];
+  if (a.ranks > 1) {  // the same for the whole grid
+    if (tid < TOKENS * kQ4Rows) *mine = sum;
+    __syncthreads();
+    cluster_sync_all();
+    if (rank == 0 && tid < TOKENS * kQ4Rows)
+      for (int r = 1; r < a.ranks; ++r) sum += load_cluster(mapa_shared(smem_u32(mine), r));
+    __syncthreads();
     cluster_sync_all();  // the others' shared memory lives until it has been read
     if (rank != 0) return;
   }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int at = threadIdx.x + i * kQ4Warps * 32;
-    const int row = row0 + at / kQ4Rows, n = static_cast<int>(tile) * kQ4Rows + at % kQ4Rows;
-    if (at < TOKENS * kQ4Rows && row < a.rows && n < a.N) {
-      const T v = Elem<T>::from_float(sum[i]);
-      a.out[static_cast<int64_t>(row) * a.N + n] = *reinterpret_cast<const uint16_t*>(&v);
-    }
+  const int r = tid / kQ4Rows, n = static_cast<int>(tile) * kQ4Rows + tid % kQ4Rows;
+  if (r < count && n < a.N) {
+    const T v = Elem<T>::from_float(sum);
+    a.out[static_cast<int64_t>(row0 + r) * a.N + n] = *reinterpret_cast<const uint16_t*>(&v);
   }
 }
 
-template <typename T, int NG, bool ZEROS, int MT> static int launch_q4(const Q4Args& a, cudaStream_t s) {
-  const auto kernel = q4_rows_kernel<T, NG, ZEROS, MT>;
+template <typename T, int NG, bool ZEROS> static int launch_q4_rows(const Q4Args& a, cudaStream_t s) {
+  const auto kernel = q4_rows_kernel<T, NG, ZEROS>;
   constexpr int smem = kQ4Warps * kQ4Ring<NG, ZEROS>;
   static std::atomic<bool> prepared[64];
   int dev = 0;
@@ -98,7 +97,7 @@ template <typename T, int NG, bool ZEROS, int MT> static int launch_q4(const Q4A
     if (dev < 64) prepared[dev].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.w.tiles * a.ranks), static_cast<unsigned>((a.rows + 8 * MT - 1) / (8 * MT)), 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(a.w.tiles * a.ranks), static_cast<unsigned>((a.rows + 7) / 8), 1);
   cfg.blockDim = dim3(kQ4Warps * 32, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -112,13 +111,7 @@ template <typename T, int NG, bool ZEROS, int MT> static int launch_q4(const Q4A
   MOE_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   return MOE_OK;
 }
-template <typename T, int NG, bool ZEROS> static int launch_q4_rows(const Q4Args& a, cudaStream_t s) {
-  if (a.rows <= 8) return launch_q4<T, NG, ZEROS, 1>(a, s);
-  if (a.rows <= 16) return launch_q4<T, NG, ZEROS, 2>(a, s);
-  return launch_q4<T, NG, ZEROS, 4>(a, s);
-}
-template <typename T> static int launch_q4_groups(const Q4Args& a, int group, cudaStream_t s) {
-  const bool z = a.w.zeros != nullptr;
+template <typename T> static int launch_q4_groups(const Q4Args& a, int group, bool z, cudaStream_t s) {
   if (group == 128) return z ? launch_q4_rows<T, 1, true>(a, s) : launch_q4_rows<T, 1, false>(a, s);
   if (group == 64) return z ? launch_q4_rows<T, 2, true>(a, s) : launch_q4_rows<T, 2, false>(a, s);
   return z ? launch_q4_rows<T, 4, true>(a, s) : launch_q4_rows<T, 4, false>(a, s);
@@ -128,9 +121,9 @@ template <typename T> static int launch_q4_groups(const Q4Args& a, int group, cu
 
 using namespace moe;
 
-extern "C" int moe_int4_matmul(const void* x, const void* data, const void* scales, const void* zeros, void* out, int64_t rows, int k_dim, int n_dim,
-                               int group, int dtype, void* stream) {
-  MOE_CHECK_ARG(rows >= 0 && rows <= (1 << 20) && k_dim > 0 && n_dim > 0, "moe_int4_matmul: %lld rows (at most 2^20), K=%d, N=%d",
+extern "C" int moe_int4_matmul(const void* x, const void* data, void* out, int64_t rows, int k_dim, int n_dim, int group, int zeros, int dtype,
+                               void* stream) {
+  MOE_CHECK_ARG(rows >= 0 && rows <= (1 << 19) && k_dim > 0 && n_dim > 0, "moe_int4_matmul: %lld rows (at most 2^19), K=%d, N=%d",
                 static_cast<long long>(rows), k_dim, n_dim);
   MOE_CHECK_ARG(group == 32 || group == 64 || group == 128, "moe_int4_matmul: groups of 32, 64 or 128 columns, got %d", group);
   MOE_CHECK_ARG(dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16, "moe_int4_matmul: unknown dtype %d", dtype);
@@ -139,14 +132,10 @@ extern "C" int moe_int4_matmul(const void* x, const void* data, const void* scal
     return MOE_ERR_UNSUPPORTED;
   }
   if (rows == 0) return MOE_OK;
-  MOE_CHECK_ARG(x && data && scales && out, "moe_int4_matmul: null pointer argument");
-  MOE_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(scales) |
-                  reinterpret_cast<uintptr_t>(zeros)) & 15) == 0,
-                "moe_int4_matmul: pointers must be 16-byte aligned");
+  MOE_CHECK_ARG(x && data && out, "moe_int4_matmul: null pointer argument");
+  MOE_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(data)) & 15) == 0, "moe_int4_matmul: pointers must be 16-byte aligned");
   Q4Args a{};
-  a.w.data = static_cast<const uint4*>(data);
-  a.w.scales = scales;
-  a.w.zeros = static_cast<const uint8_t*>(zeros);
+  a.w.data = static_cast<const uint8_t*>(data);
   a.w.tiles = (n_dim + kQ4Rows - 1) / kQ4Rows;
   a.w.steps = (k_dim + kQ4Step - 1) / kQ4Step;
   a.x = static_cast<const uint16_t*>(x);
@@ -155,9 +144,9 @@ extern "C" int moe_int4_matmul(const void* x, const void* data, const void* scal
   a.K = k_dim;
   a.N = n_dim;
   // CTAs share a tile's steps while SMs would stay idle and each of their warps has two steps
-  const int64_t row_blocks = rows <= 16 ? 1 : (rows + 31) / 32;
+  const int64_t row_blocks = (rows + 7) / 8;
   a.ranks = 1;
   while (a.ranks < 8 && a.w.tiles * row_blocks * a.ranks < 2ll * sm_count() && a.w.steps >= 4 * kQ4Warps * a.ranks) a.ranks *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == MOE_DTYPE_BF16 ? launch_q4_groups<__nv_bfloat16>(a, group, s) : launch_q4_groups<__half>(a, group, s);
+  return dtype == MOE_DTYPE_BF16 ? launch_q4_groups<__nv_bfloat16>(a, group, zeros != 0, s) : launch_q4_groups<__half>(a, group, zeros != 0, s);
 }

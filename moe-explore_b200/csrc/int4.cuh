@@ -1,11 +1,11 @@
 // Products of a few 16-bit rows with 4-bit weights: element [n, k] = (value - zero) * scale, a value of 0 to 15, scale (in the rows' type)
 // and zero (8 where there is none) per row n and group of 32, 64 or 128 columns.
 //
-// Layout.  A matrix [N, K] is cut into tiles of 16 rows and steps of 128 columns; a step of a tile is 1 KB, the steps of a tile lie one
-// behind the other, so that a warp's loads are whole lines of one stream.  Byte (half * 32 + lane) * 16 + i * 4 + b of a step belongs to
-// row (lane / 4) + 8 half and word i of that lane: columns 32 i + 8 (lane % 4) + 0..7, the even ones in the word's low half and the odd
-// ones in the high half, lowest column lowest.  Scales (and zeros) of a step: [16 rows][groups of the step].  Rows behind N and columns
-// behind K hold zeros, values and scales.
+// Layout.  A matrix [N, K] is cut into tiles of 16 rows and steps of 128 columns; a step of a tile is one block, 1 KB of values, then the
+// scales, then the zeros, and the steps of a tile lie one behind the other, so that a warp reads one stream.  Byte (half * 32 + lane) * 16
+// + i * 4 + b of the values belongs to row (lane / 4) + 8 half and word i of that lane: columns 32 i + 8 (lane % 4) + 0..7, the even ones in
+// the word's low half and the odd ones in the high half, lowest column lowest.  Scales and zeros: [16 rows][groups of the step].  Rows
+// behind N and columns behind K hold zeros, values and scales.
 //
 // A step's fragments.  m16n8k16 with the weights as its 16 rows and eight tokens as its columns: the sums over k may take the columns in
 // any order, as long as both operands do, and in the order above (word >> 4 j) & 0x000F000F is the pair of columns 2 j, 2 j + 1 of a
@@ -13,8 +13,8 @@
 // bits of 128 (bf16) or 1024 (fp16), whose last mantissa bits it then is, and subtracting 128 + zero (1024 + zero), exactly.  Word i
 // holds columns of one group of 32 for all lanes, so the scale is applied to the fp32 sums of a group: no weight is ever rounded.
 //
-// Bound by HBM for up to 16 rows.  (Tensor cores by mma.sync because the weights are made in registers and M is 16: per KB of weights a
-// warp issues 88 instructions to make them and 8 to multiply.)
+// Tensor cores by mma.sync, because the weights are made in registers and there are only 16 of their rows: per KB of weights a warp issues 88
+// instructions to make them and 8 to multiply; the 56 integer ones among them are what bounds the rate beside HBM.
 #pragma once
 
 #include "common.cuh"
@@ -41,16 +41,18 @@ template <> __device__ __forceinline__ void mma_16x8x16<__half>(float (&c)[4], c
 __device__ __forceinline__ void copy_16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// The same, or 16 zero bytes (nothing is read then).
+__device__ __forceinline__ void copy_16_or_zeros(uint32_t to, const void* from, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // All but the last N groups of this thread's copies have landed.
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// One matrix, as the kernels see it.
+// One matrix (a matrix per expert follows), as the kernels see it: [tiles][steps][block].
 struct Q4Matrix {
-  const uint4* data;     // [tiles][steps][64]
-  const void* scales;    // [tiles][steps][16][NG], NG = 128 / group
-  const uint8_t* zeros;  // the same, or null
-  int64_t tiles;         // of the whole matrix (a matrix per expert follows)
+  const uint8_t* data;
+  int64_t tiles;
   int steps;
 };
 
@@ -70,19 +72,32 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b, __half) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// A step in shared memory: the words, each lane's copied by itself, then scales and zeros, copied by the first lanes.
+// A step in shared memory: its block, then the same columns of eight tokens' rows, 256 bytes each, their 16-byte pieces turned by four in
+// every second row (so that the eight lanes of a load that are served at once read two rows without a conflict).
 template <int NG, bool ZEROS> struct Q4Stage {
-  static constexpr int kScales = 1024, kZeros = kScales + 32 * NG, kBytes = kZeros + (ZEROS ? 16 * NG : 0);
+  static constexpr int kScales = 1024, kZeros = kScales + 32 * NG, kBlock = kZeros + (ZEROS ? 16 * NG : 0), kRows = kBlock, kBytes = kRows + 2048;
 };
-template <int NG, bool ZEROS>
-__device__ __forceinline__ void q4_copy(uint32_t stage, const uint4* data, const uint16_t* scales, const uint8_t* zeros, int step, int lane) {
-  using S = Q4Stage<NG, ZEROS>;
-  const uint4* from = data + static_cast<int64_t>(step) * kQ4Words + lane;
-  copy_16(stage + lane * 16, from);
-  copy_16(stage + 512 + lane * 16, from + 32);
-  const int64_t at = static_cast<int64_t>(step) * (kQ4Rows * NG);
-  if (lane < 2 * NG) copy_16(stage + S::kScales + lane * 16, scales + at + lane * 8);
-  else if (ZEROS && lane < 3 * NG) copy_16(stage + S::kZeros + (lane - 2 * NG) * 16, zeros + at + (lane - 2 * NG) * 16);
+template <int NG, bool ZEROS> __device__ __forceinline__ void q4_copy(uint32_t stage, const uint8_t* block, int lane) {
+  const uint8_t* from = block + lane * 16;
+  const uint32_t to = stage + lane * 16;
+  copy_16(to, from);
+  copy_16(to + 512, from + 512);
+  if (lane < (ZEROS ? 3 : 2) * NG) copy_16(to + 1024, from + 1024);
+}
+// The rows' part: row(r) gives row r < count, for lanes 0..15 even rows, for the others odd ones.
+template <int NG, bool ZEROS, typename Row>
+__device__ __forceinline__ void q4_copy_rows(uint32_t stage, Row row, int count, int K, int step, int lane) {
+  const int piece = lane & 15, odd = lane >> 4, k = step * kQ4Step + 8 * piece;
+  const bool real = k < K;
+  const uint32_t to = stage + Q4Stage<NG, ZEROS>::kRows + odd * 256 + ((piece ^ (odd << 2)) << 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (2 * i >= count) break;
+    if (2 * i + odd < count) {
+      const uint16_t* x = row(i);
+      copy_16_or_zeros(to + i * 512, real ? x + k : x, real);
+    }
+  }
 }
 // What a lane takes of a step: its words of rows g and g + 8, and their scales and zeros.
 template <int NG, bool ZEROS> struct Q4Piece {
@@ -135,21 +150,22 @@ template <typename T> __device__ __forceinline__ float q4_scale(const uint32_t* 
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// The other operand of word i: eight columns of token 8 m + lane / 4.  x: that token's row, or null.
-__device__ __forceinline__ uint4 q4_row(const uint16_t* x, int K, int step, int i, int lane) {
-  const int k = step * kQ4Step + 32 * i + 8 * (lane & 3);
-  return x != nullptr && k < K ? *reinterpret_cast<const uint4*>(x + k) : make_uint4(0, 0, 0, 0);
+// Where a lane finds the other operand of word 0: eight columns of token lane / 4 (of the first one behind the last: its products are
+// nobody's); of word i at this ^ 64 (i & 1) + 128 (i / 2).
+__device__ __forceinline__ uint32_t q4_row_at(int count, int lane) {
+  const int g = lane >> 2, r = g < count ? g : 0;
+  return r * 256 + (((lane & 3) ^ ((r & 1) << 2)) << 4);
 }
 
-// acc[m][..] += the tile's product over one step, by groups.
-template <typename T, int NG, bool ZEROS, int MT>
-__device__ __forceinline__ void q4_step(float (&acc)[MT][4], const Q4Piece<NG, ZEROS>& p, const uint16_t* const (&x)[MT], int K, int step, int lane) {
+// acc += the tile's product with up to eight rows over one step, by groups.
+template <typename T, int NG, bool ZEROS>
+__device__ __forceinline__ void q4_step(float (&acc)[4], uint32_t stage, uint32_t row_at, int lane) {
   constexpr int kPerGroup = 4 / NG;  // words
+  Q4Piece<NG, ZEROS> p;
+  q4_take<NG, ZEROS>(p, stage, lane);
 #pragma unroll
   for (int j = 0; j < NG; ++j) {
-    float sum[MT][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) sum[m][0] = sum[m][1] = sum[m][2] = sum[m][3] = 0.0f;
+    float sum[4] = {};
     uint32_t bias[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -172,53 +188,16 @@ __device__ __forceinline__ void q4_step(float (&acc)[MT][4], const Q4Piece<NG, Z
           a[q >> 1][2 * (q & 1) + h] = sub2(bits, bias[h], T());
         }
       }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint4 b = q4_row(x[m], K, step, i, lane);
-        mma_16x8x16<T>(sum[m], a[0], b.x, b.y);
-        mma_16x8x16<T>(sum[m], a[1], b.z, b.w);
-      }
+      const uint4 b = lds_128(stage + Q4Stage<NG, ZEROS>::kRows + (row_at ^ (64 * (i & 1))) + 128 * (i >> 1));
+      mma_16x8x16<T>(sum, a[0], b.x, b.y);
+      mma_16x8x16<T>(sum, a[1], b.z, b.w);
     }
     const float s0 = q4_scale<T>(p.scale[0], j), s1 = q4_scale<T>(p.scale[1], j);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      acc[m][0] = fmaf(sum[m][0], s0, acc[m][0]);
-      acc[m][1] = fmaf(sum[m][1], s0, acc[m][1]);
-      acc[m][2] = fmaf(sum[m][2], s1, acc[m][2]);
-      acc[m][3] = fmaf(sum[m][3], s1, acc[m][3]);
-    }
+    acc[0] = fmaf(sum[0], s0, acc[0]);
+    acc[1] = fmaf(sum[1], s0, acc[1]);
+    acc[2] = fmaf(sum[2], s1, acc[2]);
+    acc[3] = fmaf(sum[3], s1, acc[3]);
   }
-}
-
-// Steps first, first + stride, ... of a tile, DEPTH - 1 of them on their way while one is computed.  `ring`: DEPTH stages of this warp's
-// own in shared memory.
-template <typename T, int NG, bool ZEROS, int MT, int DEPTH>
-__device__ __forceinline__ void q4_tile(float (&acc)[MT][4], const Q4Matrix& w, int64_t tile, const uint16_t* const (&x)[MT], int K, int first, int stride,
-                                        uint32_t ring, int lane) {
-  constexpr int kStage = Q4Stage<NG, ZEROS>::kBytes;
-  const uint4* data = w.data + tile * w.steps * kQ4Words;
-  const uint16_t* scales = static_cast<const uint16_t*>(w.scales) + tile * w.steps * (kQ4Rows * NG);
-  const uint8_t* zeros = ZEROS ? w.zeros + tile * w.steps * (kQ4Rows * NG) : nullptr;
-  int ahead = first;
-#pragma unroll
-  for (int s = 0; s < DEPTH - 1; ++s, ahead += stride) {
-    if (ahead < w.steps) q4_copy<NG, ZEROS>(ring + s * kStage, data, scales, zeros, ahead, lane);
-    copies_commit();
-  }
-  uint32_t stage = ring, free_stage = ring + (DEPTH - 1) * kStage;
-  for (int step = first; step < w.steps; step += stride, ahead += stride) {
-    copies_wait<DEPTH - 2>();
-    __syncwarp();  // every lane's copies of this step, and every lane is through with the stage that is filled next
-    if (ahead < w.steps) q4_copy<NG, ZEROS>(free_stage, data, scales, zeros, ahead, lane);
-    copies_commit();
-    Q4Piece<NG, ZEROS> p;
-    q4_take<NG, ZEROS>(p, stage, lane);
-    q4_step<T, NG, ZEROS, MT>(acc, p, x, K, step, lane);
-    free_stage = stage;
-    stage = stage == ring + (DEPTH - 1) * kStage ? ring : stage + kStage;
-  }
-  copies_wait<0>();
-  __syncwarp();  // the ring is free again
 }
 
 }  // namespace moe

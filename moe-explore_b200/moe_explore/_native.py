@@ -82,11 +82,11 @@ class F8RowsPass(ctypes.Structure):
 
 class FewPass(ctypes.Structure):
     """``moe_few_pass``: a whole layer for a few tokens."""
-    _fields_ = [(f, c_int32) for f in ("num_tokens", "d", "inter", "num_experts", "topk", "act", "dtype", "bits", "group", "norm_dtype",
+    _fields_ = [(f, c_int32) for f in ("num_tokens", "d", "inter", "num_experts", "topk", "act", "dtype", "bits", "group", "zeros", "norm_dtype",
                                        "router_dtype", "score_function", "normalize", "num_groups", "topk_groups", "group_best")] + \
                [("scale", c_float), ("eps", c_float)] + \
-               [(f, c_void_p) for f in ("x", "residual", "norm_w", "router_w", "router_bias", "expert_idx", "scores", "w1", "w1_scales",
-                                        "w1_zeros", "w2", "w2_scales", "w2_zeros", "addend", "out", "stream_out", "status", "workspace")] + \
+               [(f, c_void_p) for f in ("x", "residual", "norm_w", "router_w", "router_bias", "expert_idx", "scores", "w1", "w2",
+                                        "addend", "out", "stream_out", "status", "workspace")] + \
                [("workspace_bytes", c_size_t)]
 
 
@@ -133,7 +133,7 @@ SIGNATURES = {
     "moe_expert_backward": (c_int, [POINTER(ExpertPass), c_int, c_void_p]),
     "moe_act_f8_forward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
     "moe_act_f8_backward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
-    "moe_int4_matmul": (c_int, [c_void_p] * 5 + [c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "moe_int4_matmul": (c_int, [c_void_p] * 3 + [c_int64] + [c_int] * 5 + [c_void_p]),
     "moe_few_pass_size": (c_size_t, []),
     "moe_few_workspace_bytes": (c_size_t, [c_int] * 5),
     "moe_few_tokens": (c_int, [POINTER(FewPass), c_void_p]),
@@ -545,13 +545,14 @@ def act_f8_backward(q, scales, dh, dz, act):
 def int4_matmul(x, weight, out):
     """out [R, N] = x [R, K] @ weight^T for an ``Int4Weight`` (see moe_int4_matmul)."""
     with timed("int4:rows"):
-        rc = load().moe_int4_matmul(x.data_ptr(), weight.data.data_ptr(), weight.scales.data_ptr(), _ptr(weight.zeros), out.data_ptr(),
-                                    x.size(0), weight.k, weight.n, weight.group, dtype_code(x.dtype), _stream())
+        rc = load().moe_int4_matmul(x.data_ptr(), weight.data.data_ptr(), out.data_ptr(), x.size(0), weight.k, weight.n, weight.group,
+                                    weight.zeros, dtype_code(x.dtype), _stream())
     _check("moe_int4_matmul", rc)
     _count(1)
 
 
-FEW_TOKENS, FEW_SLOTS, FEW_EXPERTS, FEW_GROUPS, FEW_COLUMNS = 16, 512, 1024, 64, 1 << 20   # what moe_few_tokens takes
+FEW_TOKENS, FEW_SLOTS, FEW_EXPERTS, FEW_GROUPS = 16, 256, 1024, 64   # what moe_few_tokens takes
+FEW_COLUMNS, FEW_ROUTED_COLUMNS = 1 << 20, 16384                      # ... with norm or router
 
 
 @functools.lru_cache(maxsize=256)

@@ -50,7 +50,7 @@ def few_token_layer(input: torch.Tensor, params, residual=None, addend=None, nor
         return None
     T, d = input.shape
     E, topk = params.num_experts, params.topk
-    weights = (ep.up.data, ep.up.scales, ep.down.data, ep.down.scales) if int4 else (ep.weight1, ep.weight2)
+    weights = (ep.up.data, ep.down.data) if int4 else (ep.weight1, ep.weight2)
     bias = getattr(rp, "bias", None)
     tensors = [t for t in (input, rp.router_weight, bias, residual, addend, None if norm is None else norm.weight, *weights) if t is not None]
     if any(type(t) not in _PLAIN or not t.is_cuda for t in tensors) or not nothing_watches(*tensors) or _native.needs_gradient(*tensors):
@@ -58,7 +58,7 @@ def few_token_layer(input: torch.Tensor, params, residual=None, addend=None, nor
     options = _router_options(rp, input.dtype)
     act = None if ep.activation is None else str(ep.activation)
     if options is None or act not in _native.ACT_CODES or type(topk) is not int or rp.topk != topk or T * topk > _native.FEW_SLOTS or \
-            E > _native.FEW_EXPERTS or options[2] > _native.FEW_GROUPS or rp.router_weight.shape != (d, E) or d % 8 != 0 or d > _native.FEW_COLUMNS or \
+            E > _native.FEW_EXPERTS or options[2] > _native.FEW_GROUPS or rp.router_weight.shape != (d, E) or d % 8 != 0 or d > _native.FEW_ROUTED_COLUMNS or \
             not 0 < topk <= E // max(options[2], 1) * options[3] or options[2] < 1 or E % options[2] != 0 or not 0 < options[3] <= options[2]:
         return None
     if bias is not None and (bias.dtype is not torch.float32 or bias.shape != (E,)):
@@ -94,14 +94,12 @@ def _experts(ep, dtype, E: int, d: int, act):
     if type(ep) is Int4ExpertParams:
         up, down = ep.up, ep.down
         inter = up.n // gates
-        if up.scales.dtype is not dtype or down.scales.dtype is not dtype or (up.zeros is None) != (down.zeros is None) or up.group != down.group or \
+        if up.dtype is not dtype or down.dtype is not dtype or up.zeros != down.zeros or up.group != down.group or \
                 (up.n, up.k, down.n, down.k) != (gates * inter, d, d, inter) or up.data.size(0) != E or down.data.size(0) != E:
             return None
         up.checked(1, "up")
         down.checked(1, "down")
-        p.bits, p.group = 4, up.group
-        p.w1, p.w1_scales, p.w1_zeros = up.data.data_ptr(), up.scales.data_ptr(), _native._ptr(up.zeros)
-        p.w2, p.w2_scales, p.w2_zeros = down.data.data_ptr(), down.scales.data_ptr(), _native._ptr(down.zeros)
+        p.bits, p.group, p.zeros, p.w1, p.w2 = 4, up.group, up.zeros, up.data.data_ptr(), down.data.data_ptr()
     else:
         w1, w2 = ep.weight1, ep.weight2
         if w1.dim() != 3 or w2.dim() != 3 or w1.dtype is not dtype or w2.dtype is not dtype:
@@ -142,8 +140,8 @@ def int4_expert_compute(x, scores, indices, params: Int4ExpertParams, addend=Non
     act = None if params.activation is None else str(params.activation)
     if act not in _native.ACT_CODES:
         raise ValueError(f"Unsupported activation: {act!r}")
-    if x.dtype is not params.up.scales.dtype:
-        raise TypeError(f"rows are in the type of the scales, {params.up.scales.dtype}, got {x.dtype}")
+    if x.dtype is not params.up.dtype:
+        raise TypeError(f"rows are in the type of the scales, {params.up.dtype}, got {x.dtype}")
     if x.dim() != 2 or indices.dim() != 2 or indices.dtype is not torch.int64 or indices.size(0) != x.size(0) or scores.shape != indices.shape:
         raise ValueError("x is [tokens, d], indices (int64) and scores are [tokens, k]")
     if any(t.device != x.device for t in (scores, indices, params.up.data, params.down.data) + (() if addend is None else (addend,))):
@@ -151,18 +149,19 @@ def int4_expert_compute(x, scores, indices, params: Int4ExpertParams, addend=Non
     if addend is not None and (addend.shape != x.shape or addend.dtype is not x.dtype):
         raise ValueError("addend is like the result")
     _native.refuse_tracing()
-    if _native.needs_gradient(x, scores, addend, params.up.scales, params.down.scales):
+    if _native.needs_gradient(x, scores, addend):
         raise RuntimeError("experts in 4 bits have no backward pass: call this under torch.no_grad(), or train 16-bit experts")
     T, topk = indices.shape
     E = params.up.data.size(0)
-    if _experts(params, x.dtype, E, x.size(1), act) is None or not 0 < topk <= _native.FEW_SLOTS // _native.FEW_TOKENS or E > _native.FEW_EXPERTS:
-        raise ValueError(f"these experts do not fit together or are more than the kernel takes (1024 experts, 32 slots): input {tuple(x.shape)}, up "
+    if _experts(params, x.dtype, E, x.size(1), act) is None or not 0 < topk <= _native.FEW_SLOTS or E > _native.FEW_EXPERTS:
+        raise ValueError(f"these experts do not fit together or are more than the kernel takes (1024 experts, 256 slots): input {tuple(x.shape)}, up "
                          f"[{params.up.n}, {params.up.k}], down [{params.down.n}, {params.down.k}] for {act!r}, {E} experts, {topk} slots")
     with _native.on_device_of(x):
         ids, scores = indices.contiguous(), scores.detach().to(x.dtype).contiguous()
         outs = []
-        for t in range(0, T, _native.FEW_TOKENS):
-            part = slice(t, t + _native.FEW_TOKENS)
+        at_once = min(_native.FEW_TOKENS, _native.FEW_SLOTS // topk)
+        for t in range(0, T, at_once):
+            part = slice(t, t + at_once)
             p = _experts(params, x.dtype, E, x.size(1), act)
             p.expert_idx, p.scores = ids[part].data_ptr(), scores[part].data_ptr()
             outs.append(_launch(p, x[part], topk, None if addend is None else addend[part], (ids, scores)))

@@ -8,7 +8,6 @@ the kernels (``pack_int4``): tiles of 16 rows, cut into steps of 128 columns.  N
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
 
 import torch
 
@@ -28,41 +27,51 @@ def _up(n: int, of: int) -> int:
 @dataclass
 class Int4Weight:
     """Weights [..., n, k] in 4 bits, laid out by ``pack_int4``."""
-    data: torch.Tensor              # uint8 [..., tiles, steps, 1024]
-    scales: torch.Tensor            # bf16 or fp16 [..., tiles, steps, 16, 128 / group]
-    zeros: Optional[torch.Tensor]   # uint8, like the scales
+    data: torch.Tensor     # uint8 [..., tiles, steps, bytes of a block]: 1024 of values, then scales, then zeros
     n: int
     k: int
     group: int
+    dtype: torch.dtype     # of the scales, and of the rows: bf16 or fp16
+    zeros: bool            # whether there are zero points
+
+    @property
+    def per_step(self) -> int:
+        return STEP // self.group
+
+    @property
+    def block(self) -> int:
+        return 1024 + TILE * self.per_step * (3 if self.zeros else 2)
 
     def checked(self, dims: int, what: str) -> "Int4Weight":
         """``dims``: axes in front of the matrix."""
-        _native.require_cuda(self.data, self.scales, self.zeros)
-        tiles, steps, per_step = _up(self.n, TILE), _up(self.k, STEP), STEP // self.group if self.group in GROUPS else 0
-        lead = self.data.shape[:-3]
-        if per_step == 0 or len(lead) != dims or self.data.dtype is not torch.uint8 or tuple(self.data.shape) != (*lead, tiles, steps, 1024) or \
-                self.scales.dtype not in (torch.bfloat16, torch.float16) or tuple(self.scales.shape) != (*lead, tiles, steps, TILE, per_step) or \
-                self.scales.device != self.data.device:
-            raise ValueError(f"{what} is an Int4Weight of pack_int4 with {dims} axes in front of the matrix, got {self.data.dtype} "
-                             f"{tuple(self.data.shape)}, {self.scales.dtype} {tuple(self.scales.shape)} for [{self.n}, {self.k}] in groups of {self.group}")
-        if self.zeros is not None and (self.zeros.dtype is not torch.uint8 or self.zeros.shape != self.scales.shape or
-                                       self.zeros.device != self.data.device):
-            raise ValueError(f"{what}: zero points are uint8 and lie like the scales")
-        if any(t is not None and not (t.is_contiguous() and t.data_ptr() % 16 == 0) for t in (self.data, self.scales, self.zeros)):
-            raise ValueError(f"{what}: the parts of an Int4Weight are contiguous and 16-byte aligned, as pack_int4 makes them")
+        data = self.data
+        _native.require_cuda(data)
+        if self.group not in GROUPS or data.dim() != dims + 3 or data.dtype is not torch.uint8 or self.dtype not in (torch.bfloat16, torch.float16) or \
+                data.shape[dims:] != (_up(self.n, TILE), _up(self.k, STEP), self.block):
+            raise ValueError(f"{what} is an Int4Weight of pack_int4 with {dims} axes in front of the matrix, got {data.dtype} {tuple(data.shape)} for "
+                             f"[{self.n}, {self.k}] in groups of {self.group} with scales in {self.dtype}")
+        if not data.is_contiguous() or data.data_ptr() % 16 != 0:
+            raise ValueError(f"{what}: the data of an Int4Weight are contiguous and 16-byte aligned, as pack_int4 makes them")
         return self
 
     def unpack(self):
         """(values uint8 [..., N, K / 2] two per byte, scales [..., N, groups], zeros or None): what ``pack_int4`` was given."""
-        lead, tiles, steps = self.data.shape[:-3], self.data.size(-3), self.data.size(-2)
-        words = self.data.view(*lead, tiles, steps, 2, 8, 4, 4, 4)   # half, row, t, i, byte
+        lead, tiles, steps, n = self.data.shape[:-3], self.data.size(-3), self.data.size(-2), TILE * self.per_step
+        words = self.data[..., :1024].reshape(*lead, tiles, steps, 2, 8, 4, 4, 4)   # half, row, t, i, byte
         b0, b1, b2, b3 = words.unbind(-1)
         four = torch.stack(((b0 & 15) | (b2 << 4), (b0 >> 4) | (b2 & 240), (b1 & 15) | (b3 << 4), (b1 >> 4) | (b3 & 240)), -1)
         d = len(lead)
         rows = four.permute(*range(d), d, d + 2, d + 3, d + 1, d + 5, d + 4, d + 6).reshape(*lead, tiles * TILE, steps * STEP // 2)
+        scales = self.data[..., 1024:1024 + 2 * n].contiguous().view(self.dtype)
+        zeros = self.data[..., 1024 + 2 * n:] if self.zeros else None
         groups = _up(self.k, self.group)
-        flat = lambda t: None if t is None else t.transpose(-3, -2).reshape(*lead, tiles * TILE, -1)[..., :self.n, :groups].contiguous()
-        return rows[..., :self.n, :self.k // 2].contiguous(), flat(self.scales), flat(self.zeros)
+
+        def flat(t):
+            if t is None:
+                return None
+            t = t.reshape(*lead, tiles, steps, TILE, self.per_step).transpose(-3, -2)
+            return t.reshape(*lead, tiles * TILE, steps * self.per_step)[..., :self.n, :groups].contiguous()
+        return rows[..., :self.n, :self.k // 2].contiguous(), flat(scales), flat(zeros)
 
     def dequantize(self) -> torch.Tensor:
         """fp32 [..., N, K]."""
@@ -97,11 +106,11 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor = 
     data = torch.stack(((p0 & 15) | (p1 << 4), (p2 & 15) | (p3 << 4), (p0 >> 4) | (p1 & 240), (p2 >> 4) | (p3 & 240)), -1)
 
     def laid(t):
-        if t is None:
-            return None
         t = pad(t.detach(), (0, steps * per_step - t.size(-1), 0, tiles * TILE - n))
-        return t.reshape(*lead, tiles, TILE, steps, per_step).transpose(-3, -2).contiguous()
-    return Int4Weight(data.reshape(*lead, tiles, steps, 1024), laid(scales), laid(None if zeros is None else zeros & 15), n, k, group)
+        t = t.reshape(*lead, tiles, TILE, steps, per_step).transpose(-3, -2).contiguous()
+        return t.view(torch.uint8).reshape(*lead, tiles, steps, -1)
+    blocks = [data.reshape(*lead, tiles, steps, 1024), laid(scales)] + ([] if zeros is None else [laid(zeros & 15)])
+    return Int4Weight(torch.cat(blocks, -1), n, k, group, scales.dtype, zeros is not None)
 
 
 def quantize_int4(weight: torch.Tensor, group: int = 128, zeros: bool = False, dtype: torch.dtype = None) -> Int4Weight:
@@ -181,10 +190,10 @@ def int4_matmul(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     _native.require_cuda(x)
     if x.dim() < 1 or x.size(-1) != weight.k or x.device != weight.data.device:
         raise ValueError(f"rows of {tuple(x.shape)} on {x.device}, weights [{weight.n}, {weight.k}] on {weight.data.device}")
-    if x.dtype is not weight.scales.dtype:
-        raise TypeError(f"rows are in the type of the scales, {weight.scales.dtype}, got {x.dtype}")
+    if x.dtype is not weight.dtype:
+        raise TypeError(f"rows are in the type of the scales, {weight.dtype}, got {x.dtype}")
     _native.refuse_tracing()
-    if _native.needs_gradient(x, weight.scales):
+    if _native.needs_gradient(x):
         raise RuntimeError("products with 4-bit weights have no backward pass: call this under torch.no_grad()")
     with _native.on_device_of(x):
         rows = _dense(x.detach().reshape(-1, weight.k))

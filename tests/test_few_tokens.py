@@ -375,7 +375,6 @@ def test_refusals_of_the_library(native):
                          (dict(scores=None), -1, b"router, or"), (dict(router_w=16, num_groups=3), -1, b"groups"), (dict(router_w=16, router_dtype=7), -1, b"router options"),
                          (dict(router_w=16, score_function=2, router_bias=16), -1, b"without bias"), (dict(), -1, b"null"),
                          (dict(x=16, w1=16, w2=16, out=16, workspace=16), -1, b"workspace has"), (dict(x=8, w1=16, w2=16, out=16, workspace=16), -1, b"aligned"),
-                         (dict(x=16, w1=16, w2=16, out=16, workspace=16, bits=4, group=32), -1, b"have scales"),
                          (dict(x=16, w1=16, w2=16, out=16, workspace=16, residual=16), -1, b"residual")]:
         got = call(base(**kw))
         assert got[0] == rc and text in got[1], (kw, got)

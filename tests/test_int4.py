@@ -55,7 +55,7 @@ def test_layout_and_back(lead, n, k, group, zeros):
     assert torch.equal(back[0], given[0]) and torch.equal(back[1], given[1]) and (torch.equal(back[2], given[2]) if zeros else back[2] is None)
     assert bool((w.dequantize().double() == weight64(*given, group)).all())
     # every value where the description of the layout puts it
-    data, values = w.data.reshape(-1, -(-n // 16), -(-k // 128), 1024), given[0].reshape(-1, n, k // 2)
+    data, values = w.data.reshape(-1, -(-n // 16), -(-k // 128), w.block), given[0].reshape(-1, n, k // 2)
     for m, r, c in torch.randint(0, 1 << 20, (200, 3), generator=gen(1, "cpu")).tolist():
         m, r, c = m % data.size(0), r % n, c % k
         i, t, low = c % 128 // 32, c % 32 // 8, c % 8
@@ -73,13 +73,13 @@ def test_quantized_weights_are_near():
         for group in (32, 64, 128):
             q = quantize_int4(w, group, zeros)
             _, scales, points = q.unpack()
-            assert q.scales.dtype is torch.bfloat16 and bool((scales > 0).all())
+            assert q.dtype is torch.bfloat16 and scales.dtype is torch.bfloat16 and bool((scales > 0).all())
             step = scales.float().repeat_interleave(group, -1)[..., :200]
             assert bool(((q.dequantize() - w).abs() <= step * (0.5 + 15 * 2.0 ** -8 + (0.5 if zeros else 0))).all())
     glu = MLPParams(torch.randn(2, 64, 96), torch.randn(2, 48, 64), "swiglu")
     p = quantize_experts_int4(glu, 32)
     same = quantize_experts_int4(GLUParams(glu.weight1[..., 0::2], glu.weight1[..., 1::2], glu.weight2, "swiglu"), 32)
-    assert torch.equal(p.up.data, same.up.data) and torch.equal(p.up.scales, same.up.scales) and torch.equal(p.down.data, same.down.data)
+    assert torch.equal(p.up.data, same.up.data) and torch.equal(p.down.data, same.down.data)
     rows = p.up.dequantize().view(2, 6, 2, 8, 64)
     for h in range(2):
         part = glu.weight1[..., h::2].mT.reshape(2, 6, 8, 64)
@@ -157,12 +157,11 @@ def test_offsets_past_32_bits(native):
     """A matrix of more than 2^32 values (2 GB and more of data): its last rows are what they are by themselves."""
     n, k = 270336, 16384
     x = torch.randn(1, k, device="cuda").bfloat16()
-    data = torch.zeros(n // 16, k // 128, 1024, dtype=torch.uint8, device="cuda")
-    scales = torch.ones(n // 16, k // 128, 16, 1, dtype=torch.bfloat16, device="cuda")
+    data = torch.zeros(n // 16, k // 128, 1024 + 32, dtype=torch.uint8, device="cuda")
     tail = raw(gen(3), 48, k)
-    last = pack_int4(*tail)
-    data[-3:], scales[-3:] = last.data, last.scales
-    out = int4_matmul(x, Int4Weight(data, scales, None, n, k, 128))
+    data[-3:] = pack_int4(*tail).data
+    out = int4_matmul(x, Int4Weight(data, n, k, 128, torch.bfloat16, False))
+    assert not out[:, :-48].any()
     check(out[:, -48:], x, weight64(*tail, 128), torch.bfloat16)
 
 
@@ -188,11 +187,11 @@ def test_refusals_without_a_gpu(native):
     with pytest.raises(RuntimeError, match="CUDA"):
         int4_matmul(torch.zeros(1, 64).bfloat16(), pack_int4(values, scales, zeros, group=32))
     lib = native.load()
-    assert lib.moe_int4_matmul(None, None, None, None, None, 1, 64, 64, 128, 0, None) == -1 and b"null" in lib.moe_last_error()
-    assert lib.moe_int4_matmul(None, None, None, None, None, 1, 64, 64, 48, 0, None) == -1 and b"groups" in lib.moe_last_error()
-    assert lib.moe_int4_matmul(None, None, None, None, None, 1, 60, 64, 32, 0, None) == -2 and b"multiples of 8" in lib.moe_last_error()
-    assert lib.moe_int4_matmul(None, None, None, None, None, -1, 64, 64, 32, 0, None) == -1
-    assert lib.moe_int4_matmul(16, 32, 40, None, 64, 1, 64, 64, 32, 0, None) == -1 and b"aligned" in lib.moe_last_error()
+    assert lib.moe_int4_matmul(None, None, None, 1, 64, 64, 128, 0, 0, None) == -1 and b"null" in lib.moe_last_error()
+    assert lib.moe_int4_matmul(None, None, None, 1, 64, 64, 48, 0, 0, None) == -1 and b"groups" in lib.moe_last_error()
+    assert lib.moe_int4_matmul(None, None, None, 1, 60, 64, 32, 0, 0, None) == -2 and b"multiples of 8" in lib.moe_last_error()
+    assert lib.moe_int4_matmul(None, None, None, -1, 64, 64, 32, 0, 0, None) == -1
+    assert lib.moe_int4_matmul(16, 40, 64, 1, 64, 64, 32, 0, 0, None) == -1 and b"aligned" in lib.moe_last_error()
 
 
 @gpu
@@ -209,10 +208,11 @@ def test_refusals(native):
     with pytest.raises(ValueError, match="axes in front"):
         int4_matmul(x, pack_int4(*raw(gen(0), 2, 16, 64, group=32), group=32))
     with pytest.raises(ValueError, match="Int4Weight"):
-        int4_matmul(x, Int4Weight(w.data, w.scales, None, 16, 64, 128))
+        int4_matmul(x, Int4Weight(w.data, 16, 64, 128, w.dtype, False))
+    with pytest.raises(ValueError, match="Int4Weight"):
+        int4_matmul(x, Int4Weight(w.data, 16, 64, 32, w.dtype, True))
+    two = pack_int4(*raw(gen(0), 32, 64, group=32), group=32)
     with pytest.raises(ValueError, match="contiguous"):
-        int4_matmul(x, Int4Weight(w.data, w.scales.transpose(-1, -2).contiguous().transpose(-1, -2), None, 16, 64, 32))
-    with pytest.raises(ValueError, match="zero points"):
-        int4_matmul(x, Int4Weight(w.data, w.scales, w.scales, 16, 64, 32))
+        int4_matmul(x, Int4Weight(two.data.repeat(1, 1, 2)[:, :, :two.block], 32, 64, 32, w.dtype, False))
     with pytest.raises(RuntimeError, match="trace"):
         torch.jit.trace(lambda t: int4_matmul(t, w), (x,), check_trace=False)
