@@ -22,7 +22,7 @@ constexpr int kFewSlots = 256;      // tokens x slots
 constexpr int kFewRows = 8;         // of an entry: slots of one expert that share its weights
 constexpr int kFewExperts = 1024, kFewGroups = 64;
 constexpr int kFewCtas = 2;         // per SM
-constexpr int kFewParts = 4;        // shares of the down product's depth, at most
+constexpr int kFewParts = 4;        // shares of the down product's depth, at most (1, 2 or 4)
 
 // ---------------------------------------------------------------------------------------------------- norm and logits
 constexpr int kHeadRanks = 8;           // CTAs of a cluster share the hidden size
@@ -275,6 +275,7 @@ struct FewRouting {
   int16_t slot[kFewSlots], token[kFewSlots];    // and these slots' tokens
   uint8_t count[kFewSlots];
   int starts[kFewSlots / 32];
+  uint32_t sums[kFewWarps];        // where a warp's sums of a unit are
   int entries;
   int go_on;
 };
@@ -502,27 +503,33 @@ __device__ __forceinline__ float few_act(float x, int act) {
 }
 
 // A format of weights: how a warp copies one step of a tile with the same columns of an entry's rows to shared memory, and multiplies them.
-// A unit is an entry's rows by a few tiles of its expert's matrix over steps [begin, end).  Its tiles are shared out to the warps, `team` of
-// them to a tile (1, 2, 4 or 8, so that a unit has 8 / team tiles); warp w of a team takes steps begin + w, begin + w + team, ...
+// A unit is an entry's rows by a tile of its expert's matrix, over a share of its steps.  It belongs to a team of 1, 2, 4 or 8 warps of a
+// CTA; a team's warps take its steps in turn and join their sums.
 struct FewMatrix {
   const void* w16;
   Q4Matrix w4;
-  int K, N, steps, cols;  // cols: of a tile
-  int team, shares;       // of the depth, see below
+  int K, N, steps;
+  int cols, team, shares;  // columns of a tile; see share_out
 };
 
-// Team and shares of a product: the fullest CTA has `rounds` units, each of the steps of a warp and what the joining costs (about as much as
-// `cost` steps).  More shares, up to `most`, give more units of fewer steps, and partial sums for the fold.
-__device__ __forceinline__ void share_out(FewMatrix& m, int entries, int most, int cost) {
-  const int tiles = (m.N + m.cols - 1) / m.cols;
-  int least = 0x7FFFFFFF;
-  for (int shares = 1; shares <= most; shares *= 2)
-    for (int team = kFewWarps; team >= 1; team /= 2) {
-      const int units = entries * ((tiles * team + kFewWarps - 1) / kFewWarps) * shares;
-      const int rounds = (units + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-      const int steps = (m.steps + shares * team - 1) / (shares * team) + cost + (shares > 1);
-      if (rounds * steps < least) least = rounds * steps, m.team = team, m.shares = shares;
-    }
+// What gives the least to the team that has the most: `rounds` units of the steps of a warp and the joining, which costs about as much as
+// `cost` steps.  Where the format has a choice, tiles of fewer columns (in eights, 16 to kCols; a step costs as much as eight columns more) make
+// more units where there are few; shares of the depth, up to `most`, do too, and leave partial sums to the fold.  A lane per choice.
+template <typename F> __device__ __forceinline__ void share_out(FewMatrix& m, int entries, int most, int lane) {
+  constexpr int kWidths = (F::kCols - F::kNarrowest) / 8 + 1, kTeams = F::kLeastTeam == 8 ? 1 : 4, kAll = kWidths * kTeams * 3;
+  uint32_t least = 0xFFFFFFFFu;
+  for (int i = lane; i < kAll; i += 32) {
+    const int cols = F::kCols - 8 * (i % kWidths), team = kFewWarps >> (i / kWidths % kTeams), shares = 1 << (i / kWidths / kTeams);
+    if (shares > most) continue;
+    const int tiles = (m.N + cols - 1) / cols, teams = static_cast<int>(gridDim.x) * (kFewWarps / team);
+    const int rounds = (entries * tiles * shares + teams - 1) / teams;
+    const uint32_t work = static_cast<uint32_t>(rounds) * ((m.steps + shares * team - 1) / (shares * team) + F::kCost + (shares > 1)) * (kWidths > 1 ? cols + 8 : 1);
+    least = min(least, min(work, 0x1FFFFFFu) << 7 | i);
+  }
+  const int i = static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, least) & 127u);
+  m.cols = F::kCols - 8 * (i % kWidths);
+  m.team = kFewWarps >> (i / kWidths % kTeams);
+  m.shares = 1 << (i / kWidths / kTeams);
 }
 
 // 16 bits, [K, N] with N contiguous: 16 rows of K by up to 64 columns.  The weights are the 16 rows of m16n8k16, transposed on their way from
@@ -530,9 +537,9 @@ __device__ __forceinline__ void share_out(FewMatrix& m, int entries, int most, i
 // products, four rows to a quarter of a warp, made a request of every 16 bytes: 2.2 TB/s); in shared memory the 16-byte pieces of a row
 // are turned by its number, so that the eight rows of a matrix lie in different banks.
 template <typename T> struct FewWide {
-  static constexpr int kCols = 64, kStep = 16, kDepth = 5, kProducts = 4, kCost = 4;
+  static constexpr int kCols = 64, kNarrowest = 16, kStep = 16, kDepth = 5, kProducts = 4, kCost = 4, kLeastTeam = 8;
   static constexpr int kRowsAt = kStep * kCols * 2, kStage = kRowsAt + kFewRows * kStep * 2;
-  const uint16_t* w;   // the copy's: this lane's piece of the step's first row
+  const uint16_t* w;   // the copy's: this lane's piece of the unit's first rows
   const uint16_t* x;   // this lane's piece of its row
   int64_t row;
   int K;
@@ -545,34 +552,35 @@ template <typename T> struct FewWide {
     const int g = lane >> 2;
     row_at = kRowsAt + (g < count ? g : 0) * 32 + (lane & 3) * 4;  // (rows behind the last give products that are nobody's)
   }
-  template <typename Row> __device__ __forceinline__ void set(const FewMatrix& m, int expert, int tile, int step, Row rows, int count, int lane) {
+  template <typename Row> __device__ __forceinline__ void set(const FewMatrix& m, int expert, int tile, Row rows, int count, int lane) {
     const int piece = lane & 7, col = tile * m.cols + 8 * piece;
     inside = 8 * piece < m.cols && col < m.N;
     row = m.N;
     K = m.K;
-    w = static_cast<const uint16_t*>(m.w16) + (static_cast<int64_t>(expert) * K + step * kStep + (lane >> 3)) * row + col;
-    x = (lane >> 1) < count ? rows(lane >> 1) : nullptr;
+    w = static_cast<const uint16_t*>(m.w16) + (static_cast<int64_t>(expert) * K + (lane >> 3)) * row + col;
+    x = (lane >> 1) < count ? rows(lane >> 1) + 8 * (lane & 1) : nullptr;
   }
   __device__ __forceinline__ void copy(uint32_t stage, int step, int lane) const {
     if (!inside) return;
     const int r = lane >> 3;
     const uint32_t to = stage + r * 128;
+    const uint16_t* from = w + step * kStep * row;
     if (step * kStep + kStep <= K) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) copy_16(to + j * 512 + (((lane & 7) ^ ((r + 4 * j) & 7)) << 4), w + 4 * j * row);
+      for (int j = 0; j < 4; ++j) copy_16(to + j * 512 + (((lane & 7) ^ ((r + 4 * j) & 7)) << 4), from + 4 * j * row);
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const bool real = step * kStep + r + 4 * j < K;
-        copy_16_or_zeros(to + j * 512 + (((lane & 7) ^ ((r + 4 * j) & 7)) << 4), real ? w + 4 * j * row : w, real);
+        copy_16_or_zeros(to + j * 512 + (((lane & 7) ^ ((r + 4 * j) & 7)) << 4), real ? from + 4 * j * row : w, real);
       }
     }
   }
   __device__ __forceinline__ void copy_rows(uint32_t stage, int, int step, int lane) const {
-    const int k = step * kStep + 8 * (lane & 1);
-    if (x != nullptr) copy_16_or_zeros(stage + kRowsAt + lane * 16, k < K ? x + k : x, k < K);
+    const int k = step * kStep;
+    const bool real = k + 8 * (lane & 1) < K;
+    if (x != nullptr) copy_16_or_zeros(stage + kRowsAt + lane * 16, real ? x + k : x - 8 * (lane & 1), real);
   }
-  __device__ __forceinline__ void next(int team) { w += team * kStep * row; }
   __device__ __forceinline__ void multiply(float (&acc)[kProducts][4], uint32_t stage, int) const {
     const uint32_t b0 = lds_32(stage + row_at), b1 = lds_32(stage + row_at + 16);
 #pragma unroll
@@ -580,58 +588,59 @@ template <typename T> struct FewWide {
       uint32_t a[4];
       asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                    : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
-                   : "r"(stage + (weight_at ^ (32 * q)))
-                   : "memory");
+                   : "r"(stage + (weight_at ^ (32 * q))));
       mma_16x8x16<T>(acc[q], a, b0, b1);
     }
   }
   // column of the tile that value c of product q belongs to
   __device__ static __forceinline__ int column(int q, int c, int lane) { return 16 * q + (lane >> 2) + 8 * (c >> 1); }
-  // Columns of a tile: as many, in eights, as leave the fullest CTA with the least (a unit's own costs count as eight columns).
-  __device__ static __forceinline__ int width(int entries, int N) {
-    int best = kCols, least = 0x7FFFFFFF;
-    for (int c = kCols; c >= 16; c -= 8) {
-      const int rounds = (entries * ((N + c - 1) / c) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-      if (rounds * (c + 8) < least) least = rounds * (c + 8), best = c;
-    }
-    return best;
-  }
 };
 
-// 4 bits (int4.cuh): 16 rows of the weight by 128 columns.
+// 4 bits (int4.cuh): 32 rows of the weight by 128 columns.
 template <typename T, int NG, bool ZEROS> struct FewFour {
-  static constexpr int kCols = kQ4Rows, kStep = kQ4Step, kDepth = 4, kProducts = 1, kCost = 4;
+  static constexpr int kCols = kQ4Cols, kNarrowest = kCols, kStep = kQ4Step, kDepth = 3, kProducts = kQ4Tiles, kCost = 2, kLeastTeam = 1;
   static constexpr int kStage = Q4Stage<NG, ZEROS>::kBytes, kBlock = Q4Stage<NG, ZEROS>::kBlock;
   const uint8_t* block;
+  int64_t apart;
   const uint16_t* x[4];
   int K;
   uint32_t row_at;
   __device__ __forceinline__ void read(int count, int lane) { row_at = q4_row_at(count, lane); }
-  template <typename Row> __device__ __forceinline__ void set(const FewMatrix& m, int expert, int tile, int step, Row rows, int count, int lane) {
-    block = m.w4.data + ((expert * m.w4.tiles + tile) * m.w4.steps + step) * kBlock;
+  template <typename Row> __device__ __forceinline__ void set(const FewMatrix& m, int expert, int tile, Row rows, int count, int lane) {
+    block = m.w4.data + (expert * m.w4.tiles + kQ4Tiles * tile) * m.w4.steps * kBlock + lane * 16;
+    apart = kQ4Tiles * tile + 1 < m.w4.tiles ? static_cast<int64_t>(m.w4.steps) * kBlock : 0;
     K = m.K;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 2 * i + (lane >> 4);
-      if (r < count) x[i] = rows(r);
+      if (2 * i < count) x[i] = rows(r < count ? r : 0) + 8 * (lane & 15);
     }
   }
-  __device__ __forceinline__ void copy(uint32_t stage, int, int lane) const { q4_copy<NG, ZEROS>(stage, block, lane); }
-  __device__ __forceinline__ void copy_rows(uint32_t stage, int count, int step, int lane) const {
-    q4_copy_rows<NG, ZEROS>(stage, [&](int i) { return x[i]; }, count, K, step, lane);
+  __device__ __forceinline__ void copy(uint32_t stage, int step, int lane) const {
+    q4_copy<NG, ZEROS>(stage, block + static_cast<int64_t>(step) * kBlock, apart, lane);
   }
-  __device__ __forceinline__ void next(int team) { block += team * kBlock; }
-  __device__ __forceinline__ void multiply(float (&acc)[1][4], uint32_t stage, int lane) const { q4_step<T, NG, ZEROS>(acc[0], stage, row_at, lane); }
-  __device__ static __forceinline__ int column(int, int c, int lane) { return (lane >> 2) + 8 * (c >> 1); }
-  __device__ static __forceinline__ int width(int, int) { return kCols; }
+  __device__ __forceinline__ void copy_rows(uint32_t stage, int count, int step, int lane) const {
+    q4_copy_rows<NG, ZEROS>(stage, x, count, K, step * kStep, lane);
+  }
+  __device__ __forceinline__ void multiply(float (&acc)[kProducts][4], uint32_t stage, int lane) const {
+    q4_step<T, NG, ZEROS>(acc, stage, row_at, lane);
+  }
+  __device__ static __forceinline__ int column(int q, int c, int lane) { return kQ4Rows * q + (lane >> 2) + 8 * (c >> 1); }
 };
 
 template <typename F> struct FewPlan {
   static constexpr int kRing = F::kDepth * F::kStage;
-  static constexpr int kParts = kFewWarps * kRing;                                   // the warps' sums of a unit: [warp][row][column]
-  static constexpr int kTotal = kParts + kFewWarps * kFewRows * F::kCols * 4;
-  static_assert(kFewWarps * (kFewExperts + kFewGroups) * 4 <= kParts && kFewWarps * kFewExperts + 4 * kFewExperts <= kParts, "the router's keys lie where the rings will be");
+  static constexpr int kTotal = kFewWarps * kRing;
+  static_assert(kFewRows * F::kCols * 4 <= F::kStage, "a warp's sums of a unit, [row][column], lie in the stage that it has read last");
+  static_assert(kFewWarps * (kFewExperts + kFewGroups) * 4 <= kTotal && kFewWarps * kFewExperts + 4 * kFewExperts <= kTotal,
+                "the router's keys lie where the rings will be");
 };
+
+// The warps of a team (of a CTA's; more than one warp).
+__device__ __forceinline__ void team_sync(int team, int warp) {
+  if (team == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / team), "r"(32 * team) : "memory");
+}
 
 // The units of one product.  A warp's copies run ahead of its products by up to kDepth - 1 steps, into the next units, so that nothing
 // waits for memory while a unit's sums are joined.
@@ -640,58 +649,54 @@ template <typename F> struct FewWalk {
   const FewRouting& r;
   const uint16_t* source;  // the rows, and which of them belong to the entries' slots
   const int16_t* which;
-  int bundles, units;  // a bundle: the tiles of a unit
-  uint32_t ring;
+  int tiles, units, teams;
   int warp, lane;
   // where the copies are
   F f;
   int unit, step, end, count;
-  uint32_t to;
 
-  // the entry, this warp's tile (maybe behind the last) and its steps [begin, stop)
-  __device__ __forceinline__ void place(int u, int& entry, int& bundle, int& share) const {
-    entry = u / (bundles * m.shares);
-    const int rest = u - entry * bundles * m.shares;
-    share = rest / bundles;
-    bundle = rest - share * bundles;
+  __device__ __forceinline__ int first_unit() const { return warp / m.team * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x); }  // CTAs in turn
+  __device__ __forceinline__ void place(int u, int& entry, int& tile, int& share) const {
+    entry = u / (tiles * m.shares);
+    const int rest = u - entry * tiles * m.shares;
+    share = rest / tiles;
+    tile = rest - share * tiles;
   }
-  __device__ __forceinline__ int tile_of(int bundle) const { return bundle * (kFewWarps / m.team) + warp / m.team; }
-  __device__ __forceinline__ void steps_of(int tile, int share, int& begin, int& stop) const {
-    begin = m.steps * share / m.shares + warp % m.team;
-    stop = tile * m.cols < m.N ? m.steps * (share + 1) / m.shares : 0;
-  }
+  // this warp's steps of a share
+  __device__ __forceinline__ int begin_of(int share) const { return m.steps * share / m.shares + warp % m.team; }
+  __device__ __forceinline__ int end_of(int share) const { return m.steps * (share + 1) / m.shares; }
   __device__ __forceinline__ void seek() {  // the unit's first step of this warp's, or the next unit that has one
     while (unit < units) {
-      int n, bundle, share;
-      place(unit, n, bundle, share);
-      const int tile = tile_of(bundle);
-      steps_of(tile, share, step, end);
+      int n, tile, share;
+      place(unit, n, tile, share);
+      step = begin_of(share);
+      end = end_of(share);
       if (step < end) {
         count = r.count[n];
         const int first = r.first[n];
-        f.set(m, r.expert[n], tile, step, [&](int i) { return source + static_cast<int64_t>(which[first + i]) * m.K; }, count, lane);
+        f.set(m, r.expert[n], tile, [&](int i) { return source + static_cast<int64_t>(which[first + i]) * m.K; }, count, lane);
         return;
       }
-      unit += gridDim.x;
+      unit += teams;
     }
   }
   __device__ __forceinline__ void start() {
-    unit = blockIdx.x;
-    to = ring;
+    unit = first_unit();
     seek();
   }
   __device__ __forceinline__ void advance() {
     step += m.team;
-    if (step < end) {
-      f.next(m.team);
-    } else {
-      unit += gridDim.x;
+    if (step >= end) {
+      unit += teams;
       seek();
     }
-    to = to == ring + (F::kDepth - 1) * F::kStage ? ring : to + F::kStage;
   }
-  __device__ __forceinline__ void copy_weights() const { if (unit < units) f.copy(to, step, lane); }
-  __device__ __forceinline__ void copy_rows() const { if (unit < units) f.copy_rows(to, count, step, lane); }
+  __device__ __forceinline__ void copy(uint32_t to, bool weights, bool rows) {  // one step, and on to the next
+    if (unit >= units) return;
+    if (weights) f.copy(to, step, lane);
+    if (rows) f.copy_rows(to, count, step, lane);
+    advance();
+  }
 };
 
 template <typename T, typename F>
@@ -700,33 +705,33 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) few_experts_kernel(cons
   constexpr bool WIDE = F::kCols == 64;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ FewRouting r;
-  float* const parts = reinterpret_cast<float*>(smem + P::kParts);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t ring = smem_u32(smem) + warp * P::kRing;
+  const uint32_t base = smem_u32(smem), ring = warp * P::kRing;  // the ring's place in it
   route<T>(a, r, reinterpret_cast<float*>(smem));
   const bool gated = a.act == MOE_ACT_SWIGLU || a.act == MOE_ACT_GEGLU;
   const int slots = a.T * a.k;
-  // All units of a product whose first copies are under way; `give` takes the sums of a unit's tiles: (entry, tile, its place in the
-  // bundle, share, total(row, column)).
+  // All units of a product whose first copies are under way; `give` takes a unit's sums: (entry, tile, share, thread of the team,
+  // the team's threads, total(row, column)).
   const auto walk = [&](FewWalk<F>& c, auto give) {
     F f;
-    uint32_t from = ring;
-    const int team = c.m.team;
-    for (int unit = blockIdx.x; unit < c.units; unit += gridDim.x) {
-      int n, bundle, share, step, end;
-      c.place(unit, n, bundle, share);
-      c.steps_of(c.tile_of(bundle), share, step, end);
-      const int count = r.count[n];
+    uint32_t from = ring, spent = ring + (F::kDepth - 1) * F::kStage;
+    const int team = c.m.team, mine = warp % team * 32 + lane;
+    const uint32_t* const sums = r.sums + (warp - warp % team);
+#pragma unroll 1
+    for (int unit = c.first_unit(); unit < c.units; unit += c.teams) {
+      int n, tile, share;
+      c.place(unit, n, tile, share);
+      const int count = r.count[n], end = c.end_of(share);
       f.read(count, lane);
       float acc[F::kProducts][4] = {};
-      for (; step < end; step += team) {
+#pragma unroll 1
+      for (int step = c.begin_of(share); step < end; step += team) {
         copies_wait<F::kDepth - 2>();
         __syncwarp();  // every lane's copies of this step, and every lane is through with the stage that is filled next
-        c.copy_weights();
-        c.copy_rows();
+        c.copy(base + spent, true, true);
         copies_commit();
-        c.advance();
-        f.multiply(acc, from, lane);
+        f.multiply(acc, base + from, lane);
+        spent = from;
         from = from == ring + (F::kDepth - 1) * F::kStage ? ring : from + F::kStage;
       }
 #pragma unroll
@@ -734,51 +739,47 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) few_experts_kernel(cons
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int row = 2 * (lane & 3) + (i & 1);
-          if (row < count) parts[(warp * kFewRows + row) * F::kCols + F::column(q, i, lane)] = acc[q][i];
+          if (row < count) reinterpret_cast<float*>(smem + spent)[row * F::kCols + F::column(q, i, lane)] = acc[q][i];
         }
-      __syncthreads();
-      give(n, bundle * (kFewWarps / team), kFewWarps / team, share, [&](int place, int row, int col) {
+      if (lane == 0) r.sums[warp] = spent;
+      team_sync(team, warp);
+      give(n, tile, share, mine, team * 32, [&](int row, int col) {
         float v = 0.0f;
-        const float* p = parts + (place * team * kFewRows + row) * F::kCols + col;
-        for (int w = 0; w < team; ++w) v += p[w * kFewRows * F::kCols];
+        for (int w = 0; w < team; ++w) v += reinterpret_cast<const float*>(smem + sums[w])[row * F::kCols + col];
         return v;
       });
-      __syncthreads();
+      team_sync(team, warp);
     }
     copies_wait<0>();
     __syncwarp();
   };
   const auto open = [&](const FewMatrix& m, const uint16_t* source, const int16_t* which) {
     const int tiles = (m.N + m.cols - 1) / m.cols;
-    const int bundles = (tiles * m.team + kFewWarps - 1) / kFewWarps;
-    FewWalk<F> c{m, r, source, which, bundles, r.entries * bundles * m.shares, ring, warp, lane};
+    FewWalk<F> c{m, r, source, which, tiles, r.entries * tiles * m.shares, static_cast<int>(gridDim.x) * (kFewWarps / m.team), warp, lane};
     c.start();
     return c;
   };
 
   {
-    const int N = gated ? 2 * a.I : a.I;
-    FewMatrix up{a.w1, a.up, a.d, N, (a.d + F::kStep - 1) / F::kStep, F::width(r.entries, N), kFewWarps, 1};
-    if (!WIDE) share_out(up, r.entries, 1, F::kCost);
+    FewMatrix up{a.w1, a.up, a.d, gated ? 2 * a.I : a.I, (a.d + F::kStep - 1) / F::kStep, F::kCols, kFewWarps, 1};
+    share_out<F>(up, r.entries, 1, lane);
     auto c = open(up, static_cast<const uint16_t*>(a.x), r.token);
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < F::kDepth - 1; ++s) {
-      c.copy_weights();
-      c.copy_rows();
+      c.copy(base + ring + s * F::kStage, true, true);
       copies_commit();
-      c.advance();
     }
     const int cols = gated ? up.cols / 2 : up.cols;
-    walk(c, [&](int n, int tile, int tiles, int, auto total) {
+    walk(c, [&](int n, int tile, int, int thread, int threads, auto total) {
       const int count = r.count[n];
-      for (int at = tid; at < count * cols * tiles; at += kFewThreads) {
-        const int row = at / (cols * tiles), rest = at - row * cols * tiles;
-        const int place = rest / cols, col = rest - place * cols;
-        const int i = tile * cols + rest;
+      for (int at = thread; at < count * cols; at += threads) {
+        const int row = at / cols, col = at - row * cols;
+        const int i = tile * cols + col;
         if (i >= a.I) continue;
-        float v;
-        if (gated) v = WIDE ? few_act(total(place, row, 2 * col), a.act) * total(place, row, 2 * col + 1) : few_act(total(place, row, col), a.act) * total(place, row, col + 8);
-        else v = few_act(total(place, row, col), a.act);
+        // gate and up columns in turn, or (4 bits) in eights
+        const int gate = !gated ? col : WIDE ? 2 * col : 2 * col - col % 8;
+        float v = few_act(total(row, gate), a.act);
+        if (gated) v *= total(row, gate + (WIDE ? 1 : 8));
         const T h = Elem<T>::from_float(v);
         a.hidden[static_cast<int64_t>(r.slot[r.first[n] + row]) * a.I + i] = *reinterpret_cast<const uint16_t*>(&h);
       }
@@ -786,33 +787,29 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) few_experts_kernel(cons
   }
 
   FewMatrix down{a.w2, a.down, a.I, a.d, (a.I + F::kStep - 1) / F::kStep, F::kCols, kFewWarps, 1};
-  share_out(down, r.entries, kFewParts, F::kCost);
+  share_out<F>(down, r.entries, kFewParts, lane);
   const int shares = down.shares;
   {
     // the first weights of the down product are asked for before the wait for the rows that they multiply
     auto ahead = open(down, a.hidden, r.slot);
     auto c = ahead;
-#pragma unroll
-    for (int s = 0; s < F::kDepth - 1; ++s) {
-      ahead.copy_weights();
-      ahead.advance();
-    }
+#pragma unroll 1
+    for (int s = 0; s < F::kDepth - 1; ++s) ahead.copy(base + ring + s * F::kStage, true, false);
     if (!meet(a, 1, &r.go_on)) {
       copies_wait<0>();
       return;
     }
-#pragma unroll
+#pragma unroll 1
     for (int s = 0; s < F::kDepth - 1; ++s) {
-      c.copy_rows();
+      c.copy(base + ring + s * F::kStage, false, true);
       copies_commit();
-      c.advance();
     }
-    walk(c, [&](int n, int tile, int tiles, int share, auto total) {
-      const int count = r.count[n], cols = F::kCols * tiles;
-      for (int at = tid; at < count * cols; at += kFewThreads) {
-        const int row = at / cols, rest = at - row * cols;
-        const int i = tile * F::kCols + rest;
-        if (i < a.d) a.rows[(static_cast<int64_t>(share) * slots + r.slot[r.first[n] + row]) * a.d + i] = total(rest / F::kCols, row, rest % F::kCols);
+    walk(c, [&](int n, int tile, int share, int thread, int threads, auto total) {
+      const int count = r.count[n], cols = down.cols;
+      for (int at = thread; at < count * cols; at += threads) {
+        const int row = at / cols, col = at - row * cols;
+        const int i = tile * cols + col;
+        if (i < a.d) a.rows[(static_cast<int64_t>(share) * slots + r.slot[r.first[n] + row]) * a.d + i] = total(row, col);
       }
     });
   }
