@@ -9,8 +9,9 @@
 // The kept values are quotients of 16-bit values rounded once to fp32 and once to e4m3 (f8_quotients); everything else is fp32,
 // rounded once to 16 bits.
 //
-// Bound by HBM.  A lane takes 16 columns of a row, eight of them share a block; a warp walks a row (or, where there are few rows, a share
-// of one) 512 columns at a time and asks for the next ones before it computes.
+// Bound by HBM beside instructions (the forward pass issues about 300 per 16 columns: exponentials, reciprocals and exactly rounded quotients).
+// A lane takes 16 columns of a row, eight lanes share a block and ask for their next one before they compute.  The backward pass walks
+// a row (or, where there are few rows, a share of one) 512 columns at a time: the gradient of a slot's weight is a sum over its row.
 #include "f8.cuh"
 
 namespace moe {
@@ -85,55 +86,107 @@ __device__ __forceinline__ Wide wide_load(const void* base, int64_t row, int col
   return w;
 }
 
+// Two fp32 numbers in one register pair.
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+// f8_quotients, two at a time: the same operations, the same bits.
+__device__ __forceinline__ void act_quotients(float (&f)[16], float most) {
+  if (!(most <= 3.0e38f)) {
+    f8_quotients(f, most);
+    return;
+  }
+  const float near1 = most >= 1.0f ? 0x1p-60f : 0x1p60f;
+  const float d = most * near1, r = __frcp_rn(d);
+  const uint64_t c2 = pair_of(0.875f * near1, 0.875f * near1), r2 = pair_of(r, r), d2 = pair_of(-d, -d), top2 = pair_of(512.0f, 512.0f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint64_t v = mul_pair(pair_of(f[2 * i], f[2 * i + 1]), c2);
+    const uint64_t q = mul_pair(v, r2);
+    const uint64_t o = mul_pair(fma_pair(fma_pair(q, d2, v), r2, q), top2);
+    float o0, o1, v0, v1;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(o0), "=f"(o1) : "l"(o));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v0), "=f"(v1) : "l"(v));
+    f[2 * i] = copysignf(o0, v0);
+    f[2 * i + 1] = copysignf(o1, v1);
+  }
+}
+
+// A warp takes four blocks at a time, wherever rows end (where a row's last piece was half a warp's, 65536 x 2816 took 168 us).
 template <typename T, int ACT, bool LAYER>
 __global__ void __launch_bounds__(kActThreads, kActCtas) act_f8_forward_kernel(const ActArgs a) {
   constexpr bool GATED = act_gated(ACT);
   const int lane = threadIdx.x & 31;
   const int blocks = (a.cols + kF8Block - 1) / kF8Block;
   const int inter = GATED ? a.cols / 2 : a.cols;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kActThreads / 32);
   int64_t rows = a.rows;
   if constexpr (LAYER) rows = min(rows, static_cast<int64_t>(*a.num_mtiles) * MOE_TILE_M);
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * (kActThreads / 32) + (threadIdx.x >> 5); item < rows * a.split; item += warps) {
-    const int64_t row = item / a.split;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * (kActThreads / 8);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kActThreads / 8) + threadIdx.x / 8;
+  const int64_t stride_rows = stride / blocks;
+  const int stride_blocks = static_cast<int>(stride - stride_rows * blocks);
+  int64_t row = first / blocks;
+  int block = static_cast<int>(first - row * blocks);
+  const auto load = [&](int64_t r, int b) {
+    Wide w{};
+    if (r >= rows) return w;
     if constexpr (LAYER)
-      if (a.row_src[row] < 0) continue;
-    const int step = 512 * a.split;
-    const int first = static_cast<int>(item - row * a.split) * 512;
-    Wide next = wide_load(a.z, row, a.cols, first + lane * 16);
-    for (int c0 = first; c0 < a.cols; c0 += step) {
-      const Wide u = next;
-      const int at = c0 + lane * 16;
-      next = wide_load(a.z, row, c0 + step < a.cols ? a.cols : 0, at + step);
-      float f[16];
-      act_unpack<T>(u.a, f);
-      act_unpack<T>(u.b, f + 8);
-      if (at < a.cols) {
-        float h[16];
-        if constexpr (GATED) {
+      if (a.row_src[r] < 0) return w;
+    return wide_load(a.z, r, a.cols, b * kF8Block + (lane & 7) * 16);
+  };
+  Wide next = load(row, block);
+  while (__any_sync(0xFFFFFFFFu, row < rows)) {
+    const Wide u = next;
+    const int64_t this_row = row;
+    const int at = block * kF8Block + (lane & 7) * 16;
+    bool ok = row < rows && at < a.cols;
+    if constexpr (LAYER) ok = ok && a.row_src[this_row] >= 0;
+    row += stride_rows;
+    if ((block += stride_blocks) >= blocks) {
+      block -= blocks;
+      ++row;
+    }
+    next = load(row, block);
+    float f[16];
+    act_unpack<T>(u.a, f);
+    act_unpack<T>(u.b, f + 8);
+    if (ok) {
+      float h[16];
+      if constexpr (GATED) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = act_only<ACT>(f[2 * i]) * f[2 * i + 1];
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + row * inter + at / 2) = act_pack<T>(h);
-        } else {
+        for (int i = 0; i < 8; ++i) h[i] = act_only<ACT>(f[2 * i]) * f[2 * i + 1];
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + this_row * inter + at / 2) = act_pack<T>(h);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) h[i] = act_only<ACT>(f[i]);
-          uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + row * inter + at);
-          out[0] = act_pack<T>(h);
-          if (at + 8 < a.cols) out[1] = act_pack<T>(h + 8);
-        }
+        for (int i = 0; i < 16; ++i) h[i] = act_only<ACT>(f[i]);
+        uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.h) + this_row * inter + at);
+        out[0] = act_pack<T>(h);
+        if (at + 8 < a.cols) out[1] = act_pack<T>(h + 8);
       }
-      if (a.q == nullptr) continue;
-      float most = kF8Least;
+    }
+    if (a.q == nullptr) continue;
+    float most = kF8Least;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(f[i]));
+    for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(f[i]));
 #pragma unroll
-      for (int off = 4; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
-      f8_quotients(f, most);
-      if (at < a.cols) {
-        *reinterpret_cast<uint4*>(a.q + row * a.q_cols + at) =
-            make_uint4(f8x4(f[0], f[1], f[2], f[3]), f8x4(f[4], f[5], f[6], f[7]), f8x4(f[8], f[9], f[10], f[11]), f8x4(f[12], f[13], f[14], f[15]));
-        if ((lane & 7) == 0) a.scales[row * blocks + at / kF8Block] = most / kF8Top;
-      }
+    for (int off = 4; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
+    act_quotients(f, most);
+    if (ok) {
+      *reinterpret_cast<uint4*>(a.q + this_row * a.q_cols + at) =
+          make_uint4(f8x4(f[0], f[1], f[2], f[3]), f8x4(f[4], f[5], f[6], f[7]), f8x4(f[8], f[9], f[10], f[11]), f8x4(f[12], f[13], f[14], f[15]));
+      if ((lane & 7) == 0) a.scales[this_row * blocks + at / kF8Block] = most / kF8Top;
     }
   }
 }
@@ -278,7 +331,8 @@ static int run_act(const char* name, bool backward, ActArgs a, int inter, int ac
   a.split = 1;
   if (!layer)
     while (a.split < units && a.rows * a.split < resident) ++a.split;
-  const int64_t want = (a.rows * a.split + kActThreads / 32 - 1) / (kActThreads / 32);
+  const int64_t pieces = backward ? a.rows * a.split : (a.rows * ((a.cols + kF8Block - 1) / kF8Block) + 3) / 4;
+  const int64_t want = (pieces + kActThreads / 32 - 1) / (kActThreads / 32);
   const int64_t most = static_cast<int64_t>(sm_count()) * kActCtas;
   const int grid = static_cast<int>(want < most ? want : most);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

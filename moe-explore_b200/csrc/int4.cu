@@ -95,10 +95,114 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) q4_rows_kernel(const Q4Args 
   }
 }
 
-template <typename T, int NG, bool ZEROS> static int launch_q4_rows(const Q4Args& a, cudaStream_t s) {
-  const auto kernel = q4_rows_kernel<T, NG, ZEROS>;
-  constexpr int smem = kQ4Warps * kQ4Ring<NG, ZEROS>;
-  static std::atomic<bool> prepared[64];
+// More rows, 8 MT at a time.  A CTA takes eight tiles, two per warp, and the rows; its warps go through the steps together, so that a step's
+// columns of the rows lie in shared memory once, and the numbers made of a word are used for all rows.
+constexpr int kQ4ManyWarps = 4, kQ4ManyDepth = 3;
+template <int NG, bool ZEROS, int MT> struct Q4Many {
+  static constexpr int kBlock = Q4Stage<NG, ZEROS>::kBlock, kRows = kQ4ManyWarps * kQ4Tiles * kBlock, kStage = kRows + MT * 2048;
+  static constexpr int kCols = kQ4ManyWarps * kQ4Cols, kTokens = 8 * MT;
+  static constexpr int kSums = kTokens * kCols * 4;  // [token][column], where the stages were
+  static constexpr int kTotal = kQ4ManyDepth * kStage > kSums ? kQ4ManyDepth * kStage : kSums;
+};
+template <typename T, int NG, bool ZEROS, int MT>
+__global__ void __launch_bounds__(kQ4ManyWarps * 32, MT == 8 ? 2 : 3) q4_many_kernel(const Q4Args a) {
+  using P = Q4Many<NG, ZEROS, MT>;
+  extern __shared__ __align__(128) uint8_t stages[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = a.ranks > 1 ? static_cast<int>(blockIdx.x) % a.ranks : 0;
+  const int64_t tile = static_cast<int64_t>(blockIdx.x / a.ranks) * (kQ4ManyWarps * kQ4Tiles) + warp * kQ4Tiles;
+  const int row0 = blockIdx.y * P::kTokens, count = min(a.rows - row0, P::kTokens);
+  const uint8_t* data = a.w.data + tile * a.w.steps * P::kBlock + lane * 16;
+  const int64_t apart = tile + 1 < a.w.tiles ? static_cast<int64_t>(a.w.steps) * P::kBlock : 0;
+  const int piece = tid & 15, r8 = tid >> 4;  // of the rows: this thread copies one 16-byte piece of rows r8, r8 + 8, ...
+  const uint16_t* x = a.x + static_cast<int64_t>(row0 + (r8 < count ? r8 : 0)) * a.K + 8 * piece;
+  const uint32_t base = smem_u32(stages), row_to = P::kRows + r8 * 256 + ((piece ^ ((r8 & 1) << 2)) << 4);
+  const uint32_t row_at = P::kRows + (lane >> 2) * 256 + (((lane & 3) ^ (((lane >> 2) & 1) << 2)) << 4);
+  const auto copy = [&](uint32_t stage, int step) {
+    if (step < a.w.steps) {
+      if (tile < a.w.tiles) q4_copy<NG, ZEROS>(stage + warp * kQ4Tiles * P::kBlock, data + static_cast<int64_t>(step) * P::kBlock, apart, lane);
+      const int at = step * kQ4Step;
+      const bool real = at + 8 * piece < a.K;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        if (r8 + 8 * m < count) copy_16_or_zeros(stage + row_to + m * 2048, real ? x + static_cast<int64_t>(8 * m) * a.K + at : a.x, real);
+    }
+    copies_commit();
+  };
+  float acc[kQ4Tiles][MT][4];
+#pragma unroll
+  for (int t = 0; t < kQ4Tiles; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[t][m][0] = acc[t][m][1] = acc[t][m][2] = acc[t][m][3] = 0.0f;
+#pragma unroll
+  for (int s = 0; s < kQ4ManyDepth - 1; ++s) copy(base + s * P::kStage, rank + s * a.ranks);
+  uint32_t from = base, spent = base + (kQ4ManyDepth - 1) * P::kStage;
+#pragma unroll 1
+  for (int step = rank; step < a.w.steps; step += a.ranks) {
+    copies_wait<kQ4ManyDepth - 2>();
+    __syncthreads();  // everybody's copies of this step, and everybody is through with the stage that is filled next
+    copy(spent, step + (kQ4ManyDepth - 1) * a.ranks);
+    Q4Piece<NG, ZEROS> p[kQ4Tiles];
+#pragma unroll
+    for (int t = 0; t < kQ4Tiles; ++t) q4_take<NG, ZEROS>(p[t], from + (warp * kQ4Tiles + t) * P::kBlock, lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t n[kQ4Tiles][2][4];
+      float scale[kQ4Tiles][2];
+#pragma unroll
+      for (int t = 0; t < kQ4Tiles; ++t) {
+        q4_numbers<T, NG, ZEROS>(n[t], p[t], i);
+        scale[t][0] = q4_scale<T>(p[t].scale[0], i * NG / 4);
+        scale[t][1] = q4_scale<T>(p[t].scale[1], i * NG / 4);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const uint4 b = lds_128(from + (row_at ^ (64 * (i & 1))) + 128 * (i >> 1) + m * 2048);
+#pragma unroll
+        for (int t = 0; t < kQ4Tiles; ++t) {
+          float sum[4];
+          mma_16x8x16_first<T>(sum, n[t][0], b.x, b.y);
+          mma_16x8x16<T>(sum, n[t][1], b.z, b.w);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[t][m][c] = fmaf(sum[c], scale[t][c >> 1], acc[t][m][c]);
+        }
+      }
+    }
+    spent = from;
+    from = from == base + (kQ4ManyDepth - 1) * P::kStage ? base : from + P::kStage;
+  }
+  copies_wait<0>();
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(stages);
+#pragma unroll
+  for (int t = 0; t < kQ4Tiles; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        sums[(8 * m + 2 * (lane & 3) + (c & 1)) * P::kCols + warp * kQ4Cols + t * kQ4Rows + (lane >> 2) + 8 * (c >> 1)] = acc[t][m][c];
+  __syncthreads();
+  if (a.ranks > 1) cluster_sync_all();
+  // the ranks share out the tokens
+  const int n = static_cast<int>(blockIdx.x / a.ranks) * P::kCols + tid;
+  for (int t = rank; t < count; t += a.ranks) {
+    float v = 0.0f;
+    if (a.ranks > 1) {
+      for (int r = 0; r < a.ranks; ++r) v += load_cluster(mapa_shared(smem_u32(&sums[t * P::kCols + tid]), r));
+    } else {
+      v = sums[t * P::kCols + tid];
+    }
+    if (n < a.N) {
+      const T w = Elem<T>::from_float(v);
+      a.out[static_cast<int64_t>(row0 + t) * a.N + n] = *reinterpret_cast<const uint16_t*>(&w);
+    }
+  }
+  __syncthreads();
+  if (a.ranks > 1) cluster_sync_all();  // the others' shared memory lives until it has been read
+}
+
+template <typename Kernel> static int launch_q4(Kernel kernel, std::atomic<bool> (&prepared)[64], const Q4Args& a, int64_t groups, int rows_at_once, int warps,
+                                                int smem, cudaStream_t s) {
   int dev = 0;
   MOE_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !prepared[dev].load(std::memory_order_acquire)) {
@@ -106,9 +210,9 @@ template <typename T, int NG, bool ZEROS> static int launch_q4_rows(const Q4Args
     if (dev < 64) prepared[dev].store(true, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((a.w.tiles + kQ4Tiles - 1) / kQ4Tiles * a.ranks), static_cast<unsigned>((a.rows + 7) / 8), 1);
-  cfg.blockDim = dim3(kQ4Warps * 32, 1, 1);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(static_cast<unsigned>(groups * a.ranks), static_cast<unsigned>((a.rows + rows_at_once - 1) / rows_at_once), 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(warps * 32), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -119,6 +223,27 @@ template <typename T, int NG, bool ZEROS> static int launch_q4_rows(const Q4Args
   cfg.numAttrs = a.ranks > 1 ? 1 : 0;
   MOE_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   return MOE_OK;
+}
+// CTAs share a group of tiles while SMs would stay idle and each of them has `least` steps.
+static int q4_ranks(int64_t ctas, int64_t wanted, int steps, int least) {
+  int ranks = 1;
+  while (ranks < 8 && ctas * ranks < wanted && steps >= 2 * least * ranks) ranks *= 2;
+  return ranks;
+}
+template <typename T, int NG, bool ZEROS, int MT> static int launch_q4_many(Q4Args a, cudaStream_t s) {
+  static std::atomic<bool> prepared[64];
+  const int64_t groups = (a.w.tiles + kQ4ManyWarps * kQ4Tiles - 1) / (kQ4ManyWarps * kQ4Tiles);
+  a.ranks = q4_ranks(groups * ((a.rows + 8 * MT - 1) / (8 * MT)), sm_count(), a.w.steps, 2);
+  return launch_q4(q4_many_kernel<T, NG, ZEROS, MT>, prepared, a, groups, 8 * MT, kQ4ManyWarps, Q4Many<NG, ZEROS, MT>::kTotal, s);
+}
+template <typename T, int NG, bool ZEROS> static int launch_q4_rows(Q4Args a, cudaStream_t s) {
+  if (a.rows > 32) return launch_q4_many<T, NG, ZEROS, 8>(a, s);
+  if (a.rows > 16) return launch_q4_many<T, NG, ZEROS, 4>(a, s);
+  if (a.rows > 8) return launch_q4_many<T, NG, ZEROS, 2>(a, s);
+  static std::atomic<bool> prepared[64];
+  const int64_t pairs = (a.w.tiles + kQ4Tiles - 1) / kQ4Tiles;
+  a.ranks = q4_ranks(pairs * ((a.rows + 7) / 8), 2 * sm_count(), a.w.steps, 2 * kQ4Warps);
+  return launch_q4(q4_rows_kernel<T, NG, ZEROS>, prepared, a, pairs, 8, kQ4Warps, kQ4Warps * kQ4Ring<NG, ZEROS>, s);
 }
 template <typename T> static int launch_q4_groups(const Q4Args& a, int group, bool z, cudaStream_t s) {
   if (group == 128) return z ? launch_q4_rows<T, 1, true>(a, s) : launch_q4_rows<T, 1, false>(a, s);
@@ -132,7 +257,7 @@ using namespace moe;
 
 extern "C" int moe_int4_matmul(const void* x, const void* data, void* out, int64_t rows, int k_dim, int n_dim, int group, int zeros, int dtype,
                                void* stream) {
-  MOE_CHECK_ARG(rows >= 0 && rows <= (1 << 19) && k_dim > 0 && n_dim > 0, "moe_int4_matmul: %lld rows (at most 2^19), K=%d, N=%d",
+  MOE_CHECK_ARG(rows >= 0 && rows <= (1 << 21) && k_dim > 0 && n_dim > 0, "moe_int4_matmul: %lld rows (at most 2^21), K=%d, N=%d",
                 static_cast<long long>(rows), k_dim, n_dim);
   MOE_CHECK_ARG(group == 32 || group == 64 || group == 128, "moe_int4_matmul: groups of 32, 64 or 128 columns, got %d", group);
   MOE_CHECK_ARG(dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16, "moe_int4_matmul: unknown dtype %d", dtype);
@@ -152,10 +277,6 @@ extern "C" int moe_int4_matmul(const void* x, const void* data, void* out, int64
   a.rows = static_cast<int>(rows);
   a.K = k_dim;
   a.N = n_dim;
-  // CTAs share a pair of tiles while SMs would stay idle and each of their warps has two steps
-  const int64_t row_blocks = (rows + 7) / 8;
-  a.ranks = 1;
-  while (a.ranks < 8 && (a.w.tiles + kQ4Tiles - 1) / kQ4Tiles * row_blocks * a.ranks < 2ll * sm_count() && a.w.steps >= 4 * kQ4Warps * a.ranks) a.ranks *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == MOE_DTYPE_BF16 ? launch_q4_groups<__nv_bfloat16>(a, group, zeros != 0, s) : launch_q4_groups<__half>(a, group, zeros != 0, s);
 }

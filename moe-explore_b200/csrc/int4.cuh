@@ -201,6 +201,22 @@ __device__ __forceinline__ uint32_t q4_pair(uint32_t word, uint32_t magic) {
   return r;
 }
 
+// Word i of a tile as the two fragments of its products.
+template <typename T, int NG, bool ZEROS> __device__ __forceinline__ void q4_numbers(uint32_t (&a)[2][4], const Q4Piece<NG, ZEROS>& p, int i) {
+  const int j = i * NG / 4;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t bias = Q4Magic<T>::kEight;
+    if constexpr (ZEROS) {
+      const uint32_t z = (p.zero[h] >> (8 * j)) & 15u;
+      bias = Q4Magic<T>::kBits | z | (z << 16);
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)  // pair q of the words of rows g and g + 8: fragment q / 2, its first or second eight columns
+      a[q >> 1][2 * (q & 1) + h] = sub2(q4_pair(word_of(p.w[h], i) >> (4 * q), Q4Magic<T>::kBits), bias, T());
+  }
+}
+
 // acc[tile] += the tiles' products with up to eight rows over one step, by groups.
 template <typename T, int NG, bool ZEROS>
 __device__ __forceinline__ void q4_step(float (&acc)[kQ4Tiles][4], uint32_t stage, uint32_t row_at, int lane) {
@@ -216,18 +232,7 @@ __device__ __forceinline__ void q4_step(float (&acc)[kQ4Tiles][4], uint32_t stag
 #pragma unroll
     for (int t = 0; t < kQ4Tiles; ++t) {
       uint32_t a[2][4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t bias = Q4Magic<T>::kEight;
-        if constexpr (ZEROS) {
-          const uint32_t z = (p[t].zero[h] >> (8 * j)) & 15u;
-          bias = Q4Magic<T>::kBits | z | (z << 16);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {  // pair q of the words of rows g and g + 8: fragment q / 2, its first or second eight columns
-          a[q >> 1][2 * (q & 1) + h] = sub2(q4_pair(word_of(p[t].w[h], i) >> (4 * q), Q4Magic<T>::kBits), bias, T());
-        }
-      }
+      q4_numbers<T, NG, ZEROS>(a, p[t], i);
       if (i % kPerGroup == 0) mma_16x8x16_first<T>(sum[t], a[0], b.x, b.y);
       else mma_16x8x16<T>(sum[t], a[0], b.x, b.y);
       mma_16x8x16<T>(sum[t], a[1], b.z, b.w);
