@@ -325,7 +325,7 @@ template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int
   }
   // open experts' keys are 2 and above (NaN and -inf 2: they come last, lowest index first), taken and closed ones below
   uint32_t key[EACH];
-  const auto key_of = [](float v) { return v > -3.402823466e38f ? ordered(v) : 2u; };
+  const auto key_of = [](float v) { return v > -3.402823466e38f ? ordered(v + 0.0f) : 2u; };  // (-0 is 0)
   float most = -3.402823466e38f, sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
@@ -734,6 +734,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) few_experts_kernel(cons
         spent = from;
         from = from == ring + (F::kDepth - 1) * F::kStage ? ring : from + F::kStage;
       }
+      __syncwarp();  // every lane is through with the last stage, where the sums go
 #pragma unroll
       for (int q = 0; q < F::kProducts; ++q)
 #pragma unroll

@@ -43,6 +43,8 @@ def few_token_layer(input: torch.Tensor, params, residual=None, addend=None, nor
     tokens, a gradient, another device than the current one, something that watches the single ops, routers or sizes that they do not know.
 
     The logits are not rounded to 16 bits, equal ones are taken in ascending index; an expert's rows are not rounded before the fold."""
+    if residual is not None and norm is None:
+        raise ValueError("residual is added by the layer's norm: norm is None")
     ep, rp = params.expert_params, params.router_params
     int4 = type(ep) is Int4ExpertParams
     if not int4 and type(ep) is not MLPParams or type(input) not in _PLAIN or input.dim() != 2 or not 0 < input.size(0) <= _native.FEW_TOKENS or \

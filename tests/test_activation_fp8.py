@@ -303,6 +303,10 @@ def test_layer_in_training(normed, native):
 def test_training_step_in_a_graph(native):
     leaves, indices, dy = experts(96, 128, 8, 2, 64, "swiglu", torch.bfloat16)
     step = lambda: torch.autograd.grad(routed_expert_compute(*leaves, indices, 8, 2, "swiglu", save_fp8=True), leaves, dy)
+    # an eager graph of the same values (of the same leaves torch's engine would make the capture wait for the eager stream, and refuses)
+    others = [t.detach().clone().requires_grad_(True) for t in leaves]
+    alive = routed_expert_compute(*others, indices, 8, 2, "swiglu", save_fp8=True)
+    want = torch.autograd.grad(alive, others, dy, retain_graph=True)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -311,6 +315,9 @@ def test_training_step_in_a_graph(native):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         grads = step()
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(alive, others, dy), want))
     with torch.no_grad():
         leaves[0].copy_(torch.randn(96, 128, device="cuda"))
         indices.copy_(indices.flip(0))

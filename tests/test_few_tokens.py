@@ -223,6 +223,22 @@ def test_equal_logits_duplicates_and_bad_experts(native):
 
 
 @gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_all_slots_on_few_experts(bits, native):
+    """Every token to every expert, 16 rows each (two blocks of eight), 16 slots per token, and the deepest and the shallowest rows."""
+    g = gen(20)
+    for T, d, E, inter in ((16, 136, 16, 8), (9, 8, 3, 1032), (16, 1032, 2, 264)):
+        experts, w1, w2 = make_experts(g, bits, E, d, inter, "swiglu", torch.bfloat16, 32)
+        rp = make_router(g, "topk norm", d, E, E, torch.bfloat16)
+        x = torch.randn(T, d, generator=g, device="cuda").bfloat16()
+        with torch.no_grad():
+            out = few_token_layer(x, MOEParams(rp, experts, E, E))
+        y = x.double()
+        assert near(out, experts64(y, *route64(rp, y @ rp.router_weight.double()), w1, w2, "swiglu"), torch.bfloat16, 2)
+    native.check_status(device_status(0))
+
+
+@gpu
 def test_values_that_are_not_finite(native):
     """A token that holds NaN or an infinity spoils its own row only."""
     g = gen(10)
@@ -399,5 +415,7 @@ def test_refusals(native):
         int4_expert_compute(x, s, i, q, addend=x[:1])
     with pytest.raises(RuntimeError, match="CUDA"):
         int4_expert_compute(x, s.cpu(), i, q)
+    with pytest.raises(ValueError, match="norm is None"):
+        few_token_layer(x, MOEParams(make_router(g, "topk", 64, 8, 2, torch.bfloat16), q, 8, 2), residual=x)
     with pytest.raises(RuntimeError, match="trace"):
         torch.jit.trace(lambda t: int4_expert_compute(t, s, i, q), (x,), check_trace=False)
