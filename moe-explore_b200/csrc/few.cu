@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a)
   const int left = a.E - (col0 + 4 * cv);
   const bool whole = left >= 4 && (a.E & 3) == 0, mine = a.router != nullptr && left > 0;
   const W* router = static_cast<const W*>(a.router) + static_cast<int64_t>(k_begin) * a.E + col0 + 4 * cv;
-  constexpr int AHEAD = 4;
+  constexpr int AHEAD = 2;
   float w[AHEAD][4];
   const auto ask = [&](int i, float (&f)[4]) {
     if (mine && i < count) router_row<W>(router + static_cast<int64_t>(i) * a.E, left, whole, f);
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a)
     const T* x = static_cast<const T*>(a.x) + static_cast<int64_t>(t) * a.d + k_begin;
     const T* residual = a.residual == nullptr ? nullptr : static_cast<const T*>(a.residual) + static_cast<int64_t>(t) * a.d + k_begin;
     float sum = 0.0f, large = 0.0f, most = 0.0f;
-#pragma unroll 2
+#pragma unroll 1
     for (int i = lane * 8; i < share; i += 256) {
       float h[8] = {}, g[8];
       if (i < count) {
