@@ -9,7 +9,8 @@
 // The kept values are quotients of 16-bit values rounded once to fp32 and once to e4m3 (f8_quotients); everything else is fp32,
 // rounded once to 16 bits.
 //
-// Bound by HBM beside instructions (the forward pass issues about 300 per 16 columns: exponentials, reciprocals and exactly rounded quotients).
+// Bound by HBM beside instructions (the forward pass issues about 300 per 16 columns: exponentials, reciprocals and exactly rounded quotients;
+// 72 % of the issue slots): 65536 x 2816 swiglu 132 us forward and 129 back, 114 each at the copy's rate; geglu 182 and 188 (erff).
 // A lane takes 16 columns of a row, eight lanes share a block and ask for their next one before they compute.  The backward pass walks
 // a row (or, where there are few rows, a share of one) 512 columns at a time: the gradient of a slot's weight is a sum over its row.
 #include "f8.cuh"

@@ -4,7 +4,10 @@
 //   second:  scores and experts of every token (each CTA for itself);  hidden = round(act(y W1[e])) for the chosen experts;
 //            rows = hidden W2[e] in fp32;  out = round(sum over the slots of score * row + addend)
 //
-// Bound by reading the chosen experts' weights once.  The second kernel is one resident wave (a cooperative launch, so that its CTAs may
+// Bound by reading the chosen experts' weights once (16 bits: 16 tokens x 8 on 64 experts of 2048 x 1024, 711 MB, in 136 us, the up product's
+// part at 6.7 TB/s), by what it costs to make numbers of 4-bit ones (64 experts of 7168 x 2048, 1.2 GB, 305 us), and for one token by what
+// is not reading: of 37 us for 69 MB the first kernel and the way to the second are 8, choosing 4, meeting twice 4.  The second kernel
+// is one resident wave (a cooperative launch, so that its CTAs may
 // wait for one another): between its three phases they meet at a counter in global memory that the first kernel has set to zero.
 // Every sum has a fixed order: nothing depends on timing.
 //

@@ -13,8 +13,11 @@
 // bits of 128 (bf16) or 1024 (fp16), whose last mantissa bits it then is, and subtracting 128 + zero (1024 + zero), exactly.  Word i
 // holds columns of one group of 32 for all lanes, so the scale is applied to the fp32 sums of a group: no weight is ever rounded.
 //
-// Tensor cores by mma.sync, because the weights are made in registers and there are only 16 of their rows: per KB of weights a warp issues 88
-// instructions to make them and 8 to multiply; the 56 integer ones among them are what bounds the rate beside HBM.
+// Tensor cores by mma.sync, because the weights are made in registers and a tile has only 16 of their rows: per KB of weights a warp issues 88
+// instructions to make them (56 of them on the integer pipe, which takes one every other cycle), 8 to multiply and about 70 around them.  So
+// long streams are bound by issuing, at 3.5 to 4 TB/s of weights.  (Two tiles per warp instead of one: 382 us instead of 420 for 64
+// experts of 7168 x 2048; the pair of numbers masked and given its exponent by one lop3, which the compiler makes two of: 320; four
+// tiles: no gain.)
 #pragma once
 
 #include "common.cuh"

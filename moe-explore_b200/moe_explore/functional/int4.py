@@ -196,7 +196,7 @@ def int4_matmul(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     if _native.needs_gradient(x):
         raise RuntimeError("products with 4-bit weights have no backward pass: call this under torch.no_grad()")
     with _native.on_device_of(x):
-        rows = _dense(x.detach().reshape(-1, weight.k))
-        out = torch.empty(rows.size(0), weight.n, dtype=x.dtype, device=x.device)
+        rows = _dense(x if x.dim() == 2 else x.reshape(-1, weight.k))
+        out = x.new_empty((rows.size(0), weight.n))
         _native.int4_matmul(rows, weight, out)
-    return out.view(*x.shape[:-1], weight.n)
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], weight.n)
