@@ -651,8 +651,10 @@ int moe_act_f8_backward(const void* q, const float* scales, const void* dh, void
  *   values: byte (half * 32 + 4 r + t) * 16 + 4 i + b holds row r + 8 half, columns 32 i + 8 t + 4 (b % 2) + b / 2 (low four bits) and two
  *   behind (high);  scales, zeros: [16 rows][128 / group].  Rows behind n_dim and columns behind k_dim hold zeros.
  * x and data 16-byte aligned, k_dim and n_dim multiples of 8.
- * out [rows, n_dim] = x [rows, k_dim] @ w^T.
+ * moe_int4_matmul: out [rows, n_dim] = x [rows, k_dim] @ w^T.  moe_int4_expand: out [matrices, k_dim, n_dim], the weights in 16 bits, each
+ * rounded once; gated: eight rows of w become the even, the next eight the odd columns of 16.
  * --------------------------------------------------------------------------------- */
+int moe_int4_expand(const void* data, void* out, int64_t matrices, int k_dim, int n_dim, int group, int zeros, int gated, int dtype, void* stream);
 int moe_int4_matmul(const void* x, const void* data, void* out, int64_t rows, int k_dim, int n_dim, int group, int zeros, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------

@@ -254,6 +254,55 @@ template <typename T> static int launch_q4_groups(const Q4Args& a, int group, bo
   return z ? launch_q4_rows<T, 4, true>(a, s) : launch_q4_rows<T, 4, false>(a, s);
 }
 
+// The weights as 16-bit matrices [K, N] (N contiguous), each value times its scale rounded once: for passes of so many rows that 16-bit
+// products of whole tiles are cheaper than making the numbers again for every few of them.  GATED: eight rows of the gate and eight of
+// the up matrix in turn become columns in turn.  A CTA takes a step of four tiles: 128 rows of the result, 64 columns.
+template <typename T, int NG, bool ZEROS, bool GATED>
+__global__ void __launch_bounds__(256) q4_expand_kernel(const uint8_t* data, int64_t tiles, int steps, int K, int N, uint16_t* out) {
+  constexpr int kBlock = Q4Stage<NG, ZEROS>::kBlock, TILES = 4;
+  __shared__ __align__(16) uint8_t blocks[TILES][kBlock];
+  const int step = blockIdx.x;
+  const int64_t tile0 = static_cast<int64_t>(blockIdx.y) * TILES, matrix = blockIdx.z;
+  for (int at = threadIdx.x; at < TILES * (kBlock / 16); at += 256) {
+    const int t = at / (kBlock / 16), p = at - t * (kBlock / 16);
+    if (tile0 + t < tiles)
+      reinterpret_cast<uint4*>(blocks[t])[p] = __ldg(reinterpret_cast<const uint4*>(data + ((matrix * tiles + tile0 + t) * steps + step) * kBlock) + p);
+  }
+  __syncthreads();
+  for (int item = threadIdx.x; item < kQ4Step * TILES * 2; item += 256) {
+    const int k = item / (TILES * 2), eight = item % (TILES * 2), t = eight / 2;  // row of the result, eight of its columns
+    const int64_t column = tile0 * kQ4Rows + eight * 8;
+    if (step * kQ4Step + k >= K || column >= N) continue;
+    const int low = k % 8, j = k * NG / kQ4Step;
+    const int byte = (k % 32 / 8) * 16 + 4 * (k / 32) + (low % 2) * 2 + low / 4, shift = low % 4 / 2 * 4;
+    float v[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const int of16 = 8 * (eight % 2) + c, row = GATED ? of16 / 2 + 8 * (of16 % 2) : of16;
+      const int value = blocks[t][(row / 8 * 32 + 4 * (row % 8)) * 16 + byte] >> shift & 15;
+      const int zero = ZEROS ? blocks[t][1024 + 32 * NG + row * NG + j] : 8;
+      v[c] = static_cast<float>(value - zero) * Elem<T>::to_float(reinterpret_cast<const T*>(blocks[t] + 1024)[row * NG + j]);
+    }
+    *reinterpret_cast<uint4*>(out + (matrix * K + step * kQ4Step + k) * N + column) =
+        make_uint4(Elem<T>::pack2(v[0], v[1]), Elem<T>::pack2(v[2], v[3]), Elem<T>::pack2(v[4], v[5]), Elem<T>::pack2(v[6], v[7]));
+  }
+}
+template <typename T, int NG, bool ZEROS>
+static void launch_q4_expand(const void* data, int64_t matrices, int K, int N, bool gated, void* out, cudaStream_t s) {
+  const int64_t tiles = (N + kQ4Rows - 1) / kQ4Rows;
+  const int steps = (K + kQ4Step - 1) / kQ4Step;
+  const dim3 grid(static_cast<unsigned>(steps), static_cast<unsigned>((tiles + 3) / 4), static_cast<unsigned>(matrices));
+  const uint8_t* from = static_cast<const uint8_t*>(data);
+  uint16_t* to = static_cast<uint16_t*>(out);
+  if (gated) q4_expand_kernel<T, NG, ZEROS, true><<<grid, 256, 0, s>>>(from, tiles, steps, K, N, to);
+  else q4_expand_kernel<T, NG, ZEROS, false><<<grid, 256, 0, s>>>(from, tiles, steps, K, N, to);
+}
+template <typename T> static void launch_q4_expand_groups(const void* data, int64_t matrices, int K, int N, int group, bool z, bool gated, void* out, cudaStream_t s) {
+  if (group == 128) z ? launch_q4_expand<T, 1, true>(data, matrices, K, N, gated, out, s) : launch_q4_expand<T, 1, false>(data, matrices, K, N, gated, out, s);
+  else if (group == 64) z ? launch_q4_expand<T, 2, true>(data, matrices, K, N, gated, out, s) : launch_q4_expand<T, 2, false>(data, matrices, K, N, gated, out, s);
+  else z ? launch_q4_expand<T, 4, true>(data, matrices, K, N, gated, out, s) : launch_q4_expand<T, 4, false>(data, matrices, K, N, gated, out, s);
+}
+
 }  // namespace moe
 
 using namespace moe;
@@ -282,4 +331,24 @@ extern "C" int moe_int4_matmul(const void* x, const void* data, void* out, int64
   a.N = n_dim;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == MOE_DTYPE_BF16 ? launch_q4_groups<__nv_bfloat16>(a, group, zeros != 0, s) : launch_q4_groups<__half>(a, group, zeros != 0, s);
+}
+
+extern "C" int moe_int4_expand(const void* data, void* out, int64_t matrices, int k_dim, int n_dim, int group, int zeros, int gated, int dtype,
+                               void* stream) {
+  MOE_CHECK_ARG(matrices >= 0 && matrices <= 65535 && k_dim > 0 && n_dim > 0, "moe_int4_expand: %lld matrices (at most 65535), K=%d, N=%d",
+                static_cast<long long>(matrices), k_dim, n_dim);
+  MOE_CHECK_ARG(group == 32 || group == 64 || group == 128, "moe_int4_expand: groups of 32, 64 or 128 columns, got %d", group);
+  MOE_CHECK_ARG(dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16, "moe_int4_expand: unknown dtype %d", dtype);
+  if (k_dim % 8 != 0 || n_dim % (gated ? 16 : 8) != 0 || k_dim > (1 << 21) || n_dim > (1 << 21)) {
+    set_error("moe_int4_expand: K=%d must be a multiple of 8 and N=%d of 8 (gated: 16), up to 2^21", k_dim, n_dim);
+    return MOE_ERR_UNSUPPORTED;
+  }
+  if (matrices == 0) return MOE_OK;
+  MOE_CHECK_ARG(data && out, "moe_int4_expand: null pointer argument");
+  MOE_CHECK_ARG(((reinterpret_cast<uintptr_t>(data) | reinterpret_cast<uintptr_t>(out)) & 15) == 0, "moe_int4_expand: pointers must be 16-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == MOE_DTYPE_BF16) launch_q4_expand_groups<__nv_bfloat16>(data, matrices, k_dim, n_dim, group, zeros != 0, gated != 0, out, s);
+  else launch_q4_expand_groups<__half>(data, matrices, k_dim, n_dim, group, zeros != 0, gated != 0, out, s);
+  MOE_CUDA(cudaGetLastError());
+  return MOE_OK;
 }

@@ -134,6 +134,7 @@ SIGNATURES = {
     "moe_act_f8_forward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
     "moe_act_f8_backward": (c_int, [c_void_p] * 4 + [c_int64, c_int, c_int, c_int, c_void_p]),
     "moe_int4_matmul": (c_int, [c_void_p] * 3 + [c_int64] + [c_int] * 5 + [c_void_p]),
+    "moe_int4_expand": (c_int, [c_void_p] * 2 + [c_int64] + [c_int] * 6 + [c_void_p]),
     "moe_few_pass_size": (c_size_t, []),
     "moe_few_workspace_bytes": (c_size_t, [c_int] * 5),
     "moe_few_tokens": (c_int, [POINTER(FewPass), c_void_p]),
@@ -548,6 +549,15 @@ def int4_matmul(x, weight, out):
         rc = load().moe_int4_matmul(x.data_ptr(), weight.data.data_ptr(), out.data_ptr(), x.size(0), weight.k, weight.n, weight.group,
                                     weight.zeros, dtype_code(x.dtype), _stream())
     _check("moe_int4_matmul", rc)
+    _count(1)
+
+
+def int4_expand(weight, gated: bool, out):
+    """out [E, K, N] = the matrices of an ``Int4Weight`` with one axis in front, in 16 bits (see moe_int4_expand)."""
+    with timed("int4:expand"):
+        rc = load().moe_int4_expand(weight.data.data_ptr(), out.data_ptr(), out.size(0), weight.k, weight.n, weight.group, weight.zeros, gated,
+                                    dtype_code(out.dtype), _stream())
+    _check("moe_int4_expand", rc)
     _count(1)
 
 

@@ -9,6 +9,7 @@ from __future__ import annotations
 import torch
 
 from moe_explore import _native
+from moe_explore.expert_compute import routed_expert_compute
 from moe_explore.functional.activation import is_glu
 from moe_explore.functional.fp8 import _dense
 from moe_explore.params import ErnieRouterParams, GroupedTopkRouterParams, Int4ExpertParams, MLPParams, TopkRouterParams
@@ -131,11 +132,33 @@ def _launch(p, x, topk: int, addend, held):
     return out
 
 
+# Above, the experts' weights are brought to 16 bits once and the pass is the 16-bit one.  Both grow with the weights, so the line does not move
+# much (us, 16 tokens at a time / in 16 bits: 64 experts of 7168 x 2048, 64 tokens 1320 / 2305, 96 1877 / 2306, 256 5093 / 2307; 64 of 2048 x
+# 1024 362 / 434, 513 / 443, 1206 / 420; 60 of 2048 x 1408 304 / 497, 448 / 492, 1090 / 491).
+EXPAND_FROM = 96
+
+
+def int4_experts_in_16_bits(params: Int4ExpertParams) -> MLPParams:
+    """The experts in 16 bits, each weight rounded once: what ``int4_expert_compute`` makes for itself when there are many tokens, for callers
+    that want to keep it for a while (four times the memory)."""
+    params.up.checked(1, "up")
+    params.down.checked(1, "down")
+    act = None if params.activation is None else str(params.activation)
+    with _native.on_device_of(params.up.data):
+        made = []
+        for w, gated in ((params.up, is_glu(act)), (params.down, False)):
+            out = torch.empty(w.data.size(0), w.k, w.n, dtype=w.dtype, device=w.data.device)
+            _native.int4_expand(w, gated, out)
+            made.append(out)
+    return MLPParams(*made, params.activation)
+
+
 def int4_expert_compute(x, scores, indices, params: Int4ExpertParams, addend=None) -> torch.Tensor:
     """out[t] = sum_s scores[t, s] * (act(x[t] @ up[e]^T) @ down[e]^T) with e = indices[t, s], the weights in 4 bits.  ``x`` [T, d] in the type
     of their scales, ``scores`` (rounded to that type) and ``indices`` (int64) [T, k]; slots with an expert id out of range add nothing (and
-    are reported by the status word).  ``addend`` [T, d] is added by the fold.  For serving: no gradients.  Made for decoding: every 16
-    tokens read the weights of the experts that they chose."""
+    are reported by the status word).  ``addend`` [T, d] is added by the fold.  For serving: no gradients.  Up to 96 tokens go through the
+    kernel for a few, 16 at a time; for more the weights are brought to 16 bits first (rounded there; as much memory as 16-bit experts
+    take, for the time of the call) and the pass is ``routed_expert_compute``'s."""
     params.up.checked(1, "up")
     params.down.checked(1, "down")
     _native.require_cuda(x, scores, indices, addend)
@@ -160,6 +183,10 @@ def int4_expert_compute(x, scores, indices, params: Int4ExpertParams, addend=Non
                          f"[{params.up.n}, {params.up.k}], down [{params.down.n}, {params.down.k}] for {act!r}, {E} experts, {topk} slots")
     with _native.on_device_of(x):
         ids, scores = indices.contiguous(), scores.detach().to(x.dtype).contiguous()
+        if T > EXPAND_FROM:
+            experts = int4_experts_in_16_bits(params)
+            with torch.no_grad():
+                return routed_expert_compute(x, scores, experts.weight1, experts.weight2, ids, E, topk, act, addend=addend)
         outs = []
         at_once = min(_native.FEW_TOKENS, _native.FEW_SLOTS // topk)
         for t in range(0, T, at_once):

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from moe_explore.few_tokens import few_token_layer, int4_expert_compute
+from moe_explore.expert_compute import routed_expert_compute
+from moe_explore.few_tokens import few_token_layer, int4_expert_compute, int4_experts_in_16_bits
 from moe_explore.functional.int4 import pack_experts_int4, quantize_experts_int4
 from moe_explore.functional.topk_moe import topk_moe_forward
 from moe_explore.params import (ErnieRouterParams, GroupedTopkRouterParams, Int4ExpertParams, MLPParams, MOEParams, RMSNormParams,
@@ -236,6 +237,30 @@ def test_all_slots_on_few_experts(bits, native):
         y = x.double()
         assert near(out, experts64(y, *route64(rp, y @ rp.router_weight.double()), w1, w2, "swiglu"), torch.bfloat16, 2)
     native.check_status(device_status(0))
+
+
+@gpu
+@pytest.mark.parametrize("d,E,inter,act,dtype,group,zeros", [(136, 4, 72, "swiglu", torch.bfloat16, 32, True), (512, 8, 264, "geglu", torch.float16, 128, False),
+                                                             (72, 3, 136, "gelu", torch.bfloat16, 64, True), (256, 5, 40, "silu", torch.float16, 64, False)])
+def test_prompts_through_experts_in_4_bits(d, E, inter, act, dtype, group, zeros, native):
+    """The weights in 16 bits are their values rounded once, in the 16-bit experts' layout; many tokens are the 16-bit pass on them, few tokens
+    are near it: six roundings (gate and up weights, down weights, the activated product, an expert's row, the result)."""
+    g = gen(d + E)
+    q, w1, w2 = make_experts(g, 4, E, d, inter, act, dtype, group, zeros)
+    wide = int4_experts_in_16_bits(q)
+    assert wide.weight1.shape == w1.shape and wide.weight2.shape == w2.shape
+    assert torch.equal(wide.weight1, w1.to(dtype)) and torch.equal(wide.weight2, w2.to(dtype))
+    T, k = 300, 2
+    x, addend = (torch.randn(T, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    indices = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(t))[:k] for t in range(T)]).cuda()
+    scores = torch.rand(T, k, generator=g, device="cuda").to(dtype)
+    many = int4_expert_compute(x, scores, indices, q, addend=addend)
+    with torch.no_grad():
+        assert torch.equal(many, routed_expert_compute(x, scores, wide.weight1, wide.weight2, indices, E, k, act, addend=addend))
+    want = experts64(x.double(), scores.double(), indices, w1, w2, act) + addend.double()
+    assert near(many, want, dtype, 6)
+    few = torch.cat([int4_expert_compute(x[t:t + 90], scores[t:t + 90], indices[t:t + 90], q, addend=addend[t:t + 90]) for t in range(0, T, 90)])
+    assert near(few, want, dtype, 2)
 
 
 @gpu

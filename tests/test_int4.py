@@ -191,6 +191,9 @@ def test_refusals_without_a_gpu(native):
     assert lib.moe_int4_matmul(None, None, None, 1, 64, 64, 48, 0, 0, None) == -1 and b"groups" in lib.moe_last_error()
     assert lib.moe_int4_matmul(None, None, None, 1, 60, 64, 32, 0, 0, None) == -2 and b"multiples of 8" in lib.moe_last_error()
     assert lib.moe_int4_matmul(None, None, None, -1, 64, 64, 32, 0, 0, None) == -1
+    assert lib.moe_int4_expand(None, None, 1, 64, 64, 32, 0, 0, 0, None) == -1 and b"null" in lib.moe_last_error()
+    assert lib.moe_int4_expand(None, None, 1, 64, 24, 32, 0, 1, 0, None) == -2 and b"gated" in lib.moe_last_error()
+    assert lib.moe_int4_expand(None, None, 70000, 64, 64, 32, 0, 0, 0, None) == -1 and lib.moe_int4_expand(8, 16, 1, 64, 64, 32, 0, 0, 0, None) == -1
     assert lib.moe_int4_matmul(16, 40, 64, 1, 64, 64, 32, 0, 0, None) == -1 and b"aligned" in lib.moe_last_error()
 
 
