@@ -185,7 +185,7 @@ def quantize_experts_int4(params, group: int = 128, zeros: bool = False):
 
 def int4_matmul(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     """``x @ weight^T`` [..., N] for a few rows ``x`` [..., K] in the type of the weight's scales (any number of rows is right; the kernel is
-    made for up to 64: beyond, the weights are read again for every 32)."""
+    made for up to 64: beyond, the weights are read again for every 64)."""
     weight.checked(0, "weight")
     _native.require_cuda(x)
     if x.dim() < 1 or x.size(-1) != weight.k or x.device != weight.data.device:

@@ -264,6 +264,36 @@ def test_prompts_through_experts_in_4_bits(d, E, inter, act, dtype, group, zeros
 
 
 @gpu
+@pytest.mark.parametrize("T", [96, 97, 130])
+@pytest.mark.parametrize("E", [1, 6])
+def test_prompts_with_bad_experts_in_a_graph(T, E, native):
+    """On both sides of the line: slots of no expert add nothing and are reported, and a graph follows its inputs."""
+    g = gen(100 * T + E)
+    d, inter, k = 128, 64, 2
+    q, w1, w2 = make_experts(g, 4, E, d, inter, "swiglu", torch.bfloat16, 64, True)
+    x = torch.randn(T, d, generator=g, device="cuda").bfloat16()
+    scores = torch.rand(T, k, generator=g, device="cuda").bfloat16()
+    indices = torch.randint(0, E, (T, k), generator=g, device="cuda")   # the same expert twice, too
+    int4_expert_compute(x, scores, indices, q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = int4_expert_compute(x, scores, indices, q)
+    for bad in (False, True):
+        x.copy_(torch.randn(T, d, generator=g, device="cuda"))
+        if bad:
+            indices[0], indices[5, 1], indices[T - 1, 0] = E, -1, E + 7
+        graph.replay()
+        eager = int4_expert_compute(x, scores, indices, q)
+        assert torch.equal(out, eager)
+        real = (indices >= 0) & (indices < E)
+        want = sum(experts64(x.double(), (scores.double() * real)[:, s:s + 1], indices.clamp(0, E - 1)[:, s:s + 1], w1, w2, "swiglu") for s in range(k))
+        assert near(eager, want, torch.bfloat16, 6)
+        assert not bad or not eager[0].any()
+        assert native.read_status(device_status(0), reset=True) == (native.STATUS_BAD_EXPERT_ID if bad else 0)
+
+
+@gpu
 def test_values_that_are_not_finite(native):
     """A token that holds NaN or an infinity spoils its own row only."""
     g = gen(10)
