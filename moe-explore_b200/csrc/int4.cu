@@ -99,7 +99,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) q4_rows_kernel(const Q4Args 
 // More rows, 8 MT at a time.  A CTA takes eight tiles, two per warp, and the rows; its warps go through the steps together, so that a step's
 // columns of the rows lie in shared memory once, and the numbers made of a word are used for all rows.  16, 32, 64 rows of 4096 by 28672: 28,
 // 43, 78 us (by eights: 36, 70, 134), the tensor pipe busy for 40 % of it with two warps per scheduler; 9 and 16 rows of 7168 by 4096
-// 9.1 and 9.4 (by eights 13.7 and 14.8).
+// 9.1 and 9.4 (by eights 13.7 and 14.8).  With one tile per warp and twice the CTAs an SM, which read the rows out of shared memory twice as
+// often, 84 us for the 64 rows and 10.7 for the 16.
 constexpr int kQ4ManyWarps = 4, kQ4ManyDepth = 3;
 template <int NG, bool ZEROS, int MT> struct Q4Many {
   static constexpr int kBlock = Q4Stage<NG, ZEROS>::kBlock, kRows = kQ4ManyWarps * kQ4Tiles * kBlock, kStage = kRows + MT * 2048;
