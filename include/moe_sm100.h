@@ -660,8 +660,9 @@ int moe_int4_matmul(const void* x, const void* data, void* out, int64_t rows, in
 /* ---------------------------------------------------------------------------------
  * A whole layer for a few tokens (at most 16; 256 slots, 1024 experts) in two kernels, forward only.  No counterpart in the reference.
  *   h = round(x + residual), y = round(h / sqrt(mean h^2 + eps) * norm_w)  (norm_w NULL: y = x);  stream_out receives h
- *   logits = y router_w in fp32 (of y before its rounding);  scores and experts as in moe_router_tail / moe_grouped_topk with equal values
- *   by ascending index, or, with router_w NULL, as given (expert_idx, scores [num_tokens, topk])
+ *   logits = y router_w in fp32 (of y before its rounding);  scores and experts as in moe_grouped_topk (the choice of exact arithmetic on
+ *   these logits; NaN last), with normalize 2 as in moe_router_tail (by p + bias in fp32), with score_function 2 by the logits (NaN first),
+ *   equal values by ascending index;  with router_w NULL as given (expert_idx, scores [num_tokens, topk])
  *   out = sum over the slots of score * (round(act(y w1[e])) w2[e]) + addend, summed in fp32, rounded once
  * bits 16: w1 [num_experts, d, 2 inter] (gated: gate and up columns in turn) or [num_experts, d, inter], w2 [num_experts, inter, d].
  * bits 4: the layout of moe_int4_matmul, a matrix per expert: w1 [2 inter, d] (gated: eight rows of the gate, eight of the up matrix in

@@ -14,6 +14,7 @@
 // The logits are not rounded to 16 bits, nor are an expert's rows before the fold; y and the activated product are, because they are
 // operands of 16-bit products.
 #include "int4.cuh"
+#include "order.cuh"
 
 #include <atomic>
 
@@ -308,32 +309,116 @@ __device__ __forceinline__ bool meet(const FewArgs& a, int turn, int* go_on) {
   return *go_on != 0;
 }
 
-// A number's bits in an order that whole numbers have.
-__device__ __forceinline__ uint32_t ordered(float v) {
-  const uint32_t u = __float_as_uint(v);
-  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+template <typename V> __device__ __forceinline__ V share_of(float logit, bool sigmoid, float most, V sum) {
+  if (sigmoid) return V(1) / (V(1) + exp(-static_cast<V>(logit)));
+  return exp(static_cast<V>(logit) - static_cast<V>(most)) / sum;
+}
+
+// What a group is worth by the keys of its best two: the best one, or half the sum of both (which ranks as the sum does, and does not
+// overflow).  Without a bias the keys are those of logits.  `size`: of the members, for what fp32 is off by.
+template <typename V>
+__device__ __forceinline__ V group_worth(const FewArgs& a, bool both, typename Order<V>::Key b0, typename Order<V>::Key b1, float most, V sum, V& size) {
+  V v = Order<V>::value(b0), w = V(0);
+  if (both) {
+    w = Order<V>::value(b1);
+    if (a.bias == nullptr) {
+      v = share_of<V>(static_cast<float>(v), a.sigmoid != 0, most, sum);
+      w = share_of<V>(static_cast<float>(w), a.sigmoid != 0, most, sum);
+    }
+    v *= V(0.5);
+    w *= V(0.5);
+  }
+  size = fabs(v) + fabs(w);
+  return v + w;
+}
+
+// The choice in 64 bits, all of it in shared memory: for the rare token whose values fp32 does not tell apart.  Leaves the experts and their
+// shares; the lane's part of their sum.
+__device__ __noinline__ float choose_exactly(const FewArgs& a, int t, unsigned long long* keys, FewRouting& r, float most, int lane) {
+  typedef Order<double> O;
+  const float* from = a.logits + static_cast<int64_t>(t) * a.E;
+  const bool sigmoid = a.sigmoid != 0;
+  __syncwarp();  // the keys in 32 bits, which lie here, have been read
+  double sum = 0.0;
+  if (!sigmoid) {
+    for (int e = lane; e < a.E; e += 32) sum += exp(static_cast<double>(from[e]) - static_cast<double>(most));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+  }
+  for (int e = lane; e < a.E; e += 32)
+    keys[e] = O::key(a.bias != nullptr ? share_of<double>(from[e], sigmoid, most, sum) + static_cast<double>(a.bias[e]) : static_cast<double>(from[e]));
+  __syncwarp();
+  if (a.keep < a.groups) {
+    const int width = a.E / a.groups;
+    unsigned long long* const worth = keys + a.E;
+    for (int g = lane; g < a.groups; g += 32) {
+      unsigned long long b0 = 0, b1 = 0;
+      for (int i = 0; i < width; ++i) {
+        const unsigned long long k = keys[g * width + i], lower = k < b0 ? k : b0;
+        b1 = lower > b1 ? lower : b1;
+        b0 = k > b0 ? k : b0;
+      }
+      double size;
+      worth[g] = O::key(group_worth<double>(a, a.best == 2 && width > 1, b0, b1, most, sum, size));
+    }
+    __syncwarp();
+    for (int g = lane; g < a.groups; g += 32) {
+      int before = 0;
+      for (int o = 0; o < a.groups; ++o) before += worth[o] > worth[g] || (worth[o] == worth[g] && o < g);
+      if (before >= a.keep)
+        for (int i = 0; i < width; ++i) keys[g * width + i] = 0;
+    }
+    __syncwarp();
+  }
+  unsigned long long best = 0;
+  int at = lane;
+  const auto look = [&]() {
+    best = 0;
+    for (int e = lane; e < a.E; e += 32)
+      if (keys[e] > best) best = keys[e], at = e;
+  };
+  look();
+  float total = 0.0f;
+  for (int s = 0; s < a.k; ++s) {
+    const unsigned long long v = O::warp_max(best);
+    const uint32_t e = __reduce_min_sync(0xFFFFFFFFu, best == v ? static_cast<uint32_t>(at) : 0xFFFFu);
+    if (e == static_cast<uint32_t>(at) && best == v) {
+      const float share = static_cast<float>(share_of<double>(from[e], sigmoid, most, sum));
+      r.id[t * a.k + s] = static_cast<int16_t>(e);
+      r.score[t * a.k + s] = share;
+      total += share;
+      keys[e] = 0;
+      look();
+    }
+  }
+  return total;
 }
 
 // One warp, one token; expert lane + 32 i is the lane's i-th of up to EACH.  `keys`: scratch of this warp's own, [E] and [groups].
-template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int t, float* keys, FewRouting& r, int lane) {
+//
+// The logits decide where they are all that does (shares grow with them).  Where shares with a bias, or sums of two, are compared, the choice
+// is that of exact arithmetic on the fp32 logits: values closer than what fp32 can be off by are decided again in 64 bits -- but for
+// the router whose definition is in 32 bits (normalize 2).  Equal values by ascending index.  NaN is taken after everything else, or,
+// where the softmax runs over the selected logits, before (the row is NaN then, as it is behind torch.topk).
+template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int t, uint32_t* keys, FewRouting& r, int lane) {
   constexpr uint32_t kAll = 0xFFFFFFFFu;
+  typedef Order<float> O;
   const float* from = a.logits + static_cast<int64_t>(t) * a.E;
+  const bool biased = a.bias != nullptr;
   float p[EACH];        // logit, then its share before normalisation
   float bias[EACH];
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     const int e = lane + 32 * i;
     p[i] = e < a.E ? from[e] : -INFINITY;
-    bias[i] = e < a.E && a.bias != nullptr ? a.bias[e] : 0.0f;
+    bias[i] = e < a.E && biased ? a.bias[e] : 0.0f;
   }
-  // open experts' keys are 2 and above (NaN and -inf 2: they come last, lowest index first), taken and closed ones below
-  uint32_t key[EACH];
-  const auto key_of = [](float v) { return v > -3.402823466e38f ? ordered(v + 0.0f) : 2u; };  // (-0 is 0)
+  uint32_t key[EACH];   // 0: no expert, or taken, or in a closed group
   float most = -3.402823466e38f, sum = 0.0f;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     most = fmaxf(most, p[i]);
-    key[i] = lane + 32 * i < a.E ? key_of(p[i]) : 0u;
+    key[i] = lane + 32 * i < a.E ? a.softmax_after && p[i] != p[i] ? kAll : O::key(p[i]) : 0u;
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(kAll, most, off));
@@ -348,43 +433,69 @@ template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int
 #pragma unroll
     for (int i = 0; i < EACH; ++i) p[i] /= sum;
   }
-  if (a.bias != nullptr || a.groups > 1) {
+  if (biased) {
 #pragma unroll
     for (int i = 0; i < EACH; ++i)
-      if (lane + 32 * i < a.E) key[i] = key_of(p[i] + bias[i]);
+      if (lane + 32 * i < a.E) key[i] = O::key(p[i] + bias[i]);
   }
-  if (a.groups > 1) {
+  // How far a share can be off.  Sigmoid: the exponential by two units of 2^-23, which count with p (1 - p) <= 1/4, sum and quotient by
+  // half a unit each.  Softmax: the same, a rounding per addition, and that of logit - most, which counts most (1/e) where it is -1.
+  const float slack = a.sigmoid ? 3e-7f : (8e-7f + 1.2e-7f * EACH) / sum + 3e-8f;
+  const bool exact = a.normalize != 2;
+  bool sure = true;
+  if (a.keep < a.groups) {
     const int width = a.E / a.groups;
-    float* const worth = keys + a.E;
+    const bool both = a.best == 2 && width > 1;
+    uint32_t* const worth = keys + a.E;
 #pragma unroll
     for (int i = 0; i < EACH; ++i)
-      if (lane + 32 * i < a.E) keys[lane + 32 * i] = key[i] > 2u ? p[i] + bias[i] : -3.402823466e38f;
+      if (lane + 32 * i < a.E) keys[lane + 32 * i] = key[i];
     __syncwarp();
-    for (int g = lane; g < a.groups; g += 32) {
-      float b0 = -INFINITY, b1 = -INFINITY;
+    float off_by[2] = {};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int g = lane + 32 * j;
+      if (g >= a.groups) continue;
+      uint32_t b0 = 0, b1 = 0;
 #pragma unroll 4
       for (int i = 0; i < width; ++i) {
-        const float v = keys[g * width + i];
-        b1 = fmaxf(b1, fminf(b0, v));
-        b0 = fmaxf(b0, v);
+        const uint32_t k = keys[g * width + i];
+        b1 = max(b1, min(b0, k));
+        b0 = max(b0, k);
       }
-      worth[g] = a.best == 2 && width > 1 ? b0 + b1 : b0;
+      float size;
+      worth[g] = O::key(group_worth<float>(a, both, b0, b1, most, sum, size));
+      // each member's slack and its rounding by 2^-24 of its size, the addition's and that of the bounds below by 2^-24 of the sum (an
+      // infinite member is exact)
+      off_by[j] = size < INFINITY ? slack + 2.4e-7f * size : 0.0f;
     }
     __syncwarp();
-    uint32_t open0 = 0, open1 = 0;  // groups 0..31, 32..63
-    for (int g0 = 0; g0 < a.groups; g0 += 32) {
-      const int g = g0 + lane;
-      int before = a.keep;
+    uint32_t open[2] = {};  // groups 0..31, 32..63
+    uint32_t worst = kAll, next = 0;  // the least that an open group can be worth, and the most that a closed one can
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int g = lane + 32 * j;
+      bool is_open = false;
       if (g < a.groups) {
-        before = 0;
-        for (int o = 0; o < a.groups; ++o) before += worth[o] > worth[g] || (worth[o] == worth[g] && o < g);
+        const uint32_t mine = worth[g];
+        int before = 0;
+        for (int o = 0; o < a.groups; ++o) before += worth[o] > mine || (worth[o] == mine && o < g);
+        is_open = before < a.keep;
+        const float v = O::value(mine);
+        if (is_open) worst = min(worst, O::key(v - off_by[j]));
+        else next = max(next, O::key(v + off_by[j]));
       }
-      (g0 == 0 ? open0 : open1) = __ballot_sync(kAll, before < a.keep);
+      open[j] = __ballot_sync(kAll, is_open);
+    }
+    if (exact && (biased || both)) {  // (closed groups of minus infinity or NaN are exact)
+      worst = O::warp_min(worst);
+      next = O::warp_max(next);
+      sure = !(worst <= next && next > O::key(-INFINITY));
     }
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const int g = (lane + 32 * i) / width;
-      if (((g < 32 ? open0 : open1) >> (g & 31) & 1) == 0) key[i] = 0u;
+      if (((g < 32 ? open[0] : open[1]) >> (g & 31) & 1) == 0) key[i] = 0u;
     }
   }
   // k times the best of the lanes' best; only the lane that had it looks again
@@ -399,9 +510,10 @@ template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int
   };
   look();
   float total = 0.0f;
+  uint32_t last = 0;
   for (int s = 0; s < a.k; ++s) {
-    const uint32_t v = __reduce_max_sync(kAll, best);
-    const uint32_t e = __reduce_min_sync(kAll, best == v ? static_cast<uint32_t>(at) : 0xFFFFu);
+    last = __reduce_max_sync(kAll, best);
+    const uint32_t e = __reduce_min_sync(kAll, best == last ? static_cast<uint32_t>(at) : 0xFFFFu);
     if (e == static_cast<uint32_t>(at)) {
       r.id[t * a.k + s] = static_cast<int16_t>(e);
       r.score[t * a.k + s] = share;
@@ -412,6 +524,12 @@ template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int
       look();
     }
   }
+  if (exact && biased) {  // the last that was taken and the first that was not
+    const uint32_t next = O::warp_max(best);
+    const float above = O::value(last), below = O::value(next);
+    sure = sure && !(next != 0 && above - below <= 2.0f * slack + 1.2e-7f * (fabsf(above) + fabsf(below)));
+  }
+  if (!sure) total = choose_exactly(a, t, reinterpret_cast<unsigned long long*>(keys), r, most, lane);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(kAll, total, off);
   __syncwarp();
@@ -422,11 +540,11 @@ template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int
 
 // Scores, experts, and the list of entries: up to eight slots of one expert each.  Entries of one expert follow one another (they read
 // the same weights at the same time), experts by their first slots.
-template <typename T> __device__ __forceinline__ void route(const FewArgs& a, FewRouting& r, float* scratch) {
+template <typename T> __device__ __forceinline__ void route(const FewArgs& a, FewRouting& r, uint32_t* scratch) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int slots = a.T * a.k;
   if (a.logits != nullptr) {
-    float* const keys = scratch + warp * (a.E + a.groups);
+    uint32_t* const keys = scratch + warp * 2 * (a.E + a.groups);  // (room for 64-bit ones)
     for (int t = warp; t < a.T; t += kFewWarps) {
       if (a.E <= 64) choose<2>(a, t, keys, r, lane);
       else if (a.E <= 256) choose<8>(a, t, keys, r, lane);
@@ -635,7 +753,7 @@ template <typename F> struct FewPlan {
   static constexpr int kRing = F::kDepth * F::kStage;
   static constexpr int kTotal = kFewWarps * kRing;
   static_assert(kFewRows * F::kCols * 4 <= F::kStage, "a warp's sums of a unit, [row][column], lie in the stage that it has read last");
-  static_assert(kFewWarps * (kFewExperts + kFewGroups) * 4 <= kTotal && kFewWarps * kFewExperts + 4 * kFewExperts <= kTotal,
+  static_assert(kFewWarps * (kFewExperts + kFewGroups) * 8 <= kTotal && kFewWarps * kFewExperts + 4 * kFewExperts <= kTotal,
                 "the router's keys lie where the rings will be");
 };
 
@@ -703,14 +821,14 @@ template <typename F> struct FewWalk {
 };
 
 template <typename T, typename F>
-__global__ void __launch_bounds__(kFewThreads, kFewCtas) few_experts_kernel(const FewArgs a) {
+__global__ void __launch_bounds__(kFewThreads, kFewCtas) few_experts_kernel(const __grid_constant__ FewArgs a) {
   using P = FewPlan<F>;
   constexpr bool WIDE = F::kCols == 64;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ FewRouting r;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_u32(smem), ring = warp * P::kRing;  // the ring's place in it
-  route<T>(a, r, reinterpret_cast<float*>(smem));
+  route<T>(a, r, reinterpret_cast<uint32_t*>(smem));
   const bool gated = a.act == MOE_ACT_SWIGLU || a.act == MOE_ACT_GEGLU;
   const int slots = a.T * a.k;
   // All units of a product whose first copies are under way; `give` takes a unit's sums: (entry, tile, share, thread of the team,

@@ -43,7 +43,8 @@ def few_token_layer(input: torch.Tensor, params, residual=None, addend=None, nor
     ``residual``, (output, ``input + residual``).  ``addend`` [T, d] is added by the fold.  None where the kernels do not serve: more
     tokens, a gradient, another device than the current one, something that watches the single ops, routers or sizes that they do not know.
 
-    The logits are not rounded to 16 bits, equal ones are taken in ascending index; an expert's rows are not rounded before the fold."""
+    The logits are not rounded to 16 bits; the choice among them is the routers' own (of exact arithmetic for ``GroupedTopkRouterParams``),
+    equal values are taken in ascending index.  An expert's rows are not rounded before the fold."""
     if residual is not None and norm is None:
         raise ValueError("residual is added by the layer's norm: norm is None")
     ep, rp = params.expert_params, params.router_params

@@ -428,6 +428,116 @@ def test_a_wait_that_runs_out_is_reported(native):
         assert torch.equal(topk_moe_forward(x, p, few_tokens=True), want)
 
 
+def marked_experts(E, rows, dtype=torch.bfloat16):
+    """Experts that say who they are: for a row with a single one in it, expert e adds a one in column e; so a layer's result [T, max(rows, E)]
+    holds every expert's weight in its column."""
+    d = (max(rows, E) + 7) // 8 * 8
+    w1, w2 = torch.zeros(E, d, 8, device="cuda", dtype=dtype), torch.zeros(E, 8, d, device="cuda", dtype=dtype)
+    w1[:, :, 0] = 1
+    w2[torch.arange(E), 0, torch.arange(E)] = 1
+    return MLPParams(w1, w2, None), d
+
+
+def weights_of(logits, rp, E):
+    """The layer's weights [T, E] for these fp32 logits: row t is all zeros but for a one in column t, so its logits are row t of the router."""
+    T = logits.size(0)
+    experts, d = marked_experts(E, T)
+    rp.router_weight = torch.zeros(d, E, device="cuda", dtype=torch.float32)
+    rp.router_weight[:T] = logits
+    p = MOEParams(rp, experts, E, rp.topk)
+    with torch.no_grad():
+        out = few_token_layer(torch.eye(T, d, device="cuda", dtype=torch.bfloat16), p)
+    return out[:, :E]
+
+
+def grouped(E, k, bias, groups=1, open_=1, best=2, function="sigmoid", normalize=False):
+    return GroupedTopkRouterParams(None, k, bias=bias, num_groups=groups, topk_groups=open_, group_best=best, score_function=function,
+                                   normalize_routing=normalize, scale=1.0)
+
+
+def chosen(logits, rp):
+    """Indices of the router's own kernel, and the weights in its 32-bit scores."""
+    from moe_explore.router import grouped_topk_of_logits
+    scores, indices = grouped_topk_of_logits(logits, rp, torch.float32)
+    return torch.zeros_like(logits).scatter_(1, indices, scores), indices
+
+
+def same_choice(logits, rp):
+    """The weights are those of the experts that the router's kernel chooses: they agree to a rounding of 16 bits, the last bits of two
+    exponentials in 32 (each within 2 units of 2^-23, their sum and the division), and steps of the smallest numbers of 16 bits."""
+    want, _ = chosen(logits, rp)
+    got = weights_of(logits, rp, logits.size(1)).float()
+    assert bool(((got - want).abs() <= (2.0 ** -8 + 2.0 ** -19) * want + 2.0 ** -132).all())
+
+
+@gpu
+def test_the_choice_is_that_of_exact_arithmetic(native):
+    """Values whose difference fp32 does not hold: sigmoids near one, tiny ones beside a bias, groups of such values."""
+    E = 64
+    low = torch.full((1, E), -3.0, device="cuda")
+    zero = torch.zeros(E, device="cuda")
+    near_one = low.clone()
+    near_one[0, 7], near_one[0, 50] = 20.0, 25.0           # both sigmoids are 1 in fp32
+    same_choice(near_one, grouped(E, 1, zero))
+    assert weights_of(near_one, grouped(E, 1, zero), E).nonzero().tolist() == [[0, 50]]
+    tiny = torch.full((1, E), -60.0, device="cuda")
+    tiny[0, 9], tiny[0, 40] = -22.0, -19.0                 # sigmoids of 3e-10 and 6e-9 beside a bias of a half
+    rp = grouped(E, 1, torch.full((E,), 0.5, device="cuda"))
+    want, indices = chosen(tiny, rp)
+    assert indices.tolist() == [[40]]
+    assert weights_of(tiny, rp, E).nonzero().tolist() == [[0, 40]]
+    for best in (1, 2):                                    # groups whose best sum to the same number in fp32
+        both = low.clone()
+        both[0, 3], both[0, 5], both[0, 57], both[0, 60] = 21.0, 22.0, 23.0, 22.5
+        for bias in (None, zero):
+            rp = grouped(E, 2, bias, groups=8, open_=1, best=best)
+            assert sorted(chosen(both, rp)[1][0].tolist()) == [57, 60]
+            assert weights_of(both, rp, E).nonzero().tolist() == [[0, 57], [0, 60]]
+    soft = torch.full((1, E), -40.0, device="cuda")        # all but one share are 0 beside the bias
+    soft[0, 0], soft[0, 11], soft[0, 33] = 30.0, -1.0, 4.0
+    rp = grouped(E, 2, torch.full((E,), 1.0, device="cuda"), function="softmax")
+    assert sorted(chosen(soft, rp)[1][0].tolist()) == [0, 33]
+    assert weights_of(soft, rp, E).nonzero().tolist() == [[0, 0], [0, 33]]
+
+
+@gpu
+@pytest.mark.parametrize("function", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("E,groups,open_,best", [(64, 1, 1, 1), (64, 8, 3, 2), (256, 8, 4, 2), (256, 32, 5, 1), (768, 6, 2, 2)])
+def test_the_choice_is_the_routers(function, E, groups, open_, best, native):
+    """Sixteen tokens at a time, logits of every scale: coarse ones (equal values), wide ones (shares of 0 and 1), ordinary ones."""
+    g = gen(E + groups)
+    k = 8 if E // groups * open_ >= 8 else 4
+    for scale in (0.25, 2.0, 12.0, 30.0):
+        for coarse in (False, True):
+            logits = scale * torch.randn(16, E, generator=g, device="cuda")
+            if coarse:
+                logits = (logits / scale * 8).round() * (scale / 8)
+            for bias in (None, torch.zeros(E, device="cuda"), 0.1 * torch.randn(E, generator=g, device="cuda")):
+                same_choice(logits, grouped(E, k, bias, groups, open_, best, function))
+    native.check_status(device_status(0))
+
+
+@gpu
+def test_logits_that_are_not_finite(native):
+    """NaN comes after minus infinity where the router is one of groups; where the softmax runs over the selected logits, it comes first, as for
+    the ordinary router, and the row is NaN."""
+    E = 16
+    logits = torch.full((1, E), -math.inf, device="cuda")
+    logits[0, 0], logits[0, 1], logits[0, 12] = math.nan, math.nan, 1.0
+    for rp in (grouped(E, 3, None), grouped(E, 3, torch.zeros(E, device="cuda")), grouped(E, 3, None, groups=4, open_=2, best=1)):
+        assert chosen(logits, rp)[1][0, 0] == 12 and not any(i in (0, 1) for i in chosen(logits, rp)[1][0].tolist())
+        got = weights_of(logits, rp, E)
+        assert torch.isfinite(got).all() and got.nonzero().tolist() == [[0, 12]]
+    experts, d = marked_experts(E, 1)
+    w = torch.zeros(d, E, device="cuda").bfloat16()
+    w[0] = torch.arange(E, device="cuda")
+    w[0, 3] = math.nan
+    p = MOEParams(TopkRouterParams(w, 2, False), experts, E, 2)
+    x = torch.eye(1, d, device="cuda").bfloat16()
+    with torch.no_grad():
+        assert torch.isnan(topk_moe_forward(x, p)).all() and torch.isnan(topk_moe_forward(x, p, few_tokens=True)).all()
+
+
 # ------------------------------------------------------------------------------------------------------- refusals
 def test_refusals_of_the_library(native):
     import ctypes
