@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a)
   extern __shared__ __align__(16) float rows[];  // [TT][share]: h w
   __shared__ float parts[kFewWarps][TT][kHeadCols];
   __shared__ float joined[TT][kHeadCols];
-  __shared__ float2 squares[kFewTokens];  // sum of squares, and whether it is in units of 2^144
-  __shared__ float scale[kFewTokens];
+  __shared__ float2 squares[kFewTokens];  // sum of squares, and whether it is in units of 2^144 (the rows of this share then in ones of 2^72)
+  __shared__ float scale[kFewTokens], part_scale[kFewTokens], logit_scale[kFewTokens];  // of the share's rows, its logits, and their sums
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = static_cast<int>(cluster_ctarank());
   const int group = static_cast<int>(blockIdx.x / kHeadRanks), groups = static_cast<int>(gridDim.x / kHeadRanks);
@@ -120,35 +120,43 @@ __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a)
     const T* x = static_cast<const T*>(a.x) + static_cast<int64_t>(t) * a.d + k_begin;
     const T* residual = a.residual == nullptr ? nullptr : static_cast<const T*>(a.residual) + static_cast<int64_t>(t) * a.d + k_begin;
     float sum = 0.0f, large = 0.0f, most = 0.0f;
+    // h w, times `units`, to shared memory
+    const auto make = [&](float units, bool first) {
 #pragma unroll 1
-    for (int i = lane * 8; i < share; i += 256) {
-      float h[8] = {}, g[8];
-      if (i < count) {
-        eight<T>(*reinterpret_cast<const uint4*>(x + i), h);
-        if (residual != nullptr) {
-          float o[8];
-          eight<T>(*reinterpret_cast<const uint4*>(residual + i), o);
+      for (int i = lane * 8; i < share; i += 256) {
+        float h[8] = {}, g[8];
+        if (i < count) {
+          eight<T>(*reinterpret_cast<const uint4*>(x + i), h);
+          if (residual != nullptr) {
+            float o[8];
+            eight<T>(*reinterpret_cast<const uint4*>(residual + i), o);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) h[j] += o[j];
-          const uint4 v = make_uint4(Elem<T>::pack2(h[0], h[1]), Elem<T>::pack2(h[2], h[3]), Elem<T>::pack2(h[4], h[5]), Elem<T>::pack2(h[6], h[7]));
-          if (t % groups == group) *reinterpret_cast<uint4*>(static_cast<T*>(a.stream) + static_cast<int64_t>(t) * a.d + k_begin + i) = v;
-          eight<T>(v, h);
+            for (int j = 0; j < 8; ++j) h[j] += o[j];
+            const uint4 v = make_uint4(Elem<T>::pack2(h[0], h[1]), Elem<T>::pack2(h[2], h[3]), Elem<T>::pack2(h[4], h[5]), Elem<T>::pack2(h[6], h[7]));
+            if (first && t % groups == group) *reinterpret_cast<uint4*>(static_cast<T*>(a.stream) + static_cast<int64_t>(t) * a.d + k_begin + i) = v;
+            eight<T>(v, h);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (first) {
+              sum = fmaf(h[j], h[j], sum);
+              large = fmaf(h[j] * 0x1p-72f, h[j] * 0x1p-72f, large);  // bf16 values from 2^57 on have squares whose sum may leave fp32
+              most = fmaxf(most, fabsf(h[j]));
+            } else {
+              h[j] *= units;
+            }
+            g[j] = a.norm == nullptr ? 1.0f : a.norm_fp32 ? static_cast<const float*>(a.norm)[k_begin + i + j] : 0.0f;
+          }
+          if (a.norm != nullptr && !a.norm_fp32) eight<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.norm) + k_begin + i), g);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[j] *= g[j];
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          sum = fmaf(h[j], h[j], sum);
-          large = fmaf(h[j] * 0x1p-72f, h[j] * 0x1p-72f, large);  // bf16 values from 2^57 on have squares whose sum may leave fp32
-          most = fmaxf(most, fabsf(h[j]));
-          g[j] = a.norm == nullptr ? 1.0f : a.norm_fp32 ? static_cast<const float*>(a.norm)[k_begin + i + j] : 0.0f;
-        }
-        if (a.norm != nullptr && !a.norm_fp32) eight<T>(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.norm) + k_begin + i), g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] *= g[j];
+        float4* out = reinterpret_cast<float4*>(rows + t * share + i);
+        out[0] = make_float4(h[0], h[1], h[2], h[3]);
+        out[1] = make_float4(h[4], h[5], h[6], h[7]);
       }
-      float4* out = reinterpret_cast<float4*>(rows + t * share + i);
-      out[0] = make_float4(h[0], h[1], h[2], h[3]);
-      out[1] = make_float4(h[4], h[5], h[6], h[7]);
-    }
+    };
+    make(1.0f, true);
     if (a.norm != nullptr) {
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) {
@@ -157,6 +165,7 @@ __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a)
         most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
       }
       if (lane == 0) squares[t] = most > 0x1p50f ? make_float2(large, 1.0f) : make_float2(sum, 0.0f);
+      if (most > 0x1p50f) make(0x1p-72f, false);  // h w, and its sums with the router's weights, may leave fp32 where h r w is of order 1
     }
   }
   __syncthreads();
@@ -185,7 +194,7 @@ __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a)
   __syncwarp();
   cluster_wait();
   if (tid < TT) {
-    float r = 1.0f;
+    float r = 1.0f, parts_by = 1.0f, logits_by = 1.0f;
     if (a.norm != nullptr) {
       float2 all[kHeadRanks];
 #pragma unroll
@@ -200,9 +209,15 @@ __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a)
 #pragma unroll
       for (int q = 0; q < kHeadRanks; ++q) v += all[q].y == 0.0f && wide ? all[q].x * 0x1p-72f * 0x1p-72f : all[q].x;
       v /= static_cast<float>(a.d);
-      r = wide ? rsqrtf(v) * 0x1p-72f : rsqrtf(v + a.eps);  // (beside such squares eps is nothing)
+      // (beside such squares eps is nothing.)  The logits of a row that is large somewhere are summed in units of 2^72.
+      const bool own = squares[tid].y != 0.0f;
+      logits_by = wide ? rsqrtf(v) : rsqrtf(v + a.eps);
+      r = wide && !own ? logits_by * 0x1p-72f : logits_by;
+      parts_by = wide && !own ? 0x1p-72f : 1.0f;
     }
     scale[tid] = r;
+    part_scale[tid] = parts_by;
+    logit_scale[tid] = logits_by;
   }
 #pragma unroll
   for (int t = 0; t < TT; ++t)
@@ -217,7 +232,7 @@ __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a)
     float v = 0.0f;
 #pragma unroll
     for (int w8 = 0; w8 < kFewWarps; ++w8) v += (&parts[w8][0][0])[at];
-    (&joined[0][0])[at] = v;
+    (&joined[0][0])[at] = v * part_scale[at / kHeadCols];
   }
   __syncthreads();
   cluster_arrive();  // the logits
@@ -243,7 +258,7 @@ __global__ void __launch_bounds__(kFewThreads) few_head_kernel(const HeadArgs a)
       for (int q = 0; q < kHeadRanks; ++q) part[q] = cluster_load(mapa_shared(smem_u32(&(&joined[0][0])[at]), q));
 #pragma unroll
       for (int q = 0; q < kHeadRanks; ++q) v += part[q];
-      a.logits[static_cast<int64_t>(t) * a.E + e] = v * scale[t];
+      a.logits[static_cast<int64_t>(t) * a.E + e] = v * logit_scale[t];
     }
   }
   __syncthreads();

@@ -538,6 +538,44 @@ def test_logits_that_are_not_finite(native):
         assert torch.isnan(topk_moe_forward(x, p)).all() and torch.isnan(topk_moe_forward(x, p, few_tokens=True)).all()
 
 
+@gpu
+@pytest.mark.parametrize("weight_type", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [512, 2056])
+def test_rows_near_the_end_of_bf16_get_their_norm(d, weight_type, native):
+    """Rows whose products with the norm's weight, and with the router's, leave fp32 before they are scaled; large values in all of a row, in
+    one stretch of it only, and none.  The ordinary layer is finite and near, too."""
+    g = gen(d)
+    E, k, inter = 20, 3, 64
+    experts, w1, w2 = make_experts(g, 16, E, d, inter, "swiglu", torch.bfloat16)
+    norm = RMSNormParams((4 + 4 * torch.rand(d, generator=g, device="cuda")).to(weight_type), 1e-6)
+    rp = make_router(g, "groups fp32", d, E, k, torch.bfloat16)
+    p = MOEParams(rp, experts, E, k, None, norm)
+    x = torch.randn(8, d, generator=g, device="cuda").clamp(-3.5, 3.5)
+    x[0] *= 2.0 ** 125
+    x[1, d // 2:d // 2 + 5] *= 2.0 ** 125
+    x[2] *= 2.0 ** 70
+    x[3, -1] = 2.0 ** 127
+    x[4, :8] *= 2.0 ** 60
+    x[5] *= 2.0 ** -50
+    x = x.bfloat16()
+    residual = (0.25 * torch.randn(8, d, generator=g, device="cuda") * x.abs().amax(1, keepdim=True).clamp_max(2.0 ** 124)).bfloat16()
+    for r in (None, residual):
+        h = x if r is None else x + r
+        assert torch.isfinite(h).all()
+        y = h.double()
+        y = y / (y.square().mean(-1, keepdim=True) + 1e-6).sqrt() * norm.weight.double()
+        want = experts64(y, *route64(rp, y @ rp.router_weight.double()), w1, w2, "swiglu")
+        with torch.no_grad():
+            few = topk_moe_forward(x, p, residual=r, few_tokens=True)
+            ordinary = topk_moe_forward(x, p, residual=r)
+        if r is not None:
+            assert torch.equal(few[1], h)
+            few, ordinary = few[0], ordinary[0]
+        assert torch.isfinite(ordinary).all() and torch.isfinite(few).all()
+        for t in range(8):
+            assert near(few[t], want[t], torch.bfloat16, 4), t
+
+
 # ------------------------------------------------------------------------------------------------------- refusals
 def test_refusals_of_the_library(native):
     import ctypes
