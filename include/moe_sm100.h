@@ -501,10 +501,11 @@ typedef struct moe_expert_pass {
   int32_t own_tie_rule; /* MOE_FWD_TAIL by moe_router_topk instead */
   /* The un-activated product kept in 8 bits (NULL: in 16, in pre_act): e4m3 [padded_rows, columns rounded up to 16] with fp32 scales
    * [padded_rows, ceil(columns / 128)], columns = 2 inter (gated) or inter; rows of the padding are left as they are.  Not with
-   * `gather`, `fused_combine`, `identity` or MOE_BWD_ROUTER.  Forward: MOE_FWD_UP leaves the plain product in pre_act (scratch),
-   * MOE_FWD_ACT (part of every such pass) the activated one in hidden and the kept one here.  Backward: x holds the tokens' rows;
-   * MOE_BWD_FOLD copies the rows of grad_out to gs and those of x to xs (scratch), MOE_BWD_DOWN leaves gs W2^T in dh (scratch
-   * [padded_rows, inter]), MOE_BWD_ACT writes d_pre, d_scores and the weighted activated rows that MOE_BWD_DW2 reads (hidden, scratch). */
+   * `gather`, `fused_combine`, `identity` or MOE_BWD_ROUTER; a call that has the products and not the step between them is refused.
+   * Forward: MOE_FWD_UP leaves the plain product in pre_act (scratch), MOE_FWD_ACT (part of every such pass) the activated one in hidden
+   * and the kept one here.  Backward: x holds the tokens' rows; MOE_BWD_FOLD copies the rows of grad_out to gs and those of x to xs
+   * (scratch), MOE_BWD_DOWN leaves gs W2^T in dh (scratch [padded_rows, inter]), MOE_BWD_ACT writes d_pre, d_scores and the weighted
+   * activated rows that MOE_BWD_DW2 reads (hidden, scratch). */
   void* pre_q;
   float* pre_scales;
   void* dh;
@@ -518,9 +519,9 @@ size_t moe_expert_pass_size(void);
 #define MOE_FWD_UP 4
 #define MOE_FWD_DOWN 8
 #define MOE_FWD_FOLD 16
-#define MOE_FWD_ALL 31
 #define MOE_FWD_TAIL 32 /* first: moe_router_tail (moe_router_topk) of `logits` into `scores` and `expert_idx` */
-#define MOE_FWD_ACT 64  /* after MOE_FWD_UP: with pre_q */
+#define MOE_FWD_ACT 64  /* after MOE_FWD_UP: with pre_q (without, it is no step) */
+#define MOE_FWD_ALL 95  /* without MOE_FWD_TAIL */
 int moe_expert_forward(const moe_expert_pass* pass, int steps, void* stream);
 
 #define MOE_BWD_FOLD 1    /* gs, d_scores */
@@ -530,8 +531,8 @@ int moe_expert_forward(const moe_expert_pass* pass, int steps, void* stream);
 #define MOE_BWD_DW1 16
 #define MOE_BWD_DW2 32
 #define MOE_BWD_ROUTER 64 /* dl, dlogits, router_t */
-#define MOE_BWD_ALL 127
-#define MOE_BWD_ACT 128   /* after MOE_BWD_DOWN: with pre_q */
+#define MOE_BWD_ACT 128   /* after MOE_BWD_DOWN: with pre_q (without, it is no step) */
+#define MOE_BWD_ALL 255
 int moe_expert_backward(const moe_expert_pass* pass, int steps, void* stream);
 
 /* The functional grouped GEMM in one call, rows grouped by `group_indices` [num_experts + 1]:

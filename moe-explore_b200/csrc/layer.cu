@@ -24,6 +24,11 @@ extern "C" int moe_expert_forward(const moe_expert_pass* p, int steps, void* str
   MOE_CHECK_ARG(p != nullptr, "moe_expert_forward: null pointer argument");
   const int up_cols = glu(p->act) ? 2 * p->inter : p->inter;
   const int64_t rows = p->num_tokens * p->topk;
+  const bool kept8 = p->pre_q != nullptr;  // the un-activated product is kept in 8 bits
+  MOE_CHECK_ARG(!kept8 || (!p->identity && !p->gather && !p->fused_combine && p->pre_scales && p->pre_act && p->hidden),
+                "moe_expert_forward: pre_q goes with pre_scales, pre_act and hidden, without identity, gather and fused_combine");
+  MOE_CHECK_ARG(!kept8 || (steps & MOE_FWD_ACT) || !(steps & MOE_FWD_UP) || !(steps & MOE_FWD_DOWN),
+                "moe_expert_forward: with pre_q the down product reads what MOE_FWD_ACT writes");
   const Chain chain;
   if (p->identity) {
     // One expert, weight one: no row moves and nothing is folded.  The GEMMs read x and write out where they are.
@@ -44,9 +49,6 @@ extern "C" int moe_expert_forward(const moe_expert_pass* p, int steps, void* str
                              p->inter, p->d, 1, 0, MOE_ACT_NONE, p->dtype, 0, 1, nullptr, p->status, stream, out));
     return MOE_OK;
   }
-  const bool kept8 = p->pre_q != nullptr;  // the un-activated product is kept in 8 bits
-  MOE_CHECK_ARG(!kept8 || (!p->gather && !p->fused_combine && p->pre_scales && p->pre_act && p->hidden),
-                "moe_expert_forward: pre_q goes with pre_scales, pre_act and hidden, without gather and fused_combine");
   RowCounts counts{p->pad_offsets, p->group_indices};
   counts.routed_rows = rows;
   uint32_t* const counters = p->gather ? nullptr : reinterpret_cast<uint32_t*>(p->counters);
@@ -112,6 +114,11 @@ extern "C" int moe_expert_forward(const moe_expert_pass* p, int steps, void* str
 extern "C" int moe_expert_backward(const moe_expert_pass* p, int steps, void* stream) {
   MOE_CHECK_ARG(p != nullptr, "moe_expert_backward: null pointer argument");
   const int up_cols = glu(p->act) ? 2 * p->inter : p->inter;
+  const bool kept8 = p->pre_q != nullptr;  // d_scores and what dW2 contracts then come behind the product of the rows of grad_out
+  MOE_CHECK_ARG(!kept8 || (!p->identity && !p->gather && p->dl == nullptr && p->pre_scales && p->dh && p->xs && p->hidden),
+                "moe_expert_backward: pre_q goes with pre_scales, dh, xs and hidden, without identity, gather and the router's gradient");
+  MOE_CHECK_ARG(!kept8 || (steps & MOE_BWD_ACT) || !(steps & MOE_BWD_DOWN) || !(steps & (MOE_BWD_UP | MOE_BWD_DW1 | MOE_BWD_DW2)),
+                "moe_expert_backward: with pre_q the products behind MOE_BWD_DOWN read what MOE_BWD_ACT writes");
   const Chain chain;
   if (p->identity) {
     RowCounts in{p->pad_offsets, p->group_indices};
@@ -142,9 +149,6 @@ extern "C" int moe_expert_backward(const moe_expert_pass* p, int steps, void* st
   counts.routed_rows = p->num_tokens * p->topk;
   counts.settled = true;  // nothing of a backward pass writes the metadata or the weights
   uint32_t* const counters = reinterpret_cast<uint32_t*>(p->counters);
-  const bool kept8 = p->pre_q != nullptr;  // d_scores and what dW2 contracts then come behind the product of the rows of grad_out
-  MOE_CHECK_ARG(!kept8 || (!p->gather && p->dl == nullptr && p->pre_scales && p->dh && p->xs && p->hidden),
-                "moe_expert_backward: pre_q goes with pre_scales, dh, xs and hidden, without gather and the router's gradient");
   if ((steps & MOE_BWD_FOLD) && kept8) {
     MOE_STEP(dispatch_rows(p->grad_out, p->dst_row, p->row_src, p->num_mtiles, p->gs, p->num_tokens, p->topk, p->padded_rows, p->d,
                            p->dtype, stream, true, counters));

@@ -325,6 +325,32 @@ def test_training_step_in_a_graph(native):
     assert all(torch.equal(a, b) for a, b in zip(grads, step()))
 
 
+def test_a_pass_that_keeps_8_bits_has_its_activation(native):
+    """What the header rules out is refused before anything is launched: one expert for all rows, and products of rows that the activation's step
+    would have written.  The masks of all steps hold that step."""
+    import ctypes
+    import os
+    import re
+    lib = native.load()
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(here, "include", "moe_sm100.h")) as f:
+        masks = {name: int(value) for name, value in re.findall(r"#define (MOE_(?:FWD|BWD)_\w+) (\d+)", f.read())}
+    assert masks["MOE_FWD_ALL"] & native.FWD_ACT and masks["MOE_BWD_ALL"] & native.BWD_ACT
+    p = native.ExpertPass(num_tokens=0, padded_rows=0, d=64, inter=64, num_experts=1, topk=1, act=native.ACT_CODES["swiglu"], dtype=0)
+    for f in ("pre_act", "hidden", "xs", "dh", "pre_q", "pre_scales"):
+        setattr(p, f, 16)
+    forward = lambda steps: (lib.moe_expert_forward(ctypes.byref(p), steps, None), lib.moe_last_error())
+    backward = lambda steps: (lib.moe_expert_backward(ctypes.byref(p), steps, None), lib.moe_last_error())
+    for call, steps in ((forward, native.FWD_UP | native.FWD_DOWN), (forward, 31), (backward, native.BWD_DOWN | native.BWD_UP),
+                        (backward, native.BWD_DOWN | native.BWD_DW1), (backward, native.BWD_DOWN | native.BWD_DW2), (backward, 127)):
+        got = call(steps)
+        assert got[0] == -1 and b"_ACT" in got[1], (steps, got)
+    p.identity = 1
+    for call in (forward, backward):
+        got = call(0)
+        assert got[0] == -1 and b"identity" in got[1], got
+
+
 # ------------------------------------------------------------------------------------------------------- refusals
 def test_refusals_of_the_library(native):
     lib = native.load()
