@@ -97,6 +97,8 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor = 
         raise ValueError(f"scales are bf16 or fp16 {want} on the device of the values, got {scales.dtype} {tuple(scales.shape)}")
     if zeros is not None and (zeros.dtype is not torch.uint8 or tuple(zeros.shape) != want or zeros.device != values.device):
         raise ValueError(f"zeros are uint8 {want} on the device of the values, got {zeros.dtype} {tuple(zeros.shape)}")
+    if zeros is not None and bool((zeros > 15).any()):
+        raise ValueError(f"zeros are 0 to 15, got {int(zeros.max())}")
     tiles, steps, per_step, d = _up(n, TILE), _up(k, STEP), STEP // group, len(lead)
     pad = torch.nn.functional.pad
     p = pad(values.detach(), (0, steps * STEP // 2 - half, 0, tiles * TILE - n))
@@ -109,7 +111,7 @@ def pack_int4(values: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor = 
         t = pad(t.detach(), (0, steps * per_step - t.size(-1), 0, tiles * TILE - n))
         t = t.reshape(*lead, tiles, TILE, steps, per_step).transpose(-3, -2).contiguous()
         return t.view(torch.uint8).reshape(*lead, tiles, steps, -1)
-    blocks = [data.reshape(*lead, tiles, steps, 1024), laid(scales)] + ([] if zeros is None else [laid(zeros & 15)])
+    blocks = [data.reshape(*lead, tiles, steps, 1024), laid(scales)] + ([] if zeros is None else [laid(zeros)])
     return Int4Weight(torch.cat(blocks, -1), n, k, group, scales.dtype, zeros is not None)
 
 

@@ -197,6 +197,19 @@ def test_refusals_without_a_gpu(native):
     assert lib.moe_int4_matmul(16, 40, 64, 1, 64, 64, 32, 0, 0, None) == -1 and b"aligned" in lib.moe_last_error()
 
 
+@pytest.mark.parametrize("where", [(0, 0), (39, 4)])
+def test_zero_points_that_four_bits_do_not_hold_are_refused(where):
+    values, scales, points = raw(gen(3, "cpu"), 40, 136, group=32, zeros=True, device="cpu")
+    assert torch.equal(pack_int4(values, scales, points, group=32).unpack()[2], points)
+    points[where] = 16
+    with pytest.raises(ValueError, match="0 to 15"):
+        pack_int4(values, scales, points, group=32)
+    points[where] = 255
+    with pytest.raises(ValueError, match="0 to 15"):
+        pack_experts_int4((values[None, None], scales[None, None], points[None, None]), raw(gen(4, "cpu"), 1, 136, 40, group=32, zeros=True, device="cpu"),
+                          "silu", group=32)
+
+
 @gpu
 def test_refusals(native):
     w = pack_int4(*raw(gen(0), 16, 64, group=32), group=32)
