@@ -543,6 +543,9 @@ def act_f8_backward(q, scales, dh, dz, act):
     _count(1)
 
 
+INT4_ROWS = 1 << 21   # of one launch
+
+
 def int4_matmul(x, weight, out):
     """out [R, N] = x [R, K] @ weight^T for an ``Int4Weight`` (see moe_int4_matmul)."""
     with timed("int4:rows"):

@@ -200,5 +200,9 @@ def int4_matmul(x: torch.Tensor, weight: Int4Weight) -> torch.Tensor:
     with _native.on_device_of(x):
         rows = _dense(x if x.dim() == 2 else x.reshape(-1, weight.k))
         out = x.new_empty((rows.size(0), weight.n))
-        _native.int4_matmul(rows, weight, out)
+        if rows.size(0) <= _native.INT4_ROWS:
+            _native.int4_matmul(rows, weight, out)
+        else:
+            for part, to in zip(rows.split(_native.INT4_ROWS), out.split(_native.INT4_ROWS)):
+                _native.int4_matmul(part, weight, to)
     return out if x.dim() == 2 else out.view(*x.shape[:-1], weight.n)

@@ -165,6 +165,18 @@ def test_offsets_past_32_bits(native):
     check(out[:, -48:], x, weight64(*tail, 128), torch.bfloat16)
 
 
+@gpu
+def test_more_rows_than_one_launch_takes(native):
+    """2^21 rows are a launch's; every row is its own."""
+    weight = raw(gen(5), 16, 8, group=32)
+    rows = (1 << 21) + 70
+    x = torch.randn(rows, 8, generator=gen(6), device="cuda").bfloat16()
+    out = int4_matmul(x, pack_int4(*weight, group=32))
+    w = weight64(*weight, 32)
+    for part in (slice(0, 100), slice((1 << 21) - 64, rows)):
+        check(out[part], x[part], w, torch.bfloat16)
+
+
 # ------------------------------------------------------------------------------------------------------- refusals
 def test_refusals_without_a_gpu(native):
     values, scales, zeros = raw(gen(0, "cpu"), 16, 64, group=32, zeros=True, device="cpu")
