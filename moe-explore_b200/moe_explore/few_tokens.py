@@ -133,10 +133,21 @@ def _launch(p, x, topk: int, addend, held):
     return out
 
 
-# Above, the experts' weights are brought to 16 bits once and the pass is the 16-bit one.  Both grow with the weights, so the line does not move
-# much (us, 16 tokens at a time / in 16 bits: 64 experts of 7168 x 2048, 64 tokens 1320 / 2305, 96 1877 / 2306, 256 5093 / 2307; 64 of 2048 x
-# 1024 362 / 434, 513 / 443, 1206 / 420; 60 of 2048 x 1408 304 / 497, 448 / 492, 1090 / 491).
-EXPAND_FROM = 96
+def weights_pay_in_16_bits(tokens: int, topk: int, experts: int, elements: int) -> bool:
+    """Whether a call is shorter with the weights (``elements`` per expert) brought to 16 bits once, and the 16-bit pass over them, than by the
+    kernel for a few tokens, 16 at a time.
+
+    A slice of 16 tokens takes 21 us and reads every expert that it hits (``hit`` of them where choices are even) in 0.135 us per million
+    elements; 16 bits take 0.75 us per million elements of all experts, hit or not: written, read again.  Their launches take 90 us; 130
+    keeps small experts' weights unrounded for six slices.  Measured on both sides (us, slices / 16 bits): 64 experts of 7168 x 2048, 8 slots, 96
+    tokens 1902 / 2320, 128 2579 / 2335; 256 of 2048 x 768, 8 slots, 160 tokens 865 / 1006, 208 1129 / 1006; 256 of 2048 x 1024, 1 slot,
+    97 tokens 211 / 979, 512 995 / 1250, 1024 1980 / 1312; 1024 of 1024 x 256, 1 slot, 97 tokens 198 / 470, 1024 1488 / 633; 8 of 4096 x 14336, 2
+    slots, 64 tokens 807 / 1157, 96 1217 / 1162; 6 of 128 x 64, 2 slots, 96 tokens 158 / 91, 160 247 / 89."""
+    at_once = min(_native.FEW_TOKENS, _native.FEW_SLOTS // topk)
+    slices = -(-tokens // at_once)
+    hit = experts * (1 - (1 - 1 / experts) ** (at_once * topk))
+    millions = elements * 1e-6
+    return slices * (21 + 0.135 * millions * hit) > 130 + 0.75 * millions * experts
 
 
 def int4_experts_in_16_bits(params: Int4ExpertParams) -> MLPParams:
@@ -157,9 +168,11 @@ def int4_experts_in_16_bits(params: Int4ExpertParams) -> MLPParams:
 def int4_expert_compute(x, scores, indices, params: Int4ExpertParams, addend=None) -> torch.Tensor:
     """out[t] = sum_s scores[t, s] * (act(x[t] @ up[e]^T) @ down[e]^T) with e = indices[t, s], the weights in 4 bits.  ``x`` [T, d] in the type
     of their scales, ``scores`` (rounded to that type) and ``indices`` (int64) [T, k]; slots with an expert id out of range add nothing (and
-    are reported by the status word).  ``addend`` [T, d] is added by the fold.  For serving: no gradients.  Up to 96 tokens go through the
-    kernel for a few, 16 at a time; for more the weights are brought to 16 bits first (rounded there; as much memory as 16-bit experts
-    take, for the time of the call) and the pass is ``routed_expert_compute``'s."""
+    are reported by the status word).  ``addend`` [T, d] is added by the fold.  For serving: no gradients.  Tokens go through the kernel
+    for a few, 16 at a time, or, where that takes less time (``weights_pay_in_16_bits``: from some 100 tokens on where 16 tokens hit most
+    experts, much later where they hit few), all through ``routed_expert_compute`` with the weights brought to 16 bits first: rounded
+    there, and as much memory as 16-bit experts take for the time of the call.  ``params.expand`` = False keeps to the first, True to the
+    second."""
     params.up.checked(1, "up")
     params.down.checked(1, "down")
     _native.require_cuda(x, scores, indices, addend)
@@ -184,7 +197,10 @@ def int4_expert_compute(x, scores, indices, params: Int4ExpertParams, addend=Non
                          f"[{params.up.n}, {params.up.k}], down [{params.down.n}, {params.down.k}] for {act!r}, {E} experts, {topk} slots")
     with _native.on_device_of(x):
         ids, scores = indices.contiguous(), scores.detach().to(x.dtype).contiguous()
-        if T > EXPAND_FROM:
+        expand = params.expand
+        if expand is None:
+            expand = weights_pay_in_16_bits(T, topk, E, params.up.n * params.up.k + params.down.n * params.down.k)
+        if expand and T > 0:
             experts = int4_experts_in_16_bits(params)
             with torch.no_grad():
                 return routed_expert_compute(x, scores, experts.weight1, experts.weight2, ids, E, topk, act, addend=addend)

@@ -71,10 +71,12 @@ class Fp8ExpertParams(FFNParams):
 class Int4ExpertParams(FFNParams):
     """Experts in 4 bits, for serving (``moe_explore.functional.int4.pack_experts_int4`` and ``quantize_experts_int4`` make them): ``up``
     [E, 2I, d] with eight rows of the gate and eight of the up matrix in turn for swiglu / geglu, else [E, I, d]; ``down`` [E, d, I].
-    No reference counterpart."""
+    ``expand``: whether calls bring the weights to 16 bits first, which takes a 16-bit layer's memory for the time of the call: None where that
+    is quicker (many tokens), False never, True always.  No reference counterpart."""
     up: Int4Weight
     down: Int4Weight
     activation: Activation
+    expand: Optional[bool] = None
 
 
 @dataclass

@@ -576,6 +576,52 @@ def test_rows_near_the_end_of_bf16_get_their_norm(d, weight_type, native):
             assert near(few[t], want[t], torch.bfloat16, 4), t
 
 
+def test_which_way_experts_in_4_bits_go():
+    """By the experts that a slice of 16 tokens hits and the size of their weights, not by the number of tokens alone."""
+    from moe_explore.few_tokens import weights_pay_in_16_bits as pays
+    big = 3 * 7168 * 2048
+    assert not pays(96, 8, 64, big) and pays(128, 8, 64, big)
+    assert not pays(160, 8, 256, 3 * 2048 * 768) and pays(256, 8, 256, 3 * 2048 * 768)
+    assert not pays(97, 1, 1024, 3 * 1024 * 256) and pays(1024, 1, 1024, 3 * 1024 * 256)
+    assert not pays(512, 1, 256, 3 * 2048 * 1024) and pays(1024, 1, 256, 3 * 2048 * 1024)
+    for topk, experts, elements in ((1, 1, 64), (2, 6, 3 * 128 * 64), (8, 64, big), (64, 64, 1 << 20), (256, 1024, 1 << 16)):
+        ways = [pays(t, topk, experts, elements) for t in range(0, 2000)]
+        assert not ways[0] and ways[-1] and ways == sorted(ways)   # one line, few tokens in front of it
+
+
+@gpu
+def test_the_way_that_the_parameters_name(native):
+    """Never in 16 bits: the bits of the slices, and not the memory of the weights; always: the 16-bit pass, for few tokens too."""
+    g = gen(40)
+    d, E, k, inter, T = 512, 16, 2, 512, 400
+    q, _, _ = make_experts(g, 4, E, d, inter, "swiglu", torch.bfloat16, 64)
+    x = torch.randn(T, d, generator=g, device="cuda").bfloat16()
+    indices = torch.rand(T, E, generator=g, device="cuda").topk(k, dim=1).indices
+    scores = torch.rand(T, k, generator=g, device="cuda").bfloat16()
+    wide = int4_experts_in_16_bits(q)
+    in_16 = lambda t: routed_expert_compute(x[:t], scores[:t], wide.weight1, wide.weight2, indices[:t], E, k, "swiglu")
+    slices = torch.cat([int4_expert_compute(x[t:t + 16], scores[t:t + 16], indices[t:t + 16], q) for t in range(0, T, 16)])
+    with torch.no_grad():
+        assert torch.equal(int4_expert_compute(x, scores, indices, q), in_16(T))
+        q.expand = False
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        assert torch.equal(int4_expert_compute(x, scores, indices, q), slices)
+        torch.cuda.synchronize()
+        assert torch.cuda.max_memory_allocated() - before < (wide.weight1.numel() + wide.weight2.numel()) * 2
+        q.expand = True
+        assert torch.equal(int4_expert_compute(x[:5], scores[:5], indices[:5], q), in_16(5))
+        assert int4_expert_compute(x[:0], scores[:0], indices[:0], q).shape == (0, d)
+        # the layer asks them, too
+        p = MOEParams(make_router(g, "topk", d, E, k, torch.bfloat16), q, E, k)
+        from moe_explore.router import router
+        for expand in (True, False, None):
+            q.expand = expand
+            assert torch.equal(topk_moe_forward(x, p), int4_expert_compute(x, *router(x, p.router_params), q))
+    native.check_status(device_status(0))
+
+
 # ------------------------------------------------------------------------------------------------------- refusals
 def test_refusals_of_the_library(native):
     import ctypes
