@@ -1102,6 +1102,8 @@ extern "C" int moe_few_tokens(const moe_few_pass* p, void* stream) {
   MOE_CHECK_ARG(!routed || (p->score_function >= 0 && p->score_function <= 2 && p->normalize >= 0 && p->normalize <= 2 &&
                             (p->router_dtype == 2 || p->router_dtype == p->dtype)),
                 "moe_few_tokens: unknown router options");
+  MOE_CHECK_ARG(p->norm_w == nullptr || p->norm_dtype == 2 || p->norm_dtype == p->dtype, "moe_few_tokens: norm_w is in fp32 or the rows' type, got %d",
+                p->norm_dtype);
   if (p->num_tokens == 0) return MOE_OK;
   MOE_CHECK_ARG(p->x && p->w1 && p->w2 && p->out && p->workspace, "moe_few_tokens: null pointer argument");
   MOE_CHECK_ARG(p->residual == nullptr || (p->norm_w != nullptr && p->stream_out != nullptr), "moe_few_tokens: a residual goes with a norm and the stream");

@@ -622,6 +622,73 @@ def test_the_way_that_the_parameters_name(native):
     native.check_status(device_status(0))
 
 
+@gpu
+@pytest.mark.parametrize("groups,open_,E", [(33, 5, 99), (33, 33, 99), (64, 40, 256), (64, 1, 512), (64, 63, 1024)])
+def test_many_groups(groups, open_, E, native):
+    """More groups than lanes (the router's own kernel takes 32): against the choice in 64 bits."""
+    g = gen(groups * open_)
+    k = min(6, open_ * (E // groups))
+    for best in (1, 2):
+        rp = grouped(E, k, 0.1 * torch.randn(E, generator=g, device="cuda"), groups, open_, best, normalize=True)
+        logits = torch.randn(16, E, generator=g, device="cuda")
+        got = weights_of(logits, rp, E).double()
+        w, i = route64(rp, logits.double())
+        want = torch.zeros_like(got).scatter_(1, i, w)
+        assert torch.equal(got != 0, want != 0)
+        assert bool(((got - want).abs() <= (2.0 ** -8 + 2.0 ** -18) * want).all())   # (k sums of 32 bits beside the rounding)
+    native.check_status(device_status(0))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 16), (torch.float16, 4)])
+def test_the_widest_rows(dtype, bits, native):
+    """16 tokens of 16384 columns: as much shared memory as the first kernel asks for."""
+    g = gen(21)
+    d, E, k, inter = 16384, 18, 2, 24
+    experts, w1, w2 = make_experts(g, bits, E, d, inter, "swiglu", dtype)
+    rp = make_router(g, "topk norm", d, E, k, dtype)
+    norm = RMSNormParams((1 + 0.1 * torch.randn(d, generator=g, device="cuda")).to(dtype), 1e-5)
+    p = MOEParams(rp, experts, E, k, None, norm)
+    x, residual = (torch.randn(16, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    h = (x + residual)
+    y = h.double()
+    y = y / (y.square().mean(-1, keepdim=True) + 1e-5).sqrt() * norm.weight.double()
+    with torch.no_grad():
+        out, stream = few_token_layer(x, p, residual, None, norm)
+    assert torch.equal(stream, h)
+    assert near(out, experts64(y, *route64(rp, y @ rp.router_weight.double()), w1, w2, "swiglu"), dtype, 4)
+    native.check_status(device_status(0))
+
+
+@gpu
+@pytest.mark.parametrize("norm_type", [torch.bfloat16, torch.float32])
+def test_the_library_with_a_norm_and_given_experts(norm_type, native):
+    """The C entry without a router: one cluster norms the rows, experts and scores are the caller's."""
+    g = gen(22)
+    T, d, E, k, inter = 9, 264, 6, 2, 40
+    experts, w1, w2 = make_experts(g, 16, E, d, inter, "swiglu", torch.bfloat16)
+    weight = (1 + 0.1 * torch.randn(d, generator=g, device="cuda")).to(norm_type)
+    x, residual = (torch.randn(T, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    ids = torch.randint(0, E, (T, k), generator=g, device="cuda")
+    scores = torch.rand(T, k, generator=g, device="cuda").bfloat16()
+    out, stream = torch.empty_like(x), torch.empty_like(x)
+    workspace = torch.empty(native.few_workspace_bytes(T, d, inter, E, k), dtype=torch.uint8, device="cuda")
+    p = native.FewPass(num_tokens=T, d=d, inter=inter, num_experts=E, topk=k, act=native.ACT_CODES["swiglu"], dtype=0, bits=16, eps=1e-5,
+                       norm_dtype=native.float_code(norm_type))
+    p.x, p.residual, p.norm_w, p.stream_out, p.out = (t.data_ptr() for t in (x, residual, weight, stream, out))
+    p.w1, p.w2, p.expert_idx, p.scores = (t.data_ptr() for t in (experts.weight1, experts.weight2, ids, scores))
+    p.status, p.workspace, p.workspace_bytes = device_status(0).data_ptr(), workspace.data_ptr(), workspace.numel()
+    native.few_tokens(p)
+    h = x + residual
+    y = h.double()
+    y = y / (y.square().mean(-1, keepdim=True) + 1e-5).sqrt() * weight.double()
+    want = torch.zeros_like(y)
+    for s in range(k):   # (a token may have an expert twice)
+        want += experts64(y, scores[:, s:s + 1].double(), ids[:, s:s + 1], w1, w2, "swiglu")
+    assert torch.equal(stream, h) and near(out, want, torch.bfloat16, 4)
+    native.check_status(device_status(0))
+
+
 # ------------------------------------------------------------------------------------------------------- refusals
 def test_refusals_of_the_library(native):
     import ctypes
@@ -644,6 +711,17 @@ def test_refusals_of_the_library(native):
         got = call(base(**kw))
         assert got[0] == rc and text in got[1], (kw, got)
     assert call(base(num_tokens=0))[0] == 0
+
+
+def test_the_library_refuses_norms_of_another_type(native):
+    import ctypes
+    lib = native.load()
+    for dtype, norm_dtype in ((0, 1), (1, 0), (0, 3), (1, -1)):
+        p = native.FewPass(num_tokens=1, d=64, inter=64, num_experts=8, topk=2, act=3, dtype=dtype, bits=16, norm_dtype=norm_dtype)
+        p.expert_idx = p.scores = p.norm_w = 16
+        assert lib.moe_few_tokens(ctypes.byref(p), None) == -1 and b"norm_w" in lib.moe_last_error()
+        p.norm_w = None
+        assert lib.moe_few_tokens(ctypes.byref(p), None) == -1 and b"null" in lib.moe_last_error()
 
 
 @gpu
