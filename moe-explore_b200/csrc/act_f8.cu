@@ -12,7 +12,8 @@
 // Bound by HBM beside instructions (the forward pass issues about 300 per 16 columns: exponentials, reciprocals and exactly rounded quotients;
 // 72 % of the issue slots): 65536 x 2816 swiglu 132 us forward and 129 back, 114 each at the copy's rate; geglu 182 and 188 (erff).
 // A lane takes 16 columns of a row, eight lanes share a block and ask for their next one before they compute.  The backward pass walks
-// a row (or, where there are few rows, a share of one) 512 columns at a time: the gradient of a slot's weight is a sum over its row.
+// a row (or, where there are few rows, a share of one) 512 columns at a time: the gradient of a slot's weight is a sum over its row.  (That
+// of a layer spills 4 to 52 bytes to stay within the 64 registers of four CTAs per SM.)
 #include "f8.cuh"
 
 namespace moe {

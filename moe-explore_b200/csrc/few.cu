@@ -4,11 +4,12 @@
 //   second:  scores and experts of every token (each CTA for itself);  hidden = round(act(y W1[e])) for the chosen experts;
 //            rows = hidden W2[e] in fp32;  out = round(sum over the slots of score * row + addend)
 //
-// Bound by reading the chosen experts' weights once (16 bits: 16 tokens x 8 on 64 experts of 2048 x 1024, 711 MB, in 136 us, the up product's
-// part at 6.7 TB/s), by what it costs to make numbers of 4-bit ones (64 experts of 7168 x 2048, 1.2 GB, 305 us), and for one token by what
+// Bound by reading the chosen experts' weights (16 bits: 16 tokens x 8 on 64 experts of 2048 x 1024, 711 MB, in 139 us, the up product's
+// part at 6.7 TB/s), by what it costs to make numbers of 4-bit ones (64 experts of 7168 x 2048, 1.2 GB, 300 to 321 us), and for one token by what
 // is not reading: of 37 us for 69 MB the first kernel and the way to the second are 8, choosing 4, meeting twice 4.  The second kernel
-// is one resident wave (a cooperative launch, so that its CTAs may
-// wait for one another): between its three phases they meet at a counter in global memory that the first kernel has set to zero.
+// is one resident wave (a cooperative launch, so that its CTAs may wait for one another): between its three phases they meet at a counter
+// in global memory that the first kernel has set to zero.  Weights are copied once per entry, eight slots of an expert: twice for
+// an expert that 9 to 16 slots chose.
 // Every sum has a fixed order: nothing depends on timing.
 //
 // The logits are not rounded to 16 bits, nor are an expert's rows before the fold; y and the activated product are, because they are
@@ -347,8 +348,8 @@ __device__ __forceinline__ V group_worth(const FewArgs& a, bool both, typename O
   return v + w;
 }
 
-// The choice in 64 bits, all of it in shared memory: for the rare token whose values fp32 does not tell apart.  Leaves the experts and their
-// shares; the lane's part of their sum.
+// The choice in 64 bits, all of it in shared memory: for the rare token whose values fp32 does not tell apart (one of 64 experts in 8 groups: 9 us
+// more for the call, 256: 10, 1024: 21; all 16 tokens 15, 24 and 70).  Leaves the experts and their shares; the lane's part of their sum.
 __device__ __noinline__ float choose_exactly(const FewArgs& a, int t, unsigned long long* keys, FewRouting& r, float most, int lane) {
   typedef Order<double> O;
   const float* from = a.logits + static_cast<int64_t>(t) * a.E;

@@ -100,7 +100,8 @@ __global__ void __launch_bounds__(kQ4Warps * 32, 2) q4_rows_kernel(const Q4Args 
 // columns of the rows lie in shared memory once, and the numbers made of a word are used for all rows.  16, 32, 64 rows of 4096 by 28672: 28,
 // 43, 78 us (by eights: 36, 70, 134), the tensor pipe busy for 40 % of it with two warps per scheduler; 9 and 16 rows of 7168 by 4096
 // 9.1 and 9.4 (by eights 13.7 and 14.8).  With one tile per warp and twice the CTAs an SM, which read the rows out of shared memory twice as
-// often, 84 us for the 64 rows and 10.7 for the 16.
+// often, 84 us for the 64 rows and 10.7 for the 16.  64 and 32 rows take all registers that two (three) CTAs per SM leave, 255 (168), and
+// spill 32 to 144 (4 to 32) bytes.
 constexpr int kQ4ManyWarps = 4, kQ4ManyDepth = 3;
 template <int NG, bool ZEROS, int MT> struct Q4Many {
   static constexpr int kBlock = Q4Stage<NG, ZEROS>::kBlock, kRows = kQ4ManyWarps * kQ4Tiles * kBlock, kStage = kRows + MT * 2048;

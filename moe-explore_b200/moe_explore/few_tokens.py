@@ -2,7 +2,7 @@
 
 The ordinary pass over the experts is made of seven or eight launches around tiles of 64 rows and more; a decoding step's few rows wait
 for these launches as long as for the weights.  Here the first kernel adds the residual, norms and computes the router's logits, and the
-second chooses the experts, reads their weights once and folds the result.  No reference counterpart.
+second chooses the experts, reads their weights (once per eight slots of an expert) and folds the result.  No reference counterpart.
 """
 from __future__ import annotations
 
@@ -192,7 +192,7 @@ def int4_expert_compute(x, scores, indices, params: Int4ExpertParams, addend=Non
         raise RuntimeError("experts in 4 bits have no backward pass: call this under torch.no_grad(), or train 16-bit experts")
     T, topk = indices.shape
     E = params.up.data.size(0)
-    if _experts(params, x.dtype, E, x.size(1), act) is None or not 0 < topk <= _native.FEW_SLOTS or E > _native.FEW_EXPERTS:
+    if _experts(params, x.dtype, E, x.size(1), act) is None or not 0 < topk <= _native.FEW_SLOTS or not 0 < E <= _native.FEW_EXPERTS:
         raise ValueError(f"these experts do not fit together or are more than the kernel takes (1024 experts, 256 slots): input {tuple(x.shape)}, up "
                          f"[{params.up.n}, {params.up.k}], down [{params.down.n}, {params.down.k}] for {act!r}, {E} experts, {topk} slots")
     with _native.on_device_of(x):
