@@ -4,9 +4,9 @@
 //   second:  scores and experts of every token (each CTA for itself);  hidden = round(act(y W1[e])) for the chosen experts;
 //            rows = hidden W2[e] in fp32;  out = round(sum over the slots of score * row + addend)
 //
-// Bound by reading the chosen experts' weights (16 bits: 16 tokens x 8 on 64 experts of 2048 x 1024, 711 MB, in 139 us, the up product's
-// part at 6.7 TB/s), by what it costs to make numbers of 4-bit ones (64 experts of 7168 x 2048, 1.2 GB, 300 to 321 us), and for one token by what
-// is not reading: of 37 us for 69 MB the first kernel and the way to the second are 8, choosing 4, meeting twice 4.  The second kernel
+// Bound by reading the chosen experts' weights (16 bits: 16 tokens x 8 on 64 experts of 2048 x 1024, 711 MB, in 136 us, the up product's
+// part at 6.7 TB/s), by what it costs to make numbers of 4-bit ones (64 experts of 7168 x 2048, 1.2 GB, 318 us), and for one token by what
+// is not reading: of 36 us for 69 MB the first kernel and the way to the second are 8, choosing 4, meeting twice 4.  The second kernel
 // is one resident wave (a cooperative launch, so that its CTAs may wait for one another): between its three phases they meet at a counter
 // in global memory that the first kernel has set to zero.  Weights are copied once per entry, eight slots of an expert: twice for
 // an expert that 9 to 16 slots chose.
@@ -348,9 +348,9 @@ __device__ __forceinline__ V group_worth(const FewArgs& a, bool both, typename O
   return v + w;
 }
 
-// The choice in 64 bits, all of it in shared memory: for the rare token whose values fp32 does not tell apart (one of 64 experts in 8 groups: 9 us
-// more for the call, 256: 10, 1024: 21; all 16 tokens 15, 24 and 70).  Leaves the experts and their shares; the lane's part of their sum.
-__device__ __noinline__ float choose_exactly(const FewArgs& a, int t, unsigned long long* keys, FewRouting& r, float most, int lane) {
+// The choice in 64 bits, all of it in shared memory: for the rare token whose values fp32 does not tell apart (one token, 64 experts in 8 groups: 7
+// us more for the call, 256: 10, 1024: 20; all of 16 tokens 14, 23 and 70).  Leaves the experts and their shares; the lane's part of their sum.
+__device__ __forceinline__ float choose_exactly(const FewArgs& a, int t, unsigned long long* keys, FewRouting& r, float most, int lane) {
   typedef Order<double> O;
   const float* from = a.logits + static_cast<int64_t>(t) * a.E;
   const bool sigmoid = a.sigmoid != 0;
@@ -410,13 +410,14 @@ __device__ __noinline__ float choose_exactly(const FewArgs& a, int t, unsigned l
   return total;
 }
 
-// One warp, one token; expert lane + 32 i is the lane's i-th of up to EACH.  `keys`: scratch of this warp's own, [E] and [groups].
+// One warp, one token; expert lane + 32 i is the lane's i-th of up to EACH.  `keys`: scratch of this warp's own, [E] and [groups].  Leaves
+// the experts, their shares, the largest logit and the lane's part of the shares' sum; false where the choice is to be made exactly.
 //
 // The logits decide where they are all that does (shares grow with them).  Where shares with a bias, or sums of two, are compared, the choice
 // is that of exact arithmetic on the fp32 logits: values closer than what fp32 can be off by are decided again in 64 bits -- but for
 // the router whose definition is in 32 bits (normalize 2).  Equal values by ascending index.  NaN is taken after everything else, or,
 // where the softmax runs over the selected logits, before (the row is NaN then, as it is behind torch.topk).
-template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int t, uint32_t* keys, FewRouting& r, int lane) {
+template <int EACH> __device__ __forceinline__ bool choose(const FewArgs& a, int t, uint32_t* keys, FewRouting& r, float& most, float& total, int lane) {
   constexpr uint32_t kAll = 0xFFFFFFFFu;
   typedef Order<float> O;
   const float* from = a.logits + static_cast<int64_t>(t) * a.E;
@@ -430,7 +431,8 @@ template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int
     bias[i] = e < a.E && biased ? a.bias[e] : 0.0f;
   }
   uint32_t key[EACH];   // 0: no expert, or taken, or in a closed group
-  float most = -3.402823466e38f, sum = 0.0f;
+  float sum = 0.0f;
+  most = -3.402823466e38f;
 #pragma unroll
   for (int i = 0; i < EACH; ++i) {
     most = fmaxf(most, p[i]);
@@ -525,7 +527,7 @@ template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int
       if (key[i] > best) best = key[i], at = lane + 32 * i, share = p[i];
   };
   look();
-  float total = 0.0f;
+  total = 0.0f;
   uint32_t last = 0;
   for (int s = 0; s < a.k; ++s) {
     last = __reduce_max_sync(kAll, best);
@@ -545,26 +547,28 @@ template <int EACH> __device__ __forceinline__ void choose(const FewArgs& a, int
     const float above = O::value(last), below = O::value(next);
     sure = sure && !(next != 0 && above - below <= 2.0f * slack + 1.2e-7f * (fabsf(above) + fabsf(below)));
   }
-  if (!sure) total = choose_exactly(a, t, reinterpret_cast<unsigned long long*>(keys), r, most, lane);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(kAll, total, off);
-  __syncwarp();
-  const float by = a.softmax_after ? total : a.normalize == 2 ? fmaxf(total, 1e-12f) : a.normalize == 1 ? total + 1e-20f : 1.0f;
-  for (int s = lane; s < a.k; s += 32) r.score[t * a.k + s] = r.score[t * a.k + s] / by * (a.softmax_after ? 1.0f : a.scale);
-  __syncwarp();
+  return sure;
 }
 
 // Scores, experts, and the list of entries: up to eight slots of one expert each.  Entries of one expert follow one another (they read
-// the same weights at the same time), experts by their first slots.
-template <typename T> __device__ __forceinline__ void route(const FewArgs& a, FewRouting& r, uint32_t* scratch) {
+// the same weights at the same time), experts by their first slots.  A function of its own, so that its registers are not the products': 1
+// token on 8 experts of 4096 x 14336 in 4 bits 77 us on the device instead of 84, 16 of 64 of 7168 x 2048 318 instead of 322.
+template <typename T> __device__ __noinline__ void route(const FewArgs& a, FewRouting& r, uint32_t* scratch) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int slots = a.T * a.k;
   if (a.logits != nullptr) {
     uint32_t* const keys = scratch + warp * 2 * (a.E + a.groups);  // (room for 64-bit ones)
     for (int t = warp; t < a.T; t += kFewWarps) {
-      if (a.E <= 64) choose<2>(a, t, keys, r, lane);
-      else if (a.E <= 256) choose<8>(a, t, keys, r, lane);
-      else choose<32>(a, t, keys, r, lane);
+      float most, total;
+      const bool sure = a.E <= 64 ? choose<2>(a, t, keys, r, most, total, lane) : a.E <= 256 ? choose<8>(a, t, keys, r, most, total, lane)
+                                                                                 : choose<32>(a, t, keys, r, most, total, lane);
+      if (!sure) total = choose_exactly(a, t, reinterpret_cast<unsigned long long*>(keys), r, most, lane);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, off);
+      __syncwarp();
+      const float by = a.softmax_after ? total : a.normalize == 2 ? fmaxf(total, 1e-12f) : a.normalize == 1 ? total + 1e-20f : 1.0f;
+      for (int s = lane; s < a.k; s += 32) r.score[t * a.k + s] = r.score[t * a.k + s] / by * (a.softmax_after ? 1.0f : a.scale);
+      __syncwarp();
     }
   } else if (tid < slots) {
     const int64_t e = a.ids[tid];
